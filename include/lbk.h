@@ -771,6 +771,76 @@ int lbk_block_ell_topk_columns(const void* dense, int64_t ld, int32_t elem_bytes
  */
 int lbk_ternary_check_codes(const uint32_t* words, int64_t n_words, int32_t* bad_count, void* stream);
 
+/*
+ * Microscaled 4-bit floating point (MXFP4).  Groups of 32 consecutive input features share a power of
+ * two: scale byte b stands for 2^(b - 127), b = clamp(floor(log2 max|x|) - 2 + 127, 0, 254), or 255
+ * (NaN) where the group holds an Inf or a NaN.  A code is a sign bit and one of 0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6: the nearest to x / 2^(b - 127), ties to the even code, beyond 6 to 6.  Two codes a byte, the even
+ * index in the low half.  No counterpart in the reference.
+ */
+enum { LBK_BF16 = 0, LBK_FP16 = 1, LBK_FP32 = 2 };
+
+/* One Block-ELL weight in 4 bits: groups run along B_in, so B is 32 or 64.
+ *   codes  [R, K, B_out, B_in/2], 16-byte aligned;  scales [R, K, B_out, B_in/32]. */
+typedef struct lbk_bell_mx {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const int32_t* col_idx;
+    int32_t R, K, B;
+} lbk_bell_mx;
+
+/* Rows of x [N, F] (row stride ldx elements, F a multiple of 32, rows 16-byte aligned) -> codes
+ * [N, F/2], scales [N, F/32], and back to `dtype` (contiguous). */
+int lbk_mx_quantize(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx, uint8_t* codes,
+                    uint8_t* scales, void* stream);
+int lbk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t N, int32_t F, int32_t dtype,
+                      void* out, void* stream);
+/* Tiles [R, K, B_in, B_out] <-> the codes and scales of an lbk_bell_mx. */
+int lbk_mx_quantize_tiles(const void* values, int32_t dtype, int32_t R, int32_t K, int32_t B, uint8_t* codes,
+                          uint8_t* scales, void* stream);
+int lbk_mx_dequantize_tiles(const uint8_t* codes, const uint8_t* scales, int32_t R, int32_t K, int32_t B,
+                            int32_t dtype, void* values, void* stream);
+
+/*
+ * y[N, R*B] = Q(x)[N, in_features] W (+ bias), x and y contiguous bf16, Q the quantisation above (done
+ * in the call).  Slots whose column is negative or >= in_features / B contribute nothing.
+ */
+size_t lbk_mx_matmul_workspace_bytes(int64_t N, int32_t in_features, const lbk_bell_mx* w);
+int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const lbk_bell_mx* w, const float* bias,
+                       uint16_t* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * out = W_down Q(h) (+ b_down) (+ x),  h = silu(W_gate Q(x) + b_gate) * (W_up Q(x) + b_up) in fp32.
+ * Biases are fp32, each optional.  The call's hidden state lives quantised in the workspace.
+ */
+size_t lbk_mx_swiglu_workspace_bytes(int64_t N, int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx* up,
+                                     const lbk_bell_mx* down);
+int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const lbk_bell_mx* gate,
+                           const lbk_bell_mx* up, const lbk_bell_mx* down, const float* b_gate, const float* b_up,
+                           const float* b_down, int add_residual, uint16_t* out, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
+ * The dense gated FFN: out = (act(x w_gate^T) * (x w_up^T)) w_down^T (+ x), dense weights [out, in]
+ * (w_gate, w_up [d_ff, d_model], w_down [d_model, d_ff]), everything of one type, LBK_BF16 or LBK_FP16,
+ * contiguous and 16-byte aligned; d_model and d_ff are multiples of 8.  The dense form of the
+ * reference's PyTorch layer (interop/pt_model.py:851-903).
+ *
+ * The forward gives h = act(gate) * up, gate_pre and up_out [N, d_ff] for the backward, all three or
+ * none.  The backward's four gradients are each optional; w_* are the forward's.
+ */
+enum { LBK_SILU = 0, LBK_GELU = 1 };   /* LBK_GELU: the tanh form */
+
+size_t lbk_gated_fwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff, int want_intermediates);
+int lbk_gated_fwd(int32_t dtype, int32_t act, const void* x, int64_t N, int32_t d_model, int32_t d_ff,
+                  const void* w_gate, const void* w_up, const void* w_down, int add_residual, void* out, void* h_out,
+                  void* gate_pre_out, void* up_out, void* workspace, size_t workspace_bytes, void* stream);
+size_t lbk_gated_bwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff);
+int lbk_gated_bwd(int32_t dtype, int32_t act, const void* grad_out, const void* x, const void* gate_pre,
+                  const void* up_out, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
+                  const void* w_up, const void* w_down, int add_residual, void* dx, void* dw_gate, void* dw_up,
+                  void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

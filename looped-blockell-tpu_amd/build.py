@@ -25,7 +25,8 @@ LIB = os.path.join(PKG, "liblbk.so")
 EXT = os.path.join(PKG, "_titan_ext.so")
 
 HIP_SOURCES = ["lbk_bf16.hip", "lbk_split.hip", "lbk_tile64.hip", "lbk_decode.hip", "lbk_ternary.hip", "lbk_tsplit.hip", "lbk_bwd.hip", "lbk_topo.hip", "lbk_format.hip",
-               "lbk_abi.hip", "lbk_noalloc.hip"]
+               "lbk_mx.hip", "lbk_gated.hip", "lbk_abi.hip", "lbk_noalloc.hip"]
+EXT_SOURCES = ["torch_ops.cpp", "torch_ffn.cpp"]
 ARCH = os.environ.get("LBK_OFFLOAD_ARCH", "gfx950")
 
 # Packed-fp32 VALU forms are kept out of the generated code.
@@ -85,11 +86,18 @@ def build_ext() -> str:
     libdirs = ce.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     py_inc = sysconfig.get_paths()["include"]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           f"-I{INCLUDE}", f"-I{py_inc}"]
-    cmd += [f"-I{p}" for p in incs]
-    cmd += [os.path.join(CSRC, "torch_ops.cpp")]
+    from concurrent.futures import ThreadPoolExecutor
+
+    objdir = os.path.join(HERE, "_build")
+    os.makedirs(objdir, exist_ok=True)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             f"-I{INCLUDE}", f"-I{CSRC}", f"-I{py_inc}", *[f"-I{p}" for p in incs]]
+    objs = [os.path.join(objdir, src.replace(".cpp", ".o")) for src in EXT_SOURCES]
+    cmds = [["g++", *flags, "-c", os.path.join(CSRC, src), "-o", obj] for src, obj in zip(EXT_SOURCES, objs)]
+    with ThreadPoolExecutor(len(cmds)) as pool:
+        for fut in [pool.submit(_run, c) for c in cmds]:
+            fut.result()
+    cmd = ["g++", "-shared", *objs]
     cmd += [f"-L{p}" for p in libdirs]
     cmd += ["-L/opt/rocm/lib", f"-L{PKG}", "-llbk", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
             "-ltorch_hip", "-lamdhip64", "-Wl,-rpath,$ORIGIN"]

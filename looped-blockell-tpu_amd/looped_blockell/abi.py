@@ -40,6 +40,17 @@ class BellTernary(C.Structure):
                 ("R", C.c_int32), ("K", C.c_int32), ("B", C.c_int32)]
 
 
+class BellMx(C.Structure):
+    """``lbk_bell_mx``: 4-bit codes, scale bytes, column indices."""
+
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("col_idx", C.c_void_p),
+                ("R", C.c_int32), ("K", C.c_int32), ("B", C.c_int32)]
+
+
+LBK_BF16, LBK_FP16, LBK_FP32 = 0, 1, 2
+LBK_SILU, LBK_GELU = 0, 1
+
+
 class TernaryAcc(C.Structure):
     """``lbk_ternary_acc``: optional accumulator exports of the ternary SwiGLU (device pointers)."""
 
@@ -65,6 +76,7 @@ _SZ = C.c_size_t
 _F = C.c_float
 _PB = C.POINTER(Bell)
 _PT = C.POINTER(BellTernary)
+_PM = C.POINTER(BellMx)
 SIGNATURES = {
     "lbk_status_string": (C.c_char_p, [C.c_int]),
     "lbk_version": (C.c_int, []),
@@ -157,6 +169,19 @@ SIGNATURES = {
     "lbk_ternary_prepared_workspace_bytes": (_SZ, [_I64, _I32, _PT, _PT, _PT]),
     "lbk_swiglu_fwd_ternary_prepared": (C.c_int, [_P, _P, _I64, _I32, _PT, _PT, _PT, _P, _SZ, _P, _P, _P, _P, _P,
                                                   C.POINTER(TernaryAcc), _P, _SZ, _P]),
+    "lbk_mx_quantize": (C.c_int, [_P, _I32, _I64, _I32, _I64, _P, _P, _P]),
+    "lbk_mx_dequantize": (C.c_int, [_P, _P, _I64, _I32, _I32, _P, _P]),
+    "lbk_mx_quantize_tiles": (C.c_int, [_P, _I32, _I32, _I32, _I32, _P, _P, _P]),
+    "lbk_mx_dequantize_tiles": (C.c_int, [_P, _P, _I32, _I32, _I32, _I32, _P, _P]),
+    "lbk_mx_matmul_workspace_bytes": (_SZ, [_I64, _I32, _PM]),
+    "lbk_mx_matmul_bf16": (C.c_int, [_P, _I64, _I32, _PM, _P, _P, _P, _SZ, _P]),
+    "lbk_mx_swiglu_workspace_bytes": (_SZ, [_I64, _I32, _PM, _PM, _PM]),
+    "lbk_mx_swiglu_fwd_bf16": (C.c_int, [_P, _I64, _I32, _PM, _PM, _PM, _P, _P, _P, C.c_int, _P, _P, _SZ, _P]),
+    "lbk_gated_fwd_workspace_bytes": (_SZ, [_I64, _I32, _I32, C.c_int]),
+    "lbk_gated_fwd": (C.c_int, [_I32, _I32, _P, _I64, _I32, _I32, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P, _SZ, _P]),
+    "lbk_gated_bwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
+    "lbk_gated_bwd": (C.c_int, [_I32, _I32, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P,
+                                _SZ, _P]),
 }
 
 _lib = None

@@ -446,3 +446,75 @@ def ternary_swiglu_fwd_accumulators(xq, sx, gate, up, down, x_resid=None):
     (reference ``bonsai-test/bitlinear.py:34-69``) with one scale per block."""
     _gpu(xq)
     return ops().block_ell_swiglu_fwd_ternary_accumulators(xq, sx, *gate, *up, *down, x_resid)
+
+
+# ---------------------------------------------------------------- microscaled 4-bit path
+
+def mx_quantize(x):
+    """x [..., F] (bf16, fp16 or fp32, F a multiple of 32) in microscaled 4-bit floating point:
+    ``(codes uint8 [..., F/2], scales uint8 [..., F/32])``.  Groups of 32 features share the power
+    of two ``2^(scale - 127)``; a code is a sign and the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties
+    to the even code, beyond 6 to 6), two a byte, the even feature low.  A group that holds an Inf or
+    a NaN gets scale 255 and reads back as NaN."""
+    _gpu(x)
+    lead = x.shape[:-1]
+    codes, scales = ops().mx_quantize(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    return codes.reshape(*lead, codes.shape[-1]), scales.reshape(*lead, scales.shape[-1])
+
+
+def mx_dequantize(codes, scales, dtype: torch.dtype = torch.bfloat16):
+    """The values that ``mx_quantize``'s codes and scales stand for, [..., F]."""
+    _gpu(codes, scales)
+    out = ops().mx_dequantize(codes.reshape(-1, codes.shape[-1]), scales.reshape(-1, scales.shape[-1]), dtype)
+    return out.reshape(*codes.shape[:-1], out.shape[-1])
+
+
+def mx_quantize_tiles(values):
+    """Tiles [R, K, B_in, B_out] (B 32 or 64) -> ``(codes uint8 [R, K, B_out, B_in/2], scales uint8
+    [R, K, B_out, B_in/32])``, in groups of 32 input features."""
+    _gpu(values)
+    return ops().mx_quantize_tiles(values)
+
+
+def mx_dequantize_tiles(codes, scales, dtype: torch.dtype = torch.bfloat16):
+    """The tiles [R, K, B_in, B_out] that ``mx_quantize_tiles``'s codes and scales stand for."""
+    _gpu(codes, scales)
+    return ops().mx_dequantize_tiles(codes, scales, dtype)
+
+
+def mx_matmul(x, codes, scales, col_indices, bias=None):
+    """x [..., C*B] -> [..., R*B] through a Block-ELL weight in 4 bits (``mx_quantize_tiles``), x
+    quantised in the call, sums in fp32; not differentiable."""
+    _gpu(x, codes, scales, col_indices)
+    lead = x.shape[:-1]
+    y = ops().block_ell_matmul_mx(x.reshape(-1, x.shape[-1]).to(torch.bfloat16), codes, scales, col_indices, bias)
+    return y.reshape(*lead, y.shape[-1])
+
+
+def mx_swiglu(x, gate, up, down, add_residual: bool = False, b_gate=None, b_up=None, b_down=None):
+    """The SwiGLU FFN on weights in 4 bits: gate, up and down are (codes, scales, col_indices) triples.
+    x and the hidden state ``silu(gate) * up`` (formed in fp32) are quantised in the call; not
+    differentiable."""
+    _gpu(x, gate[0], up[0], down[0])
+    lead = x.shape[:-1]
+    y = ops().block_ell_swiglu_fwd_mx(x.reshape(-1, x.shape[-1]).to(torch.bfloat16), *gate, b_gate, *up, b_up, *down, b_down,
+                                      add_residual)
+    return y.reshape(*lead, y.shape[-1])
+
+
+# ---------------------------------------------------------------- dense gated FFN
+
+def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", add_residual: bool = False):
+    """``(act(x w_gate^T) * (x w_up^T)) w_down^T (+ x)`` with dense weights [out, in], all bf16 or all
+    fp16; ``activation`` 'silu' or 'gelu' (tanh form); d_model and d_ff multiples of 8.
+    Differentiable in x and the weights as one native autograd node (``titan::gated_ffn_train``),
+    gradients in the inputs' type; without gradients nothing is kept."""
+    _gpu(x, w_gate, w_up, w_down)
+    lead = x.shape[:-1]
+    x2 = x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+        _no_transforms()
+        y = ops().gated_ffn_train(x2, w_gate, w_up, w_down, activation, add_residual)
+    else:
+        y = ops().gated_ffn_fwd(x2, w_gate, w_up, w_down, activation, add_residual)
+    return y.reshape(*lead, y.shape[-1])
