@@ -15,6 +15,9 @@
 // the other 16: a group of 32 outputs is requantised with one exchange.
 #include "lbk.h"
 #include "lbk_device.h"
+#include "lbk_internal.h"
+
+#include <type_traits>
 
 namespace lbk {
 
@@ -189,6 +192,50 @@ __global__ __launch_bounds__(256) void mx_dequantize_tiles_kernel(const uint8_t*
   }
 }
 
+// ------------------------------------------------------------------ token panels
+// The quantised tokens that the panel products read: blocks of TB = 32 MT tokens, each [group][token] codes
+// of 16 bytes, then [group][token % 32][token / 32] scale bytes, both padded to 1 KB: a workgroup copies a
+// block to LDS as it lies, 32 lanes read consecutive 16-byte pieces there, and one read gives the scale
+// bytes of a lane's MT tokens.  Tokens behind the last one hold whatever was there: they reach no output.
+struct Panel {
+  int64_t codes, bytes;      // bytes of a block's codes, and of the block
+};
+__host__ __device__ inline Panel panel_of(int G, int TB) {
+  const int64_t c = ((int64_t)G * TB * 16 + 1023) & ~(int64_t)1023;
+  return {c, c + (((int64_t)G * TB + 1023) & ~(int64_t)1023)};
+}
+
+// x [N, F] bf16 -> panel blocks.  A wave takes 16 tokens and two groups (a 128-byte line of each token):
+// four lanes a token and group, 8 features each.
+__global__ __launch_bounds__(256) void mx_quantize_panel_kernel(const uint16_t* __restrict__ x, int64_t N, int F, int TB,
+                                                                uint8_t* __restrict__ panels) {
+  const int lane = threadIdx.x & 63, G = F >> 5, pairs = (G + 1) >> 1;
+  const int64_t wv = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t n = wv / pairs * 16 + (lane >> 2);
+  const int g0 = (int)(wv % pairs) * 2, part = lane & 3;
+  if (n >= N) return;                                             // four lanes of a token leave together
+  const Panel P = panel_of(G, TB);
+  uint8_t* blk = panels + n / TB * P.bytes;
+  const int tt = (int)(n % TB), MT = TB / 32;
+  float f[2][8];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (g0 + k < G) load8<LBK_BF16>(x + n * F + (g0 + k) * 32 + part * 8, f[k]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (g0 + k >= G) break;
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, absbits(f[k][e]));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+    const uint32_t b = mx_scale(m);
+    const int64_t at = (int64_t)(g0 + k) * TB;
+    *reinterpret_cast<uint32_t*>(blk + (at + tt) * 16 + part * 4) = mx_code8(f[k], mx_pow2(b));
+    if (part == 0) blk[P.codes + at + (tt & 31) * MT + (tt >> 5)] = (uint8_t)b;
+  }
+}
+
 // ------------------------------------------------------------------ products
 struct MxArgs {
   const uint8_t* xc; const uint8_t* xs;     // quantised tokens [N, F / 2], [N, F / 32]
@@ -293,6 +340,216 @@ __global__ __launch_bounds__(256) void mx_rowblock_kernel(MxArgs a) {
       store_bf16x<4>(a.y + n * ld + o, f);
     }
   }
+}
+
+// ------------------------------------------------------------------ products on token panels
+struct MxPanelArgs {
+  const uint8_t* x;                         // panels of 32 MT tokens
+  int64_t N;
+  int F, slices;
+  lbk_bell_mx w0, w1;
+  const float* b0; const float* b1;
+  const uint16_t* resid;
+  uint16_t* y;                              // MODE 0
+  uint8_t* h; int TBh;                      // MODE 1: panels of TBh tokens
+};
+
+// A workgroup of 8 waves holds 32 MT tokens in LDS and one of `slices` shares of the 32-row output tiles;
+// a wave takes every 8th tile of the share.  The (tile, weight, slot pair) positions of a wave form one
+// stream: their codes (16 bytes a lane), scale and column are loaded D positions ahead, always all three,
+// so that the compiler's load counters stay exact across tiles.  A dead slot, and the second half of an odd
+// row's last pair, multiplies zeros with unit scales.
+template <int B, int MODE, int MT>
+__global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
+  constexpr int TB = 32 * MT, NW = 8, D = 4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6), half = lane >> 5, i = lane & 31;
+  const int G = a.F >> 5, C = a.F / B;
+  const Panel P = panel_of(G, TB);
+  const int64_t tb = blockIdx.x / a.slices;
+  const int sl = (int)(blockIdx.x % a.slices);
+  const int tiles = a.w0.R * (B / 32);
+  const int mEnd = (int)((int64_t)tiles * (sl + 1) / a.slices), m0 = (int)((int64_t)tiles * sl / a.slices) + w;
+
+  typedef __attribute__((address_space(3))) unsigned char lds_byte;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
+  const uint8_t* src = a.x + tb * P.bytes + lane * 16;
+  for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_load16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  if (m0 >= mEnd) return;
+
+  constexpr int STEP = 64 / B;
+  const int P0 = (a.w0.K + STEP - 1) / STEP, P1 = MODE == 1 ? (a.w1.K + STEP - 1) / STEP : 0;
+  // loading position, D ahead of the computing one
+  int lm = m0, lup = 0, lj = 0;
+  u32x4 wr[D];
+  uint32_t sr[D];
+  int cr[D];
+  auto load = [&](int d) {
+    const lbk_bell_mx& wt = lup ? a.w1 : a.w0;
+    const int K = wt.K, row = lm * 32, r = row / B, j = row % B + i;
+    const int slot = min(B == 32 ? 2 * lj + half : lj, K - 1);
+    const int64_t idx = (int64_t)r * K + slot, at = (idx * B + j) * (B / 32) + (B == 64 ? half : 0);
+    wr[d] = reinterpret_cast<const u32x4*>(wt.codes)[at];
+    sr[d] = wt.scales[at];
+    cr[d] = wt.col_idx[idx];
+    if (++lj == (lup ? P1 : P0)) {
+      lj = 0;
+      if (MODE == 1 && !lup) lup = 1;
+      else {
+        lup = 0;
+        lm = lm + NW < mEnd ? lm + NW : lm;      // behind the last tile: its loads again, for nobody
+      }
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(d);
+
+  f32x16 acc[MODE + 1][MT] = {};
+  const unsigned char* xs = smem + P.codes;
+  int cm = m0, cup = 0, cj = 0;
+  auto compute = [&](int d, f32x16 (&c)[MT], int K) {
+    const int col = cr[d];
+    const bool live = (B == 64 || 2 * cj + half < K) && (uint32_t)col < (uint32_t)C;
+    const int g = live ? (B == 32 ? col : 2 * col + half) : 0;
+    const u32x4 wv = live ? wr[d] : u32x4{0, 0, 0, 0};
+    const uint32_t sa = live ? sr[d] : 127u;
+    uint32_t sb;
+    if constexpr (MT == 4) sb = reinterpret_cast<const uint32_t*>(xs)[g * 32 + i];
+    else if constexpr (MT == 2) sb = reinterpret_cast<const uint16_t*>(xs)[g * 32 + i];
+    else sb = xs[g * 32 + i];
+    sb = live ? sb : 0x7f7f7f7fu;
+    const u32x4* xp = reinterpret_cast<const u32x4*>(smem) + g * TB + i;
+    const i32x8_t A = {(int)wv[0], (int)wv[1], (int)wv[2], (int)wv[3], 0, 0, 0, 0};
+    auto mm = [&](int t, auto sel) {
+      const u32x4 xv = xp[32 * t];
+      const i32x8_t Bm = {(int)xv[0], (int)xv[1], (int)xv[2], (int)xv[3], 0, 0, 0, 0};
+      c[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, Bm, c[t], 4, 4, 0, (int)sa, decltype(sel)::value, (int)sb);
+    };
+    mm(0, std::integral_constant<int, 0>{});
+    if constexpr (MT > 1) mm(1, std::integral_constant<int, 1>{});
+    if constexpr (MT > 2) {
+      mm(2, std::integral_constant<int, 2>{});
+      mm(3, std::integral_constant<int, 3>{});
+    }
+  };
+  auto store = [&]() {
+    const int o0 = cm * 32;
+    if constexpr (MODE == 1) {
+      const int Gh = a.w0.R * (B / 32);
+      const Panel Ph = panel_of(Gh, a.TBh);
+      const int MTh = a.TBh / 32;
+      float bg[16], bu[16];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const int o = o0 + (q & 3) + 8 * (q >> 2) + 4 * half;
+        bg[q] = a.b0 ? a.b0[o] : 0.0f;
+        bu[q] = a.b1 ? a.b1[o] : 0.0f;
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) v[q] = silu_f(acc[0][t][q] + bg[q]) * (acc[MODE][t][q] + bu[q]);
+        const int64_t n = tb * TB + 32 * t + i, hb = n / a.TBh;
+        const int tt = (int)(n - hb * a.TBh);
+        uint8_t* blk = a.h + hb * Ph.bytes;
+        mx_store_group(v, half, blk + ((int64_t)cm * a.TBh + tt) * 16,
+                       blk + Ph.codes + (int64_t)cm * a.TBh + (tt & 31) * MTh + (tt >> 5), n < a.N);
+      }
+    } else {
+      const int64_t ld = (int64_t)a.w0.R * B;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int64_t n = tb * TB + 32 * t + i;
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          // 4 features of each of q and q + 1 -> 8 consecutive ones: half 0 takes those of q, half 1 of q + 1
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[0][t][4 * q + e]),
+                                                             __float_as_uint(acc[0][t][4 * q + 4 + e]), false, false);
+            f[e] = __uint_as_float(sw[0]);
+            f[4 + e] = __uint_as_float(sw[1]);
+          }
+          const int o = o0 + 8 * (q + half);
+          if (a.b0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] += a.b0[o + e];
+          }
+          if (n < a.N) {
+            if (a.resid) {
+              float r[8];
+              load_bf16x<8>(a.resid + n * ld + o, r);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] += r[e];
+            }
+            store_bf16x<8>(a.y + n * ld + o, f);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      acc[0][t] = f32x16{};
+      if constexpr (MODE == 1) acc[MODE][t] = f32x16{};
+    }
+  };
+  for (;;) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (MODE == 1 && cup) compute(d, acc[MODE], a.w1.K);
+      else compute(d, acc[0], a.w0.K);
+      load(d);
+      if (++cj == (cup ? P1 : P0)) {
+        cj = 0;
+        if (MODE == 1 && !cup) cup = 1;
+        else {
+          store();
+          cup = 0;
+          cm += NW;
+          if (cm >= mEnd) return;
+        }
+      }
+    }
+  }
+}
+
+// Tokens a workgroup holds: the most whose codes and scales fit in LDS (0: none does)
+inline int mx_block_tokens(int F) {
+  for (int TB = 128; TB >= 32; TB /= 2)
+    if (panel_of(F / 32, TB).bytes <= 160 * 1024) return TB;
+  return 0;
+}
+
+template <int B, int MODE, int MT>
+int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
+  auto* k = mx_panel_kernel<B, MODE, MT>;
+  const int64_t lds = panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
+  const int tiles = a.w0.R * (B / 32);
+  // shares of the output tiles: enough workgroups for 256 CUs, at least a tile a wave
+  const int64_t want = (256 + nb - 1) / nb, most = (tiles + 7) / 8;
+  a.slices = (int)(want < most ? want : most);
+  if (nb * a.slices > 0x7fffff) return -1;
+  static std::atomic<uint64_t> done{0};
+  if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), 160 * 1024, done) != 0) return -1;
+  k<<<(unsigned)(nb * a.slices), 512, lds, st>>>(a);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+template <int MODE>
+int launch_mx_panel(int TB, const MxPanelArgs& a, hipStream_t st) {
+  const bool b32 = a.w0.B == 32;
+  if (TB == 128) return b32 ? launch_mx_panel_t<32, MODE, 4>(a, st) : launch_mx_panel_t<64, MODE, 4>(a, st);
+  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2>(a, st) : launch_mx_panel_t<64, MODE, 2>(a, st);
+  return b32 ? launch_mx_panel_t<32, MODE, 1>(a, st) : launch_mx_panel_t<64, MODE, 1>(a, st);
+}
+
+int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* panels, hipStream_t st) {
+  const int64_t waves = (N + 15) / 16 * ((F / 32 + 1) / 2);
+  if (waves > 0x3ffffff) return -1;
+  mx_quantize_panel_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(x, N, F, TB, panels);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 template <int MODE>
@@ -400,6 +657,42 @@ int check_ffn_mx(const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_
   return (int64_t)down->R * down->B == d_model ? LBK_OK : LBK_ERR_SHAPE;
 }
 
+// Tokens of a panel block for a product of these input features, 0: rows of codes (mx_rowblock_kernel,
+// also where a weight has no slots)
+int in_tokens(int64_t F, const lbk_bell_mx* w) { return w->K > 0 ? mx_block_tokens((int)F) : 0; }
+
+// Both products of an FFN read tokens of one kind, so that the gate/up kernel writes what the down one reads
+struct FfnTokens {
+  int x, h;
+};
+FfnTokens ffn_tokens(int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_mx* down) {
+  const FfnTokens t{up->K > 0 ? in_tokens(d_model, gate) : 0, in_tokens((int64_t)gate->R * gate->B, down)};
+  return t.x && t.h ? t : FfnTokens{0, 0};
+}
+size_t tokens_bytes(int64_t N, int64_t F, int TB) {
+  return TB ? (size_t)((N + TB - 1) / TB * panel_of((int)(F / 32), TB).bytes) : quantised_bytes(N, F);
+}
+
+int quantize_tokens(const uint16_t* x, int64_t N, int F, int TB, void* ws, hipStream_t st) {
+  if (TB) return launch_quantize_panel(x, N, F, TB, static_cast<uint8_t*>(ws), st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  const Quantised q = quantised_at(ws, N, F);
+  return lbk_mx_quantize(x, LBK_BF16, N, F, F, q.c, q.s, st);
+}
+
+// y = tokens (quantised as quantize_tokens leaves them) times w
+int product(void* tokens, int64_t N, int F, int TB, const lbk_bell_mx& w, const float* bias, const uint16_t* resid,
+            uint16_t* y, hipStream_t st) {
+  if (TB) {
+    MxPanelArgs a{};
+    a.x = static_cast<uint8_t*>(tokens); a.N = N; a.F = F; a.w0 = w; a.b0 = bias; a.resid = resid; a.y = y;
+    return launch_mx_panel<0>(TB, a, st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  }
+  const Quantised q = quantised_at(tokens, N, F);
+  MxArgs a{};
+  a.xc = q.c; a.xs = q.s; a.N = N; a.F = F; a.w0 = w; a.b0 = bias; a.resid = resid; a.y = y;
+  return launch_mx_rowblock<0>(a, st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+}
+
 }  // namespace
 
 extern "C" {
@@ -447,7 +740,7 @@ int lbk_mx_dequantize_tiles(const uint8_t* codes, const uint8_t* scales, int32_t
 
 size_t lbk_mx_matmul_workspace_bytes(int64_t N, int32_t in_features, const lbk_bell_mx* w) {
   if (!w || N <= 0 || in_features <= 0) return 0;
-  return quantised_bytes(N, in_features);
+  return tokens_bytes(N, in_features, in_tokens(in_features, w));
 }
 
 int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const lbk_bell_mx* w, const float* bias,
@@ -459,18 +752,17 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
   if (!x || !y) return LBK_ERR_NULL;
   if (!a16(x) || !a16(y) || !a16(workspace)) return LBK_ERR_ALIGN;
   const size_t need = lbk_mx_matmul_workspace_bytes(N, in_features, w);
-  if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
-  const Quantised q = quantised_at(workspace, N, in_features);
-  if (int st = lbk_mx_quantize(x, LBK_BF16, N, in_features, in_features, q.c, q.s, stream)) return st;
-  MxArgs a{};
-  a.xc = q.c; a.xs = q.s; a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
-  return launch_mx_rowblock<0>(a, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
+  const int TB = in_tokens(in_features, w);
+  if (int st = quantize_tokens(x, N, in_features, TB, workspace, S(stream))) return st;
+  return product(workspace, N, in_features, TB, *w, bias, nullptr, y, S(stream));
 }
 
 size_t lbk_mx_swiglu_workspace_bytes(int64_t N, int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx* up,
                                      const lbk_bell_mx* down) {
   if (!gate || !up || !down || N <= 0 || d_model <= 0) return 0;
-  return quantised_bytes(N, d_model) + quantised_bytes(N, (int64_t)gate->R * gate->B);
+  const FfnTokens t = ffn_tokens(d_model, gate, up, down);
+  return tokens_bytes(N, d_model, t.x) + tokens_bytes(N, (int64_t)gate->R * gate->B, t.h);
 }
 
 int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const lbk_bell_mx* gate,
@@ -484,18 +776,23 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
   if (!a16(x) || !a16(out) || !a16(workspace)) return LBK_ERR_ALIGN;
   const size_t need = lbk_mx_swiglu_workspace_bytes(N, d_model, gate, up, down);
   if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
-  const int64_t d_ff = (int64_t)gate->R * gate->B;
-  const Quantised q = quantised_at(workspace, N, d_model);
-  const Quantised h = quantised_at(static_cast<uint8_t*>(workspace) + quantised_bytes(N, d_model), N, d_ff);
-  if (int st = lbk_mx_quantize(x, LBK_BF16, N, d_model, d_model, q.c, q.s, stream)) return st;
-  MxArgs g{};
-  g.xc = q.c; g.xs = q.s; g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
-  g.hc = h.c; g.hs = h.s;
-  if (launch_mx_rowblock<1>(g, S(stream)) != 0) return LBK_ERR_LAUNCH;
-  MxArgs d{};
-  d.xc = h.c; d.xs = h.s; d.N = N; d.F = (int)d_ff; d.w0 = *down; d.b0 = b_down; d.y = out;
-  d.resid = add_residual ? x : nullptr;
-  return launch_mx_rowblock<0>(d, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  const int d_ff = gate->R * gate->B;
+  const FfnTokens t = ffn_tokens(d_model, gate, up, down);
+  uint8_t* hp = static_cast<uint8_t*>(workspace) + tokens_bytes(N, d_model, t.x);
+  if (int st = quantize_tokens(x, N, d_model, t.x, workspace, S(stream))) return st;
+  if (t.x) {
+    MxPanelArgs g{};
+    g.x = static_cast<uint8_t*>(workspace); g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
+    g.h = hp; g.TBh = t.h;
+    if (launch_mx_panel<1>(t.x, g, S(stream)) != 0) return LBK_ERR_LAUNCH;
+  } else {
+    const Quantised q = quantised_at(workspace, N, d_model), h = quantised_at(hp, N, d_ff);
+    MxArgs g{};
+    g.xc = q.c; g.xs = q.s; g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
+    g.hc = h.c; g.hs = h.s;
+    if (launch_mx_rowblock<1>(g, S(stream)) != 0) return LBK_ERR_LAUNCH;
+  }
+  return product(hp, N, d_ff, t.h, *down, b_down, add_residual ? x : nullptr, out, S(stream));
 }
 
 }  // extern "C"
