@@ -11,6 +11,8 @@
 #include "lbk_device.h"
 #include "lbk_internal.h"
 
+#include <type_traits>
+
 namespace lbk {
 namespace {
 
@@ -48,6 +50,12 @@ __device__ __forceinline__ void load4h(const uint16_t* p, float (&f)[4]) {
 template <bool H>
 __device__ __forceinline__ void store4h(uint16_t* p, const float (&f)[4]) {
   *reinterpret_cast<u32x2*>(p) = u32x2{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3])};
+}
+
+template <bool H>
+__device__ __forceinline__ void store8h(uint16_t* p, const float (&f)[8]) {
+  *reinterpret_cast<u32x4*>(p) = u32x4{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3]), Half<H>::pack2(f[4], f[5]),
+                                       Half<H>::pack2(f[6], f[7])};
 }
 
 // sixteen zero bytes that out-of-range pieces of a tile are loaded from
@@ -88,195 +96,328 @@ struct Gemm {
   int64_t ldd;
 };
 
-constexpr int BK = 64;
+constexpr int KS = 32;       // K of a matrix instruction
+constexpr int BK = 64;       // K of a stage
 
-// A tile lies in LDS as 16-byte chunks, [row][chunk], the chunk's place XORed with a function of the
-// row so that the lanes of a read phase fall on all banks (the direct loads write 1 KB of consecutive
-// places; each lane fetches the chunk that belongs at its place):
-//   KC: rows of 8 chunks.  A 16-row fragment takes rows 16 (i / 4) + 4 t + i % 4 of 64, so that a lane of
-//       four fragments ends with 16 consecutive features; eight lanes of a phase, eight f.
-//   MC: K rows of ROWS / 8 chunks, read transposed; 32 lanes of a phase read 32 bytes of 8 rows.
-__device__ __forceinline__ int f_kc(int row) { return (row & 3) | (((row >> 4) & 1) << 2); }
+// The 32 K of a step of an operand lie in LDS as 16-byte chunks whose place is XORed with a function of the row, so
+// that the lanes of a read phase fall on all banks (the direct loads write 1 KB of consecutive places; each
+// lane fetches the chunk that belongs at its place):
+//   KC: [row][4 chunks], fragment t is rows 16 t + i.  A read phase is lanes 0 .. 3, 12 .. 15 and 20 .. 27 (or
+//       the others) of a half-wave: rows of all four (row / 4) % 4, two each of two neighbouring chunks.
+//   MC: [k][ROWS / 8 chunks], read transposed; 32 lanes of a phase read 32 bytes of 8 K rows.
+__device__ __forceinline__ int f_kc(int row) { return -(row >> 2) & 3; }
 __device__ __forceinline__ int f_mc(int k) { return 2 * ((k & 3) | (((k >> 3) & 1) << 2)); }
 
-template <bool H, bool AMC, bool BMC, int EPI, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void gemm_kernel(Gemm p) {
-  constexpr int WAVES = (BM / WM) * (BN / WN), MW = BM / WM;
-  constexpr int MT = WM / 16, NT = WN / 16;
-  constexpr int ABYTES = BM * BK * 2, BBYTES = BN * BK * 2, STAGE = ABYTES + BBYTES;
-  constexpr int APW = ABYTES / 1024 / WAVES, BPW = BBYTES / 1024 / WAVES;
-  static_assert(ABYTES % (1024 * WAVES) == 0 && BBYTES % (1024 * WAVES) == 0, "whole loads per wave");
+// The matrix row that row i of A's fragment t holds.  KC: a lane (i, q) of the products' results holds rows
+// 4 q .. + 3 of each fragment, so 16 consecutive features of four fragments.  EPI_GATE: fragments 0 and 1 of
+// four are gate's, 2 and 3 up's, 8 consecutive features of a lane each.
+template <bool GATE>
+__device__ __forceinline__ int a_row(int t, int i) {
+  return GATE ? (t >> 2) * 32 + 8 * (i >> 2) + 4 * (t & 1) + (i & 3) : (t >> 2) * 64 + 16 * (i >> 2) + 4 * (t & 3) + (i & 3);
+}
+
+// Output tiles of TILE x TILE, waves of TILE / 2 x 64.  Two K stages in LDS, of two steps each; a step's
+// fragments are read while the step before is multiplied.  Workgroups are persistent, and the K stages of
+// their output tiles form one stream of loads: the next output tile's are in flight during the epilogue.
+// TAIL: K is no multiple of 64.
+template <bool H, bool AMC, bool BMC, int EPI, int TILE, bool TAIL>
+__global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
+  constexpr int BM = TILE, BN = TILE, WAVES = TILE / 32;
+  constexpr int WM = BM / 2, WN = 64, MT = WM / 16, NT = WN / 16;
+  constexpr int ABYTES = BM * KS * 2, STEP = ABYTES + BN * KS * 2, STAGE = 2 * STEP;
+  constexpr int PA = ABYTES / 1024 / WAVES, PB = PA, PIECES = PA + PB;             // 1 KB loads of a wave and step
+  constexpr bool GATE = EPI == EPI_GATE;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
   const int i = lane & 15, q = lane >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
 
-  constexpr int FM = EPI == EPI_GATE ? BM / 2 : BM;       // features of a tile (of each weight)
-  const int64_t mt = (p.M + FM - 1) / FM, nt = (p.N + BN - 1) / BN;
-  // workgroup -> tile: workgroups are dealt to the 8 XCDs round robin; each XCD takes a run of the
-  // tiles (features fastest), so that its L2 keeps the B rows of a run
-  const int64_t tiles = mt * nt * p.splits;
-  const int64_t per = (tiles + 7) / 8;
-  const int64_t id = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || id >= tiles) return;
-  const int64_t m0 = (id % mt) * FM, n0 = (id / mt % nt) * BN;
-  const int split = (int)(id / (mt * nt));
+  constexpr int FM = GATE ? BM / 2 : BM;                        // features of a tile
+  const int mt = (int)((p.M + FM - 1) / FM), nt = (int)((p.N + BN - 1) / BN);
+  const int tiles = mt * nt * p.splits;                         // < 2^30 (launch_tile)
+  // workgroups are dealt to the 8 XCDs round robin; an XCD takes a run of the tiles, which go eight
+  // columns at a time, so that the tiles in work on it share operand rows in its L2
+  const int per = (tiles + 7) / 8, xcd = (int)(blockIdx.x & 7), stride = (int)(gridDim.x >> 3);
+  const int last = min((xcd + 1) * per, tiles);
+  int id = xcd * per + (int)(blockIdx.x >> 3);
+  if (id >= last) return;
 
-  // K in tiles of BK; tile t belongs to pair t / kt
   const int kt = (int)((p.K + BK - 1) / BK), all = kt * p.pairs;
-  const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
+  struct Where {
+    int m0, n0, split, t0, t1;
+  };
+  auto where = [&](int idx) {
+    Where v;
+    v.split = idx / (mt * nt);
+    const int r = idx - v.split * (mt * nt), ng = r / (mt * 8), rr = r - ng * mt * 8;
+    const int wide = min(8, nt - ng * 8);
+    v.m0 = uniform(rr / wide * FM);
+    v.n0 = uniform((ng * 8 + rr % wide) * BN);
+    v.t0 = uniform((int)((int64_t)all * v.split / p.splits));
+    v.t1 = uniform((int)((int64_t)all * (v.split + 1) / p.splits));
+    return v;
+  };
 
-  // the 1 KB loads of one operand tile; R: rows of the tile, `which`: whether the row is in range, and where
-  auto stage = [&](int t, uint32_t base) {
-    const int pr = t >= kt ? 1 : 0;
-    const int64_t k0 = (int64_t)(t - pr * kt) * BK;
+  // byte offsets of this lane's chunks from an output tile's first row (KC) or column (MC); rows behind the
+  // matrix read its last row, and reach no output
+  uint32_t aoff[PA], boff[PB];
+  auto offsets = [&](const Where& v) {
+    const int r4 = lane >> 2, ch = (lane & 3) ^ f_kc(lane >> 2);
 #pragma unroll
-    for (int c = 0; c < APW + BPW; ++c) {
-      const bool isA = c < APW;
-      const int piece = isA ? w * APW + c : w * BPW + (c - APW);
-      const int L = piece * 64 + lane;                     // 16-byte place in the operand's tile
-      const uint32_t at = base + (isA ? 0 : ABYTES) + (uint32_t)piece * 1024;
-      const uint16_t* src;
-      if (isA ? AMC : BMC) {
-        const int CH = (isA ? BM : BN) / 8, kr = L / CH, ch = (L % CH) ^ f_mc(kr);
-        const int64_t k = k0 + kr, r = (isA ? m0 : n0) + ch * 8;
-        const uint16_t* X = isA ? p.A[pr] : p.B[pr];
-        src = k < p.K && r < (isA ? p.M : p.N) ? X + k * (isA ? p.lda : p.ldb) + r : (const uint16_t*)&zero16;
+    for (int c = 0; c < PA; ++c) {
+      const int piece = w * PA + c;
+      if constexpr (AMC) {
+        const int kr = (piece * 64 + lane) / (BM / 8), r = ((lane % (BM / 8)) ^ f_mc(kr)) * 8;
+        aoff[c] = (uint32_t)((kr * p.lda + min(r, (int)(p.M - 8 - v.m0))) * 2);
       } else {
-        const int row = L / 8, ch = (L % 8) ^ f_kc(row);
-        const int64_t k = k0 + ch * 8;
-        const uint16_t* X = isA ? p.A[EPI == EPI_GATE ? (row >> 6) & 1 : pr] : p.B[pr];
-        const int64_t r = isA ? (EPI == EPI_GATE ? m0 + (row >> 7) * 64 + (row & 63) : m0 + row) : n0 + row;
-        src = k < p.K && r < (isA ? p.M : p.N) ? X + r * (isA ? p.lda : p.ldb) + k : (const uint16_t*)&zero16;
+        aoff[c] = (uint32_t)((min(a_row<GATE>(piece, r4), (int)(p.M - 1 - v.m0)) * p.lda + ch * 8) * 2);
       }
-      lds_load16(src, at);
+    }
+#pragma unroll
+    for (int c = 0; c < PB; ++c) {
+      const int piece = w * PB + c;
+      if constexpr (BMC) {
+        const int kr = (piece * 64 + lane) / (BN / 8), r = ((lane % (BN / 8)) ^ f_mc(kr)) * 8;
+        boff[c] = (uint32_t)((kr * p.ldb + min(r, (int)(p.N - 8 - v.n0))) * 2);
+      } else {
+        boff[c] = (uint32_t)((min(piece * 16 + r4, (int)(p.N - 1 - v.n0)) * p.ldb + ch * 8) * 2);
+      }
+    }
+  };
+  // the stream of loads: K stage lt of output tile lv; its bases, and how much of K is left there
+  Where lv = where(id);
+  int lid = id, lt = lv.t0, left = 0;
+  const char *sa0 = nullptr, *sa1 = nullptr, *sb0 = nullptr;
+  auto ptr = [](const uint16_t* b, int64_t elems) {
+    const uint64_t v = reinterpret_cast<uint64_t>(b + elems);
+    return reinterpret_cast<const char*>((uint64_t)(uint32_t)uniform((int)(uint32_t)v) |
+                                         (uint64_t)(uint32_t)uniform((int)(uint32_t)(v >> 32)) << 32);
+  };
+  const int64_t da = AMC ? BK * 2 * p.lda : BK * 2, db = BMC ? BK * 2 * p.ldb : BK * 2;
+  auto source = [&]() {
+    const int pr = lt >= kt ? 1 : 0;
+    const int64_t k0 = (int64_t)(lt - pr * kt) * BK;
+    const int64_t ao = AMC ? k0 * p.lda + lv.m0 : lv.m0 * p.lda + k0, bo = BMC ? k0 * p.ldb + lv.n0 : lv.n0 * p.ldb + k0;
+    sa0 = ptr(GATE || !pr ? p.A[0] : p.A[1], ao);
+    if constexpr (GATE) sa1 = ptr(p.A[1], ao);
+    sb0 = ptr(pr ? p.B[1] : p.B[0], bo);
+    left = (int)(p.K - k0);
+  };
+  auto advance = [&]() {                // behind the stream's end its last K stage is loaded again, for nobody
+    ++lt;
+    if (lt == lv.t1 || lt == kt) {
+      if (lt == lv.t1) {
+        if (lid + stride < last) {
+          lid += stride;
+          lv = where(lid);
+          offsets(lv);
+          lt = lv.t0;
+        } else {
+          --lt;
+        }
+      }
+      source();
+    } else {
+      sa0 += da;
+      sa1 += da;
+      sb0 += db;
+      left -= BK;
+    }
+  };
+  // load c (0 .. 2 PIECES - 1) of the K stage at `base`: both steps' chunks of a row one after the other
+  const int64_t ha = AMC ? KS * 2 * p.lda : KS * 2, hb = BMC ? KS * 2 * p.ldb : KS * 2;
+  auto load = [&](uint32_t base, int c) {
+    const int ks = c & 1, cp = c >> 1;
+    const bool isA = cp < PA;
+    const int cc = isA ? cp : cp - PA, piece = isA ? w * PA + cc : w * PB + cc;
+    const uint32_t at = base + ks * STEP + (isA ? 0 : ABYTES) + (uint32_t)piece * 1024, off = isA ? aoff[cc] : boff[cc];
+    // EPI_GATE: a load is a fragment's 16 rows, all of one weight
+    const char* b = (!isA ? sb0 : GATE && (piece & 2) ? sa1 : sa0) + (ks ? (isA ? ha : hb) : 0);
+    if constexpr (TAIL) {
+      const int R = isA ? BM : BN;
+      const int k = ks * KS + ((isA ? AMC : BMC) ? (piece * 64 + lane) / (R / 8) : ((lane & 3) ^ f_kc(lane >> 2)) * 8);
+      lds_load16(k < left ? b + off : reinterpret_cast<const char*>(&zero16), at);
+    } else {
+      lds_load16(b, off, at);
     }
   };
 
-  f32x4 acc[MT][NT];
+  const int wm = (w & 1) * WM, wn = (w >> 1) * WN;
+  // fragment addresses in a step: KC one (fragments are immediates), MC one a fragment
+  uint32_t ra[AMC ? MT : 1], rb[BMC ? NT : 1];
 #pragma unroll
-  for (int a = 0; a < MT; ++a)
+  for (int t = 0; t < (AMC ? MT : 1); ++t)
+    ra[t] = AMC ? (uint32_t)((8 * q + (i >> 2)) * (BM * 2) +
+                             (((wm + 16 * t) / 8 + ((i & 3) >> 1)) ^ f_mc(8 * q + (i >> 2))) * 16 + (i & 1) * 8)
+                : (uint32_t)((wm + i) * 64 + ((q ^ f_kc(i)) << 4));
 #pragma unroll
-    for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int wm = (w % MW) * WM, wn = (w / MW) * WN;
-  // fragment t of a 64-row span at row `r0` of an operand's tile, K step ks
-  auto frag_kc = [&](const unsigned char* s, int r0, int t, int ks) {
-    const int row = r0 + (t >> 2) * 64 + 16 * (i >> 2) + 4 * (t & 3) + (i & 3);
-    return *reinterpret_cast<const u32x4*>(s + row * 128 + (((ks * 4 + q) ^ f_kc(row)) << 4));
-  };
-  auto frag_mc = [&](const unsigned char* s, int r0, int t, int ks, int rows) {
-    const int k = ks * 32 + 8 * q + (i >> 2);
-    const int ch = (r0 + 16 * t) / 8 + ((i & 3) >> 1);
-    const unsigned char* a = s + (k * (rows / 8) + (ch ^ f_mc(k))) * 16 + (i & 1) * 8;
-    const unsigned char* b = s + ((k + 4) * (rows / 8) + (ch ^ f_mc(k + 4))) * 16 + (i & 1) * 8;
-    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_g*)(lds_byte*)a));
-    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_g*)(lds_byte*)b));
+  for (int t = 0; t < (BMC ? NT : 1); ++t)
+    rb[t] = (uint32_t)ABYTES +
+            (BMC ? (uint32_t)((8 * q + (i >> 2)) * (BN * 2) +
+                              (((wn + 16 * t) / 8 + ((i & 3) >> 1)) ^ f_mc(8 * q + (i >> 2))) * 16 + (i & 1) * 8)
+                 : (uint32_t)((wn + i) * 64 + ((q ^ f_kc(i)) << 4)));
+  auto tr = [&](const unsigned char* s, int row) {
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_g*)(lds_byte*)s));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_g*)(lds_byte*)(s + 4 * row)));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
-  // B rows of a KC operand in their own order: column i of fragment t is row 16 t + i
-  auto frag_b = [&](const unsigned char* s, int t, int ks) {
-    const int row = wn + 16 * t + i;
-    return *reinterpret_cast<const u32x4*>(s + row * 128 + (((ks * 4 + q) ^ f_kc(row)) << 4));
+  auto frag_a = [&](const unsigned char* s, int t) {
+    if constexpr (AMC) return tr(s + ra[t], BM * 2);
+    else return *reinterpret_cast<const u32x4*>(s + ra[0] + t * 1024);
+  };
+  auto frag_b = [&](const unsigned char* s, int t) {
+    if constexpr (BMC) return tr(s + rb[t], BN * 2);
+    else return *reinterpret_cast<const u32x4*>(s + rb[0] + t * 1024);
   };
 
-  if (t0 < t1) stage(t0, lds0);
-  for (int t = t0; t < t1; ++t) {
+  offsets(lv);
+  source();
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+#pragma unroll
+    for (int c = 0; c < 2 * PIECES; ++c) load(lds0 + st * STAGE, c);
+    advance();
+  }
+  f32x4 acc[MT][NT];
+  auto clear = [&]() {
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+      for (int b = 0; b < NT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  clear();
+  u32x4 fa[2][MT], fb[2][NT];
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * PIECES) : "memory");
+#pragma unroll
+  for (int b = 0; b < NT; ++b) fb[0][b] = frag_b(smem, b);
+#pragma unroll
+  for (int a = 0; a < MT; ++a) fa[0][a] = frag_a(smem, a);
+  // a step's products, the next step's fragments read beside the first of them; the order is pinned, or the
+  // compiler gathers the reads behind the products and waits for them
+  auto step = [&](auto set, const unsigned char* next, auto&& beside) {
+    constexpr int c = decltype(set)::value, n = 1 - c;
+#pragma unroll
+    for (int a = 0; a < MT; ++a) {
+      beside(a);
+      if (a < NT) fb[n][a] = frag_b(next, a);
+      if (2 * a < MT) {
+        fa[n][2 * a] = frag_a(next, 2 * a);
+        fa[n][2 * a + 1] = frag_a(next, 2 * a + 1);
+      }
+#pragma unroll
+      for (int b = 0; b < NT; ++b) acc[a][b] = Half<H>::mfma(fa[c][a], fb[c][b], acc[a][b]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  Where done = where(id);
+  uint32_t cur = 0;                     // the stage in work
+  for (int t = done.t0;;) {
+    step(std::integral_constant<int, 0>{}, smem + cur + STEP, [](int) {});
+    // the stage is read, and the next one has landed, for every wave
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const uint32_t cur = (uint32_t)((t - t0) & 1) * STAGE;
-    if (t + 1 < t1) stage(t + 1, lds0 + (STAGE - cur));
-    const unsigned char* sa = smem + cur;
-    const unsigned char* sb = sa + ABYTES;
+    step(std::integral_constant<int, 1>{}, smem + (STAGE - cur), [&](int a) {
 #pragma unroll
-    for (int ks = 0; ks < BK / 32; ++ks) {
-      u32x4 fb[NT];
-#pragma unroll
-      for (int b = 0; b < NT; ++b) fb[b] = BMC ? frag_mc(sb, wn, b, ks, BN) : frag_b(sb, b, ks);
-#pragma unroll
-      for (int a = 0; a < MT; ++a) {
-        const u32x4 fa = AMC ? frag_mc(sa, wm, a, ks, BM) : frag_kc(sa, wm, a, ks);
-#pragma unroll
-        for (int b = 0; b < NT; ++b) acc[a][b] = Half<H>::mfma(fa, fb[b], acc[a][b]);
-      }
-    }
-  }
+      for (int c = 0; c < 2 * PIECES / MT; ++c) load(lds0 + cur, a * (2 * PIECES / MT) + c);
+    });
+    cur = STAGE - cur;
+    advance();
+    if (++t < done.t1) continue;
 
-  // lane (i, q) of acc[a][b]: column n = n0 + wn + 16 b + i; features from wm + 64 (a / 4) + 16 q + 4 (a % 4)
-  // (KC) or wm + 16 a + 4 q (MC), four consecutive
+    // lane (i, q) of acc[a][b]: column n, features from f, consecutive: KC 16 of four fragments (EPI_GATE
+    // 8 of each weight), MC 4 of each
 #pragma unroll
-  for (int b = 0; b < NT; ++b) {
-    const int64_t n = n0 + wn + 16 * b + i;
-    if (n >= p.N) continue;
-    if constexpr (EPI == EPI_GATE) {
+    for (int b = 0; b < NT; ++b) {
+      const int64_t n = done.n0 + wn + 16 * b + i;
+      if (n >= p.N) continue;
+      if constexpr (EPI == EPI_GATE) {
 #pragma unroll
-      for (int a = 0; a < MT / 2; ++a) {
-        const int64_t f = m0 + wm / 2 + (a >> 2) * 64 + 16 * q + 4 * (a & 3);
-        if (f >= p.M) continue;
-        const f32x4 &g = acc[(a >> 2) * 8 + (a & 3)][b], &u = acc[(a >> 2) * 8 + 4 + (a & 3)][b];
-        float h[4], gv[4], uv[4];
+        for (int a = 0; a < MT; a += 4) {
+          const int64_t f = done.m0 + wm / 2 + (a >> 2) * 32 + 8 * q;
+          if (f >= p.M) continue;
+          float h[8], gv[8], uv[8];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) gv[v] = g[v], uv[v] = u[v], h[v] = act_f(g[v], p.act) * u[v];
-        store4h<H>(p.d0 + n * p.ldd + f, h);
-        if (p.d1) {
-          store4h<H>(p.d1 + n * p.ldd + f, gv);
-          store4h<H>(p.d2 + n * p.ldd + f, uv);
+          for (int e = 0; e < 8; ++e) {
+            gv[e] = acc[a + (e >> 2)][b][e & 3];
+            uv[e] = acc[a + 2 + (e >> 2)][b][e & 3];
+            h[e] = act_f(gv[e], p.act) * uv[e];
+          }
+          store8h<H>(p.d0 + n * p.ldd + f, h);
+          if (p.d1) {
+            store8h<H>(p.d1 + n * p.ldd + f, gv);
+            store8h<H>(p.d2 + n * p.ldd + f, uv);
+          }
         }
-      }
-    } else {
+      } else {
 #pragma unroll
-      for (int a = 0; a < MT; ++a) {
-        const int64_t f = m0 + wm + (AMC ? 16 * a + 4 * q : (a >> 2) * 64 + 16 * q + 4 * (a & 3));
-        if (f >= p.M) continue;
-        const int64_t at = n * p.ldd + f;
-        float v[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-        if constexpr (EPI == EPI_PART) {
-          *reinterpret_cast<f32x4*>(p.part + (int64_t)split * p.N * p.ldd + at) = acc[a][b];
-        } else if constexpr (EPI == EPI_STORE) {
-          if (p.s0) {
-            float r[4];
-            load4h<H>(p.s0 + at, r);
+        for (int a = 0; a < MT; ++a) {
+          const int64_t f = done.m0 + wm + (AMC ? 16 * a + 4 * q : (a >> 2) * 64 + 16 * q + 4 * (a & 3));
+          if (f >= p.M) continue;
+          const int64_t at = n * p.ldd + f;
+          float x[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+          if constexpr (EPI == EPI_PART) {
+            *reinterpret_cast<f32x4*>(p.part + (int64_t)done.split * p.N * p.ldd + at) = acc[a][b];
+          } else if constexpr (EPI == EPI_STORE) {
+            if (p.s0) {
+              float r[4];
+              load4h<H>(p.s0 + at, r);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += r[e];
+              for (int e = 0; e < 4; ++e) x[e] += r[e];
+            }
+            store4h<H>(p.d0 + at, x);
+          } else {
+            float g[4], u[4], dg[4], du[4];
+            load4h<H>(p.s0 + at, g);
+            load4h<H>(p.s1 + at, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float ac, de;
+              act_both(g[e], p.act, ac, de);
+              dg[e] = x[e] * u[e] * de;
+              du[e] = x[e] * ac;
+            }
+            store4h<H>(p.d0 + at, dg);
+            store4h<H>(p.d1 + at, du);
           }
-          store4h<H>(p.d0 + at, v);
-        } else {
-          float g[4], u[4], dg[4], du[4];
-          load4h<H>(p.s0 + at, g);
-          load4h<H>(p.s1 + at, u);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float ac, de;
-            act_both(g[e], p.act, ac, de);
-            dg[e] = v[e] * u[e] * de;
-            du[e] = v[e] * ac;
-          }
-          store4h<H>(p.d0 + at, dg);
-          store4h<H>(p.d1 + at, du);
         }
       }
     }
+    id += stride;
+    if (id >= last) break;
+    done = where(id);
+    t = done.t0;
+    clear();
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the loads behind the stream's end
 }
 
-template <bool H, bool AMC, bool BMC, int EPI, int BM, int BN, int WM, int WN>
+// gradients of no tokens: the tiled product needs a K of 1 and more
+__global__ __launch_bounds__(256) void zero_kernel(u32x4* __restrict__ p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0, 0, 0, 0};
+}
+
+template <bool H, bool AMC, bool BMC, int EPI, int TILE, bool TAIL>
 int launch_tile(const Gemm& p, hipStream_t st) {
-  constexpr int FM = EPI == EPI_GATE ? BM / 2 : BM;
-  const int64_t tiles = (p.M + FM - 1) / FM * ((p.N + BN - 1) / BN) * p.splits;
+  constexpr int FM = EPI == EPI_GATE ? TILE / 2 : TILE;
+  const int64_t tiles = (p.M + FM - 1) / FM * ((p.N + TILE - 1) / TILE) * p.splits;
   if (tiles == 0) return LBK_OK;
-  const int64_t blocks = (tiles + 7) / 8 * 8;
-  if (blocks > 0x3fffff) return LBK_ERR_TOO_LARGE;
-  constexpr int lds = 2 * (BM + BN) * BK * 2;
-  auto* k = gemm_kernel<H, AMC, BMC, EPI, BM, BN, WM, WN>;
+  // every share of K holds a K stage: the kernel's stream of loads counts on it
+  if (p.K < 1 || p.splits > (p.K + BK - 1) / BK * p.pairs) return LBK_ERR_ARG;
+  if (tiles > 0x3fffffff) return LBK_ERR_TOO_LARGE;
+  // workgroups that run at once, all XCDs alike
+  const int64_t most = TILE == 256 ? 256 : 512, blocks = tiles >= most ? most : (tiles + 7) / 8 * 8;
+  constexpr int lds = 2 * 2 * TILE * BK * 2;
+  auto* k = gemm_kernel<H, AMC, BMC, EPI, TILE, TAIL>;
   static std::atomic<uint64_t> done{0};
   if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), lds, done) != 0) return LBK_ERR_LAUNCH;
-  k<<<(unsigned)blocks, (BM / WM) * (BN / WN) * 64, lds, st>>>(p);
+  k<<<(unsigned)blocks, TILE * 2, lds, st>>>(p);
   return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH;
 }
 
 template <bool H, bool AMC, bool BMC, int EPI>
 int launch_gemm(const Gemm& p, hipStream_t st) {
-  if constexpr (EPI == EPI_GATE) return launch_tile<H, AMC, BMC, EPI, 128, 128, 128, 32>(p, st);
-  else return launch_tile<H, AMC, BMC, EPI, 128, 128, 64, 64>(p, st);
+  const int64_t big = (p.M * (EPI == EPI_GATE ? 2 : 1) + 255) / 256 * ((p.N + 255) / 256) * p.splits;
+  if (p.K % BK) return big >= 128 ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, true>(p, st);
+  return big >= 128 ? launch_tile<H, AMC, BMC, EPI, 256, false>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
 }
 
 Gemm operands(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K) {
@@ -309,6 +450,11 @@ int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* 
 template <bool H>
 int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* g, const void* u, const void* h, int residual,
               void* dx, void* dwg, void* dwu, void* dwd, void* dg, void* du, hipStream_t st) {
+  if (a.N == 0) {
+    for (void* d : {dwg, dwu, dwd})
+      if (d) zero_kernel<<<256, 256, 0, st>>>(static_cast<u32x4*>(d), a.D * a.F / 8);
+    return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH;
+  }
   if (dx || dwg || dwu) {
     Gemm p = operands(a.wd, a.F, dy, a.D, a.F, a.N, a.D);
     p.act = a.act, p.ldd = a.F;
@@ -345,7 +491,8 @@ inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 int check_gated(int32_t dtype, int32_t act, int64_t N, int32_t D, int32_t F) {
   if ((dtype != LBK_BF16 && dtype != LBK_FP16) || (act != LBK_SILU && act != LBK_GELU) || N < 0) return LBK_ERR_ARG;
   if (D <= 0 || F <= 0 || D % 8 || F % 8) return LBK_ERR_SHAPE;
-  return N > ((int64_t)1 << 31) ? LBK_ERR_TOO_LARGE : LBK_OK;
+  // row and column numbers are 32-bit, and so are the byte offsets within a tile's rows
+  return N > 0x7ffffe00 || D > (1 << 22) || F > (1 << 22) ? LBK_ERR_TOO_LARGE : LBK_OK;
 }
 
 }  // namespace
