@@ -2,15 +2,19 @@
 // (gfx950, bf16 or fp16 MFMA, fp32 sums), and its entry points of include/lbk.h.
 //
 // Weights are dense Linear weights [out, in].  Six matrix products, all on one tiled kernel:
-//   forward   g, u = x Wg^T, x Wu^T with h = act(g) u in the epilogue;  out = h Wd^T (+ x)
-//   backward  dh = dy Wd with dg = dh u act'(g), du = dh act(g) in the epilogue;
+//   forward   g, u = x Wg^T, x Wu^T with h = act(g) u in the epilogue, and for the backward the factors
+//             cg = u act'(g), cu = act(g);  out = h Wd^T (+ x)
+//   backward  dh = dy Wd with dg = dh cg, du = dh cu in the epilogue;
 //             dx = dg Wg + du Wu (+ dy) as one product over both;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
-// g, u, h, dg and du are rounded to the inputs' type between the products (they are the matrix
-// instructions' operands, and g and u are kept for the backward); sums are fp32.
+// h, dg and du are rounded to the inputs' type between the products (they are the matrix instructions'
+// operands), and so are cg and cu, which the forward makes from fp32 values: kept in 32 bits they would add
+// 268 MB to a step of 16384 tokens and 4096 hidden features.  Kept in place of g and u they cost the same bytes
+// and spare the backward's epilogue the activation.  Sums are fp32.
 #include "lbk.h"
 #include "lbk_device.h"
 #include "lbk_internal.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace lbk {
@@ -41,21 +45,20 @@ template <> struct Half<true> {
   static __device__ __forceinline__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2_t, w)[1]; }
 };
 
-// four consecutive values
+// eight consecutive values
 template <bool H>
-__device__ __forceinline__ void load4h(const uint16_t* p, float (&f)[4]) {
-  const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-  f[0] = Half<H>::lo(w[0]), f[1] = Half<H>::hi(w[0]), f[2] = Half<H>::lo(w[1]), f[3] = Half<H>::hi(w[1]);
+__device__ __forceinline__ void unpack8h(const u32x4& w, float (&f)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[2 * k] = Half<H>::lo(w[k]), f[2 * k + 1] = Half<H>::hi(w[k]);
 }
-template <bool H>
-__device__ __forceinline__ void store4h(uint16_t* p, const float (&f)[4]) {
-  *reinterpret_cast<u32x2*>(p) = u32x2{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3])};
-}
-
-template <bool H>
+// STREAM: results that nobody reads before the backward go past the caches, which keep h for the next product
+// (a training step of 16384 tokens, 1024 / 4096: 1285 -> 1263 us; dg and du, which the next products read, lose
+// by it: 1263 -> 1308).
+template <bool H, bool STREAM = false>
 __device__ __forceinline__ void store8h(uint16_t* p, const float (&f)[8]) {
-  *reinterpret_cast<u32x4*>(p) = u32x4{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3]), Half<H>::pack2(f[4], f[5]),
-                                       Half<H>::pack2(f[6], f[7])};
+  const u32x4 v = {Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3]), Half<H>::pack2(f[4], f[5]), Half<H>::pack2(f[6], f[7])};
+  if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));
+  else *reinterpret_cast<u32x4*>(p) = v;
 }
 
 // sixteen zero bytes that out-of-range pieces of a tile are loaded from
@@ -78,8 +81,8 @@ __device__ __forceinline__ void act_both(float z, int act, float& a, float& d) {
 // D[n][m] = sum_k A(m, k) B(n, k) over one or two (A, B) pairs, in fp32; rows m of A are the features
 // that lie consecutive in D.  An operand is stored [rows][K] (KC: K consecutive) or [K][rows] (MC).
 //   EPI_STORE  D (+ resid) rounded to the type       EPI_PART  fp32 partial sums of a share of K
-//   EPI_GATE   A holds two weights; h = act(g) u, and g, u if asked
-//   EPI_GRAD   D = dh; from g and u: dg = dh u act'(g), du = dh act(g)
+//   EPI_GATE   A holds two weights; h = act(g) u, and cg, cu if asked
+//   EPI_GRAD   D = dh; dg = dh cg, du = dh cu
 enum { EPI_STORE = 0, EPI_PART = 1, EPI_GATE = 2, EPI_GRAD = 3 };
 
 struct Gemm {
@@ -88,10 +91,11 @@ struct Gemm {
   int64_t lda, ldb;          // row strides (elements) of the stored matrices
   int64_t M, N, K;           // K of one pair
   int pairs;                 // K runs over pairs * K
+  int parts;                 // 2: two products of one A, with B[0] and B[1], results d0 and d1 (or both in part)
   int splits;                // shares of K (EPI_PART)
   int act;
-  uint16_t* d0; uint16_t* d1; uint16_t* d2;   // STORE: D | GATE: h, g, u | GRAD: dg, du
-  const uint16_t* s0; const uint16_t* s1;     // STORE: resid | GRAD: g, u
+  uint16_t* d0; uint16_t* d1; uint16_t* d2;   // STORE: D | GATE: h, cg, cu | GRAD: dg, du
+  const uint16_t* s0; const uint16_t* s1;     // STORE: resid | GRAD: cg, cu
   float* part;
   int64_t ldd;
 };
@@ -108,12 +112,23 @@ constexpr int BK = 64;       // K of a stage
 __device__ __forceinline__ int f_kc(int row) { return -(row >> 2) & 3; }
 __device__ __forceinline__ int f_mc(int k) { return 2 * ((k & 3) | (((k >> 3) & 1) << 2)); }
 
-// The matrix row that row i of A's fragment t holds.  KC: a lane (i, q) of the products' results holds rows
-// 4 q .. + 3 of each fragment, so 16 consecutive features of four fragments.  EPI_GATE: fragments 0 and 1 of
-// four are gate's, 2 and 3 up's, 8 consecutive features of a lane each.
+// The matrix row that row i of A's fragment t holds.  A lane (i, q) of the products' results holds rows 4 q ..
+// + 3 of each fragment.  KC: with this order two fragments give 8 consecutive features, and the four q of a
+// column 32; EPI_GATE: fragments 0 and 1 of four are gate's, 2 and 3 the same features of up.
 template <bool GATE>
 __device__ __forceinline__ int a_row(int t, int i) {
-  return GATE ? (t >> 2) * 32 + 8 * (i >> 2) + 4 * (t & 1) + (i & 3) : (t >> 2) * 64 + 16 * (i >> 2) + 4 * (t & 3) + (i & 3);
+  return (GATE ? t >> 2 : t >> 1) * 32 + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
+}
+
+// MC fragments hold rows in their own order: fragments a and a + 1 of lane q = 0 .. 3 become 8 consecutive
+// features, those of fragment a + (q & 1) from 8 (q / 2) on, by exchanging neighbouring rows of 16 lanes
+__device__ __forceinline__ void pair_rows(const f32x4& x, const f32x4& y, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[e]), __float_as_uint(y[e]), false, false);
+    f[e] = __uint_as_float(s[0]);
+    f[4 + e] = __uint_as_float(s[1]);
+  }
 }
 
 // Output tiles of TILE x TILE, waves of TILE / 2 x 64.  Two K stages in LDS, of two steps each; a step's
@@ -133,7 +148,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
 
   constexpr int FM = GATE ? BM / 2 : BM;                        // features of a tile
-  const int mt = (int)((p.M + FM - 1) / FM), nt = (int)((p.N + BN - 1) / BN);
+  const int mt = (int)((p.M + FM - 1) / FM), nt1 = (int)((p.N + BN - 1) / BN), nt = nt1 * p.parts;
   const int tiles = mt * nt * p.splits;                         // < 2^30 (launch_tile)
   // workgroups are dealt to the 8 XCDs round robin; an XCD takes a run of the tiles, which go eight
   // columns at a time, so that the tiles in work on it share operand rows in its L2
@@ -144,7 +159,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
 
   const int kt = (int)((p.K + BK - 1) / BK), all = kt * p.pairs;
   struct Where {
-    int m0, n0, split, t0, t1;
+    int m0, n0, part, split, t0, t1;
   };
   auto where = [&](int idx) {
     Where v;
@@ -152,7 +167,9 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
     const int r = idx - v.split * (mt * nt), ng = r / (mt * 8), rr = r - ng * mt * 8;
     const int wide = min(8, nt - ng * 8);
     v.m0 = uniform(rr / wide * FM);
-    v.n0 = uniform((ng * 8 + rr % wide) * BN);
+    const int c = ng * 8 + rr % wide;
+    v.part = uniform(c >= nt1 ? 1 : 0);
+    v.n0 = uniform((c - v.part * nt1) * BN);
     v.t0 = uniform((int)((int64_t)all * v.split / p.splits));
     v.t1 = uniform((int)((int64_t)all * (v.split + 1) / p.splits));
     return v;
@@ -200,7 +217,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
     const int64_t ao = AMC ? k0 * p.lda + lv.m0 : lv.m0 * p.lda + k0, bo = BMC ? k0 * p.ldb + lv.n0 : lv.n0 * p.ldb + k0;
     sa0 = ptr(GATE || !pr ? p.A[0] : p.A[1], ao);
     if constexpr (GATE) sa1 = ptr(p.A[1], ao);
-    sb0 = ptr(pr ? p.B[1] : p.B[0], bo);
+    sb0 = ptr(pr | lv.part ? p.B[1] : p.B[0], bo);
     left = (int)(p.K - k0);
   };
   auto advance = [&]() {                // behind the stream's end its last K stage is loaded again, for nobody
@@ -323,60 +340,79 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
     advance();
     if (++t < done.t1) continue;
 
-    // lane (i, q) of acc[a][b]: column n, features from f, consecutive: KC 16 of four fragments (EPI_GATE
-    // 8 of each weight), MC 4 of each
+    // column n of lane (i, q), features f .. f + 7 of two fragments (EPI_GATE: of two of each weight)
+    const int64_t f0 = done.m0 + (GATE ? wm / 2 : wm) + (AMC ? 16 * (q & 1) + 8 * (q >> 1) : 8 * q);
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
       const int64_t n = done.n0 + wn + 16 * b + i;
-      if (n >= p.N) continue;
-      if constexpr (EPI == EPI_GATE) {
+      const bool in_n = n < p.N;
+      if constexpr (GATE) {
+        if (!in_n) continue;
 #pragma unroll
         for (int a = 0; a < MT; a += 4) {
-          const int64_t f = done.m0 + wm / 2 + (a >> 2) * 32 + 8 * q;
+          const int64_t f = f0 + a * 8, at = n * p.ldd + f;
           if (f >= p.M) continue;
-          float h[8], gv[8], uv[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            gv[e] = acc[a + (e >> 2)][b][e & 3];
-            uv[e] = acc[a + 2 + (e >> 2)][b][e & 3];
-            h[e] = act_f(gv[e], p.act) * uv[e];
-          }
-          store8h<H>(p.d0 + n * p.ldd + f, h);
+          float h[8], cg[8], cu[8];
           if (p.d1) {
-            store8h<H>(p.d1 + n * p.ldd + f, gv);
-            store8h<H>(p.d2 + n * p.ldd + f, uv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float g = acc[a + (e >> 2)][b][e & 3], u = acc[a + 2 + (e >> 2)][b][e & 3];
+              float d;
+              act_both(g, p.act, cu[e], d);
+              h[e] = cu[e] * u;
+              cg[e] = u * d;
+            }
+            store8h<H, true>(p.d1 + at, cg);
+            store8h<H, true>(p.d2 + at, cu);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              h[e] = act_f(acc[a + (e >> 2)][b][e & 3], p.act) * acc[a + 2 + (e >> 2)][b][e & 3];
           }
+          store8h<H>(p.d0 + at, h);
         }
       } else {
+        // resid, or cg and cu: a column's features first, then what is made of them
+        u32x4 r0[MT / 2], r1[MT / 2];
+        const bool reads = EPI == EPI_GRAD || (EPI == EPI_STORE && p.s0);
 #pragma unroll
-        for (int a = 0; a < MT; ++a) {
-          const int64_t f = done.m0 + wm + (AMC ? 16 * a + 4 * q : (a >> 2) * 64 + 16 * q + 4 * (a & 3));
-          if (f >= p.M) continue;
-          const int64_t at = n * p.ldd + f;
-          float x[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+        for (int a = 0; a < MT; a += 2) {
+          const int64_t f = f0 + a * 16;
+          if (!reads || !in_n || f >= p.M) continue;
+          r0[a / 2] = *reinterpret_cast<const u32x4*>(p.s0 + n * p.ldd + f);
+          if constexpr (EPI == EPI_GRAD) r1[a / 2] = *reinterpret_cast<const u32x4*>(p.s1 + n * p.ldd + f);
+        }
+#pragma unroll
+        for (int a = 0; a < MT; a += 2) {
+          float x[8];
+          if constexpr (AMC) {
+            pair_rows(acc[a][b], acc[a + 1][b], x);       // all lanes take part
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = acc[a + (e >> 2)][b][e & 3];
+          }
+          const int64_t f = f0 + a * 16, at = n * p.ldd + f;
+          if (!in_n || f >= p.M) continue;
           if constexpr (EPI == EPI_PART) {
-            *reinterpret_cast<f32x4*>(p.part + (int64_t)done.split * p.N * p.ldd + at) = acc[a][b];
+            float* d = p.part + (int64_t)(done.split * p.parts + done.part) * p.N * p.ldd + at;
+            *reinterpret_cast<f32x4*>(d) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[4], x[5], x[6], x[7]};
           } else if constexpr (EPI == EPI_STORE) {
             if (p.s0) {
-              float r[4];
-              load4h<H>(p.s0 + at, r);
+              float r[8];
+              unpack8h<H>(r0[a / 2], r);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] += r[e];
+              for (int e = 0; e < 8; ++e) x[e] += r[e];
             }
-            store4h<H>(p.d0 + at, x);
+            store8h<H>((done.part ? p.d1 : p.d0) + at, x);
           } else {
-            float g[4], u[4], dg[4], du[4];
-            load4h<H>(p.s0 + at, g);
-            load4h<H>(p.s1 + at, u);
+            float dg[8], du[8];
+            unpack8h<H>(r0[a / 2], dg);
+            unpack8h<H>(r1[a / 2], du);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float ac, de;
-              act_both(g[e], p.act, ac, de);
-              dg[e] = x[e] * u[e] * de;
-              du[e] = x[e] * ac;
-            }
-            store4h<H>(p.d0 + at, dg);
-            store4h<H>(p.d1 + at, du);
+            for (int e = 0; e < 8; ++e) dg[e] *= x[e], du[e] *= x[e];
+            store8h<H>(p.d0 + at, dg);
+            store8h<H>(p.d1 + at, du);
           }
         }
       }
@@ -395,10 +431,67 @@ __global__ __launch_bounds__(256) void zero_kernel(u32x4* __restrict__ p, int64_
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0, 0, 0, 0};
 }
 
+// The partial products of the shares of K, summed in their order, + resid, rounded; `total` elements of each
+// of `parts` results.  HBM-bound (or the memory-side cache's).
+template <bool H>
+__global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ part, int splits, int parts, int64_t total,
+                                                     const uint16_t* __restrict__ resid, uint16_t* __restrict__ d0,
+                                                     uint16_t* __restrict__ d1) {
+  const int64_t all = total * parts, step = (int64_t)gridDim.x * 256 * 8;
+  for (int64_t e0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; e0 < all; e0 += step) {
+    float x[8] = {};
+    for (int s = 0; s < splits; ++s) {
+      const f32x4 *p = reinterpret_cast<const f32x4*>(part + s * all + e0), v = p[0], u = p[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += v[e], x[4 + e] += u[e];
+    }
+    const bool second = e0 >= total;
+    const int64_t at = second ? e0 - total : e0;
+    if (resid) {
+      float r[8];
+      unpack8h<H>(*reinterpret_cast<const u32x4*>(resid + at), r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] += r[e];
+    }
+    store8h<H>((second ? d1 : d0) + at, x);
+  }
+}
+
+// How a product of M features, N columns and K (over all pairs) runs: output tiles of 256 or 128, K in
+// `splits` shares.  The least of the estimated times in us: a 256 tile takes 1.75 a K stage and 8 more, one to
+// a CU; a 128 tile 0.8 and 4 alone on a CU, 1.15 and 5 beside another; shares write their fp32 sums, and a
+// second launch adds them up.  (Measured: 16384 x 1024, K 4096: 124 us with 256 tiles, 163 with 128 ones;
+// 1024 x 4096, K 16384: 204 us with 128 tiles, 124 and the sums with 256 ones in four shares.)
+struct Plan {
+  int tile, splits;
+};
+Plan plan(int64_t M, int64_t N, int64_t K, int parts, bool gate, bool may_split) {
+  Plan best{256, 1};
+  double least = 1e30;
+  const int64_t st = (K + BK - 1) / BK;
+  for (int tile : {256, 128}) {
+    const int64_t fm = gate ? tile / 2 : tile, t1 = (M + fm - 1) / fm * ((N + tile - 1) / tile) * parts;
+    for (int s = 1; s <= 16 && (s == 1 || (may_split && st >= 4 * s)); s *= 2) {
+      const int64_t t = t1 * s;
+      const double k = (double)((st + s - 1) / s);
+      double us;
+      if (tile == 256) us = (double)((t + 255) / 256) * (1.75 * k + 8);
+      else us = t <= 256 ? 0.8 * k + 4 : (double)((t + 511) / 512) * (1.15 * k + 5);
+      if (s > 1) us += 4 + (double)M * N * parts * (8 * s + 2) / 4.5e6;
+      if (us < least) least = us, best = {tile, s};
+    }
+  }
+  return best;
+}
+size_t part_bytes(int64_t M, int64_t N, int64_t K, int parts) {
+  const Plan p = plan(M, N, K, parts, false, true);
+  return p.splits > 1 ? (size_t)M * N * parts * p.splits * 4 : 0;
+}
+
 template <bool H, bool AMC, bool BMC, int EPI, int TILE, bool TAIL>
 int launch_tile(const Gemm& p, hipStream_t st) {
   constexpr int FM = EPI == EPI_GATE ? TILE / 2 : TILE;
-  const int64_t tiles = (p.M + FM - 1) / FM * ((p.N + TILE - 1) / TILE) * p.splits;
+  const int64_t tiles = (p.M + FM - 1) / FM * ((p.N + TILE - 1) / TILE) * p.parts * p.splits;
   if (tiles == 0) return LBK_OK;
   // every share of K holds a K stage: the kernel's stream of loads counts on it
   if (p.K < 1 || p.splits > (p.K + BK - 1) / BK * p.pairs) return LBK_ERR_ARG;
@@ -414,10 +507,26 @@ int launch_tile(const Gemm& p, hipStream_t st) {
 }
 
 template <bool H, bool AMC, bool BMC, int EPI>
-int launch_gemm(const Gemm& p, hipStream_t st) {
-  const int64_t big = (p.M * (EPI == EPI_GATE ? 2 : 1) + 255) / 256 * ((p.N + 255) / 256) * p.splits;
-  if (p.K % BK) return big >= 128 ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, true>(p, st);
-  return big >= 128 ? launch_tile<H, AMC, BMC, EPI, 256, false>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
+int launch_gemm(const Gemm& p, int tile, hipStream_t st) {
+  // EPI_GRAD's epilogue moves four times the results' bytes: two workgroups a CU hide it better than one of
+  // 256 x 256 (16384 x 4096, K 1024: 286 against 381 us)
+  if constexpr (EPI == EPI_GRAD)
+    return p.K % BK ? launch_tile<H, AMC, BMC, EPI, 128, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
+  if (p.K % BK) return tile == 256 ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, true>(p, st);
+  return tile == 256 ? launch_tile<H, AMC, BMC, EPI, 256, false>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
+}
+
+// EPI_STORE, whole or in shares of K by way of `part`
+template <bool H, bool AMC, bool BMC>
+int store_gemm(Gemm p, float* part, hipStream_t st) {
+  const Plan pl = plan(p.M, p.N, p.K * p.pairs, p.parts, false, part != nullptr);
+  if (pl.splits == 1) return launch_gemm<H, AMC, BMC, EPI_STORE>(p, pl.tile, st);
+  p.splits = pl.splits;
+  p.part = part;
+  if (int s = launch_gemm<H, AMC, BMC, EPI_PART>(p, pl.tile, st)) return s;
+  const int64_t total = p.N * p.ldd, threads = (total * p.parts / 8 + 255) / 256;
+  reduce_kernel<H><<<(unsigned)(threads < 2048 ? threads : 2048), 256, 0, st>>>(part, pl.splits, p.parts, total, p.s0, p.d0, p.d1);
+  return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH;
 }
 
 Gemm operands(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K) {
@@ -425,7 +534,7 @@ Gemm operands(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M,
   p.A[0] = p.A[1] = static_cast<const uint16_t*>(A);
   p.B[0] = p.B[1] = static_cast<const uint16_t*>(B);
   p.lda = lda, p.ldb = ldb, p.M = M, p.N = N, p.K = K;
-  p.pairs = p.splits = 1;
+  p.pairs = p.parts = p.splits = 1;
   return p;
 }
 
@@ -436,20 +545,20 @@ struct GatedArgs {
 };
 
 template <bool H>
-int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* h, void* g, void* u, hipStream_t st) {
+int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* h, void* cg, void* cu, float* part, hipStream_t st) {
   Gemm p = operands(a.wg, a.D, x, a.D, a.F, a.N, a.D);
   p.A[1] = static_cast<const uint16_t*>(a.wu);
   p.act = a.act, p.ldd = a.F;
-  p.d0 = static_cast<uint16_t*>(h), p.d1 = static_cast<uint16_t*>(g), p.d2 = static_cast<uint16_t*>(u);
-  if (int s = launch_gemm<H, false, false, EPI_GATE>(p, st)) return s;
+  p.d0 = static_cast<uint16_t*>(h), p.d1 = static_cast<uint16_t*>(cg), p.d2 = static_cast<uint16_t*>(cu);
+  if (int s = launch_gemm<H, false, false, EPI_GATE>(p, plan(p.M, p.N, p.K, 1, true, false).tile, st)) return s;
   Gemm d = operands(a.wd, a.F, h, a.F, a.D, a.N, a.F);
   d.ldd = a.D, d.d0 = static_cast<uint16_t*>(out), d.s0 = residual ? static_cast<const uint16_t*>(x) : nullptr;
-  return launch_gemm<H, false, false, EPI_STORE>(d, st);
+  return store_gemm<H, false, false>(d, part, st);
 }
 
 template <bool H>
-int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* g, const void* u, const void* h, int residual,
-              void* dx, void* dwg, void* dwu, void* dwd, void* dg, void* du, hipStream_t st) {
+int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* cg, const void* cu, const void* h, int residual,
+              void* dx, void* dwg, void* dwu, void* dwd, void* dg, void* du, float* part, hipStream_t st) {
   if (a.N == 0) {
     for (void* d : {dwg, dwu, dwd})
       if (d) zero_kernel<<<256, 256, 0, st>>>(static_cast<u32x4*>(d), a.D * a.F / 8);
@@ -457,29 +566,28 @@ int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* g, 
   }
   if (dx || dwg || dwu) {
     Gemm p = operands(a.wd, a.F, dy, a.D, a.F, a.N, a.D);
-    p.act = a.act, p.ldd = a.F;
+    p.ldd = a.F;
     p.d0 = static_cast<uint16_t*>(dg), p.d1 = static_cast<uint16_t*>(du);
-    p.s0 = static_cast<const uint16_t*>(g), p.s1 = static_cast<const uint16_t*>(u);
-    if (int s = launch_gemm<H, true, false, EPI_GRAD>(p, st)) return s;
+    p.s0 = static_cast<const uint16_t*>(cg), p.s1 = static_cast<const uint16_t*>(cu);
+    if (int s = launch_gemm<H, true, false, EPI_GRAD>(p, 128, st)) return s;
   }
   if (dx) {
     Gemm p = operands(a.wg, a.D, dg, a.F, a.D, a.N, a.F);
     p.A[1] = static_cast<const uint16_t*>(a.wu), p.B[1] = static_cast<const uint16_t*>(du), p.pairs = 2;
     p.ldd = a.D, p.d0 = static_cast<uint16_t*>(dx), p.s0 = residual ? static_cast<const uint16_t*>(dy) : nullptr;
-    if (int s = launch_gemm<H, true, false, EPI_STORE>(p, st)) return s;
+    if (int s = store_gemm<H, true, false>(p, part, st)) return s;
   }
-  const void* gr[2] = {dg, du};
-  void* dw[2] = {dwg, dwu};
-  for (int k = 0; k < 2; ++k)
-    if (dw[k]) {
-      Gemm p = operands(x, a.D, gr[k], a.F, a.D, a.F, a.N);
-      p.ldd = a.D, p.d0 = static_cast<uint16_t*>(dw[k]);
-      if (int s = launch_gemm<H, true, true, EPI_STORE>(p, st)) return s;
-    }
+  if (dwg || dwu) {
+    // one launch for both, which share x, where both are wanted
+    Gemm p = operands(x, a.D, dwg ? dg : du, a.F, a.D, a.F, a.N);
+    p.ldd = a.D, p.d0 = static_cast<uint16_t*>(dwg ? dwg : dwu), p.parts = dwg && dwu ? 2 : 1;
+    p.B[1] = static_cast<const uint16_t*>(du), p.d1 = static_cast<uint16_t*>(dwu);
+    if (int s = store_gemm<H, true, true>(p, part, st)) return s;
+  }
   if (dwd) {
     Gemm p = operands(h, a.F, dy, a.D, a.F, a.D, a.N);
     p.ldd = a.F, p.d0 = static_cast<uint16_t*>(dwd);
-    if (int s = launch_gemm<H, true, true, EPI_STORE>(p, st)) return s;
+    if (int s = store_gemm<H, true, true>(p, part, st)) return s;
   }
   return LBK_OK;
 }
@@ -504,51 +612,57 @@ extern "C" {
 
 size_t lbk_gated_fwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff, int want_intermediates) {
   if (N <= 0 || d_model <= 0 || d_ff <= 0) return 0;
-  return want_intermediates ? 0 : align256((size_t)N * d_ff * 2);
+  return (want_intermediates ? 0 : align256((size_t)N * d_ff * 2)) + part_bytes(d_model, N, d_ff, 1);
 }
 
 int lbk_gated_fwd(int32_t dtype, int32_t act, const void* x, int64_t N, int32_t d_model, int32_t d_ff,
                   const void* w_gate, const void* w_up, const void* w_down, int add_residual, void* out, void* h_out,
-                  void* gate_pre_out, void* up_out, void* workspace, size_t workspace_bytes, void* stream) {
+                  void* gate_factor_out, void* up_factor_out, void* workspace, size_t workspace_bytes, void* stream) {
   if (int st = check_gated(dtype, act, N, d_model, d_ff)) return st;
   if (N == 0) return LBK_OK;
   if (!x || !w_gate || !w_up || !w_down || !out) return LBK_ERR_NULL;
-  const bool inter = h_out || gate_pre_out || up_out;
-  if (inter && (!h_out || !gate_pre_out || !up_out)) return LBK_ERR_NULL;
-  for (const void* p : {x, w_gate, w_up, w_down, (const void*)out, (const void*)h_out, (const void*)gate_pre_out,
-                        (const void*)up_out, (const void*)workspace})
+  const bool inter = h_out || gate_factor_out || up_factor_out;
+  if (inter && (!h_out || !gate_factor_out || !up_factor_out)) return LBK_ERR_NULL;
+  for (const void* p : {x, w_gate, w_up, w_down, (const void*)out, (const void*)h_out, (const void*)gate_factor_out,
+                        (const void*)up_factor_out, (const void*)workspace})
     if (!a16(p)) return LBK_ERR_ALIGN;
   const size_t need = lbk_gated_fwd_workspace_bytes(N, d_model, d_ff, inter);
   if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
   const GatedArgs a{N, d_model, d_ff, act, w_gate, w_up, w_down};
   void* h = inter ? h_out : workspace;
-  return dtype == LBK_FP16 ? gated_fwd<true>(a, x, add_residual, out, h, gate_pre_out, up_out, S(stream))
-                           : gated_fwd<false>(a, x, add_residual, out, h, gate_pre_out, up_out, S(stream));
+  float* part = part_bytes(d_model, N, d_ff, 1)
+                    ? reinterpret_cast<float*>(static_cast<char*>(workspace) + (inter ? 0 : align256((size_t)N * d_ff * 2)))
+                    : nullptr;
+  return dtype == LBK_FP16 ? gated_fwd<true>(a, x, add_residual, out, h, gate_factor_out, up_factor_out, part, S(stream))
+                           : gated_fwd<false>(a, x, add_residual, out, h, gate_factor_out, up_factor_out, part, S(stream));
 }
 
 size_t lbk_gated_bwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff) {
   if (N <= 0 || d_model <= 0 || d_ff <= 0) return 0;
-  return 2 * align256((size_t)N * d_ff * 2);
+  const size_t parts[] = {part_bytes(d_model, N, 2 * (int64_t)d_ff, 1), part_bytes(d_model, d_ff, N, 2),
+                          part_bytes(d_model, d_ff, N, 1), part_bytes(d_ff, d_model, N, 1)};
+  return 2 * align256((size_t)N * d_ff * 2) + *std::max_element(parts, parts + 4);
 }
 
-int lbk_gated_bwd(int32_t dtype, int32_t act, const void* grad_out, const void* x, const void* gate_pre,
-                  const void* up_out, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
+int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const void* gate_factor,
+                  const void* up_factor, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
                   const void* w_up, const void* w_down, int add_residual, void* dx, void* dw_gate, void* dw_up,
                   void* dw_down, void* workspace, size_t workspace_bytes, void* stream) {
-  if (int st = check_gated(dtype, act, N, d_model, d_ff)) return st;
+  if (int st = check_gated(dtype, LBK_SILU, N, d_model, d_ff)) return st;
   if (!w_gate || !w_up || !w_down) return LBK_ERR_NULL;
-  if (N > 0 && (!grad_out || !x || !gate_pre || !up_out || !h)) return LBK_ERR_NULL;
-  for (const void* p : {grad_out, x, gate_pre, up_out, h, w_gate, w_up, w_down, (const void*)dx, (const void*)dw_gate,
+  if (N > 0 && (!grad_out || !x || !gate_factor || !up_factor || !h)) return LBK_ERR_NULL;
+  for (const void* p : {grad_out, x, gate_factor, up_factor, h, w_gate, w_up, w_down, (const void*)dx, (const void*)dw_gate,
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!a16(p)) return LBK_ERR_ALIGN;
   const size_t need = lbk_gated_bwd_workspace_bytes(N, d_model, d_ff);
   if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
-  const GatedArgs a{N, d_model, d_ff, act, w_gate, w_up, w_down};
+  const GatedArgs a{N, d_model, d_ff, LBK_SILU, w_gate, w_up, w_down};
   void* dg = workspace;
   void* du = static_cast<char*>(workspace) + align256((size_t)N * d_ff * 2);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(du) + align256((size_t)N * d_ff * 2));
   return dtype == LBK_FP16
-             ? gated_bwd<true>(a, grad_out, x, gate_pre, up_out, h, add_residual, dx, dw_gate, dw_up, dw_down, dg, du, S(stream))
-             : gated_bwd<false>(a, grad_out, x, gate_pre, up_out, h, add_residual, dx, dw_gate, dw_up, dw_down, dg, du, S(stream));
+             ? gated_bwd<true>(a, grad_out, x, gate_factor, up_factor, h, add_residual, dx, dw_gate, dw_up, dw_down, dg, du, part, S(stream))
+             : gated_bwd<false>(a, grad_out, x, gate_factor, up_factor, h, add_residual, dx, dw_gate, dw_up, dw_down, dg, du, part, S(stream));
 }
 
 }  // extern "C"

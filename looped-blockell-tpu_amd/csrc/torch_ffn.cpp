@@ -219,19 +219,20 @@ Tensor gated_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
   return std::get<0>(gated_fwd_impl(x, wg, wu, wd, act, add_residual, false, "gated_ffn_fwd"));
 }
 
+// (out, h, u act'(g), act(g))
 Four gated_fwd_train(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, c10::string_view act,
                      bool add_residual) {
   return gated_fwd_impl(x, wg, wu, wd, act, add_residual, true, "gated_ffn_fwd_train");
 }
 
-// (dx, dw_gate, dw_up, dw_down); those not wanted come back empty
+// (dx, dw_gate, dw_up, dw_down) from gated_fwd_train's factors and h; those not wanted come back empty
 Four gated_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& g_, const Tensor& u_, const Tensor& h_, const Tensor& wg,
-               const Tensor& wu, const Tensor& wd, c10::string_view act, bool add_residual, std::array<bool, 4> want) {
+               const Tensor& wu, const Tensor& wd, bool add_residual, std::array<bool, 4> want) {
   const char* op = "gated_ffn_bwd";
   check_gpu(x_, op, "x");
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x_.device());
-  const Gated a = make_gated(x_, wg, wu, wd, act, op);
-  const std::pair<const Tensor*, const char*> ts[] = {{&dy_, "grad_out"}, {&g_, "gate_pre"}, {&u_, "up_out"}, {&h_, "h"}};
+  const Gated a = make_gated(x_, wg, wu, wd, "silu", op);     // the factors hold the activation
+  const std::pair<const Tensor*, const char*> ts[] = {{&dy_, "grad_out"}, {&g_, "gate_factor"}, {&u_, "up_factor"}, {&h_, "h"}};
   for (const auto& [t, name] : ts) {
     check_with(*t, x_, op, name);
     TORCH_CHECK(t->scalar_type() == x_.scalar_type() && t->dim() == 2 && t->size(0) == a.N &&
@@ -250,7 +251,7 @@ Four gated_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& g_, const Tens
   const size_t wsb = lbk_gated_bwd_workspace_bytes(a.N, (int32_t)a.D, (int32_t)a.F);
   Tensor ws = workspace(wsb, a.x);
   LBK_CALL("gated_ffn_bwd",
-           lbk_gated_bwd(a.dt, a.act, dy.data_ptr(), a.x.data_ptr(), g.data_ptr(), u.data_ptr(), h.data_ptr(), a.N, (int32_t)a.D,
+           lbk_gated_bwd(a.dt, dy.data_ptr(), a.x.data_ptr(), g.data_ptr(), u.data_ptr(), h.data_ptr(), a.N, (int32_t)a.D,
                          (int32_t)a.F, a.wg.data_ptr(), a.wu.data_ptr(), a.wd.data_ptr(), add_residual ? 1 : 0, p[0], p[1],
                          p[2], p[3], ws.data_ptr(), wsb, cur_stream(a.x)));
   return {r[0], r[1], r[2], r[3]};
@@ -265,10 +266,10 @@ Four call_gated_fwd_train(const Tensor& x, const Tensor& wg, const Tensor& wu, c
 }
 
 Four call_gated_bwd(const Tensor& dy, const Tensor& x, const Tensor& g, const Tensor& u, const Tensor& h, const Tensor& wg,
-                    const Tensor& wu, const Tensor& wd, c10::string_view act, bool add_residual, std::array<bool, 4> want) {
+                    const Tensor& wu, const Tensor& wd, bool add_residual, std::array<bool, 4> want) {
   static const auto op =
       c10::Dispatcher::singleton().findSchemaOrThrow("titan::gated_ffn_bwd", "").typed<decltype(gated_bwd)>();
-  return op.call(dy, x, g, u, h, wg, wu, wd, act, add_residual, want);
+  return op.call(dy, x, g, u, h, wg, wu, wd, add_residual, want);
 }
 
 struct GatedTrain : public torch::autograd::Function<GatedTrain> {
@@ -277,7 +278,6 @@ struct GatedTrain : public torch::autograd::Function<GatedTrain> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [out, h, g, u] = call_gated_fwd_train(x, wg, wu, wd, act, add_residual);
     ctx->save_for_backward({x, g, u, h, wg, wu, wd});
-    ctx->saved_data["act"] = std::string(act);
     ctx->saved_data["res"] = add_residual;
     return out;
   }
@@ -288,8 +288,7 @@ struct GatedTrain : public torch::autograd::Function<GatedTrain> {
     const auto s = ctx->get_saved_variables();
     std::array<bool, 4> want;
     for (int k = 0; k < 4; ++k) want[k] = ctx->needs_input_grad(k);
-    const std::string act = ctx->saved_data["act"].toStringRef();
-    auto d = call_gated_bwd(grads[0].to(s[0].scalar_type()), s[0], s[1], s[2], s[3], s[4], s[5], s[6], act,
+    auto d = call_gated_bwd(grads[0].to(s[0].scalar_type()), s[0], s[1], s[2], s[3], s[4], s[5], s[6],
                             ctx->saved_data["res"].toBool(), want);
     if (want[0]) r[0] = std::get<0>(d);
     if (want[1]) r[1] = std::get<1>(d);
@@ -322,8 +321,8 @@ TORCH_LIBRARY_FRAGMENT(titan, m) {
   m.def("gated_ffn_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation, bool add_residual) -> Tensor");
   m.def("gated_ffn_fwd_train(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation, bool add_residual) "
         "-> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("gated_ffn_bwd(Tensor grad_out, Tensor x, Tensor gate_pre, Tensor up_out, Tensor h, Tensor w_gate, Tensor w_up, "
-        "Tensor w_down, str activation, bool add_residual, bool[4] want) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("gated_ffn_bwd(Tensor grad_out, Tensor x, Tensor gate_factor, Tensor up_factor, Tensor h, Tensor w_gate, "
+        "Tensor w_up, Tensor w_down, bool add_residual, bool[4] want) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("gated_ffn_train(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, str activation, bool add_residual) -> Tensor");
 }
 
@@ -380,7 +379,7 @@ TORCH_LIBRARY_IMPL(titan, Meta, m) {
     return std::make_tuple(at::empty_like(x), act(), act(), act());
   });
   m.impl("gated_ffn_bwd", [](const Tensor&, const Tensor& x, const Tensor&, const Tensor&, const Tensor&, const Tensor& wg,
-                             const Tensor& wu, const Tensor& wd, c10::string_view, bool, std::array<bool, 4> want) {
+                             const Tensor& wu, const Tensor& wd, bool, std::array<bool, 4> want) {
     auto d = [&](int k, const Tensor& t) { return want[k] ? at::empty(t.sizes(), x.options()) : at::empty({0}, x.options()); };
     return std::make_tuple(d(0, x), d(1, wg), d(2, wu), d(3, wd));
   });

@@ -180,7 +180,7 @@ SIGNATURES = {
     "lbk_gated_fwd_workspace_bytes": (_SZ, [_I64, _I32, _I32, C.c_int]),
     "lbk_gated_fwd": (C.c_int, [_I32, _I32, _P, _I64, _I32, _I32, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P, _SZ, _P]),
     "lbk_gated_bwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
-    "lbk_gated_bwd": (C.c_int, [_I32, _I32, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P,
+    "lbk_gated_bwd": (C.c_int, [_I32, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P,
                                 _SZ, _P]),
 }
 

@@ -144,8 +144,8 @@ def act_eval(z, a):
 
 def gated(x, wg, wu, wd, dy, kind, residual):
     """{name: (value, bound)} of the forward, and with dy of the four gradients, from float64 copies of the
-    inputs.  The bounds count 32-bit sums and one rounding to the inputs' type of each of g, u, h, dg, du;
-    the last rounding of a result is `close`'s."""
+    inputs.  The bounds count 32-bit sums and one rounding to the inputs' type of each of h, dg, du and
+    of the factors u act'(g) and act(g) that the forward keeps; the last rounding of a result is `close`'s."""
     hs = HALF_STEP[x.dtype]
     dt = x.dtype
     # a rounding near or below the subnormals is off by at most half their step instead
@@ -176,18 +176,16 @@ def gated(x, wg, wu, wd, dy, kind, residual):
         return res
     Y = dy.double()
     dh, edh = mm(Y, D)
-    egr = eg * (1 + hs) + hs * g.abs() + sub          # g and u as kept for the backward
-    eur = eu * (1 + hs) + hs * u.abs() + sub
-    ear = 1.2 * egr + act_eval(g, a)
-    edr = dd * egr + act_eval(g, da)
     dg, du = dh * u * da, dh * a
 
-    def triple(p, ep, q, eq, r, er):
-        full = (p.abs() + ep) * (q.abs() + eq) * (r.abs() + er)
-        return full - (p * q * r).abs() + 4 * U32 * full
+    def times(p, ep, q, eq):
+        full = (p.abs() + ep) * (q.abs() + eq)
+        return full - (p * q).abs() + 2 * U32 * full
 
-    edg = triple(dh, edh, u, eur, da, edr)
-    edu = triple(dh, edh, a, ear, torch.ones_like(a), torch.zeros_like(a))
+    ecg = times(u, eu, da, dd * eg + act_eval(g, da))
+    ecg = ecg * (1 + hs) + hs * (u * da).abs() + sub
+    ecu = ea * (1 + hs) + hs * a.abs() + sub
+    edg, edu = times(dh, edh, u * da, ecg), times(dh, edh, a, ecu)
     edg = edg * (1 + hs) + hs * dg.abs() + sub
     edu = edu * (1 + hs) + hs * du.abs() + sub
     F = dg.shape[1]

@@ -75,8 +75,8 @@ def test_gated_validation_codes():
     assert fwd(N=0, x=None, out=None, ws=None, nb=0) == A.LBK_OK
     assert lib.lbk_gated_fwd_workspace_bytes(8, 64, 128, 0) >= 8 * 128 * 2
 
-    def bwd(dt=0, act=0, dy=P, N=8, d=64, ff=128, wd=P, dx=P, ws=P, nb=1 << 20):
-        return lib.lbk_gated_bwd(dt, act, dy, P, P, P, P, N, d, ff, P, P, wd, 0, dx, P, P, P, ws, nb, None)
+    def bwd(dt=0, dy=P, N=8, d=64, ff=128, wd=P, dx=P, ws=P, nb=1 << 20):
+        return lib.lbk_gated_bwd(dt, dy, P, P, P, P, N, d, ff, P, P, wd, 0, dx, P, P, P, ws, nb, None)
 
     assert bwd(dt=3) == A.LBK_ERR_ARG and bwd(d=4) == A.LBK_ERR_SHAPE and bwd(dy=None) == A.LBK_ERR_NULL
     assert bwd(wd=None) == A.LBK_ERR_NULL and bwd(dx=P + 4) == A.LBK_ERR_ALIGN
@@ -107,7 +107,7 @@ def test_shape_functions():
     assert kernels.gated_ffn(x, *w).shape == (7, 64)
     out, h, g, u = o.gated_ffn_fwd_train(x, *w, "gelu", True)
     assert h.shape == g.shape == u.shape == (7, 128)
-    r = o.gated_ffn_bwd(out, x, g, u, h, *w, "gelu", True, [True, False, True, True])
+    r = o.gated_ffn_bwd(out, x, g, u, h, *w, True, [True, False, True, True])
     assert [tuple(t.shape) for t in r] == [(7, 64), (0,), (128, 64), (64, 128)]
 
 
