@@ -516,6 +516,150 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ few tokens
+// A workgroup of 8 waves makes one 32-row output tile of 32 tokens: the slots are dealt to the waves (MODE 1:
+// gate's to waves 0 .. 3, up's to 4 .. 7) and their sums joined through LDS in a fixed order.  The weights are
+// read once, four positions on their way per wave; tokens come as bf16 rows, quantised where they are used
+// (one launch less, and a row of the slot's columns is 64 bytes a lane), or as panels of 32 (XQ: the hidden
+// state).  Latency-bound at these sizes: 16 tokens, 4096 / 14336 at 0.1, 9 MB of weights.
+template <int B, int MODE, bool XQ>
+__global__ __launch_bounds__(512, 4) void mx_decode_kernel(MxPanelArgs a, const uint16_t* __restrict__ x) {
+  constexpr int U = XQ ? 4 : 2, STEP = 64 / B, DEAL = MODE == 1 ? 4 : 8;
+  __shared__ f32x4 part[8][4][64];
+  __shared__ uint32_t top[4][64];
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6), half = lane >> 5, i = lane & 31;
+  const int64_t n = (int64_t)blockIdx.y * 32 + i;
+  const int C = a.F / B, o0 = blockIdx.x * 32, r = o0 / B, j = o0 % B + i;
+  const bool up = MODE == 1 && w >= 4;
+  const lbk_bell_mx& wt = up ? a.w1 : a.w0;
+  const int K = wt.K, P = (K + STEP - 1) / STEP;
+  const Panel Px = panel_of(a.F >> 5, 32);
+  const uint8_t* panel = a.x + blockIdx.y * Px.bytes;
+  f32x16 acc = {};
+  for (int p0 = w & (DEAL - 1); p0 < P; p0 += DEAL * U) {
+    u32x4 wv[U], xv[U][XQ ? 1 : 4];
+    uint32_t sa[U], sb[U];
+    int col[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int pos = p0 + u * DEAL;
+      if (pos >= P) break;
+      const int slot = B == 32 ? 2 * pos + half : pos;
+      const int64_t idx = (int64_t)r * K + min(slot, K - 1), at = (idx * B + j) * (B / 32) + (B == 64 ? half : 0);
+      wv[u] = reinterpret_cast<const u32x4*>(wt.codes)[at];
+      sa[u] = wt.scales[at];
+      col[u] = slot < K ? wt.col_idx[idx] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p0 + u * DEAL >= P) break;
+      const bool live = (uint32_t)col[u] < (uint32_t)C;
+      const int g = live ? (B == 32 ? col[u] : 2 * col[u] + half) : 0;
+      if (!live) wv[u] = u32x4{0, 0, 0, 0}, sa[u] = 127;
+      if constexpr (XQ) {
+        xv[u][0] = reinterpret_cast<const u32x4*>(panel)[g * 32 + i];
+        sb[u] = live ? panel[Px.codes + g * 32 + i] : 127u;
+      } else {
+        const u32x4* src = reinterpret_cast<const u32x4*>(x + n * a.F + g * 32);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) xv[u][k] = live && n < a.N ? src[k] : u32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p0 + u * DEAL >= P) break;
+      u32x4 b;
+      if constexpr (XQ) {
+        b = xv[u][0];
+      } else {
+        // the largest magnitude over packed pairs: as 16-bit integers in the upper and the lower halves
+        uint32_t hi = 0, lo = 0;
+        float f[4][8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          unpack8_bf16(xv[u][k], f[k]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            hi = max(hi, xv[u][k][e] & 0x7fffffffu);
+            lo = max(lo, xv[u][k][e] << 16 & 0x7fffffffu);
+          }
+        }
+        sb[u] = mx_scale(max(hi, lo));
+        const float s = mx_pow2(sb[u]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = mx_code8(f[k], s);
+      }
+      acc = mfma_fp4(wv[u], b, acc, sa[u], sb[u]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) part[w][q][lane] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  // wave q < 4: features 8 q + 4 half .. + 3 of the tile
+  const int q = w & 3, o = o0 + 8 * q + 4 * half;
+  float f[4] = {}, v[4] = {};
+  if (w < 4) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const f32x4 t = part[s][q][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) (MODE == 1 && s >= 4 ? v : f)[e] += t[e];
+    }
+  }
+  if constexpr (MODE == 1) {
+    uint32_t m = 0;
+    if (w < 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = silu_f(f[e] + (a.b0 ? a.b0[o + e] : 0.0f)) * (v[e] + (a.b1 ? a.b1[o + e] : 0.0f));
+        m = max(m, absbits(f[e]));
+      }
+      top[q][lane] = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    }
+    __syncthreads();
+    if (w < 4 && n < a.N) {
+      m = max(max(top[0][lane], top[1][lane]), max(top[2][lane], top[3][lane]));
+      const uint32_t b = mx_scale(m);
+      const float s = mx_pow2(b);
+      uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], s, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], s, 1);
+      const Panel Ph = panel_of(a.w0.R * (B / 32), 32);
+      uint8_t* blk = a.h + blockIdx.y * Ph.bytes;
+      const int at = blockIdx.x * 32 + i;
+      *reinterpret_cast<uint16_t*>(blk + at * 16 + 4 * q + 2 * half) = (uint16_t)c;
+      if (q == 0 && half == 0) blk[Ph.codes + at] = (uint8_t)b;
+    }
+  } else {
+    if (w >= 4 || n >= a.N) return;
+    const int64_t at = n * ((int64_t)a.w0.R * B) + o;
+    if (a.b0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += a.b0[o + e];
+    }
+    if (a.resid) {
+      float t[4];
+      load_bf16x<4>(a.resid + at, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += t[e];
+    }
+    store_bf16x<4>(a.y + at, f);
+  }
+}
+
+// x: bf16 rows, or NULL for a.x's panels
+template <int MODE>
+int launch_mx_decode(const MxPanelArgs& a, const uint16_t* x, hipStream_t st) {
+  const dim3 grid((unsigned)(a.w0.R * (a.w0.B / 32)), (unsigned)((a.N + 31) / 32));
+  if (a.w0.B == 32) {
+    if (x) mx_decode_kernel<32, MODE, false><<<grid, 512, 0, st>>>(a, x);
+    else mx_decode_kernel<32, MODE, true><<<grid, 512, 0, st>>>(a, x);
+  } else {
+    if (x) mx_decode_kernel<64, MODE, false><<<grid, 512, 0, st>>>(a, x);
+    else mx_decode_kernel<64, MODE, true><<<grid, 512, 0, st>>>(a, x);
+  }
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
 // Tokens a workgroup holds: the most whose codes and scales fit in LDS (0: none does)
 inline int mx_block_tokens(int F) {
   for (int TB = 128; TB >= 32; TB /= 2)
@@ -657,6 +801,9 @@ int check_ffn_mx(const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_
   return (int64_t)down->R * down->B == d_model ? LBK_OK : LBK_ERR_SHAPE;
 }
 
+// Tokens that mx_decode_kernel takes
+constexpr int64_t kDecode = 32;
+
 // Tokens of a panel block for a product of these input features, 0: rows of codes (mx_rowblock_kernel,
 // also where a weight has no slots)
 int in_tokens(int64_t F, const lbk_bell_mx* w) { return w->K > 0 ? mx_block_tokens((int)F) : 0; }
@@ -739,7 +886,7 @@ int lbk_mx_dequantize_tiles(const uint8_t* codes, const uint8_t* scales, int32_t
 }
 
 size_t lbk_mx_matmul_workspace_bytes(int64_t N, int32_t in_features, const lbk_bell_mx* w) {
-  if (!w || N <= 0 || in_features <= 0) return 0;
+  if (!w || N <= kDecode || in_features <= 0) return 0;
   return tokens_bytes(N, in_features, in_tokens(in_features, w));
 }
 
@@ -752,7 +899,12 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
   if (!x || !y) return LBK_ERR_NULL;
   if (!a16(x) || !a16(y) || !a16(workspace)) return LBK_ERR_ALIGN;
   const size_t need = lbk_mx_matmul_workspace_bytes(N, in_features, w);
-  if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
+  if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
+  if (N <= kDecode) {
+    MxPanelArgs a{};
+    a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
+    return launch_mx_decode<0>(a, x, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  }
   const int TB = in_tokens(in_features, w);
   if (int st = quantize_tokens(x, N, in_features, TB, workspace, S(stream))) return st;
   return product(workspace, N, in_features, TB, *w, bias, nullptr, y, S(stream));
@@ -761,6 +913,7 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
 size_t lbk_mx_swiglu_workspace_bytes(int64_t N, int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx* up,
                                      const lbk_bell_mx* down) {
   if (!gate || !up || !down || N <= 0 || d_model <= 0) return 0;
+  if (N <= kDecode) return tokens_bytes(N, (int64_t)gate->R * gate->B, 32);
   const FfnTokens t = ffn_tokens(d_model, gate, up, down);
   return tokens_bytes(N, d_model, t.x) + tokens_bytes(N, (int64_t)gate->R * gate->B, t.h);
 }
@@ -777,6 +930,15 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
   const size_t need = lbk_mx_swiglu_workspace_bytes(N, d_model, gate, up, down);
   if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
   const int d_ff = gate->R * gate->B;
+  if (N <= kDecode) {
+    MxPanelArgs g{};
+    g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up; g.h = static_cast<uint8_t*>(workspace);
+    if (launch_mx_decode<1>(g, x, S(stream)) != 0) return LBK_ERR_LAUNCH;
+    MxPanelArgs d{};
+    d.x = static_cast<uint8_t*>(workspace); d.N = N; d.F = d_ff; d.w0 = *down; d.b0 = b_down; d.y = out;
+    d.resid = add_residual ? x : nullptr;
+    return launch_mx_decode<0>(d, nullptr, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  }
   const FfnTokens t = ffn_tokens(d_model, gate, up, down);
   uint8_t* hp = static_cast<uint8_t*>(workspace) + tokens_bytes(N, d_model, t.x);
   if (int st = quantize_tokens(x, N, d_model, t.x, workspace, S(stream))) return st;

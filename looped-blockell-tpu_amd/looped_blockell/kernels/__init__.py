@@ -457,14 +457,18 @@ def mx_quantize(x):
     to the even code, beyond 6 to 6), two a byte, the even feature low.  A group that holds an Inf or
     a NaN gets scale 255 and reads back as NaN."""
     _gpu(x)
+    if x.dim() == 2:
+        return ops().mx_quantize(x)
     lead = x.shape[:-1]
-    codes, scales = ops().mx_quantize(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    codes, scales = ops().mx_quantize(x.reshape(-1, x.shape[-1]))
     return codes.reshape(*lead, codes.shape[-1]), scales.reshape(*lead, scales.shape[-1])
 
 
 def mx_dequantize(codes, scales, dtype: torch.dtype = torch.bfloat16):
     """The values that ``mx_quantize``'s codes and scales stand for, [..., F]."""
     _gpu(codes, scales)
+    if codes.dim() == 2 and scales.dim() == 2:
+        return ops().mx_dequantize(codes, scales, dtype)
     out = ops().mx_dequantize(codes.reshape(-1, codes.shape[-1]), scales.reshape(-1, scales.shape[-1]), dtype)
     return out.reshape(*codes.shape[:-1], out.shape[-1])
 
@@ -486,6 +490,9 @@ def mx_matmul(x, codes, scales, col_indices, bias=None):
     """x [..., C*B] -> [..., R*B] through a Block-ELL weight in 4 bits (``mx_quantize_tiles``), x
     quantised in the call, sums in fp32; not differentiable."""
     _gpu(x, codes, scales, col_indices)
+    if x.dim() == 2:
+        return ops().block_ell_matmul_mx(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), codes, scales, col_indices,
+                                         bias)
     lead = x.shape[:-1]
     y = ops().block_ell_matmul_mx(x.reshape(-1, x.shape[-1]).to(torch.bfloat16), codes, scales, col_indices, bias)
     return y.reshape(*lead, y.shape[-1])
@@ -496,6 +503,8 @@ def mx_swiglu(x, gate, up, down, add_residual: bool = False, b_gate=None, b_up=N
     x and the hidden state ``silu(gate) * up`` (formed in fp32) are quantised in the call; not
     differentiable."""
     _gpu(x, gate[0], up[0], down[0])
+    if x.dim() == 2 and x.dtype == torch.bfloat16:
+        return ops().block_ell_swiglu_fwd_mx(x, *gate, b_gate, *up, b_up, *down, b_down, add_residual)
     lead = x.shape[:-1]
     y = ops().block_ell_swiglu_fwd_mx(x.reshape(-1, x.shape[-1]).to(torch.bfloat16), *gate, b_gate, *up, b_up, *down, b_down,
                                       add_residual)
@@ -510,11 +519,10 @@ def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", add_residual: b
     Differentiable in x and the weights as one native autograd node (``titan::gated_ffn_train``),
     gradients in the inputs' type; without gradients nothing is kept."""
     _gpu(x, w_gate, w_up, w_down)
-    lead = x.shape[:-1]
-    x2 = x.reshape(-1, x.shape[-1])
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         _no_transforms()
         y = ops().gated_ffn_train(x2, w_gate, w_up, w_down, activation, add_residual)
     else:
         y = ops().gated_ffn_fwd(x2, w_gate, w_up, w_down, activation, add_residual)
-    return y.reshape(*lead, y.shape[-1])
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
