@@ -51,6 +51,10 @@ __device__ __forceinline__ void unpack8h(const u32x4& w, float (&f)[8]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) f[2 * k] = Half<H>::lo(w[k]), f[2 * k + 1] = Half<H>::hi(w[k]);
 }
+template <bool H>
+__device__ __forceinline__ void store4h(uint16_t* p, const float (&f)[4]) {
+  *reinterpret_cast<u32x2*>(p) = u32x2{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3])};
+}
 // STREAM: results that nobody reads before the backward go past the caches, which keep h for the next product
 // (a training step of 16384 tokens, 1024 / 4096: 1285 -> 1263 us; dg and du, which the next products read, lose
 // by it: 1263 -> 1308).
@@ -431,6 +435,118 @@ __global__ __launch_bounds__(256) void zero_kernel(u32x4* __restrict__ p, int64_
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0, 0, 0, 0};
 }
 
+// ------------------------------------------------------------------ few tokens
+// D of up to 16 NT columns (tokens) where A is KC: the weights are streamed once.  A workgroup makes 16
+// features (GATE: of both weights), its waves take K in turns of 64 (128 bytes of a row), U turns on their way;
+// the waves' sums meet in LDS and are added in their order.
+// EIGHT (up to 8 columns): 8 features, rows and columns 8 .. 15 of the matrix instructions taking the next 64 K
+// of the same features and tokens, so that twice the workgroups stream with whole loads.
+// HBM-bound: 1 token, 2048 / 8192, 100 MB of weights: 143 us on the tiled kernel, 25 so.
+template <bool H, bool GATE, int NT, int NW, bool EIGHT>
+__global__ __launch_bounds__(NW * 64) void skinny_kernel(Gemm p) {
+  constexpr int MATS = GATE ? 2 : 1, ROWS = EIGHT ? 8 : 16, TURN = EIGHT ? 128 : 64;
+  constexpr int U = NT == 1 ? 4 : 2;
+  static_assert(!EIGHT || NT == 1, "one tile");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  f32x4* part = reinterpret_cast<f32x4*>(smem);                 // [NW][MATS][NT][64]
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6), i = lane & 15, q = lane >> 4;
+  const int ii = EIGHT ? i & 7 : i, k0 = 16 * q + (EIGHT ? (i >> 3) * 64 : 0);
+  const int64_t f0 = (int64_t)blockIdx.x * ROWS;
+  const int S = (int)((p.K + TURN - 1) / TURN);
+  const uint16_t *wp[MATS], *xp[NT];
+#pragma unroll
+  for (int m = 0; m < MATS; ++m) wp[m] = p.A[m] + min(f0 + ii, p.M - 1) * p.lda + k0;
+#pragma unroll
+  for (int b = 0; b < NT; ++b) xp[b] = p.B[0] + min((int64_t)(16 * b + ii), p.N - 1) * p.ldb + k0;
+  f32x4 acc[MATS][NT] = {};
+  for (int s0 = w; s0 < S; s0 += NW * U) {
+    u32x4 wv[U][MATS][2], xv[U][NT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * NW;
+      if (s >= S) break;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const bool in = (int64_t)s * TURN + k0 + 8 * c < p.K;   // K is a multiple of 8
+        const int64_t at = (int64_t)s * TURN + 8 * c;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+          wv[u][m][c] = in ? *reinterpret_cast<const u32x4*>(wp[m] + at) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < NT; ++b) xv[u][b][c] = in ? *reinterpret_cast<const u32x4*>(xp[b] + at) : u32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * NW >= S) break;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+          for (int b = 0; b < NT; ++b) acc[m][b] = Half<H>::mfma(wv[u][m][c], xv[u][b][c], acc[m][b]);
+    }
+  }
+  auto slot = [&](int wave, int m, int b) { return ((wave * MATS + m) * NT + b) * 64 + lane; };
+#pragma unroll
+  for (int m = 0; m < MATS; ++m)
+#pragma unroll
+    for (int b = 0; b < NT; ++b) part[slot(w, m, b)] = acc[m][b];
+  __syncthreads();
+  if (w >= NT) return;
+  // wave w: columns 16 w + i, features f .. f + 3
+  if (EIGHT && (i >= 8 || q >= 2)) return;
+  const int64_t n = 16 * w + i, f = f0 + 4 * q, at = n * p.ldd + f;
+  f32x4 v[MATS] = {};
+#pragma unroll
+  for (int s = 0; s < NW; ++s)
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) {
+      v[m] += part[slot(s, m, w)];
+      if constexpr (EIGHT) v[m] += part[slot(s, m, w) + 8 + 32];      // rows and columns 8 further on
+    }
+  if (n >= p.N || f >= p.M) return;
+  float x[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+  if constexpr (GATE) {
+    float cg[4], cu[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float d;
+      act_both(x[e], p.act, cu[e], d);
+      cg[e] = v[1][e] * d;
+      x[e] = cu[e] * v[1][e];
+    }
+    if (p.d1) {
+      store4h<H>(p.d1 + at, cg);
+      store4h<H>(p.d2 + at, cu);
+    }
+  } else if (p.s0) {
+    const u32x2 t = *reinterpret_cast<const u32x2*>(p.s0 + at);
+    x[0] += Half<H>::lo(t[0]), x[1] += Half<H>::hi(t[0]), x[2] += Half<H>::lo(t[1]), x[3] += Half<H>::hi(t[1]);
+  }
+  store4h<H>(p.d0 + at, x);
+}
+
+// Whether the weights are streamed: where the tokens' own reads, once a workgroup, do not outweigh the tiled
+// kernel's idle columns.  us of a forward, streamed / tiled (33 tokens): 2048 / 8192 16 tokens 36 / 47, 32 tokens
+// 51 / 47; 1024 / 4096 32 tokens 20 / 25; 4096 / 14336 16 tokens 93 / 95, 8 tokens 80.
+bool skinny(int64_t N, int64_t D, int64_t F) { return N <= 16 || (N <= 32 && D * F <= (int64_t)1 << 23); }
+
+template <bool H, bool GATE, int NT, int NW, bool EIGHT = false>
+int launch_skinny_t(const Gemm& p, hipStream_t st) {
+  constexpr int lds = NW * (GATE ? 2 : 1) * NT * 64 * 16, rows = EIGHT ? 8 : 16;
+  static_assert(lds <= 65536, "within the default limit");
+  skinny_kernel<H, GATE, NT, NW, EIGHT><<<(unsigned)((p.M + rows - 1) / rows), NW * 64, lds, st>>>(p);
+  return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH;
+}
+template <bool H, bool GATE>
+int launch_skinny(const Gemm& p, hipStream_t st) {
+  const bool few = p.M < 256 * 16;          // fewer workgroups of 16 features than CUs
+  if (p.N <= 8 && few) return launch_skinny_t<H, GATE, 1, 16, true>(p, st);
+  if (p.N <= 16) return few ? launch_skinny_t<H, GATE, 1, 16>(p, st) : launch_skinny_t<H, GATE, 1, 8>(p, st);
+  return few ? launch_skinny_t<H, GATE, 2, 16>(p, st) : launch_skinny_t<H, GATE, 2, 8>(p, st);
+}
+
 // The partial products of the shares of K, summed in their order, + resid, rounded; `total` elements of each
 // of `parts` results.  HBM-bound (or the memory-side cache's).
 template <bool H>
@@ -487,6 +603,9 @@ size_t part_bytes(int64_t M, int64_t N, int64_t K, int parts) {
   const Plan p = plan(M, N, K, parts, false, true);
   return p.splits > 1 ? (size_t)M * N * parts * p.splits * 4 : 0;
 }
+
+// of the forward's second product
+size_t down_part_bytes(int64_t N, int64_t D, int64_t F) { return skinny(N, D, F) ? 0 : part_bytes(D, N, F, 1); }
 
 template <bool H, bool AMC, bool BMC, int EPI, int TILE, bool TAIL>
 int launch_tile(const Gemm& p, hipStream_t st) {
@@ -550,10 +669,12 @@ int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* 
   p.A[1] = static_cast<const uint16_t*>(a.wu);
   p.act = a.act, p.ldd = a.F;
   p.d0 = static_cast<uint16_t*>(h), p.d1 = static_cast<uint16_t*>(cg), p.d2 = static_cast<uint16_t*>(cu);
-  if (int s = launch_gemm<H, false, false, EPI_GATE>(p, plan(p.M, p.N, p.K, 1, true, false).tile, st)) return s;
+  if (int s = skinny(a.N, a.D, a.F) ? launch_skinny<H, true>(p, st)
+                             : launch_gemm<H, false, false, EPI_GATE>(p, plan(p.M, p.N, p.K, 1, true, false).tile, st))
+    return s;
   Gemm d = operands(a.wd, a.F, h, a.F, a.D, a.N, a.F);
   d.ldd = a.D, d.d0 = static_cast<uint16_t*>(out), d.s0 = residual ? static_cast<const uint16_t*>(x) : nullptr;
-  return store_gemm<H, false, false>(d, part, st);
+  return skinny(a.N, a.D, a.F) ? launch_skinny<H, false>(d, st) : store_gemm<H, false, false>(d, part, st);
 }
 
 template <bool H>
@@ -612,7 +733,7 @@ extern "C" {
 
 size_t lbk_gated_fwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff, int want_intermediates) {
   if (N <= 0 || d_model <= 0 || d_ff <= 0) return 0;
-  return (want_intermediates ? 0 : align256((size_t)N * d_ff * 2)) + part_bytes(d_model, N, d_ff, 1);
+  return (want_intermediates ? 0 : align256((size_t)N * d_ff * 2)) + down_part_bytes(N, d_model, d_ff);
 }
 
 int lbk_gated_fwd(int32_t dtype, int32_t act, const void* x, int64_t N, int32_t d_model, int32_t d_ff,
@@ -630,7 +751,7 @@ int lbk_gated_fwd(int32_t dtype, int32_t act, const void* x, int64_t N, int32_t 
   if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
   const GatedArgs a{N, d_model, d_ff, act, w_gate, w_up, w_down};
   void* h = inter ? h_out : workspace;
-  float* part = part_bytes(d_model, N, d_ff, 1)
+  float* part = down_part_bytes(N, d_model, d_ff)
                     ? reinterpret_cast<float*>(static_cast<char*>(workspace) + (inter ? 0 : align256((size_t)N * d_ff * 2)))
                     : nullptr;
   return dtype == LBK_FP16 ? gated_fwd<true>(a, x, add_residual, out, h, gate_factor_out, up_factor_out, part, S(stream))
