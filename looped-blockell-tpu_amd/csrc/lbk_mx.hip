@@ -252,9 +252,16 @@ struct MxArgs {
 // (v % 4) + 8 (v / 4) + 4 half; the partner lane l ^ 32 has the others) -> codes and scale.  The group's
 // maximum and code halves cross by one exchange each; each lane stores 8 of the 16 code bytes.
 __device__ __forceinline__ void mx_store_group(const float (&h)[16], int half, uint8_t* hc, uint8_t* hs, bool live) {
-  uint32_t m = 0;
+  // positive values are largest as signed integers, negative ones as unsigned (NaNs above all, either way):
+  // half an instruction a value each, where masking the sign off took a whole one
+  int mp = 0;
+  uint32_t mn = 0;
 #pragma unroll
-  for (int v = 0; v < 16; ++v) m = max(m, absbits(h[v]));
+  for (int v = 0; v < 16; ++v) {
+    mp = max(mp, __float_as_int(h[v]));
+    mn = max(mn, __float_as_uint(h[v]));
+  }
+  uint32_t m = max((uint32_t)mp, mn & 0x7fffffffu);
   m = max(m, (uint32_t)__shfl_xor((int)m, 32));
   const uint32_t b = mx_scale(m);
   const float s = mx_pow2(b);
@@ -354,14 +361,17 @@ struct MxPanelArgs {
   uint8_t* h; int TBh;                      // MODE 1: panels of TBh tokens
 };
 
-// A workgroup of 8 waves holds 32 MT tokens in LDS and one of `slices` shares of the 32-row output tiles;
-// a wave takes every 8th tile of the share.  The (tile, weight, slot pair) positions of a wave form one
-// stream: their codes (16 bytes a lane), scale and column are loaded D positions ahead, always all three,
-// so that the compiler's load counters stay exact across tiles.  A dead slot, and the second half of an odd
-// row's last pair, multiplies zeros with unit scales.
-template <int B, int MODE, int MT>
-__global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
-  constexpr int TB = 32 * MT, NW = 8, D = 4;
+// A workgroup of NW waves holds 32 MT tokens in LDS and one of `slices` shares of the 32-row output tiles; a
+// wave takes every NW-th tile of the share.  The (tile, weight, slot pair) positions of a wave form one stream:
+// their codes (16 bytes a lane), scale and column are loaded D positions ahead, always all three, so that the
+// compiler's load counters stay exact across tiles.  A dead slot, and the second half of an odd row's last
+// pair, multiplies zeros with unit scales.
+// MODE 1 is bound by the epilogue's vector work (silu's exp and reciprocal, the maximum and the conversion:
+// about 54 cycles a hidden value and wave, against 16 of the matrix unit at 8 slots), so four waves a SIMD of
+// 64 tokens beat two of 128, whose weights are read half as often.
+template <int B, int MODE, int MT, int NW, bool BIAS>
+__global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a) {
+  constexpr int TB = 32 * MT, D = 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6), half = lane >> 5, i = lane & 31;
   const int G = a.F >> 5, C = a.F / B;
@@ -375,62 +385,100 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
   const uint8_t* src = a.x + tb * P.bytes + lane * 16;
   for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_load16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  if (m0 >= mEnd) return;
 
-  constexpr int STEP = 64 / B;
-  const int P0 = (a.w0.K + STEP - 1) / STEP, P1 = MODE == 1 ? (a.w1.K + STEP - 1) / STEP : 0;
-  // loading position, D ahead of the computing one
-  int lm = m0, lup = 0, lj = 0;
-  u32x4 wr[D];
-  uint32_t sr[D];
-  int cr[D];
+  // a position is QP instructions' slots (STEP each)
+  constexpr int STEP = 64 / B, QP = 2;
+  const int P0 = (a.w0.K + STEP * QP - 1) / (STEP * QP), P1 = MODE == 1 ? (a.w1.K + STEP * QP - 1) / (STEP * QP) : 0;
+  // loading position, D ahead of the computing one: the row's codes, scales and columns, and this lane's place
+  // in a slot's tile; a tile on is NW * 32 / B block rows on
+  struct Row {
+    const uint8_t *c, *s;
+    const int32_t* i;
+  };
+  int lm = min(m0, mEnd - 1), lup = 0, lj = 0;
+  auto row_of = [&](const lbk_bell_mx& wt) {
+    const int64_t base = (int64_t)(lm * 32 / B) * wt.K;
+    return Row{wt.codes + base * (B * B / 2), wt.scales + base * (B * B / 32), wt.col_idx + base};
+  };
+  Row r0 = row_of(a.w0), r1 = MODE == 1 ? row_of(a.w1) : Row{};
+  const uint32_t place = (uint32_t)(lm * 32 % B + i) * (B / 32) + (B == 64 ? half : 0);
+  u32x4 wr[D][QP];
+  uint32_t sr[D][QP];
+  int cr[D][QP];
   auto load = [&](int d) {
-    const lbk_bell_mx& wt = lup ? a.w1 : a.w0;
-    const int K = wt.K, row = lm * 32, r = row / B, j = row % B + i;
-    const int slot = min(B == 32 ? 2 * lj + half : lj, K - 1);
-    const int64_t idx = (int64_t)r * K + slot, at = (idx * B + j) * (B / 32) + (B == 64 ? half : 0);
-    wr[d] = reinterpret_cast<const u32x4*>(wt.codes)[at];
-    sr[d] = wt.scales[at];
-    cr[d] = wt.col_idx[idx];
-    if (++lj == (lup ? P1 : P0)) {
+    const Row& r = MODE == 1 && lup ? r1 : r0;
+    const int K = MODE == 1 && lup ? a.w1.K : a.w0.K;
+#pragma unroll
+    for (int p = 0; p < QP; ++p) {
+      const uint32_t slot = (uint32_t)min(B == 32 ? 2 * (lj * QP + p) + half : lj * QP + p, K - 1);
+      const uint32_t piece = slot * (B * (B / 32)) + place;
+      wr[d][p] = reinterpret_cast<const u32x4*>(r.c)[piece];
+      sr[d][p] = r.s[piece];
+      cr[d][p] = r.i[slot];
+    }
+    if (++lj == (MODE == 1 && lup ? P1 : P0)) {
       lj = 0;
-      if (MODE == 1 && !lup) lup = 1;
-      else {
+      if (MODE == 1 && !lup) {
+        lup = 1;
+      } else {
         lup = 0;
-        lm = lm + NW < mEnd ? lm + NW : lm;      // behind the last tile: its loads again, for nobody
+        if (lm + NW < mEnd) {                    // behind the last tile: its loads again, for nobody
+          lm += NW;
+          r0 = row_of(a.w0);
+          if constexpr (MODE == 1) r1 = row_of(a.w1);
+        }
       }
     }
   };
 #pragma unroll
   for (int d = 0; d < D; ++d) load(d);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * D * QP) : "memory"); // the panel is in LDS
+  if (m0 >= mEnd) return;
 
   f32x16 acc[MODE + 1][MT] = {};
   const unsigned char* xs = smem + P.codes;
   int cm = m0, cup = 0, cj = 0;
-  auto compute = [&](int d, f32x16 (&c)[MT], int K) {
-    const int col = cr[d];
-    const bool live = (B == 64 || 2 * cj + half < K) && (uint32_t)col < (uint32_t)C;
-    const int g = live ? (B == 32 ? col : 2 * col + half) : 0;
-    const u32x4 wv = live ? wr[d] : u32x4{0, 0, 0, 0};
-    const uint32_t sa = live ? sr[d] : 127u;
-    uint32_t sb;
-    if constexpr (MT == 4) sb = reinterpret_cast<const uint32_t*>(xs)[g * 32 + i];
-    else if constexpr (MT == 2) sb = reinterpret_cast<const uint16_t*>(xs)[g * 32 + i];
-    else sb = xs[g * 32 + i];
-    sb = live ? sb : 0x7f7f7f7fu;
-    const u32x4* xp = reinterpret_cast<const u32x4*>(smem) + g * TB + i;
-    const i32x8_t A = {(int)wv[0], (int)wv[1], (int)wv[2], (int)wv[3], 0, 0, 0, 0};
-    auto mm = [&](int t, auto sel) {
-      const u32x4 xv = xp[32 * t];
-      const i32x8_t Bm = {(int)xv[0], (int)xv[1], (int)xv[2], (int)xv[3], 0, 0, 0, 0};
-      c[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, Bm, c[t], 4, 4, 0, (int)sa, decltype(sel)::value, (int)sb);
-    };
-    mm(0, std::integral_constant<int, 0>{});
-    if constexpr (MT > 1) mm(1, std::integral_constant<int, 1>{});
-    if constexpr (MT > 2) {
-      mm(2, std::integral_constant<int, 2>{});
-      mm(3, std::integral_constant<int, 3>{});
+  auto compute = [&](int d, f32x16 (&c)[MT], int K, bool first) {
+    u32x4 wv[QP], xv[QP][MT];
+    uint32_t sa[QP], sb[QP];
+    int g[QP];
+    bool live[QP], whole = true;
+#pragma unroll
+    for (int p = 0; p < QP; ++p) {
+      live[p] = (B == 64 ? cj * QP + p : 2 * (cj * QP + p) + half) < K && (uint32_t)cr[d][p] < (uint32_t)C;
+      whole &= live[p];
+      g[p] = B == 32 ? cr[d][p] : 2 * cr[d][p] + half;
+      wv[p] = wr[d][p];
+      sa[p] = sr[d][p];
+    }
+    const bool dead = __ballot(whole) != ~0ull;
+    if (dead) {
+#pragma unroll
+      for (int p = 0; p < QP; ++p)
+        if (!live[p]) g[p] = 0, wv[p] = u32x4{0, 0, 0, 0}, sa[p] = 127u;
+    }
+#pragma unroll
+    for (int p = 0; p < QP; ++p) {
+      if constexpr (MT == 2) sb[p] = reinterpret_cast<const uint16_t*>(xs)[g[p] * 32 + i];
+      else sb[p] = xs[g[p] * 32 + i];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xv[p][t] = reinterpret_cast<const u32x4*>(smem)[g[p] * TB + 32 * t + i];
+    }
+    if (dead) {
+#pragma unroll
+      for (int p = 0; p < QP; ++p)
+        if (!live[p]) sb[p] = 0x7f7fu;
+    }
+#pragma unroll
+    for (int p = 0; p < QP; ++p) {
+      const i32x8_t A = {(int)wv[p][0], (int)wv[p][1], (int)wv[p][2], (int)wv[p][3], 0, 0, 0, 0};
+      auto mm = [&](int t, auto sel) {
+        const i32x8_t Bm = {(int)xv[p][t][0], (int)xv[p][t][1], (int)xv[p][t][2], (int)xv[p][t][3], 0, 0, 0, 0};
+        if (first && p == 0) c[t] = f32x16{};
+        c[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(A, Bm, c[t], 4, 4, 0, (int)sa[p], decltype(sel)::value, (int)sb[p]);
+      };
+      mm(0, std::integral_constant<int, 0>{});
+      if constexpr (MT == 2) mm(1, std::integral_constant<int, 1>{});
     }
   };
   auto store = [&]() {
@@ -439,23 +487,31 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
       const int Gh = a.w0.R * (B / 32);
       const Panel Ph = panel_of(Gh, a.TBh);
       const int MTh = a.TBh / 32;
-      float bg[16], bu[16];
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const int o = o0 + (q & 3) + 8 * (q >> 2) + 4 * half;
-        bg[q] = a.b0 ? a.b0[o] : 0.0f;
-        bu[q] = a.b1 ? a.b1[o] : 0.0f;
-      }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         float v[16];
 #pragma unroll
-        for (int q = 0; q < 16; ++q) v[q] = silu_f(acc[0][t][q] + bg[q]) * (acc[MODE][t][q] + bu[q]);
-        const int64_t n = tb * TB + 32 * t + i, hb = n / a.TBh;
-        const int tt = (int)(n - hb * a.TBh);
-        uint8_t* blk = a.h + hb * Ph.bytes;
-        mx_store_group(v, half, blk + ((int64_t)cm * a.TBh + tt) * 16,
-                       blk + Ph.codes + (int64_t)cm * a.TBh + (tt & 31) * MTh + (tt >> 5), n < a.N);
+        for (int q = 0; q < 4; ++q) {
+          f32x4 bg = {}, bu = {};
+          if constexpr (BIAS) {
+            const int o = o0 + 8 * q + 4 * half;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (a.b0) bg[e] = a.b0[o + e];
+              if (a.b1) bu[e] = a.b1[o + e];
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float g = acc[0][t][4 * q + e], u = acc[MODE][t][4 * q + e];
+            v[4 * q + e] = BIAS ? silu_f(g + bg[e]) * (u + bu[e]) : silu_f(g) * u;
+          }
+        }
+        const int64_t tile = tb * MT + t;                       // of 32 tokens; TBh is 32 or 64
+        const int sub = (int)tile & (MTh - 1);
+        uint8_t* blk = a.h + (tile >> (MTh - 1)) * Ph.bytes;
+        mx_store_group(v, half, blk + (cm * a.TBh + sub * 32 + i) * 16, blk + Ph.codes + cm * a.TBh + i * MTh + sub,
+                       tile * 32 + i < a.N);
       }
     } else {
       const int64_t ld = (int64_t)a.w0.R * B;
@@ -474,7 +530,7 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
             f[4 + e] = __uint_as_float(sw[1]);
           }
           const int o = o0 + 8 * (q + half);
-          if (a.b0) {
+          if constexpr (BIAS) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] += a.b0[o + e];
           }
@@ -490,19 +546,20 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
         }
       }
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      acc[0][t] = f32x16{};
-      if constexpr (MODE == 1) acc[MODE][t] = f32x16{};
-    }
   };
   for (;;) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      if (MODE == 1 && cup) compute(d, acc[MODE], a.w1.K);
-      else compute(d, acc[0], a.w0.K);
+      // a tile's first products add to the constant 0 of the instruction, in code of their own
+      if (MODE == 1 && cup) {
+        if (cj == 0) compute(d, acc[MODE], a.w1.K, true);
+        else compute(d, acc[MODE], a.w1.K, false);
+      } else {
+        if (cj == 0) compute(d, acc[0], a.w0.K, true);
+        else compute(d, acc[0], a.w0.K, false);
+      }
       load(d);
-      if (++cj == (cup ? P1 : P0)) {
+      if (++cj == (MODE == 1 && cup ? P1 : P0)) {
         cj = 0;
         if (MODE == 1 && !cup) cup = 1;
         else {
@@ -514,6 +571,51 @@ __global__ __launch_bounds__(512, 2) void mx_panel_kernel(MxPanelArgs a) {
       }
     }
   }
+}
+
+// Tokens a workgroup holds: the most, up to 64, whose codes and scales fit in LDS (0: none does)
+inline int mx_block_tokens(int F) {
+  for (int TB = 64; TB >= 32; TB /= 2)
+    if (panel_of(F / 32, TB).bytes <= 160 * 1024) return TB;
+  return 0;
+}
+
+template <int B, int MODE, int MT, bool BIAS>
+int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
+  constexpr int NW = MODE == 1 && MT == 2 ? 12 : 16;     // 160 registers of the two accumulators' kernel
+  auto* k = mx_panel_kernel<B, MODE, MT, NW, BIAS>;
+  const int64_t lds = panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
+  const int tiles = a.w0.R * (B / 32);
+  // shares of the output tiles: the fewest rounds of 256 workgroups times tiles a wave, a workgroup's start
+  // counted as one tile
+  a.slices = 1;
+  int64_t least = INT64_MAX;
+  for (int sl = 1; sl <= 32 && sl * NW <= tiles + NW - 1; ++sl) {
+    const int64_t cost = (nb * sl + 255) / 256 * ((tiles + sl * NW - 1) / (sl * NW) + 1);
+    if (cost < least) least = cost, a.slices = sl;
+  }
+  if (nb * a.slices > 0x3fffff) return -1;
+  static std::atomic<uint64_t> done{0};
+  if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), 160 * 1024, done) != 0) return -1;
+  k<<<(unsigned)(nb * a.slices), NW * 64, lds, st>>>(a);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+template <int MODE, bool BIAS>
+int launch_mx_panel_b(int TB, const MxPanelArgs& a, hipStream_t st) {
+  const bool b32 = a.w0.B == 32;
+  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2, BIAS>(a, st) : launch_mx_panel_t<64, MODE, 2, BIAS>(a, st);
+  return b32 ? launch_mx_panel_t<32, MODE, 1, BIAS>(a, st) : launch_mx_panel_t<64, MODE, 1, BIAS>(a, st);
+}
+template <int MODE>
+int launch_mx_panel(int TB, const MxPanelArgs& a, hipStream_t st) {
+  return a.b0 || (MODE == 1 && a.b1) ? launch_mx_panel_b<MODE, true>(TB, a, st) : launch_mx_panel_b<MODE, false>(TB, a, st);
+}
+
+int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* panels, hipStream_t st) {
+  const int64_t waves = (N + 15) / 16 * ((F / 32 + 1) / 2);
+  if (waves > 0x3ffffff) return -1;
+  mx_quantize_panel_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(x, N, F, TB, panels);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 // ------------------------------------------------------------------ few tokens
@@ -657,42 +759,6 @@ int launch_mx_decode(const MxPanelArgs& a, const uint16_t* x, hipStream_t st) {
     if (x) mx_decode_kernel<64, MODE, false><<<grid, 512, 0, st>>>(a, x);
     else mx_decode_kernel<64, MODE, true><<<grid, 512, 0, st>>>(a, x);
   }
-  return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-
-// Tokens a workgroup holds: the most whose codes and scales fit in LDS (0: none does)
-inline int mx_block_tokens(int F) {
-  for (int TB = 128; TB >= 32; TB /= 2)
-    if (panel_of(F / 32, TB).bytes <= 160 * 1024) return TB;
-  return 0;
-}
-
-template <int B, int MODE, int MT>
-int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
-  auto* k = mx_panel_kernel<B, MODE, MT>;
-  const int64_t lds = panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
-  const int tiles = a.w0.R * (B / 32);
-  // shares of the output tiles: enough workgroups for 256 CUs, at least a tile a wave
-  const int64_t want = (256 + nb - 1) / nb, most = (tiles + 7) / 8;
-  a.slices = (int)(want < most ? want : most);
-  if (nb * a.slices > 0x7fffff) return -1;
-  static std::atomic<uint64_t> done{0};
-  if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), 160 * 1024, done) != 0) return -1;
-  k<<<(unsigned)(nb * a.slices), 512, lds, st>>>(a);
-  return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-template <int MODE>
-int launch_mx_panel(int TB, const MxPanelArgs& a, hipStream_t st) {
-  const bool b32 = a.w0.B == 32;
-  if (TB == 128) return b32 ? launch_mx_panel_t<32, MODE, 4>(a, st) : launch_mx_panel_t<64, MODE, 4>(a, st);
-  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2>(a, st) : launch_mx_panel_t<64, MODE, 2>(a, st);
-  return b32 ? launch_mx_panel_t<32, MODE, 1>(a, st) : launch_mx_panel_t<64, MODE, 1>(a, st);
-}
-
-int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* panels, hipStream_t st) {
-  const int64_t waves = (N + 15) / 16 * ((F / 32 + 1) / 2);
-  if (waves > 0x3ffffff) return -1;
-  mx_quantize_panel_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(x, N, F, TB, panels);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
