@@ -781,7 +781,7 @@ int lbk_ternary_check_codes(const uint32_t* words, int64_t n_words, int32_t* bad
 enum { LBK_BF16 = 0, LBK_FP16 = 1, LBK_FP32 = 2 };
 
 /* One Block-ELL weight in 4 bits: groups run along B_in, so B is 32 or 64.
- *   codes  [R, K, B_out, B_in/2], 16-byte aligned;  scales [R, K, B_out, B_in/32]. */
+ *   codes  [R, K, B_out, B_in/2], 16-byte aligned;  scales [R, K, B_out, B_in/32], 2-byte aligned. */
 typedef struct lbk_bell_mx {
     const uint8_t* codes;
     const uint8_t* scales;

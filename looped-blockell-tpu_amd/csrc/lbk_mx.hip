@@ -351,7 +351,8 @@ __global__ __launch_bounds__(256) void mx_rowblock_kernel(MxArgs a) {
 
 // ------------------------------------------------------------------ products on token panels
 struct MxPanelArgs {
-  const uint8_t* x;                         // panels of 32 MT tokens
+  const uint8_t* x;                         // panels of 32 MT tokens, or
+  const uint16_t* xb;                       // (not NULL) bf16 rows [N, F], quantised by the workgroup
   int64_t N;
   int F, slices;
   lbk_bell_mx w0, w1;
@@ -369,7 +370,7 @@ struct MxPanelArgs {
 // MODE 1 is bound by the epilogue's vector work (silu's exp and reciprocal, the maximum and the conversion:
 // about 54 cycles a hidden value and wave, against 16 of the matrix unit at 8 slots), so four waves a SIMD of
 // 64 tokens beat two of 128, whose weights are read half as often.
-template <int B, int MODE, int MT, int NW, bool BIAS>
+template <int B, int MODE, int MT, int NW, bool BIAS, bool FILL>
 __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a) {
   constexpr int TB = 32 * MT, D = 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -383,11 +384,39 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
 
   typedef __attribute__((address_space(3))) unsigned char lds_byte;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
-  const uint8_t* src = a.x + tb * P.bytes + lane * 16;
-  for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_load16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
+  if (FILL) {
+    // 16 tokens and two groups (a 128-byte line of each token) a wave and turn, four lanes a group
+    const int tl = lane >> 2, part = lane & 3, pairs = (G + 1) >> 1;
+#pragma unroll 2
+    for (int v = w; v < 2 * MT * pairs; v += NW) {
+      const int tt = v % (2 * MT) * 16 + tl, g0 = v / (2 * MT) * 2;
+      const int64_t n = min(tb * TB + tt, a.N - 1);
+      const uint16_t* row = a.xb + n * a.F + part * 8;
+      float f[2][8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (g0 + k < G) load8<LBK_BF16>(row + (g0 + k) * 32, f[k]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (g0 + k >= G) break;
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, absbits(f[k][e]));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 1));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 2));
+        const uint32_t b = mx_scale(m);
+        const int at = (g0 + k) * TB;
+        *reinterpret_cast<uint32_t*>(smem + (at + tt) * 16 + part * 4) = mx_code8(f[k], mx_pow2(b));
+        if (part == 0) smem[P.codes + at + (tt & 31) * MT + (tt >> 5)] = (uint8_t)b;
+      }
+    }
+  } else {
+    const uint8_t* src = a.x + tb * P.bytes + lane * 16;
+    for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_load16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
+  }
 
   // a position is QP instructions' slots (STEP each)
-  constexpr int STEP = 64 / B, QP = 2;
+  constexpr int STEP = 64 / B, QP = 2;     // (the scales' and columns' passing on is for two)
   const int P0 = (a.w0.K + STEP * QP - 1) / (STEP * QP), P1 = MODE == 1 ? (a.w1.K + STEP * QP - 1) / (STEP * QP) : 0;
   // loading position, D ahead of the computing one: the row's codes, scales and columns, and this lane's place
   // in a slot's tile; a tile on is NW * 32 / B block rows on
@@ -402,20 +431,27 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
   };
   Row r0 = row_of(a.w0), r1 = MODE == 1 ? row_of(a.w1) : Row{};
   const uint32_t place = (uint32_t)(lm * 32 % B + i) * (B / 32) + (B == 64 ? half : 0);
+  // Every load takes its turn of 16 cycles of the CU's address unit, whatever its size, so one fetches the
+  // position's scales (two bytes a lane: B = 32 the four slots' 128 bytes as they lie, B = 64 both input halves
+  // of the tile's 32 rows of two slots) and one its columns (even lanes those of the first instruction, odd ones
+  // of the second); the lanes pass them on in compute.
   u32x4 wr[D][QP];
-  uint32_t sr[D][QP];
-  int cr[D][QP];
+  uint32_t sr[D];
+  int cr[D];
+  const int odd = lane & 1;
+  const uint32_t splace = B == 32 ? 2 * lane : (uint32_t)(lm * 32 % B + i) * 2;
   auto load = [&](int d) {
     const Row& r = MODE == 1 && lup ? r1 : r0;
     const int K = MODE == 1 && lup ? a.w1.K : a.w0.K;
 #pragma unroll
     for (int p = 0; p < QP; ++p) {
       const uint32_t slot = (uint32_t)min(B == 32 ? 2 * (lj * QP + p) + half : lj * QP + p, K - 1);
-      const uint32_t piece = slot * (B * (B / 32)) + place;
-      wr[d][p] = reinterpret_cast<const u32x4*>(r.c)[piece];
-      sr[d][p] = r.s[piece];
-      cr[d][p] = r.i[slot];
+      wr[d][p] = reinterpret_cast<const u32x4*>(r.c)[slot * (B * (B / 32)) + place];
     }
+    const uint32_t sat = B == 32 ? min((uint32_t)lj * 128 + splace, (uint32_t)K * 32 - 2)
+                                 : (uint32_t)min(lj * QP + half, K - 1) * 128 + splace;
+    sr[d] = *reinterpret_cast<const uint16_t*>(r.s + sat);
+    cr[d] = r.i[min(B == 32 ? lj * 4 + 2 * odd + half : lj * QP + odd, K - 1)];
     if (++lj == (MODE == 1 && lup ? P1 : P0)) {
       lj = 0;
       if (MODE == 1 && !lup) {
@@ -432,7 +468,9 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
   };
 #pragma unroll
   for (int d = 0; d < D; ++d) load(d);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(3 * D * QP) : "memory"); // the panel is in LDS
+  // the panel is in LDS
+  if (FILL) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((QP + 2) * D) : "memory");
   if (m0 >= mEnd) return;
 
   f32x16 acc[MODE + 1][MT] = {};
@@ -443,13 +481,16 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
     uint32_t sa[QP], sb[QP];
     int g[QP];
     bool live[QP], whole = true;
+    const int other = __builtin_amdgcn_mov_dpp(cr[d], 0xb1, 0xf, 0xf, true);      // the neighbouring lane's
+    const int col[QP] = {odd ? other : cr[d], odd ? cr[d] : other};
 #pragma unroll
     for (int p = 0; p < QP; ++p) {
-      live[p] = (B == 64 ? cj * QP + p : 2 * (cj * QP + p) + half) < K && (uint32_t)cr[d][p] < (uint32_t)C;
+      live[p] = (B == 64 ? cj * QP + p : 2 * (cj * QP + p) + half) < K && (uint32_t)col[p] < (uint32_t)C;
       whole &= live[p];
-      g[p] = B == 32 ? cr[d][p] : 2 * cr[d][p] + half;
+      g[p] = B == 32 ? col[p] : 2 * col[p] + half;
       wv[p] = wr[d][p];
-      sa[p] = sr[d][p];
+      const int from = B == 32 ? (2 * p + half) * 16 + (i >> 1) : 32 * p + i;
+      sa[p] = (uint32_t)__builtin_amdgcn_ds_bpermute(from * 4, (int)sr[d]) >> (B == 32 ? 8 * odd : 8 * half);
     }
     const bool dead = __ballot(whole) != ~0ull;
     if (dead) {
@@ -481,6 +522,15 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
       if constexpr (MT == 2) mm(1, std::integral_constant<int, 1>{});
     }
   };
+  // a tile's biases, one a lane (lanes 32 .. 63: up's), loaded with its first position and passed on from there
+  float bias = 0.0f;
+  auto load_bias = [&]() {
+    const float* b = MODE == 1 && half ? a.b1 : a.b0;
+    bias = b ? b[cm * 32 + i] : 0.0f;
+  };
+  auto bias_at = [&](int q, int from) {
+    return __int_as_float(__builtin_amdgcn_ds_bpermute((from + (q & 3) + 8 * (q >> 2) + 4 * half) * 4, __float_as_int(bias)));
+  };
   auto store = [&]() {
     const int o0 = cm * 32;
     if constexpr (MODE == 1) {
@@ -491,21 +541,9 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
       for (int t = 0; t < MT; ++t) {
         float v[16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4 bg = {}, bu = {};
-          if constexpr (BIAS) {
-            const int o = o0 + 8 * q + 4 * half;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (a.b0) bg[e] = a.b0[o + e];
-              if (a.b1) bu[e] = a.b1[o + e];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float g = acc[0][t][4 * q + e], u = acc[MODE][t][4 * q + e];
-            v[4 * q + e] = BIAS ? silu_f(g + bg[e]) * (u + bu[e]) : silu_f(g) * u;
-          }
+        for (int q = 0; q < 16; ++q) {
+          const float g = acc[0][t][q], u = acc[MODE][t][q];
+          v[q] = BIAS ? silu_f(g + bias_at(q, 0)) * (u + bias_at(q, 32)) : silu_f(g) * u;
         }
         const int64_t tile = tb * MT + t;                       // of 32 tokens; TBh is 32 or 64
         const int sub = (int)tile & (MTh - 1);
@@ -532,7 +570,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
           const int o = o0 + 8 * (q + half);
           if constexpr (BIAS) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] += a.b0[o + e];
+            for (int e = 0; e < 8; ++e)
+              f[e] += __int_as_float(__builtin_amdgcn_ds_bpermute((8 * (q + half) + e) * 4, __float_as_int(bias)));
           }
           if (n < a.N) {
             if (a.resid) {
@@ -555,8 +594,12 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
         if (cj == 0) compute(d, acc[MODE], a.w1.K, true);
         else compute(d, acc[MODE], a.w1.K, false);
       } else {
-        if (cj == 0) compute(d, acc[0], a.w0.K, true);
-        else compute(d, acc[0], a.w0.K, false);
+        if (cj == 0) {
+          if constexpr (BIAS) load_bias();
+          compute(d, acc[0], a.w0.K, true);
+        } else {
+          compute(d, acc[0], a.w0.K, false);
+        }
       }
       load(d);
       if (++cj == (MODE == 1 && cup ? P1 : P0)) {
@@ -580,35 +623,47 @@ inline int mx_block_tokens(int F) {
   return 0;
 }
 
-template <int B, int MODE, int MT, bool BIAS>
-int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
-  constexpr int NW = MODE == 1 && MT == 2 ? 12 : 16;     // 160 registers of the two accumulators' kernel
-  auto* k = mx_panel_kernel<B, MODE, MT, NW, BIAS>;
-  const int64_t lds = panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
-  const int tiles = a.w0.R * (B / 32);
-  // shares of the output tiles: the fewest rounds of 256 workgroups times tiles a wave, a workgroup's start
-  // counted as one tile
-  a.slices = 1;
+// Waves of a workgroup, and the shares of the output tiles: the fewest rounds of 256 workgroups times tiles a
+// wave, a workgroup's start counted as one tile
+template <int MODE>
+constexpr int mx_panel_waves(int MT) { return MODE == 1 && MT == 2 ? 12 : 16; }     // registers of two accumulators
+template <int MODE>
+int mx_panel_slices(int64_t N, int TB, int tiles) {
+  const int NW = mx_panel_waves<MODE>(TB / 32);
+  const int64_t nb = (N + TB - 1) / TB;
+  int best = 1;
   int64_t least = INT64_MAX;
   for (int sl = 1; sl <= 32 && sl * NW <= tiles + NW - 1; ++sl) {
     const int64_t cost = (nb * sl + 255) / 256 * ((tiles + sl * NW - 1) / (sl * NW) + 1);
-    if (cost < least) least = cost, a.slices = sl;
+    if (cost < least) least = cost, best = sl;
   }
+  return best;
+}
+
+template <int B, int MODE, int MT, bool BIAS, bool FILL>
+int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
+  constexpr int NW = mx_panel_waves<MODE>(MT);
+  auto* k = mx_panel_kernel<B, MODE, MT, NW, BIAS, FILL>;
+  const int64_t lds = panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
+  a.slices = mx_panel_slices<MODE>(a.N, 32 * MT, a.w0.R * (B / 32));
   if (nb * a.slices > 0x3fffff) return -1;
   static std::atomic<uint64_t> done{0};
   if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), 160 * 1024, done) != 0) return -1;
   k<<<(unsigned)(nb * a.slices), NW * 64, lds, st>>>(a);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
-template <int MODE, bool BIAS>
+template <int MODE, bool BIAS, bool FILL>
 int launch_mx_panel_b(int TB, const MxPanelArgs& a, hipStream_t st) {
   const bool b32 = a.w0.B == 32;
-  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2, BIAS>(a, st) : launch_mx_panel_t<64, MODE, 2, BIAS>(a, st);
-  return b32 ? launch_mx_panel_t<32, MODE, 1, BIAS>(a, st) : launch_mx_panel_t<64, MODE, 1, BIAS>(a, st);
+  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2, BIAS, FILL>(a, st) : launch_mx_panel_t<64, MODE, 2, BIAS, FILL>(a, st);
+  return b32 ? launch_mx_panel_t<32, MODE, 1, BIAS, FILL>(a, st) : launch_mx_panel_t<64, MODE, 1, BIAS, FILL>(a, st);
 }
+// a.x or a.xb given
 template <int MODE>
 int launch_mx_panel(int TB, const MxPanelArgs& a, hipStream_t st) {
-  return a.b0 || (MODE == 1 && a.b1) ? launch_mx_panel_b<MODE, true>(TB, a, st) : launch_mx_panel_b<MODE, false>(TB, a, st);
+  const bool bias = a.b0 || (MODE == 1 && a.b1);
+  if (a.xb) return bias ? launch_mx_panel_b<MODE, true, true>(TB, a, st) : launch_mx_panel_b<MODE, false, true>(TB, a, st);
+  return bias ? launch_mx_panel_b<MODE, true, false>(TB, a, st) : launch_mx_panel_b<MODE, false, false>(TB, a, st);
 }
 
 int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* panels, hipStream_t st) {
@@ -800,6 +855,7 @@ int check_mx(const lbk_bell_mx* w) {
   if ((int64_t)w->R * w->B > 0x7fffffff) return LBK_ERR_SHAPE;
   if ((int64_t)w->R * w->K > 0 && (!w->codes || !w->scales || !w->col_idx)) return LBK_ERR_NULL;
   if (w->codes && !a16(w->codes)) return LBK_ERR_ALIGN;
+  if (w->scales && (reinterpret_cast<uintptr_t>(w->scales) & 1u)) return LBK_ERR_ALIGN;
   return LBK_OK;
 }
 
@@ -867,6 +923,11 @@ int check_ffn_mx(const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_
   return (int64_t)down->R * down->B == d_model ? LBK_OK : LBK_ERR_SHAPE;
 }
 
+// Shares of the output tiles up to which each quantises its tokens itself: one share spares the quantising
+// launch (16384 tokens, 1024 -> 4096: 80 -> 70 us), three redo its work too often (4099 tokens, 2048 / 8192:
+// 89 -> 93 us)
+constexpr int kFillSlices = 2;
+
 // Tokens that mx_decode_kernel takes
 constexpr int64_t kDecode = 32;
 
@@ -885,6 +946,10 @@ FfnTokens ffn_tokens(int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx
 size_t tokens_bytes(int64_t N, int64_t F, int TB) {
   return TB ? (size_t)((N + TB - 1) / TB * panel_of((int)(F / 32), TB).bytes) : quantised_bytes(N, F);
 }
+
+// Whether the panel kernel's workgroups quantise their own tokens: where few of them share a token
+template <int MODE>
+bool fills(int64_t N, int TB, const lbk_bell_mx* w) { return mx_panel_slices<MODE>(N, TB, w->R * (w->B / 32)) <= kFillSlices; }
 
 int quantize_tokens(const uint16_t* x, int64_t N, int F, int TB, void* ws, hipStream_t st) {
   if (TB) return launch_quantize_panel(x, N, F, TB, static_cast<uint8_t*>(ws), st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
@@ -972,6 +1037,11 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
     return launch_mx_decode<0>(a, x, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
   }
   const int TB = in_tokens(in_features, w);
+  if (TB && fills<0>(N, TB, w)) {
+    MxPanelArgs a{};
+    a.xb = x; a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
+    return launch_mx_panel<0>(TB, a, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  }
   if (int st = quantize_tokens(x, N, in_features, TB, workspace, S(stream))) return st;
   return product(workspace, N, in_features, TB, *w, bias, nullptr, y, S(stream));
 }
@@ -1007,10 +1077,12 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
   }
   const FfnTokens t = ffn_tokens(d_model, gate, up, down);
   uint8_t* hp = static_cast<uint8_t*>(workspace) + tokens_bytes(N, d_model, t.x);
-  if (int st = quantize_tokens(x, N, d_model, t.x, workspace, S(stream))) return st;
+  const bool fill = t.x && fills<1>(N, t.x, gate);
+  if (!fill)
+    if (int st = quantize_tokens(x, N, d_model, t.x, workspace, S(stream))) return st;
   if (t.x) {
     MxPanelArgs g{};
-    g.x = static_cast<uint8_t*>(workspace); g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
+    g.x = static_cast<uint8_t*>(workspace); g.xb = fill ? x : nullptr; g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
     g.h = hp; g.TBh = t.h;
     if (launch_mx_panel<1>(t.x, g, S(stream)) != 0) return LBK_ERR_LAUNCH;
   } else {

@@ -89,7 +89,7 @@ void check_mx_tiles(Tensor& c, Tensor& s, const char* op, const char* name) {
                   s.size(3) * 32 == c.size(2),
               "titan::", op, ": ", name, " scales must be [R, K, B, B/32], got ", s.sizes());
   c = dense16(c);
-  s = s.contiguous();
+  s = dense16(s);
 }
 
 Tensor mx_dequantize_tiles(const Tensor& codes_, const Tensor& scales_, at::ScalarType dtype) {
