@@ -17,6 +17,7 @@
 #include "lbk_device.h"
 #include "lbk_internal.h"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace lbk {
@@ -237,17 +238,6 @@ __global__ __launch_bounds__(256) void mx_quantize_panel_kernel(const uint16_t* 
 }
 
 // ------------------------------------------------------------------ products
-struct MxArgs {
-  const uint8_t* xc; const uint8_t* xs;     // quantised tokens [N, F / 2], [N, F / 32]
-  int64_t N;
-  int F;                                    // input features
-  lbk_bell_mx w0, w1;                       // the product's weight, or gate and up
-  const float* b0; const float* b1;
-  const uint16_t* resid;                    // MODE 0, optional [N, R B]
-  uint16_t* y;                              // MODE 0: [N, R B]
-  uint8_t* hc; uint8_t* hs;                 // MODE 1: quantised silu(gate) * up
-};
-
 // Gate/up epilogue: this lane's 16 values of a group of 32 hidden features of one token (features
 // (v % 4) + 8 (v / 4) + 4 half; the partner lane l ^ 32 has the others) -> codes and scale.  The group's
 // maximum and code halves cross by one exchange each; each lane stores 8 of the 16 code bytes.
@@ -282,73 +272,6 @@ __device__ __forceinline__ void mx_store_group(const float (&h)[16], int half, u
   }
 }
 
-// MODE 0: y = Q(x) W (+ bias) (+ resid).  MODE 1: quantised silu(gate + b0) * (up + b1).
-// The general kernel: four waves of 32 tokens share 32 outputs; every operand comes from global memory
-// (L1 and L2).  Any N, K and F.
-template <int B, int MODE>
-__global__ __launch_bounds__(256) void mx_rowblock_kernel(MxArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, i = lane & 31;
-  const int64_t n = ((int64_t)blockIdx.y * 4 + wave) * 32 + i;
-  if (((int64_t)blockIdx.y * 4 + wave) * 32 >= a.N) return;
-  const int64_t nc = n < a.N ? n : a.N - 1;
-  const uint8_t* xc = a.xc + nc * (a.F >> 1);
-  const uint8_t* xs = a.xs + nc * (a.F >> 5);
-  const int o0 = blockIdx.x * 32, r = o0 / B, j = o0 % B + i, C = a.F / B;
-
-  auto product = [&](const lbk_bell_mx& w) {
-    f32x16 acc = {};
-    constexpr int STEP = 64 / B;            // slots of one MFMA
-    for (int k = 0; k < w.K; k += STEP) {
-      const int slot = B == 32 ? k + half : k;
-      const int col = slot < w.K ? w.col_idx[(int64_t)r * w.K + slot] : -1;
-      const bool live = col >= 0 && col < C;
-      u32x4 wa = {}, xb = {};
-      uint32_t sa = 127, sb = 127;          // a dead slot multiplies zeros
-      if (live) {
-        const int64_t at = (((int64_t)r * w.K + slot) * B + j) * (B / 32) + (B == 64 ? half : 0);
-        const int g = B == 32 ? col : 2 * col + half;
-        wa = reinterpret_cast<const u32x4*>(w.codes)[at];
-        sa = w.scales[at];
-        xb = reinterpret_cast<const u32x4*>(xc)[g];
-        sb = xs[g];
-      }
-      acc = mfma_fp4(wa, xb, acc, sa, sb);
-    }
-    return acc;
-  };
-
-  const f32x16 p0 = product(a.w0);
-  float v[16];
-  if constexpr (MODE == 1) {
-    const f32x16 p1 = product(a.w1);
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      const int o = o0 + (q & 3) + 8 * (q >> 2) + 4 * half;
-      const float g = p0[q] + (a.b0 ? a.b0[o] : 0.0f), u = p1[q] + (a.b1 ? a.b1[o] : 0.0f);
-      v[q] = silu_f(g) * u;
-    }
-    const int64_t grp = nc * ((int64_t)a.w0.R * B / 32) + blockIdx.x;
-    mx_store_group(v, half, a.hc + grp * 16, a.hs + grp, n < a.N);
-  } else {
-    if (n >= a.N) return;
-    const int64_t ld = (int64_t)a.w0.R * B;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int o = o0 + 8 * q + 4 * half;
-      float f[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = p0[4 * q + e] + (a.b0 ? a.b0[o + e] : 0.0f);
-      if (a.resid) {
-        float t[4];
-        load_bf16x<4>(a.resid + n * ld + o, t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] += t[e];
-      }
-      store_bf16x<4>(a.y + n * ld + o, f);
-    }
-  }
-}
-
 // ------------------------------------------------------------------ products on token panels
 struct MxPanelArgs {
   const uint8_t* x;                         // panels of 32 MT tokens, or
@@ -370,7 +293,9 @@ struct MxPanelArgs {
 // MODE 1 is bound by the epilogue's vector work (silu's exp and reciprocal, the maximum and the conversion:
 // about 54 cycles a hidden value and wave, against 16 of the matrix unit at 8 slots), so four waves a SIMD of
 // 64 tokens beat two of 128, whose weights are read half as often.
-template <int B, int MODE, int MT, int NW, bool BIAS, bool FILL>
+// FROM: where a workgroup's tokens are: 0 a panel copied to LDS, 1 bf16 rows that it quantises into LDS itself,
+// 2 the panel in global memory (too wide for LDS: 32 lanes read 512 consecutive bytes there too).
+template <int B, int MODE, int MT, int NW, bool BIAS, int FROM>
 __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a) {
   constexpr int TB = 32 * MT, D = 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -384,7 +309,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
 
   typedef __attribute__((address_space(3))) unsigned char lds_byte;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
-  if (FILL) {
+  if constexpr (FROM == 1) {
     // 16 tokens and two groups (a 128-byte line of each token) a wave and turn, four lanes a group
     const int tl = lane >> 2, part = lane & 3, pairs = (G + 1) >> 1;
 #pragma unroll 2
@@ -410,7 +335,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
         if (part == 0) smem[P.codes + at + (tt & 31) * MT + (tt >> 5)] = (uint8_t)b;
       }
     }
-  } else {
+  } else if constexpr (FROM == 0) {
     const uint8_t* src = a.x + tb * P.bytes + lane * 16;
     for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_load16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
   }
@@ -469,12 +394,13 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
 #pragma unroll
   for (int d = 0; d < D; ++d) load(d);
   // the panel is in LDS
-  if (FILL) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((QP + 2) * D) : "memory");
+  if constexpr (FROM == 1) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (FROM == 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((QP + 2) * D) : "memory");
   if (m0 >= mEnd) return;
 
   f32x16 acc[MODE + 1][MT] = {};
-  const unsigned char* xs = smem + P.codes;
+  const unsigned char* const xc = FROM == 2 ? a.x + tb * P.bytes : smem;
+  const unsigned char* const xs = xc + P.codes;
   int cm = m0, cup = 0, cj = 0;
   auto compute = [&](int d, f32x16 (&c)[MT], int K, bool first) {
     u32x4 wv[QP], xv[QP][MT];
@@ -503,7 +429,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
       if constexpr (MT == 2) sb[p] = reinterpret_cast<const uint16_t*>(xs)[g[p] * 32 + i];
       else sb[p] = xs[g[p] * 32 + i];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) xv[p][t] = reinterpret_cast<const u32x4*>(smem)[g[p] * TB + 32 * t + i];
+      for (int t = 0; t < MT; ++t) xv[p][t] = reinterpret_cast<const u32x4*>(xc)[g[p] * TB + 32 * t + i];
     }
     if (dead) {
 #pragma unroll
@@ -616,12 +542,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
   }
 }
 
-// Tokens a workgroup holds: the most, up to 64, whose codes and scales fit in LDS (0: none does)
-inline int mx_block_tokens(int F) {
-  for (int TB = 64; TB >= 32; TB /= 2)
-    if (panel_of(F / 32, TB).bytes <= 160 * 1024) return TB;
-  return 0;
-}
+// Whether the codes and scales of 32 tokens are too wide for LDS, and the tokens of a panel block.  (Tokens of
+// 8192 features read from global memory, 64 at a time, instead of 32 in LDS: 54 -> 51 us at 2048 tokens of
+// 4096 / 8192, but 26 -> 31 at 512 and 48 -> 57 with the four times shorter rows of 2048 / 8192.)
+inline bool mx_wide(int F) { return F > 9600; }
+inline int mx_block_tokens(int F) { return mx_wide(F) || panel_of(F / 32, 64).bytes <= 160 * 1024 ? 64 : 32; }
 
 // Waves of a workgroup, and the shares of the output tiles: the fewest rounds of 256 workgroups times tiles a
 // wave, a workgroup's start counted as one tile
@@ -640,11 +565,11 @@ int mx_panel_slices(int64_t N, int TB, int tiles) {
   return best;
 }
 
-template <int B, int MODE, int MT, bool BIAS, bool FILL>
+template <int B, int MODE, int MT, bool BIAS, int FROM>
 int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
   constexpr int NW = mx_panel_waves<MODE>(MT);
-  auto* k = mx_panel_kernel<B, MODE, MT, NW, BIAS, FILL>;
-  const int64_t lds = panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
+  auto* k = mx_panel_kernel<B, MODE, MT, NW, BIAS, FROM>;
+  const int64_t lds = FROM == 2 ? 0 : panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
   a.slices = mx_panel_slices<MODE>(a.N, 32 * MT, a.w0.R * (B / 32));
   if (nb * a.slices > 0x3fffff) return -1;
   static std::atomic<uint64_t> done{0};
@@ -652,18 +577,21 @@ int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
   k<<<(unsigned)(nb * a.slices), NW * 64, lds, st>>>(a);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
-template <int MODE, bool BIAS, bool FILL>
+template <int MODE, bool BIAS, int FROM>
 int launch_mx_panel_b(int TB, const MxPanelArgs& a, hipStream_t st) {
   const bool b32 = a.w0.B == 32;
-  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2, BIAS, FILL>(a, st) : launch_mx_panel_t<64, MODE, 2, BIAS, FILL>(a, st);
-  return b32 ? launch_mx_panel_t<32, MODE, 1, BIAS, FILL>(a, st) : launch_mx_panel_t<64, MODE, 1, BIAS, FILL>(a, st);
+  if (TB == 64) return b32 ? launch_mx_panel_t<32, MODE, 2, BIAS, FROM>(a, st) : launch_mx_panel_t<64, MODE, 2, BIAS, FROM>(a, st);
+  if constexpr (FROM != 2)
+    return b32 ? launch_mx_panel_t<32, MODE, 1, BIAS, FROM>(a, st) : launch_mx_panel_t<64, MODE, 1, BIAS, FROM>(a, st);
+  return -1;
 }
 // a.x or a.xb given
 template <int MODE>
 int launch_mx_panel(int TB, const MxPanelArgs& a, hipStream_t st) {
   const bool bias = a.b0 || (MODE == 1 && a.b1);
-  if (a.xb) return bias ? launch_mx_panel_b<MODE, true, true>(TB, a, st) : launch_mx_panel_b<MODE, false, true>(TB, a, st);
-  return bias ? launch_mx_panel_b<MODE, true, false>(TB, a, st) : launch_mx_panel_b<MODE, false, false>(TB, a, st);
+  if (mx_wide(a.F)) return bias ? launch_mx_panel_b<MODE, true, 2>(TB, a, st) : launch_mx_panel_b<MODE, false, 2>(TB, a, st);
+  if (a.xb) return bias ? launch_mx_panel_b<MODE, true, 1>(TB, a, st) : launch_mx_panel_b<MODE, false, 1>(TB, a, st);
+  return bias ? launch_mx_panel_b<MODE, true, 0>(TB, a, st) : launch_mx_panel_b<MODE, false, 0>(TB, a, st);
 }
 
 int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* panels, hipStream_t st) {
@@ -805,34 +733,25 @@ __global__ __launch_bounds__(512, 4) void mx_decode_kernel(MxPanelArgs a, const 
 
 // x: bf16 rows, or NULL for a.x's panels
 template <int MODE>
-int launch_mx_decode(const MxPanelArgs& a, const uint16_t* x, hipStream_t st) {
-  const dim3 grid((unsigned)(a.w0.R * (a.w0.B / 32)), (unsigned)((a.N + 31) / 32));
-  if (a.w0.B == 32) {
-    if (x) mx_decode_kernel<32, MODE, false><<<grid, 512, 0, st>>>(a, x);
-    else mx_decode_kernel<32, MODE, true><<<grid, 512, 0, st>>>(a, x);
-  } else {
-    if (x) mx_decode_kernel<64, MODE, false><<<grid, 512, 0, st>>>(a, x);
-    else mx_decode_kernel<64, MODE, true><<<grid, 512, 0, st>>>(a, x);
-  }
-  return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-
-template <int MODE>
-int launch_mx_rowblock(const MxArgs& a, hipStream_t st) {
-  const int B = a.w0.B;
-  const int64_t blocks = (a.N + 127) / 128;
+int launch_mx_decode(const MxPanelArgs& a0, const uint16_t* x0, hipStream_t st) {
+  const int64_t blocks = (a0.N + 31) / 32, O = (int64_t)a0.w0.R * a0.w0.B;
   for (int64_t b0 = 0; b0 < blocks; b0 += 65535) {                // grid.y's limit
-    MxArgs p = a;
-    const int64_t n0 = b0 * 128, F = a.F, O = (int64_t)a.w0.R * B;
-    p.N = a.N - n0 < 65535 * 128 ? a.N - n0 : 65535 * 128;
-    p.xc += n0 * (F >> 1);
-    p.xs += n0 * (F >> 5);
-    if (p.resid) p.resid += n0 * O;
-    if (p.y) p.y += n0 * O;
-    if (p.hc) p.hc += n0 * (O / 2), p.hs += n0 * (O / 32);
-    const dim3 grid((unsigned)(O / 32), (unsigned)((p.N + 127) / 128));
-    if (B == 32) mx_rowblock_kernel<32, MODE><<<grid, 256, 0, st>>>(p);
-    else mx_rowblock_kernel<64, MODE><<<grid, 256, 0, st>>>(p);
+    MxPanelArgs a = a0;
+    const int64_t n0 = b0 * 32;
+    a.N = a0.N - n0 < 65535 * 32 ? a0.N - n0 : 65535 * 32;
+    const uint16_t* x = x0 ? x0 + n0 * a.F : nullptr;
+    if (a.x) a.x += b0 * panel_of(a.F / 32, 32).bytes;
+    if (a.h) a.h += b0 * panel_of((int)(O / 32), 32).bytes;
+    if (a.resid) a.resid += n0 * O;
+    if (a.y) a.y += n0 * O;
+    const dim3 grid((unsigned)(O / 32), (unsigned)((a.N + 31) / 32));
+    if (a.w0.B == 32) {
+      if (x) mx_decode_kernel<32, MODE, false><<<grid, 512, 0, st>>>(a, x);
+      else mx_decode_kernel<32, MODE, true><<<grid, 512, 0, st>>>(a, x);
+    } else {
+      if (x) mx_decode_kernel<64, MODE, false><<<grid, 512, 0, st>>>(a, x);
+      else mx_decode_kernel<64, MODE, true><<<grid, 512, 0, st>>>(a, x);
+    }
   }
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
@@ -847,6 +766,7 @@ inline bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) =
 inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 constexpr int64_t kMaxThreads = 0xffffff00;     // of one launch
+constexpr int64_t kMaxTokens = (int64_t)1 << 27;  // the products' launches, 32 tokens a workgroup
 
 int check_mx(const lbk_bell_mx* w) {
   if (!w) return LBK_ERR_NULL;
@@ -857,17 +777,6 @@ int check_mx(const lbk_bell_mx* w) {
   if (w->codes && !a16(w->codes)) return LBK_ERR_ALIGN;
   if (w->scales && (reinterpret_cast<uintptr_t>(w->scales) & 1u)) return LBK_ERR_ALIGN;
   return LBK_OK;
-}
-
-// codes and scales of [N, F] in a workspace
-struct Quantised {
-  uint8_t* c;
-  uint8_t* s;
-};
-size_t quantised_bytes(int64_t N, int64_t F) { return align256((size_t)N * F / 2) + align256((size_t)N * F / 32); }
-Quantised quantised_at(void* p, int64_t N, int64_t F) {
-  uint8_t* c = static_cast<uint8_t*>(p);
-  return {c, c + align256((size_t)N * F / 2)};
 }
 
 template <template <int> class L, typename... A>
@@ -927,49 +836,22 @@ int check_ffn_mx(const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_
 // launch (16384 tokens, 1024 -> 4096: 80 -> 70 us), three redo its work too often (4099 tokens, 2048 / 8192:
 // 89 -> 93 us)
 constexpr int kFillSlices = 2;
-
-// Tokens that mx_decode_kernel takes
-constexpr int64_t kDecode = 32;
-
-// Tokens of a panel block for a product of these input features, 0: rows of codes (mx_rowblock_kernel,
-// also where a weight has no slots)
-int in_tokens(int64_t F, const lbk_bell_mx* w) { return w->K > 0 ? mx_block_tokens((int)F) : 0; }
-
-// Both products of an FFN read tokens of one kind, so that the gate/up kernel writes what the down one reads
-struct FfnTokens {
-  int x, h;
-};
-FfnTokens ffn_tokens(int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_mx* down) {
-  const FfnTokens t{up->K > 0 ? in_tokens(d_model, gate) : 0, in_tokens((int64_t)gate->R * gate->B, down)};
-  return t.x && t.h ? t : FfnTokens{0, 0};
-}
-size_t tokens_bytes(int64_t N, int64_t F, int TB) {
-  return TB ? (size_t)((N + TB - 1) / TB * panel_of((int)(F / 32), TB).bytes) : quantised_bytes(N, F);
-}
-
-// Whether the panel kernel's workgroups quantise their own tokens: where few of them share a token
 template <int MODE>
-bool fills(int64_t N, int TB, const lbk_bell_mx* w) { return mx_panel_slices<MODE>(N, TB, w->R * (w->B / 32)) <= kFillSlices; }
-
-int quantize_tokens(const uint16_t* x, int64_t N, int F, int TB, void* ws, hipStream_t st) {
-  if (TB) return launch_quantize_panel(x, N, F, TB, static_cast<uint8_t*>(ws), st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
-  const Quantised q = quantised_at(ws, N, F);
-  return lbk_mx_quantize(x, LBK_BF16, N, F, F, q.c, q.s, st);
+bool fills(int64_t N, int F, const lbk_bell_mx* w) {
+  return !mx_wide(F) && mx_panel_slices<MODE>(N, mx_block_tokens(F), w->R * (w->B / 32)) <= kFillSlices;
 }
 
-// y = tokens (quantised as quantize_tokens leaves them) times w
-int product(void* tokens, int64_t N, int F, int TB, const lbk_bell_mx& w, const float* bias, const uint16_t* resid,
-            uint16_t* y, hipStream_t st) {
-  if (TB) {
-    MxPanelArgs a{};
-    a.x = static_cast<uint8_t*>(tokens); a.N = N; a.F = F; a.w0 = w; a.b0 = bias; a.resid = resid; a.y = y;
-    return launch_mx_panel<0>(TB, a, st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
-  }
-  const Quantised q = quantised_at(tokens, N, F);
-  MxArgs a{};
-  a.xc = q.c; a.xs = q.s; a.N = N; a.F = F; a.w0 = w; a.b0 = bias; a.resid = resid; a.y = y;
-  return launch_mx_rowblock<0>(a, st) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+// Tokens up to which mx_decode_kernel takes them.  FFN in us, so / on panels: 4096 / 14336 at 0.1 64 tokens 15 / 35,
+// 128 tokens 22 / 36, 256 tokens 38 / 38; 4096 / 16384 at 0.125 256 tokens 55 / 47; 1024 / 4096 at 1.0 256 tokens
+// 26 / 42.  It also takes weights without slots, at any number.
+constexpr int64_t kDecode = 128;
+bool decodes(int64_t N, std::initializer_list<const lbk_bell_mx*> ws) {
+  bool empty = false;
+  for (const lbk_bell_mx* w : ws) empty |= w->K == 0;
+  return N <= kDecode || empty;
 }
+
+size_t panels_bytes(int64_t N, int64_t F, int TB) { return (size_t)((N + TB - 1) / TB * panel_of((int)(F / 32), TB).bytes); }
 
 }  // namespace
 
@@ -1017,8 +899,8 @@ int lbk_mx_dequantize_tiles(const uint8_t* codes, const uint8_t* scales, int32_t
 }
 
 size_t lbk_mx_matmul_workspace_bytes(int64_t N, int32_t in_features, const lbk_bell_mx* w) {
-  if (!w || N <= kDecode || in_features <= 0) return 0;
-  return tokens_bytes(N, in_features, in_tokens(in_features, w));
+  if (!w || N <= 0 || in_features <= 0 || check_mx(w) || decodes(N, {w}) || fills<0>(N, in_features, w)) return 0;
+  return panels_bytes(N, in_features, mx_block_tokens(in_features));
 }
 
 int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const lbk_bell_mx* w, const float* bias,
@@ -1029,29 +911,31 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
   if (N == 0 || w->R == 0) return LBK_OK;
   if (!x || !y) return LBK_ERR_NULL;
   if (!a16(x) || !a16(y) || !a16(workspace)) return LBK_ERR_ALIGN;
+  if (N > kMaxTokens) return LBK_ERR_TOO_LARGE;
   const size_t need = lbk_mx_matmul_workspace_bytes(N, in_features, w);
   if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
-  if (N <= kDecode) {
-    MxPanelArgs a{};
-    a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
-    return launch_mx_decode<0>(a, x, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
+  MxPanelArgs a{};
+  a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
+  int err;
+  if (decodes(N, {w})) {
+    err = launch_mx_decode<0>(a, x, S(stream));
+  } else {
+    const int TB = mx_block_tokens(in_features);
+    a.x = static_cast<uint8_t*>(workspace);
+    if (fills<0>(N, in_features, w)) a.xb = x;
+    else if (launch_quantize_panel(x, N, in_features, TB, static_cast<uint8_t*>(workspace), S(stream))) return LBK_ERR_LAUNCH;
+    err = launch_mx_panel<0>(TB, a, S(stream));
   }
-  const int TB = in_tokens(in_features, w);
-  if (TB && fills<0>(N, TB, w)) {
-    MxPanelArgs a{};
-    a.xb = x; a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
-    return launch_mx_panel<0>(TB, a, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
-  }
-  if (int st = quantize_tokens(x, N, in_features, TB, workspace, S(stream))) return st;
-  return product(workspace, N, in_features, TB, *w, bias, nullptr, y, S(stream));
+  return err == 0 ? LBK_OK : LBK_ERR_LAUNCH;
 }
 
 size_t lbk_mx_swiglu_workspace_bytes(int64_t N, int32_t d_model, const lbk_bell_mx* gate, const lbk_bell_mx* up,
                                      const lbk_bell_mx* down) {
-  if (!gate || !up || !down || N <= 0 || d_model <= 0) return 0;
-  if (N <= kDecode) return tokens_bytes(N, (int64_t)gate->R * gate->B, 32);
-  const FfnTokens t = ffn_tokens(d_model, gate, up, down);
-  return tokens_bytes(N, d_model, t.x) + tokens_bytes(N, (int64_t)gate->R * gate->B, t.h);
+  if (N <= 0 || check_ffn_mx(gate, up, down, d_model)) return 0;
+  const int d_ff = gate->R * gate->B;
+  if (decodes(N, {gate, up, down})) return panels_bytes(N, d_ff, 32);
+  return (fills<1>(N, d_model, gate) ? 0 : panels_bytes(N, d_model, mx_block_tokens(d_model))) +
+         panels_bytes(N, d_ff, mx_block_tokens(d_ff));
 }
 
 int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const lbk_bell_mx* gate,
@@ -1063,36 +947,31 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
   if (N == 0) return LBK_OK;
   if (!x || !out) return LBK_ERR_NULL;
   if (!a16(x) || !a16(out) || !a16(workspace)) return LBK_ERR_ALIGN;
+  if (N > kMaxTokens) return LBK_ERR_TOO_LARGE;
   const size_t need = lbk_mx_swiglu_workspace_bytes(N, d_model, gate, up, down);
   if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
   const int d_ff = gate->R * gate->B;
-  if (N <= kDecode) {
-    MxPanelArgs g{};
-    g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up; g.h = static_cast<uint8_t*>(workspace);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  MxPanelArgs g{}, d{};
+  g.N = d.N = N; g.F = d_model; d.F = d_ff;
+  g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
+  d.w0 = *down; d.b0 = b_down; d.resid = add_residual ? x : nullptr; d.y = out;
+  if (decodes(N, {gate, up, down})) {
+    g.h = ws; d.x = ws;
     if (launch_mx_decode<1>(g, x, S(stream)) != 0) return LBK_ERR_LAUNCH;
-    MxPanelArgs d{};
-    d.x = static_cast<uint8_t*>(workspace); d.N = N; d.F = d_ff; d.w0 = *down; d.b0 = b_down; d.y = out;
-    d.resid = add_residual ? x : nullptr;
     return launch_mx_decode<0>(d, nullptr, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
   }
-  const FfnTokens t = ffn_tokens(d_model, gate, up, down);
-  uint8_t* hp = static_cast<uint8_t*>(workspace) + tokens_bytes(N, d_model, t.x);
-  const bool fill = t.x && fills<1>(N, t.x, gate);
-  if (!fill)
-    if (int st = quantize_tokens(x, N, d_model, t.x, workspace, S(stream))) return st;
-  if (t.x) {
-    MxPanelArgs g{};
-    g.x = static_cast<uint8_t*>(workspace); g.xb = fill ? x : nullptr; g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
-    g.h = hp; g.TBh = t.h;
-    if (launch_mx_panel<1>(t.x, g, S(stream)) != 0) return LBK_ERR_LAUNCH;
+  const int TBx = mx_block_tokens(d_model), TBh = mx_block_tokens(d_ff);
+  if (fills<1>(N, d_model, gate)) {
+    g.xb = x;
   } else {
-    const Quantised q = quantised_at(workspace, N, d_model), h = quantised_at(hp, N, d_ff);
-    MxArgs g{};
-    g.xc = q.c; g.xs = q.s; g.N = N; g.F = d_model; g.w0 = *gate; g.w1 = *up; g.b0 = b_gate; g.b1 = b_up;
-    g.hc = h.c; g.hs = h.s;
-    if (launch_mx_rowblock<1>(g, S(stream)) != 0) return LBK_ERR_LAUNCH;
+    if (launch_quantize_panel(x, N, d_model, TBx, ws, S(stream)) != 0) return LBK_ERR_LAUNCH;
+    g.x = ws;
+    ws += panels_bytes(N, d_model, TBx);
   }
-  return product(hp, N, d_ff, t.h, *down, b_down, add_residual ? x : nullptr, out, S(stream));
+  g.h = ws; g.TBh = TBh; d.x = ws;
+  if (launch_mx_panel<1>(TBx, g, S(stream)) != 0) return LBK_ERR_LAUNCH;
+  return launch_mx_panel<0>(TBh, d, S(stream)) == 0 ? LBK_OK : LBK_ERR_LAUNCH;
 }
 
 }  // extern "C"

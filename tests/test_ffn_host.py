@@ -37,14 +37,16 @@ def test_mx_validation_codes():
     assert lib.lbk_mx_dequantize_tiles(P, P, 2, 2, 128, 0, P, None) == A.LBK_ERR_TILE
 
     m = lib.lbk_mx_matmul_bf16
-    need = lib.lbk_mx_matmul_workspace_bytes(200, 128, w())
-    assert need > 0 and lib.lbk_mx_matmul_workspace_bytes(0, 128, w()) == 0
+    need = lib.lbk_mx_matmul_workspace_bytes(200, 128, w(R=512))
+    assert need > 0 and lib.lbk_mx_matmul_workspace_bytes(0, 128, w(R=512)) == 0
     assert m(P, 8, 128, w(B=16), None, P, P, need, None) == A.LBK_ERR_TILE
     assert m(P, 8, 100, w(), None, P, P, need, None) == A.LBK_ERR_SHAPE
     assert m(P, 8, 128, w(scales=None), None, P, P, need, None) == A.LBK_ERR_NULL
     assert m(P, 8, 128, w(codes=P + 8), None, P, P, need, None) == A.LBK_ERR_ALIGN
-    assert m(P, 200, 128, w(), None, P, P, need - 1, None) == A.LBK_ERR_WORKSPACE
-    assert m(P, 200, 128, w(), None, P, None, need, None) == A.LBK_ERR_WORKSPACE
+    assert m(P, 8, 128, w(scales=P + 1), None, P, P, need, None) == A.LBK_ERR_ALIGN
+    assert m(P, 1 << 28, 128, w(), None, P, P, 1 << 62, None) == A.LBK_ERR_TOO_LARGE
+    assert m(P, 200, 128, w(R=512), None, P, P, need - 1, None) == A.LBK_ERR_WORKSPACE
+    assert m(P, 200, 128, w(R=512), None, P, None, need, None) == A.LBK_ERR_WORKSPACE
     assert m(P, -1, 128, w(), None, P, P, need, None) == A.LBK_ERR_ARG
     assert m(None, 0, 128, w(), None, None, None, 0, None) == A.LBK_OK
 
