@@ -97,6 +97,11 @@ __device__ __forceinline__ void lds_load16(const void* base, uint32_t off, uint3
                : "memory", "m0");
 }
 
+// The same loads for the kernels of lbk_gated.hip and lbk_mx.hip.  A scalar base that a vector instruction writes
+// (readfirstlane) needs five wait states before them, which the caller leaves.
+__device__ __forceinline__ void lds_fetch16(const void* p, uint32_t lds) { lds_load16(p, lds); }
+__device__ __forceinline__ void lds_fetch16(const void* base, uint32_t off, uint32_t lds) { lds_load16(base, off, lds); }
+
 // Wave-uniform value (forces scalar registers / scalar branches).
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 

@@ -223,6 +223,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
     if constexpr (GATE) sa1 = ptr(p.A[1], ao);
     sb0 = ptr(pr | lv.part ? p.B[1] : p.B[0], bo);
     left = (int)(p.K - k0);
+    asm volatile("s_nop 4" : "+s"(sa0), "+s"(sa1), "+s"(sb0));      // wait states from readfirstlane to a load's base
   };
   auto advance = [&]() {                // behind the stream's end its last K stage is loaded again, for nobody
     ++lt;
@@ -257,9 +258,9 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
     if constexpr (TAIL) {
       const int R = isA ? BM : BN;
       const int k = ks * KS + ((isA ? AMC : BMC) ? (piece * 64 + lane) / (R / 8) : ((lane & 3) ^ f_kc(lane >> 2)) * 8);
-      lds_load16(k < left ? b + off : reinterpret_cast<const char*>(&zero16), at);
+      lds_fetch16(k < left ? b + off : reinterpret_cast<const char*>(&zero16), at);
     } else {
-      lds_load16(b, off, at);
+      lds_fetch16(b, off, at);
     }
   };
 

@@ -337,7 +337,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void mx_panel_kernel(MxPanelArgs a
     }
   } else if constexpr (FROM == 0) {
     const uint8_t* src = a.x + tb * P.bytes + lane * 16;
-    for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_load16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
+    for (int p = w; p < (int)(P.bytes >> 10); p += NW) lds_fetch16(src + (int64_t)p * 1024, lds0 + (uint32_t)p * 1024);
   }
 
   // a position is QP instructions' slots (STEP each)
