@@ -595,8 +595,7 @@ int launch_mx_panel(int TB, const MxPanelArgs& a, hipStream_t st) {
 }
 
 int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* panels, hipStream_t st) {
-  const int64_t waves = (N + 15) / 16 * ((F / 32 + 1) / 2);
-  if (waves > 0x3ffffff) return -1;
+  const int64_t waves = (N + 15) / 16 * ((F / 32 + 1) / 2);      // < 2^26 (too_many)
   mx_quantize_panel_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(x, N, F, TB, panels);
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
@@ -767,12 +766,15 @@ inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 constexpr int64_t kMaxThreads = 0xffffff00;     // of one launch
 constexpr int64_t kMaxTokens = (int64_t)1 << 27;  // the products' launches, 32 tokens a workgroup
+constexpr int32_t kMaxFeatures = 1 << 24;         // and slots of a row: places in a panel and in a row are 32-bit
+// of a product's input: the quantising launch takes 1024 elements a wave
+bool too_many(int64_t N, int32_t F) { return N > kMaxTokens || N > ((int64_t)1 << 35) / F; }
 
 int check_mx(const lbk_bell_mx* w) {
   if (!w) return LBK_ERR_NULL;
   if (w->B != 32 && w->B != 64) return LBK_ERR_TILE;
   if (w->R < 0 || w->K < 0) return LBK_ERR_SHAPE;
-  if ((int64_t)w->R * w->B > 0x7fffffff) return LBK_ERR_SHAPE;
+  if ((int64_t)w->R * w->B > kMaxFeatures || w->K > kMaxFeatures) return LBK_ERR_TOO_LARGE;
   if ((int64_t)w->R * w->K > 0 && (!w->codes || !w->scales || !w->col_idx)) return LBK_ERR_NULL;
   if (w->codes && !a16(w->codes)) return LBK_ERR_ALIGN;
   if (w->scales && (reinterpret_cast<uintptr_t>(w->scales) & 1u)) return LBK_ERR_ALIGN;
@@ -815,13 +817,13 @@ template <int DT> struct DequantizeTiles {
 int check_rows(int32_t dtype, int64_t N, int32_t F) {
   if (dtype < LBK_BF16 || dtype > LBK_FP32 || N < 0) return LBK_ERR_ARG;
   if (F <= 0 || F % 32) return LBK_ERR_SHAPE;
-  if (N > 0 && (N * (int64_t)F) / F != N) return LBK_ERR_TOO_LARGE;
-  return N * (int64_t)F / 8 > kMaxThreads ? LBK_ERR_TOO_LARGE : LBK_OK;
+  return N > kMaxThreads / (F / 8) ? LBK_ERR_TOO_LARGE : LBK_OK;
 }
 int check_tiles(int32_t dtype, int32_t R, int32_t K, int32_t B) {
   if (dtype < LBK_BF16 || dtype > LBK_FP32) return LBK_ERR_ARG;
   if (B != 32 && B != 64) return LBK_ERR_TILE;
-  return R < 0 || K < 0 ? LBK_ERR_SHAPE : LBK_OK;
+  if (R < 0 || K < 0) return LBK_ERR_SHAPE;
+  return (int64_t)R * K > kMaxThreads / (B * (B / 32)) ? LBK_ERR_TOO_LARGE : LBK_OK;
 }
 
 int check_ffn_mx(const lbk_bell_mx* gate, const lbk_bell_mx* up, const lbk_bell_mx* down, int32_t d_model) {
@@ -881,7 +883,6 @@ int lbk_mx_quantize_tiles(const void* values, int32_t dtype, int32_t R, int32_t 
   if (int st = check_tiles(dtype, R, K, B)) return st;
   const int64_t n = (int64_t)R * K * B * (B / 32);
   if (n == 0) return LBK_OK;
-  if (n > kMaxThreads) return LBK_ERR_TOO_LARGE;
   if (!values || !codes || !scales) return LBK_ERR_NULL;
   if (!a16(codes)) return LBK_ERR_ALIGN;
   return by_dtype<QuantizeTiles>(dtype, values, n, (int)B, codes, scales, S(stream));
@@ -892,7 +893,6 @@ int lbk_mx_dequantize_tiles(const uint8_t* codes, const uint8_t* scales, int32_t
   if (int st = check_tiles(dtype, R, K, B)) return st;
   const int64_t n = (int64_t)R * K * B * (B / 32);
   if (n == 0) return LBK_OK;
-  if (n > kMaxThreads) return LBK_ERR_TOO_LARGE;
   if (!codes || !scales || !values) return LBK_ERR_NULL;
   if (!a16(codes)) return LBK_ERR_ALIGN;
   return by_dtype<DequantizeTiles>(dtype, codes, scales, n, (int)B, values, S(stream));
@@ -908,10 +908,11 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
   if (int st = check_mx(w)) return st;
   if (N < 0) return LBK_ERR_ARG;
   if (in_features <= 0 || in_features % w->B) return LBK_ERR_SHAPE;
+  if (in_features > kMaxFeatures) return LBK_ERR_TOO_LARGE;
   if (N == 0 || w->R == 0) return LBK_OK;
   if (!x || !y) return LBK_ERR_NULL;
   if (!a16(x) || !a16(y) || !a16(workspace)) return LBK_ERR_ALIGN;
-  if (N > kMaxTokens) return LBK_ERR_TOO_LARGE;
+  if (too_many(N, in_features)) return LBK_ERR_TOO_LARGE;
   const size_t need = lbk_mx_matmul_workspace_bytes(N, in_features, w);
   if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
   MxPanelArgs a{};
@@ -947,7 +948,7 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
   if (N == 0) return LBK_OK;
   if (!x || !out) return LBK_ERR_NULL;
   if (!a16(x) || !a16(out) || !a16(workspace)) return LBK_ERR_ALIGN;
-  if (N > kMaxTokens) return LBK_ERR_TOO_LARGE;
+  if (too_many(N, d_model)) return LBK_ERR_TOO_LARGE;
   const size_t need = lbk_mx_swiglu_workspace_bytes(N, d_model, gate, up, down);
   if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
   const int d_ff = gate->R * gate->B;

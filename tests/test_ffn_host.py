@@ -62,6 +62,29 @@ def test_mx_validation_codes():
 
 
 @needs_lib
+def test_mx_limits_are_refused_on_the_host():
+    """Places in a panel and in a weight's row are 32-bit numbers, and a launch has a largest grid: sizes beyond
+    are refused by name, none wraps round."""
+    from looped_blockell import abi as A
+    lib = A.load()
+
+    def w(R=4, K=2, B=32):
+        return C.byref(A.BellMx(P, P, P, R, K, B))
+
+    m, big = lib.lbk_mx_matmul_bf16, 1 << 62
+    for F, N, wt in ((1 << 25, 200, w()), (128, 200, w(R=1 << 20)), (128, 200, w(R=1 << 19, B=64)), (128, 200, w(K=1 << 25)),
+                     (1 << 20, 1 << 16, w()), (128, (1 << 27) + 1, w()), (2**31 - 64, 200, w(B=64))):
+        assert m(P, N, F, wt, None, P, P, big, None) == A.LBK_ERR_TOO_LARGE, (F, N)
+    f = lib.lbk_mx_swiglu_fwd_bf16
+    assert f(P, 200, 128, w(R=1 << 21), w(R=1 << 21), w(), None, None, None, 0, P, P, big, None) == A.LBK_ERR_TOO_LARGE
+    assert f(P, 1 << 27, 1024, w(), w(), w(R=32), None, None, None, 0, P, P, big, None) == A.LBK_ERR_TOO_LARGE
+    big_tiles = 2**31 - 1
+    assert lib.lbk_mx_quantize_tiles(P, 0, big_tiles, big_tiles, 64, P, P, None) == A.LBK_ERR_TOO_LARGE
+    assert lib.lbk_mx_dequantize_tiles(P, P, big_tiles, 1 << 30, 32, 0, P, None) == A.LBK_ERR_TOO_LARGE
+    assert lib.lbk_mx_quantize(P, 0, 2**62, 64, 64, P, P, None) == A.LBK_ERR_TOO_LARGE
+
+
+@needs_lib
 def test_gated_validation_codes():
     from looped_blockell import abi as A
     lib = A.load()
