@@ -349,6 +349,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
     const int64_t f0 = done.m0 + (GATE ? wm / 2 : wm) + (AMC ? 16 * (q & 1) + 8 * (q >> 1) : 8 * q);
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
+      __builtin_amdgcn_sched_barrier(0);      // or the columns' loads are gathered, and registers spill
       const int64_t n = done.n0 + wn + 16 * b + i;
       const bool in_n = n < p.N;
       if constexpr (GATE) {
@@ -377,15 +378,14 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
           store8h<H>(p.d0 + at, h);
         }
       } else {
-        // resid, or cg and cu: a column's features first, then what is made of them
+        // cg and cu: a column's features first, then what is made of them
         u32x4 r0[MT / 2], r1[MT / 2];
-        const bool reads = EPI == EPI_GRAD || (EPI == EPI_STORE && p.s0);
 #pragma unroll
         for (int a = 0; a < MT; a += 2) {
           const int64_t f = f0 + a * 16;
-          if (!reads || !in_n || f >= p.M) continue;
+          if (EPI != EPI_GRAD || !in_n || f >= p.M) continue;
           r0[a / 2] = *reinterpret_cast<const u32x4*>(p.s0 + n * p.ldd + f);
-          if constexpr (EPI == EPI_GRAD) r1[a / 2] = *reinterpret_cast<const u32x4*>(p.s1 + n * p.ldd + f);
+          r1[a / 2] = *reinterpret_cast<const u32x4*>(p.s1 + n * p.ldd + f);
         }
 #pragma unroll
         for (int a = 0; a < MT; a += 2) {
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
           } else if constexpr (EPI == EPI_STORE) {
             if (p.s0) {
               float r[8];
-              unpack8h<H>(r0[a / 2], r);
+              unpack8h<H>(*reinterpret_cast<const u32x4*>(p.s0 + at), r);
 #pragma unroll
               for (int e = 0; e < 8; ++e) x[e] += r[e];
             }
@@ -630,10 +630,11 @@ template <bool H, bool AMC, bool BMC, int EPI>
 int launch_gemm(const Gemm& p, int tile, hipStream_t st) {
   // EPI_GRAD's epilogue moves four times the results' bytes: two workgroups a CU hide it better than one of
   // 256 x 256 (16384 x 4096, K 1024: 286 against 381 us)
-  if constexpr (EPI == EPI_GRAD)
+  if (EPI == EPI_GRAD || tile == 128)
     return p.K % BK ? launch_tile<H, AMC, BMC, EPI, 128, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
-  if (p.K % BK) return tile == 256 ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, true>(p, st);
-  return tile == 256 ? launch_tile<H, AMC, BMC, EPI, 256, false>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
+  if constexpr (EPI != EPI_GRAD)
+    return p.K % BK ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 256, false>(p, st);
+  return LBK_ERR_ARG;
 }
 
 // EPI_STORE, whole or in shares of K by way of `part`
