@@ -40,6 +40,20 @@ def test_training(gpu, N, d, ff, dtype, act, residual):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,d,ff", [(1213, 136, 1288), (2304, 1048, 1160), (9001, 264, 2056)])
+def test_many_output_tiles(gpu, N, d, ff, dtype):
+    """More groups of eight columns of output tiles than XCDs, some of them across two; tiles of both sizes, whole
+    and in shares of K, with and without a rest of K: each output tile is made once."""
+    x, w, dy = _make(N, d, ff, dtype, 6, grad=True)
+    out = kernels.gated_ffn(x, *w, add_residual=True)
+    grads = torch.autograd.grad(out, [x, *w], dy)
+    want = ref.gated(x, *w, dy, "silu", True)
+    ref.close(out.detach(), *want["out"])
+    for n, g in zip(NAMES, grads):
+        ref.close(g, *want[n])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("N,d,ff", SIZES + [(2, 2048, 8192), (5, 1024, 4096), (48, 1280, 4480), (4097, 256, 512)])
 def test_inference(gpu, N, d, ff, dtype):
     x, w, _ = _make(N, d, ff, dtype, 1)
