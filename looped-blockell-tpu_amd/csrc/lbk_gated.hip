@@ -382,15 +382,6 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
           store8h<H>(p.d0 + at, h);
         }
       } else {
-        // cg and cu: a column's features first, then what is made of them
-        u32x4 r0[MT / 2], r1[MT / 2];
-#pragma unroll
-        for (int a = 0; a < MT; a += 2) {
-          const int64_t f = f0 + a * 16;
-          if (EPI != EPI_GRAD || !in_n || f >= p.M) continue;
-          r0[a / 2] = *reinterpret_cast<const u32x4*>(p.s0 + n * p.ldd + f);
-          r1[a / 2] = *reinterpret_cast<const u32x4*>(p.s1 + n * p.ldd + f);
-        }
 #pragma unroll
         for (int a = 0; a < MT; a += 2) {
           float x[8];
@@ -416,8 +407,8 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
             store8h<H>((done.part ? p.d1 : p.d0) + at, x);
           } else {
             float dg[8], du[8];
-            unpack8h<H>(r0[a / 2], dg);
-            unpack8h<H>(r1[a / 2], du);
+            unpack8h<H>(*reinterpret_cast<const u32x4*>(p.s0 + at), dg);
+            unpack8h<H>(*reinterpret_cast<const u32x4*>(p.s1 + at), du);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dg[e] *= x[e], du[e] *= x[e];
             store8h<H>(p.d0 + at, dg);
@@ -582,22 +573,25 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 // `splits` shares.  The least of the estimated times in us: a 256 tile takes 1.75 a K stage and 8 more, one to
 // a CU; a 128 tile 0.8 and 4 alone on a CU, 1.15 and 5 beside another; shares write their fp32 sums, and a
 // second launch adds them up.  (Measured: 16384 x 1024, K 4096: 124 us with 256 tiles, 163 with 128 ones;
-// 1024 x 4096, K 16384: 204 us with 128 tiles, 124 and the sums with 256 ones in four shares.)
+// 1024 x 4096, K 16384: 204 us with 128 tiles, 124 and the sums with 256 ones in four shares.)  EPI_GRAD's
+// epilogue moves four times the results' bytes, which a 256 tile does not overlap with products of its own CU
+// (16384 x 4096, K 1024: 241 us with 256 tiles, 257 with 128 ones; 4096 x 4096: 11 us the other way).
 struct Plan {
   int tile, splits;
 };
-Plan plan(int64_t M, int64_t N, int64_t K, int parts, bool gate, bool may_split) {
+Plan plan(int64_t M, int64_t N, int64_t K, int parts, int epi, bool may_split) {
   Plan best{256, 1};
   double least = 1e30;
   const int64_t st = (K + BK - 1) / BK;
   for (int tile : {256, 128}) {
-    const int64_t fm = gate ? tile / 2 : tile, t1 = (M + fm - 1) / fm * ((N + tile - 1) / tile) * parts;
+    const int64_t fm = epi == EPI_GATE ? tile / 2 : tile, t1 = (M + fm - 1) / fm * ((N + tile - 1) / tile) * parts;
     for (int s = 1; s <= 16 && (s == 1 || (may_split && st >= 4 * s)); s *= 2) {
       const int64_t t = t1 * s;
       const double k = (double)((st + s - 1) / s);
       double us;
-      if (tile == 256) us = (double)((t + 255) / 256) * (1.75 * k + 8);
-      else us = t <= 256 ? 0.8 * k + 4 : (double)((t + 511) / 512) * (1.15 * k + 5);
+      const bool grad = epi == EPI_GRAD;
+      if (tile == 256) us = (double)((t + 255) / 256) * (1.75 * k + (grad ? 29 : 8)) + (grad ? 16 : 0);
+      else us = t <= 256 ? 0.8 * k + (grad ? 13 : 4) : (double)((t + 511) / 512) * (1.15 * k + (grad ? 14 : 5));
       if (s > 1) us += 4 + (double)M * N * parts * (8 * s + 2) / 4.5e6;
       if (us < least) least = us, best = {tile, s};
     }
@@ -605,7 +599,7 @@ Plan plan(int64_t M, int64_t N, int64_t K, int parts, bool gate, bool may_split)
   return best;
 }
 size_t part_bytes(int64_t M, int64_t N, int64_t K, int parts) {
-  const Plan p = plan(M, N, K, parts, false, true);
+  const Plan p = plan(M, N, K, parts, EPI_PART, true);
   return p.splits > 1 ? (size_t)M * N * parts * p.splits * 4 : 0;
 }
 
@@ -632,19 +626,14 @@ int launch_tile(const Gemm& p, hipStream_t st) {
 
 template <bool H, bool AMC, bool BMC, int EPI>
 int launch_gemm(const Gemm& p, int tile, hipStream_t st) {
-  // EPI_GRAD's epilogue moves four times the results' bytes: two workgroups a CU hide it better than one of
-  // 256 x 256 (16384 x 4096, K 1024: 286 against 381 us)
-  if (EPI == EPI_GRAD || tile == 128)
-    return p.K % BK ? launch_tile<H, AMC, BMC, EPI, 128, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
-  if constexpr (EPI != EPI_GRAD)
-    return p.K % BK ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 256, false>(p, st);
-  return LBK_ERR_ARG;
+  if (p.K % BK) return tile == 256 ? launch_tile<H, AMC, BMC, EPI, 256, true>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, true>(p, st);
+  return tile == 256 ? launch_tile<H, AMC, BMC, EPI, 256, false>(p, st) : launch_tile<H, AMC, BMC, EPI, 128, false>(p, st);
 }
 
 // EPI_STORE, whole or in shares of K by way of `part`
 template <bool H, bool AMC, bool BMC>
 int store_gemm(Gemm p, float* part, hipStream_t st) {
-  const Plan pl = plan(p.M, p.N, p.K * p.pairs, p.parts, false, part != nullptr);
+  const Plan pl = plan(p.M, p.N, p.K * p.pairs, p.parts, EPI_PART, part != nullptr);
   if (pl.splits == 1) return launch_gemm<H, AMC, BMC, EPI_STORE>(p, pl.tile, st);
   p.splits = pl.splits;
   p.part = part;
@@ -676,7 +665,7 @@ int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* 
   p.act = a.act, p.ldd = a.F;
   p.d0 = static_cast<uint16_t*>(h), p.d1 = static_cast<uint16_t*>(cg), p.d2 = static_cast<uint16_t*>(cu);
   if (int s = skinny(a.N, a.D, a.F) ? launch_skinny<H, true>(p, st)
-                             : launch_gemm<H, false, false, EPI_GATE>(p, plan(p.M, p.N, p.K, 1, true, false).tile, st))
+                             : launch_gemm<H, false, false, EPI_GATE>(p, plan(p.M, p.N, p.K, 1, EPI_GATE, false).tile, st))
     return s;
   Gemm d = operands(a.wd, a.F, h, a.F, a.D, a.N, a.F);
   d.ldd = a.D, d.d0 = static_cast<uint16_t*>(out), d.s0 = residual ? static_cast<const uint16_t*>(x) : nullptr;
@@ -696,7 +685,7 @@ int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* cg,
     p.ldd = a.F;
     p.d0 = static_cast<uint16_t*>(dg), p.d1 = static_cast<uint16_t*>(du);
     p.s0 = static_cast<const uint16_t*>(cg), p.s1 = static_cast<const uint16_t*>(cu);
-    if (int s = launch_gemm<H, true, false, EPI_GRAD>(p, 128, st)) return s;
+    if (int s = launch_gemm<H, true, false, EPI_GRAD>(p, plan(p.M, p.N, p.K, 1, EPI_GRAD, false).tile, st)) return s;
   }
   if (dx) {
     Gemm p = operands(a.wg, a.D, dg, a.F, a.D, a.N, a.F);
