@@ -41,7 +41,7 @@ enum {
     LBK_ERR_LAUNCH = 6,        /* HIP reported an error launching a kernel */
     LBK_ERR_ARG = 7,           /* other invalid argument (N < 0, L < 0, eps < 0 ...) */
     LBK_ERR_COLUMN = 8,        /* reserved: column index >= C found by lbk_check_columns */
-    LBK_ERR_TOO_LARGE = 9      /* the geometry needs more than the no-alloc entry point's fixed scratch */
+    LBK_ERR_TOO_LARGE = 9      /* larger than the entry point takes (no-alloc: than its fixed scratch) */
 };
 
 /* Size of the fixed device scratch array behind lbk_swiglu_fwd_bf16_noalloc (per GPU). */

@@ -488,7 +488,7 @@ def mx_dequantize_tiles(codes, scales, dtype: torch.dtype = torch.bfloat16):
 
 def mx_matmul(x, codes, scales, col_indices, bias=None):
     """x [..., C*B] -> [..., R*B] through a Block-ELL weight in 4 bits (``mx_quantize_tiles``), x
-    quantised in the call, sums in fp32; not differentiable."""
+    (rounded to bf16 if it is of another type) quantised in the call, sums in fp32; not differentiable."""
     _gpu(x, codes, scales, col_indices)
     if x.dim() == 2:
         return ops().block_ell_matmul_mx(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), codes, scales, col_indices,
@@ -500,8 +500,8 @@ def mx_matmul(x, codes, scales, col_indices, bias=None):
 
 def mx_swiglu(x, gate, up, down, add_residual: bool = False, b_gate=None, b_up=None, b_down=None):
     """The SwiGLU FFN on weights in 4 bits: gate, up and down are (codes, scales, col_indices) triples.
-    x and the hidden state ``silu(gate) * up`` (formed in fp32) are quantised in the call; not
-    differentiable."""
+    x (rounded to bf16 if it is of another type) and the hidden state ``silu(gate) * up`` (formed in
+    fp32) are quantised in the call; not differentiable."""
     _gpu(x, gate[0], up[0], down[0])
     if x.dim() == 2 and x.dtype == torch.bfloat16:
         return ops().block_ell_swiglu_fwd_mx(x, *gate, b_gate, *up, b_up, *down, b_down, add_residual)
