@@ -827,18 +827,19 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
  * reference's PyTorch layer (interop/pt_model.py:851-903).
  *
  * With g = x w_gate^T and u = x w_up^T the forward gives h = act(g) u, gate_factor = u act'(g) and
- * up_factor = act(g) [N, d_ff] for the backward, all three or none.  The backward's four gradients are
- * each optional; w_* are the forward's.
+ * up_factor = act(g) for the backward, all three or none.  h is [N, d_ff]; the factors are 3 * N * d_ff
+ * bytes each, fp32 rounded to 24 bits: the upper 2 bytes of all values, then their third bytes.
+ * The backward's four gradients are each optional; w_* are the forward's.
  */
 enum { LBK_SILU = 0, LBK_GELU = 1 };   /* LBK_GELU: the tanh form */
 
 size_t lbk_gated_fwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff, int want_intermediates);
 int lbk_gated_fwd(int32_t dtype, int32_t act, const void* x, int64_t N, int32_t d_model, int32_t d_ff,
                   const void* w_gate, const void* w_up, const void* w_down, int add_residual, void* out, void* h_out,
-                  void* gate_factor_out, void* up_factor_out, void* workspace, size_t workspace_bytes, void* stream);
+                  uint8_t* gate_factor_out, uint8_t* up_factor_out, void* workspace, size_t workspace_bytes, void* stream);
 size_t lbk_gated_bwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff);
-int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const void* gate_factor,
-                  const void* up_factor, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
+int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const uint8_t* gate_factor,
+                  const uint8_t* up_factor, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
                   const void* w_up, const void* w_down, int add_residual, void* dx, void* dw_gate, void* dw_up,
                   void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -6,10 +6,9 @@
 //             cg = u act'(g), cu = act(g);  out = h Wd^T (+ x)
 //   backward  dh = dy Wd with dg = dh cg, du = dh cu in the epilogue;
 //             dx = dg Wg + du Wu (+ dy) as one product over both;  dWg = dg^T x, dWu = du^T x, dWd = dy^T h
-// h, dg and du are rounded to the inputs' type between the products (they are the matrix instructions'
-// operands), and so are cg and cu, which the forward makes from fp32 values: kept in 32 bits they would add
-// 268 MB to a step of 16384 tokens and 4096 hidden features.  Kept in place of g and u they cost the same bytes
-// and spare the backward's epilogue the activation.  Sums are fp32.
+// h, dg and du are rounded to the inputs' type between the products: they are the matrix instructions' operands.
+// cg and cu, which the forward makes from fp32 values, are kept in 24 bits.  In place of g and u they spare the
+// backward's epilogue the activation.  Sums are fp32.
 #include "lbk.h"
 #include "lbk_device.h"
 #include "lbk_internal.h"
@@ -55,14 +54,52 @@ template <bool H>
 __device__ __forceinline__ void store4h(uint16_t* p, const float (&f)[4]) {
   *reinterpret_cast<u32x2*>(p) = u32x2{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3])};
 }
-// STREAM: results that nobody reads before the backward go past the caches, which keep h for the next product
-// (a training step of 16384 tokens, 1024 / 4096: 1285 -> 1263 us; dg and du, which the next products read, lose
-// by it: 1263 -> 1308).
-template <bool H, bool STREAM = false>
+template <bool H>
 __device__ __forceinline__ void store8h(uint16_t* p, const float (&f)[8]) {
-  const u32x4 v = {Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3]), Half<H>::pack2(f[4], f[5]), Half<H>::pack2(f[6], f[7])};
-  if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));
-  else *reinterpret_cast<u32x4*>(p) = v;
+  *reinterpret_cast<u32x4*>(p) =
+      u32x4{Half<H>::pack2(f[0], f[1]), Half<H>::pack2(f[2], f[3]), Half<H>::pack2(f[4], f[5]), Half<H>::pack2(f[6], f[7])};
+}
+
+// The factors that the forward keeps: fp32 rounded to 24 bits (sign, 8 bits of exponent, 15 of mantissa), the
+// upper 2 bytes of all in one plane and the third bytes, `third` bytes on, in another.  In 16 bits they left the
+// gradients 1.7 times as far off as the rounding of the results alone does, so 1.4 times (what is left is dg's and
+// du's); a training step of 16384 tokens, 1024 / 4096, costs 4 % more by it, one of 4096 tokens 11 %.  One
+// plane of 3-byte groups (24 bytes a lane) was much worse: 1560 against 1265 us.
+// A factor is read by the backward only, and its larger plane goes past the caches, which keep h for the next
+// product (1286 -> 1265 us; the third bytes lose by it: 1265 -> 1286, and so do dg and du, which the next products
+// read).
+__device__ __forceinline__ void store_factor8(uint8_t* p, int64_t third, const float (&f)[8]) {
+  uint32_t b[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) b[k] = __float_as_uint(f[k]) + 0x80u;
+  u32x4 hi;
+  uint32_t t[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    hi[k] = __builtin_amdgcn_perm(b[2 * k + 1], b[2 * k], 0x07060302u);
+    t[k] = __builtin_amdgcn_perm(b[2 * k + 1], b[2 * k], 0x0c0c0501u);
+  }
+  __builtin_nontemporal_store(hi, reinterpret_cast<u32x4*>(p));
+  *reinterpret_cast<u32x2*>(p + third) = u32x2{t[0] | t[1] << 16, t[2] | t[3] << 16};
+}
+__device__ __forceinline__ void store_factor4(uint8_t* p, int64_t third, const float (&f)[4]) {
+  uint32_t b[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(f[k]) + 0x80u;
+  *reinterpret_cast<u32x2*>(p) =
+      u32x2{__builtin_amdgcn_perm(b[1], b[0], 0x07060302u), __builtin_amdgcn_perm(b[3], b[2], 0x07060302u)};
+  *reinterpret_cast<uint32_t*>(p + third) =
+      __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0501u) | __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0501u) << 16;
+}
+__device__ __forceinline__ void load_factor8(const uint8_t* p, int64_t third, float (&f)[8]) {
+  const u32x4 hi = *reinterpret_cast<const u32x4*>(p);
+  const u32x2 lo = *reinterpret_cast<const u32x2*>(p + third);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t j = 2 * (k & 1), l = lo[k >> 1];      // zero, the third byte, the upper half
+    f[2 * k] = __uint_as_float(__builtin_amdgcn_perm(hi[k], l, 0x0504000cu | j << 8));
+    f[2 * k + 1] = __uint_as_float(__builtin_amdgcn_perm(hi[k], l, 0x0706000cu | (j + 1) << 8));
+  }
 }
 
 // sixteen zero bytes that out-of-range pieces of a tile are loaded from
@@ -98,8 +135,9 @@ struct Gemm {
   int parts;                 // 2: two products of one A, with B[0] and B[1], results d0 and d1 (or both in part)
   int splits;                // shares of K (EPI_PART)
   int act;
-  uint16_t* d0; uint16_t* d1; uint16_t* d2;   // STORE: D | GATE: h, cg, cu | GRAD: dg, du
-  const uint16_t* s0; const uint16_t* s1;     // STORE: resid | GRAD: cg, cu
+  uint16_t* d0; uint16_t* d1;                 // STORE: D of each part | GATE: h | GRAD: dg, du
+  uint8_t* c0; uint8_t* c1;                   // GATE (or NULL), GRAD: cg, cu
+  const uint16_t* s0;                         // STORE: resid, or NULL
   float* part;
   int64_t ldd;
 };
@@ -360,10 +398,10 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
         if (!in_n) continue;
 #pragma unroll
         for (int a = 0; a < MT; a += 4) {
-          const int64_t f = f0 + a * 8, at = n * p.ldd + f;
+          const int64_t f = f0 + a * 8, at = n * p.ldd + f, third = 2 * p.N * p.ldd - at;
           if (f >= p.M) continue;
           float h[8], cg[8], cu[8];
-          if (p.d1) {
+          if (p.c0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float g = acc[a + (e >> 2)][b][e & 3], u = acc[a + 2 + (e >> 2)][b][e & 3];
@@ -372,8 +410,8 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
               h[e] = cu[e] * u;
               cg[e] = u * d;
             }
-            store8h<H, true>(p.d1 + at, cg);
-            store8h<H, true>(p.d2 + at, cu);
+            store_factor8(p.c0 + 2 * at, third, cg);
+            store_factor8(p.c1 + 2 * at, third, cu);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -391,7 +429,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = acc[a + (e >> 2)][b][e & 3];
           }
-          const int64_t f = f0 + a * 16, at = n * p.ldd + f;
+          const int64_t f = f0 + a * 16, at = n * p.ldd + f, third = 2 * p.N * p.ldd - at;
           if (!in_n || f >= p.M) continue;
           if constexpr (EPI == EPI_PART) {
             float* d = p.part + (int64_t)(done.split * p.parts + done.part) * p.N * p.ldd + at;
@@ -407,8 +445,8 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
             store8h<H>((done.part ? p.d1 : p.d0) + at, x);
           } else {
             float dg[8], du[8];
-            unpack8h<H>(*reinterpret_cast<const u32x4*>(p.s0 + at), dg);
-            unpack8h<H>(*reinterpret_cast<const u32x4*>(p.s1 + at), du);
+            load_factor8(p.c0 + 2 * at, third, dg);
+            load_factor8(p.c1 + 2 * at, third, du);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dg[e] *= x[e], du[e] *= x[e];
             store8h<H>(p.d0 + at, dg);
@@ -512,9 +550,9 @@ __global__ __launch_bounds__(NW * 64) void skinny_kernel(Gemm p) {
       cg[e] = v[1][e] * d;
       x[e] = cu[e] * v[1][e];
     }
-    if (p.d1) {
-      store4h<H>(p.d1 + at, cg);
-      store4h<H>(p.d2 + at, cu);
+    if (p.c0) {
+      store_factor4(p.c0 + 2 * at, 2 * p.N * p.ldd - at, cg);
+      store_factor4(p.c1 + 2 * at, 2 * p.N * p.ldd - at, cu);
     }
   } else if (p.s0) {
     const u32x2 t = *reinterpret_cast<const u32x2*>(p.s0 + at);
@@ -659,11 +697,12 @@ struct GatedArgs {
 };
 
 template <bool H>
-int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* h, void* cg, void* cu, float* part, hipStream_t st) {
+int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* h, uint8_t* cg, uint8_t* cu, float* part,
+              hipStream_t st) {
   Gemm p = operands(a.wg, a.D, x, a.D, a.F, a.N, a.D);
   p.A[1] = static_cast<const uint16_t*>(a.wu);
   p.act = a.act, p.ldd = a.F;
-  p.d0 = static_cast<uint16_t*>(h), p.d1 = static_cast<uint16_t*>(cg), p.d2 = static_cast<uint16_t*>(cu);
+  p.d0 = static_cast<uint16_t*>(h), p.c0 = cg, p.c1 = cu;
   if (int s = skinny(a.N, a.D, a.F) ? launch_skinny<H, true>(p, st)
                              : launch_gemm<H, false, false, EPI_GATE>(p, plan(p.M, p.N, p.K, 1, EPI_GATE, false).tile, st))
     return s;
@@ -673,7 +712,7 @@ int gated_fwd(const GatedArgs& a, const void* x, int residual, void* out, void* 
 }
 
 template <bool H>
-int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* cg, const void* cu, const void* h, int residual,
+int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const uint8_t* cg, const uint8_t* cu, const void* h, int residual,
               void* dx, void* dwg, void* dwu, void* dwd, void* dg, void* du, float* part, hipStream_t st) {
   if (a.N == 0) {
     for (void* d : {dwg, dwu, dwd})
@@ -684,7 +723,7 @@ int gated_bwd(const GatedArgs& a, const void* dy, const void* x, const void* cg,
     Gemm p = operands(a.wd, a.F, dy, a.D, a.F, a.N, a.D);
     p.ldd = a.F;
     p.d0 = static_cast<uint16_t*>(dg), p.d1 = static_cast<uint16_t*>(du);
-    p.s0 = static_cast<const uint16_t*>(cg), p.s1 = static_cast<const uint16_t*>(cu);
+    p.c0 = const_cast<uint8_t*>(cg), p.c1 = const_cast<uint8_t*>(cu);      // read
     if (int s = launch_gemm<H, true, false, EPI_GRAD>(p, plan(p.M, p.N, p.K, 1, EPI_GRAD, false).tile, st)) return s;
   }
   if (dx) {
@@ -733,7 +772,7 @@ size_t lbk_gated_fwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff, i
 
 int lbk_gated_fwd(int32_t dtype, int32_t act, const void* x, int64_t N, int32_t d_model, int32_t d_ff,
                   const void* w_gate, const void* w_up, const void* w_down, int add_residual, void* out, void* h_out,
-                  void* gate_factor_out, void* up_factor_out, void* workspace, size_t workspace_bytes, void* stream) {
+                  uint8_t* gate_factor_out, uint8_t* up_factor_out, void* workspace, size_t workspace_bytes, void* stream) {
   if (int st = check_gated(dtype, act, N, d_model, d_ff)) return st;
   if (N == 0) return LBK_OK;
   if (!x || !w_gate || !w_up || !w_down || !out) return LBK_ERR_NULL;
@@ -760,14 +799,14 @@ size_t lbk_gated_bwd_workspace_bytes(int64_t N, int32_t d_model, int32_t d_ff) {
   return 2 * align256((size_t)N * d_ff * 2) + *std::max_element(parts, parts + 4);
 }
 
-int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const void* gate_factor,
-                  const void* up_factor, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
+int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const uint8_t* gate_factor,
+                  const uint8_t* up_factor, const void* h, int64_t N, int32_t d_model, int32_t d_ff, const void* w_gate,
                   const void* w_up, const void* w_down, int add_residual, void* dx, void* dw_gate, void* dw_up,
                   void* dw_down, void* workspace, size_t workspace_bytes, void* stream) {
   if (int st = check_gated(dtype, LBK_SILU, N, d_model, d_ff)) return st;
   if (!w_gate || !w_up || !w_down) return LBK_ERR_NULL;
   if (N > 0 && (!grad_out || !x || !gate_factor || !up_factor || !h)) return LBK_ERR_NULL;
-  for (const void* p : {grad_out, x, gate_factor, up_factor, h, w_gate, w_up, w_down, (const void*)dx, (const void*)dw_gate,
+  for (const void* p : {grad_out, x, (const void*)gate_factor, (const void*)up_factor, h, w_gate, w_up, w_down, (const void*)dx, (const void*)dw_gate,
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!a16(p)) return LBK_ERR_ALIGN;
   const size_t need = lbk_gated_bwd_workspace_bytes(N, d_model, d_ff);

@@ -202,14 +202,14 @@ Four gated_fwd_impl(const Tensor& x_, const Tensor& wg, const Tensor& wu, const 
   Tensor out = at::empty({a.N, a.D}, a.x.options()), h, g, u;
   if (train) {
     h = at::empty({a.N, a.F}, a.x.options());
-    g = at::empty({a.N, a.F}, a.x.options());
-    u = at::empty({a.N, a.F}, a.x.options());
+    g = at::empty({a.N, 3 * a.F}, a.x.options().dtype(at::kByte));
+    u = at::empty({a.N, 3 * a.F}, g.options());
   }
   const size_t wsb = lbk_gated_fwd_workspace_bytes(a.N, (int32_t)a.D, (int32_t)a.F, train ? 1 : 0);
   Tensor ws = wsb ? workspace(wsb, a.x) : Tensor();
   const int st = lbk_gated_fwd(a.dt, a.act, a.x.data_ptr(), a.N, (int32_t)a.D, (int32_t)a.F, a.wg.data_ptr(), a.wu.data_ptr(),
                                a.wd.data_ptr(), add_residual ? 1 : 0, out.data_ptr(), train ? h.data_ptr() : nullptr,
-                               train ? g.data_ptr() : nullptr, train ? u.data_ptr() : nullptr, wsb ? ws.data_ptr() : nullptr,
+                               train ? g.data_ptr<uint8_t>() : nullptr, train ? u.data_ptr<uint8_t>() : nullptr, wsb ? ws.data_ptr() : nullptr,
                                wsb, cur_stream(a.x));
   TORCH_CHECK(st == LBK_OK, "titan::", op, ": ", lbk_status_string(st), " (status ", st, ")");
   return {out, h, g, u};
@@ -219,7 +219,7 @@ Tensor gated_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
   return std::get<0>(gated_fwd_impl(x, wg, wu, wd, act, add_residual, false, "gated_ffn_fwd"));
 }
 
-// (out, h, u act'(g), act(g))
+// (out, h, u act'(g), act(g)), the factors in 24 bits (include/lbk.h)
 Four gated_fwd_train(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, c10::string_view act,
                      bool add_residual) {
   return gated_fwd_impl(x, wg, wu, wd, act, add_residual, true, "gated_ffn_fwd_train");
@@ -235,10 +235,11 @@ Four gated_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& g_, const Tens
   const std::pair<const Tensor*, const char*> ts[] = {{&dy_, "grad_out"}, {&g_, "gate_factor"}, {&u_, "up_factor"}, {&h_, "h"}};
   for (const auto& [t, name] : ts) {
     check_with(*t, x_, op, name);
-    TORCH_CHECK(t->scalar_type() == x_.scalar_type() && t->dim() == 2 && t->size(0) == a.N &&
-                    t->size(1) == (t == &dy_ ? a.D : a.F),
-                "titan::", op, ": ", name, " must be ", x_.scalar_type(), " [", a.N, ", ", t == &dy_ ? a.D : a.F, "], got ",
-                t->scalar_type(), " ", t->sizes());
+    const bool factor = t == &g_ || t == &u_;
+    const auto type = factor ? at::kByte : x_.scalar_type();
+    const int64_t cols = factor ? 3 * a.F : t == &dy_ ? a.D : a.F;
+    TORCH_CHECK(t->scalar_type() == type && t->dim() == 2 && t->size(0) == a.N && t->size(1) == cols, "titan::", op, ": ", name,
+                " must be ", type, " [", a.N, ", ", cols, "], got ", t->scalar_type(), " ", t->sizes());
   }
   const Tensor dy = dense16(dy_), g = dense16(g_), u = dense16(u_), h = dense16(h_);
   Tensor r[4];
@@ -251,7 +252,7 @@ Four gated_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& g_, const Tens
   const size_t wsb = lbk_gated_bwd_workspace_bytes(a.N, (int32_t)a.D, (int32_t)a.F);
   Tensor ws = workspace(wsb, a.x);
   LBK_CALL("gated_ffn_bwd",
-           lbk_gated_bwd(a.dt, dy.data_ptr(), a.x.data_ptr(), g.data_ptr(), u.data_ptr(), h.data_ptr(), a.N, (int32_t)a.D,
+           lbk_gated_bwd(a.dt, dy.data_ptr(), a.x.data_ptr(), g.data_ptr<uint8_t>(), u.data_ptr<uint8_t>(), h.data_ptr(), a.N, (int32_t)a.D,
                          (int32_t)a.F, a.wg.data_ptr(), a.wu.data_ptr(), a.wd.data_ptr(), add_residual ? 1 : 0, p[0], p[1],
                          p[2], p[3], ws.data_ptr(), wsb, cur_stream(a.x)));
   return {r[0], r[1], r[2], r[3]};
@@ -375,8 +376,8 @@ TORCH_LIBRARY_IMPL(titan, Meta, m) {
   m.impl("gated_ffn_fwd", like_x);
   m.impl("gated_ffn_train", like_x);
   m.impl("gated_ffn_fwd_train", [](const Tensor& x, const Tensor& wg, const Tensor&, const Tensor&, c10::string_view, bool) {
-    auto act = [&]() { return at::empty({x.size(0), wg.size(0)}, x.options()); };
-    return std::make_tuple(at::empty_like(x), act(), act(), act());
+    auto factor = [&]() { return at::empty({x.size(0), 3 * wg.size(0)}, x.options().dtype(at::kByte)); };
+    return std::make_tuple(at::empty_like(x), at::empty({x.size(0), wg.size(0)}, x.options()), factor(), factor());
   });
   m.impl("gated_ffn_bwd", [](const Tensor&, const Tensor& x, const Tensor&, const Tensor&, const Tensor&, const Tensor& wg,
                              const Tensor& wu, const Tensor& wd, bool, std::array<bool, 4> want) {

@@ -144,8 +144,8 @@ def act_eval(z, a):
 
 def gated(x, wg, wu, wd, dy, kind, residual):
     """{name: (value, bound)} of the forward, and with dy of the four gradients, from float64 copies of the
-    inputs.  The bounds count 32-bit sums and one rounding to the inputs' type of each of h, dg, du and
-    of the factors u act'(g) and act(g) that the forward keeps; the last rounding of a result is `close`'s."""
+    inputs.  The bounds count 32-bit sums and one rounding to the inputs' type of each of h, dg and du,
+    and to 24 bits (a half step of 2^-16) of the factors u act'(g) and act(g) that the forward keeps; the last rounding of a result is `close`'s."""
     hs = HALF_STEP[x.dtype]
     dt = x.dtype
     # a rounding near or below the subnormals is off by at most half their step instead
@@ -183,8 +183,9 @@ def gated(x, wg, wu, wd, dy, kind, residual):
         return full - (p * q).abs() + 2 * U32 * full
 
     ecg = times(u, eu, da, dd * eg + act_eval(g, da))
-    ecg = ecg * (1 + hs) + hs * (u * da).abs() + sub
-    ecu = ea * (1 + hs) + hs * a.abs() + sub
+    hf = 2.0 ** -16
+    ecg = ecg * (1 + hf) + hf * (u * da).abs()
+    ecu = ea * (1 + hf) + hf * a.abs()
     edg, edu = times(dh, edh, u * da, ecg), times(dh, edh, a, ecu)
     edg = edg * (1 + hs) + hs * dg.abs() + sub
     edu = edu * (1 + hs) + hs * du.abs() + sub

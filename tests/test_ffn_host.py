@@ -131,7 +131,7 @@ def test_shape_functions():
     x, w = e(7, 64), (e(128, 64), e(128, 64), e(64, 128))
     assert kernels.gated_ffn(x, *w).shape == (7, 64)
     out, h, g, u = o.gated_ffn_fwd_train(x, *w, "gelu", True)
-    assert h.shape == g.shape == u.shape == (7, 128)
+    assert h.shape == (7, 128) and g.shape == u.shape == (7, 384) and g.dtype == u.dtype == torch.uint8
     r = o.gated_ffn_bwd(out, x, g, u, h, *w, True, [True, False, True, True])
     assert [tuple(t.shape) for t in r] == [(7, 64), (0,), (128, 64), (64, 128)]
 
