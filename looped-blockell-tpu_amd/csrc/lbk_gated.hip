@@ -91,9 +91,16 @@ __device__ __forceinline__ void store_factor4(uint8_t* p, int64_t third, const f
   *reinterpret_cast<uint32_t*>(p + third) =
       __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0501u) | __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0501u) << 16;
 }
-__device__ __forceinline__ void load_factor8(const uint8_t* p, int64_t third, float (&f)[8]) {
-  const u32x4 hi = *reinterpret_cast<const u32x4*>(p);
-  const u32x2 lo = *reinterpret_cast<const u32x2*>(p + third);
+struct Factor8 {
+  u32x4 hi;
+  u32x2 lo;
+};
+__device__ __forceinline__ Factor8 load_factor8(const uint8_t* p, int64_t third) {
+  return {*reinterpret_cast<const u32x4*>(p), *reinterpret_cast<const u32x2*>(p + third)};
+}
+__device__ __forceinline__ void unpack_factor8(const Factor8& v, float (&f)[8]) {
+  const u32x4& hi = v.hi;
+  const u32x2& lo = v.lo;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const uint32_t j = 2 * (k & 1), l = lo[k >> 1];      // zero, the third byte, the upper half
@@ -420,8 +427,20 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
           store8h<H>(p.d0 + at, h);
         }
       } else {
+        constexpr int AHEAD = EPI == EPI_GRAD ? 2 : 1;
+        Factor8 r0[AHEAD], r1[AHEAD];
 #pragma unroll
         for (int a = 0; a < MT; a += 2) {
+          // the factors of two groups together, ahead of the stores that loads wait behind (16384 x 4096, K 1024: 303 ->
+          // 281 us; of four, with spilled registers, 343)
+          if (EPI == EPI_GRAD && a / 2 % AHEAD == 0) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+              const int64_t at = min(n, p.N - 1) * p.ldd + min(f0 + (a + 2 * k) * 16, p.M - 8), third = 2 * p.N * p.ldd - at;
+              r0[k] = load_factor8(p.c0 + 2 * at, third);
+              r1[k] = load_factor8(p.c1 + 2 * at, third);
+            }
+          }
           float x[8];
           if constexpr (AMC) {
             pair_rows(acc[a][b], acc[a + 1][b], x);       // all lanes take part
@@ -429,7 +448,7 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = acc[a + (e >> 2)][b][e & 3];
           }
-          const int64_t f = f0 + a * 16, at = n * p.ldd + f, third = 2 * p.N * p.ldd - at;
+          const int64_t f = f0 + a * 16, at = n * p.ldd + f;
           if (!in_n || f >= p.M) continue;
           if constexpr (EPI == EPI_PART) {
             float* d = p.part + (int64_t)(done.split * p.parts + done.part) * p.N * p.ldd + at;
@@ -445,8 +464,8 @@ __global__ __launch_bounds__(TILE * 2, 2) void gemm_kernel(Gemm p) {
             store8h<H>((done.part ? p.d1 : p.d0) + at, x);
           } else {
             float dg[8], du[8];
-            load_factor8(p.c0 + 2 * at, third, dg);
-            load_factor8(p.c1 + 2 * at, third, du);
+            unpack_factor8(r0[a / 2 % AHEAD], dg);
+            unpack_factor8(r1[a / 2 % AHEAD], du);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dg[e] *= x[e], du[e] *= x[e];
             store8h<H>(p.d0 + at, dg);
@@ -612,8 +631,8 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 // a CU; a 128 tile 0.8 and 4 alone on a CU, 1.15 and 5 beside another; shares write their fp32 sums, and a
 // second launch adds them up.  (Measured: 16384 x 1024, K 4096: 124 us with 256 tiles, 163 with 128 ones;
 // 1024 x 4096, K 16384: 204 us with 128 tiles, 124 and the sums with 256 ones in four shares.)  EPI_GRAD's
-// epilogue moves four times the results' bytes, which a 256 tile does not overlap with products of its own CU
-// (16384 x 4096, K 1024: 241 us with 256 tiles, 257 with 128 ones; 4096 x 4096: 11 us the other way).
+// epilogue moves five times the results' bytes, which a 256 tile does not overlap with products of its own CU
+// (16384 x 4096, K 1024: 293 us with 256 tiles, 301 with 128 ones; a training step of 4096 tokens: 429 and 422).
 struct Plan {
   int tile, splits;
 };
