@@ -150,3 +150,39 @@ def test_refusals(gpu):
     g = torch.autograd.grad(kernels.gated_ffn(x, *w), x, dy, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("N", [1, 40])
+def test_factors_beyond_the_inputs_type(gpu, N):
+    """fp16: u act'(g) passes the type's largest value where the gradients do not; the factors hold it."""
+    d, ff = 8, 64
+    x = torch.full((N, d), 200.0, device="cuda", dtype=torch.float16)
+    x[1:] = 0                                              # the weight gradients are one token's
+    w = [torch.zeros(ff, d, device="cuda", dtype=torch.float16), torch.full((ff, d), 200.0, device="cuda", dtype=torch.float16),
+         torch.full((d, ff), 2.0 ** -10, device="cuda", dtype=torch.float16)]
+    dy = torch.full((N, d), 0.125, device="cuda", dtype=torch.float16)
+    for t in (x, *w):
+        t.requires_grad_(True)
+    grads = torch.autograd.grad(kernels.gated_ffn(x, *w), [x, *w], dy)
+    want = ref.gated(x, *w, dy, "silu", False)
+    assert float((x[:1].double() @ w[1].double().T).max()) * 0.5 > torch.finfo(torch.float16).max
+    for n, g in zip(NAMES, grads):
+        assert torch.isfinite(g).all()
+        ref.close(g, *want[n])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [9, 300])
+def test_values_that_are_no_numbers_stay_in_their_rows(gpu, N, dtype):
+    x, w, dy = _make(N, 64, 136, dtype, 8)
+    clean = [t.clone() for t in (x, *w)]
+    x[2, 5], x[4, 7], dy[6, 1] = float("nan"), float("inf"), float("-inf")
+    for t in (x, *w, *clean):
+        t.requires_grad_(True)
+    out = kernels.gated_ffn(x, *w)
+    dx, dwg = torch.autograd.grad(out, [x, w[0]], dy)
+    good = [n for n in range(N) if n not in (2, 4, 6)]
+    ref_out = kernels.gated_ffn(clean[0], *clean[1:])
+    (ref_dx,) = torch.autograd.grad(ref_out, [clean[0]], torch.nan_to_num(dy, neginf=0.0))
+    assert torch.equal(out[good], ref_out[good]) and torch.equal(dx[good], ref_dx[good])
+    assert out[2].isnan().all() and not dx[2].isfinite().any() and not dx[6].isfinite().any() and not dwg.isfinite().any()
