@@ -24,6 +24,12 @@ void check_with(const Tensor& t, const Tensor& x, const char* op, const char* na
   TORCH_CHECK(t.device() == x.device(), "titan::", op, ": ", name, " is on ", t.device(), ", the input on ", x.device());
 }
 
+// of a weight [R, K, ...]
+void check_slots(const Tensor& t, const char* op) {
+  dim32(t.size(0), op, "block rows");
+  dim32(t.size(1), op, "slots of a row");
+}
+
 // ------------------------------------------------------------------ quantisation
 std::tuple<Tensor, Tensor> mx_quantize(const Tensor& x_) {
   const char* op = "mx_quantize";
@@ -32,12 +38,13 @@ std::tuple<Tensor, Tensor> mx_quantize(const Tensor& x_) {
   TORCH_CHECK(x_.dim() == 2 && x_.size(1) > 0 && x_.size(1) % 32 == 0, "titan::", op,
               ": x must be [N, F] with F a multiple of 32, got ", x_.sizes());
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x_.device());
-  const int64_t N = x_.size(0), F = x_.size(1), per16 = dt == LBK_FP32 ? 4 : 8;
+  const int64_t N = x_.size(0), per16 = dt == LBK_FP32 ? 4 : 8;
+  const int32_t F = dim32(x_.size(1), op, "x's features");
   const bool rows = x_.stride(1) == 1 && x_.stride(0) >= F && x_.stride(0) % per16 == 0 &&
                     (reinterpret_cast<uintptr_t>(x_.data_ptr()) & 15) == 0;
   const Tensor x = rows ? x_ : dense16(x_);
   Tensor codes = at::empty({N, F / 2}, x.options().dtype(at::kByte)), scales = at::empty({N, F / 32}, codes.options());
-  LBK_CALL("mx_quantize", lbk_mx_quantize(x.data_ptr(), dt, N, (int32_t)F, N > 1 ? x.stride(0) : F, codes.data_ptr<uint8_t>(),
+  LBK_CALL("mx_quantize", lbk_mx_quantize(x.data_ptr(), dt, N, F, N > 1 ? x.stride(0) : F, codes.data_ptr<uint8_t>(),
                                           scales.data_ptr<uint8_t>(), cur_stream(x)));
   return {codes, scales};
 }
@@ -53,10 +60,11 @@ Tensor mx_dequantize(const Tensor& codes_, const Tensor& scales_, at::ScalarType
                   codes_.size(0) == scales_.size(0),
               "titan::", op, ": codes must be [N, F/2] and scales [N, F/32], got ", codes_.sizes(), " and ", scales_.sizes());
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(codes_.device());
+  const int64_t N = codes_.size(0);
+  const int32_t F = dim32(2 * codes_.size(1), op, "features");
   const Tensor codes = dense16(codes_), scales = scales_.contiguous();
-  const int64_t N = codes.size(0), F = 2 * codes.size(1);
   Tensor out = at::empty({N, F}, codes.options().dtype(dtype));
-  LBK_CALL("mx_dequantize", lbk_mx_dequantize(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), N, (int32_t)F, dt,
+  LBK_CALL("mx_dequantize", lbk_mx_dequantize(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), N, F, dt,
                                               out.data_ptr(), cur_stream(codes)));
   return out;
 }
@@ -66,14 +74,16 @@ std::tuple<Tensor, Tensor> mx_quantize_tiles(const Tensor& v_) {
   check_gpu(v_, op, "values");
   const int32_t dt = elem_type(v_.scalar_type(), op, "values");
   TORCH_CHECK(v_.dim() == 4 && v_.size(2) == v_.size(3), "titan::", op, ": values must be [R, K, B, B], got ", v_.sizes());
-  const int64_t R = v_.size(0), K = v_.size(1), B = v_.size(2);
-  TORCH_CHECK(B == 32 || B == 64, "titan::", op, ": B must be 32 or 64 (a group of 32 inputs lies in one tile), got ", B);
+  TORCH_CHECK(v_.size(2) == 32 || v_.size(2) == 64, "titan::", op,
+              ": B must be 32 or 64 (a group of 32 inputs lies in one tile), got ", v_.size(2));
+  check_slots(v_, op);
+  const int32_t R = (int32_t)v_.size(0), K = (int32_t)v_.size(1), B = (int32_t)v_.size(2);
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(v_.device());
   const Tensor v = v_.contiguous();
   Tensor codes = at::empty({R, K, B, B / 2}, v.options().dtype(at::kByte)),
          scales = at::empty({R, K, B, B / 32}, codes.options());
-  LBK_CALL("mx_quantize_tiles", lbk_mx_quantize_tiles(v.data_ptr(), dt, (int32_t)R, (int32_t)K, (int32_t)B,
-                                                      codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), cur_stream(v)));
+  LBK_CALL("mx_quantize_tiles", lbk_mx_quantize_tiles(v.data_ptr(), dt, R, K, B, codes.data_ptr<uint8_t>(),
+                                                      scales.data_ptr<uint8_t>(), cur_stream(v)));
   return {codes, scales};
 }
 
@@ -88,6 +98,7 @@ void check_mx_tiles(Tensor& c, Tensor& s, const char* op, const char* name) {
   TORCH_CHECK(s.dim() == 4 && s.size(0) == c.size(0) && s.size(1) == c.size(1) && s.size(2) == c.size(2) &&
                   s.size(3) * 32 == c.size(2),
               "titan::", op, ": ", name, " scales must be [R, K, B, B/32], got ", s.sizes());
+  check_slots(c, op);
   c = dense16(c);
   s = dense16(s);
 }
@@ -99,10 +110,10 @@ Tensor mx_dequantize_tiles(const Tensor& codes_, const Tensor& scales_, at::Scal
   check_gpu(c, op, "codes");
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(c.device());
   check_mx_tiles(c, s, op, "weight");
-  const int64_t R = c.size(0), K = c.size(1), B = c.size(2);
+  const int32_t R = (int32_t)c.size(0), K = (int32_t)c.size(1), B = (int32_t)c.size(2);
   Tensor v = at::empty({R, K, B, B}, c.options().dtype(dtype));
-  LBK_CALL("mx_dequantize_tiles", lbk_mx_dequantize_tiles(c.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), (int32_t)R, (int32_t)K,
-                                                          (int32_t)B, dt, v.data_ptr(), cur_stream(c)));
+  LBK_CALL("mx_dequantize_tiles", lbk_mx_dequantize_tiles(c.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), R, K, B, dt, v.data_ptr(),
+                                                          cur_stream(c)));
   return v;
 }
 
@@ -119,7 +130,10 @@ lbk_bell_mx make_mx(Tensor& c, Tensor& s, Tensor& ci, const Tensor& x, const cha
                      (int32_t)c.size(1), (int32_t)c.size(2)};
 }
 
-Tensor x2d16(const Tensor& x, const char* op) { return dense16(check_x2d(x, op)); }
+Tensor x2d16(const Tensor& x, const char* op) {
+  if (x.dim() == 2) dim32(x.size(1), op, "x's features");      // ahead of a copy
+  return dense16(check_x2d(x, op));
+}
 
 Tensor matmul_mx(const Tensor& x_, const Tensor& c_, const Tensor& s_, const Tensor& ci_, const OptTensor& bias_) {
   const char* op = "block_ell_matmul_mx";
@@ -127,13 +141,14 @@ Tensor matmul_mx(const Tensor& x_, const Tensor& c_, const Tensor& s_, const Ten
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x_.device());
   Tensor c = c_, s = s_, ci = ci_, x = x2d16(x_, op);
   const lbk_bell_mx w = make_mx(c, s, ci, x, op, "weight");
-  const int64_t N = x.size(0), F = x.size(1), O = (int64_t)w.R * w.B;
+  const int64_t N = x.size(0), O = (int64_t)w.R * w.B;
+  const int32_t F = (int32_t)x.size(1);
   TORCH_CHECK(F > 0 && F % w.B == 0, "titan::", op, ": in_features ", F, " not a multiple of B=", w.B);
   const Tensor bias = opt_bias(bias_, O, x, op, "bias");
   Tensor y = at::empty({N, O}, x.options());
-  const size_t wsb = lbk_mx_matmul_workspace_bytes(N, (int32_t)F, &w);
+  const size_t wsb = lbk_mx_matmul_workspace_bytes(N, F, &w);
   Tensor ws = wsb ? workspace(wsb, x) : Tensor();
-  LBK_CALL("block_ell_matmul_mx", lbk_mx_matmul_bf16(bf(x), N, (int32_t)F, &w, fptr(bias), bfm(y),
+  LBK_CALL("block_ell_matmul_mx", lbk_mx_matmul_bf16(bf(x), N, F, &w, fptr(bias), bfm(y),
                                                      wsb ? ws.data_ptr() : nullptr, wsb, cur_stream(x)));
   return y;
 }
@@ -147,7 +162,8 @@ Tensor swiglu_mx(const Tensor& x_, const Tensor& cg_, const Tensor& sg_, const T
   Tensor x = x2d16(x_, op), cg = cg_, sg = sg_, ig = ig_, cu = cu_, su = su_, iu = iu_, cd = cd_, sd = sd_, id = id_;
   const lbk_bell_mx g = make_mx(cg, sg, ig, x, op, "gate"), u = make_mx(cu, su, iu, x, op, "up"),
                     d = make_mx(cd, sd, id, x, op, "down");
-  const int64_t N = x.size(0), D = x.size(1), F = (int64_t)g.R * g.B;
+  const int64_t N = x.size(0), F = (int64_t)g.R * g.B;
+  const int32_t D = (int32_t)x.size(1);
   TORCH_CHECK(g.B == u.B && g.B == d.B, "titan::", op, ": the three weights must have one tile size");
   TORCH_CHECK(g.R == u.R && g.R > 0, "titan::", op, ": gate and up must have the same (non-zero) output features");
   TORCH_CHECK(D > 0 && (int64_t)d.R * d.B == D, "titan::", op, ": down's ", (int64_t)d.R * d.B,
@@ -155,10 +171,10 @@ Tensor swiglu_mx(const Tensor& x_, const Tensor& cg_, const Tensor& sg_, const T
   const Tensor bg = opt_bias(bg_, F, x, op, "b_gate"), bu = opt_bias(bu_, F, x, op, "b_up"),
                bd = opt_bias(bd_, D, x, op, "b_down");
   Tensor out = at::empty({N, D}, x.options());
-  const size_t wsb = lbk_mx_swiglu_workspace_bytes(N, (int32_t)D, &g, &u, &d);
+  const size_t wsb = lbk_mx_swiglu_workspace_bytes(N, D, &g, &u, &d);
   Tensor ws = workspace(wsb, x);
   LBK_CALL("block_ell_swiglu_fwd_mx",
-           lbk_mx_swiglu_fwd_bf16(bf(x), N, (int32_t)D, &g, &u, &d, fptr(bg), fptr(bu), fptr(bd), add_residual ? 1 : 0,
+           lbk_mx_swiglu_fwd_bf16(bf(x), N, D, &g, &u, &d, fptr(bg), fptr(bu), fptr(bd), add_residual ? 1 : 0,
                                   bfm(out), ws.data_ptr(), wsb, cur_stream(x)));
   return out;
 }
@@ -188,6 +204,7 @@ Gated make_gated(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
               wd.sizes(), " for d_model=", D);
   TORCH_CHECK(D > 0 && F > 0 && D % 8 == 0 && F % 8 == 0, "titan::", op, ": d_model=", D, " and d_ff=", F,
               " must be multiples of 8");
+  dim32(D, op, "x's features"), dim32(F, op, "hidden features");
   return {dense16(x), dense16(wg), dense16(wu), dense16(wd), x.size(0), D, F,
           x.scalar_type() == at::kHalf ? LBK_FP16 : LBK_BF16, act == "gelu" ? LBK_GELU : LBK_SILU};
 }
@@ -349,28 +366,41 @@ TORCH_LIBRARY_IMPL(titan, Autograd, m) {
 
 TORCH_LIBRARY_IMPL(titan, Meta, m) {
   m.impl("mx_quantize", [](const Tensor& x) {
+    dim32(x.size(1), "mx_quantize", "x's features");
     const auto o = x.options().dtype(at::kByte);
     return std::make_tuple(at::empty({x.size(0), x.size(1) / 2}, o), at::empty({x.size(0), x.size(1) / 32}, o));
   });
   m.impl("mx_dequantize", [](const Tensor& c, const Tensor&, at::ScalarType t) {
-    return at::empty({c.size(0), 2 * c.size(1)}, c.options().dtype(t));
+    return at::empty({c.size(0), dim32(2 * c.size(1), "mx_dequantize", "features")}, c.options().dtype(t));
   });
   m.impl("mx_quantize_tiles", [](const Tensor& v) {
+    check_slots(v, "mx_quantize_tiles");
     const auto o = v.options().dtype(at::kByte);
     return std::make_tuple(at::empty({v.size(0), v.size(1), v.size(2), v.size(2) / 2}, o),
                            at::empty({v.size(0), v.size(1), v.size(2), v.size(2) / 32}, o));
   });
   m.impl("mx_dequantize_tiles", [](const Tensor& c, const Tensor&, at::ScalarType t) {
+    check_slots(c, "mx_dequantize_tiles");
     return at::empty({c.size(0), c.size(1), c.size(2), c.size(2)}, c.options().dtype(t));
   });
   m.impl("block_ell_matmul_mx", [](const Tensor& x, const Tensor& c, const Tensor&, const Tensor&, const OptTensor&) {
+    dim32(x.size(1), "block_ell_matmul_mx", "x's features");
+    check_slots(c, "block_ell_matmul_mx");
     return at::empty({x.size(0), c.size(0) * c.size(2)}, x.options());
   });
   m.impl("block_ell_swiglu_fwd_mx",
-         [](const Tensor& x, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const Tensor&, const Tensor&,
-            const Tensor&, const OptTensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
-            bool) { return at::empty_like(x); });
-  auto like_x = [](const Tensor& x, const Tensor&, const Tensor&, const Tensor&, c10::string_view, bool) {
+         [](const Tensor& x, const Tensor& cg, const Tensor&, const Tensor&, const OptTensor&, const Tensor& cu, const Tensor&,
+            const Tensor&, const OptTensor&, const Tensor& cd, const Tensor&, const Tensor&, const OptTensor&, bool) {
+           dim32(x.size(1), "block_ell_swiglu_fwd_mx", "x's features");
+           for (const Tensor& c : {cg, cu, cd}) check_slots(c, "block_ell_swiglu_fwd_mx");
+           return at::empty_like(x);
+         });
+  auto gated_dims = [](const Tensor& x, const Tensor& wg, const char* op) {
+    dim32(x.size(1), op, "x's features");
+    dim32(wg.size(0), op, "hidden features");
+  };
+  auto like_x = [gated_dims](const Tensor& x, const Tensor& wg, const Tensor&, const Tensor&, c10::string_view, bool) {
+    gated_dims(x, wg, "gated_ffn_fwd");
     return at::empty_like(x);
   };
   m.impl("gated_ffn_fwd", like_x);

@@ -10,6 +10,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cstdint>
 #include <vector>
 
 #include "lbk.h"
@@ -31,6 +32,12 @@ inline uint16_t* bfm(at::Tensor& t) { return reinterpret_cast<uint16_t*>(t.data_
 
 inline void check_gpu(const at::Tensor& t, const char* op, const char* name) {
   TORCH_CHECK(t.is_cuda(), "titan::", op, ": ", name, " must be a GPU (HIP) tensor");
+}
+
+// a size as the C ABI's 32-bit argument
+inline int32_t dim32(int64_t n, const char* op, const char* what) {
+  TORCH_CHECK(n <= INT32_MAX, "titan::", op, ": ", what, " are ", n, ", more than 2^31 - 1");
+  return (int32_t)n;
 }
 
 inline at::Tensor check_x2d(const at::Tensor& x, const char* op) {
