@@ -325,6 +325,9 @@ Tensor gated_train_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu,
   return GatedTrain::apply(x, wg, wu, wd, act, add_residual);
 }
 
+// for the shape functions: the operators' results are contiguous, whatever x's strides
+Tensor rows_like(const Tensor& x) { return at::empty(x.sizes(), x.options()); }
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(titan, m) {
@@ -393,7 +396,7 @@ TORCH_LIBRARY_IMPL(titan, Meta, m) {
             const Tensor&, const OptTensor&, const Tensor& cd, const Tensor&, const Tensor&, const OptTensor&, bool) {
            dim32(x.size(1), "block_ell_swiglu_fwd_mx", "x's features");
            for (const Tensor& c : {cg, cu, cd}) check_slots(c, "block_ell_swiglu_fwd_mx");
-           return at::empty_like(x);
+           return rows_like(x);
          });
   auto gated_dims = [](const Tensor& x, const Tensor& wg, const char* op) {
     dim32(x.size(1), op, "x's features");
@@ -401,13 +404,13 @@ TORCH_LIBRARY_IMPL(titan, Meta, m) {
   };
   auto like_x = [gated_dims](const Tensor& x, const Tensor& wg, const Tensor&, const Tensor&, c10::string_view, bool) {
     gated_dims(x, wg, "gated_ffn_fwd");
-    return at::empty_like(x);
+    return rows_like(x);
   };
   m.impl("gated_ffn_fwd", like_x);
   m.impl("gated_ffn_train", like_x);
   m.impl("gated_ffn_fwd_train", [](const Tensor& x, const Tensor& wg, const Tensor&, const Tensor&, c10::string_view, bool) {
     auto factor = [&]() { return at::empty({x.size(0), 3 * wg.size(0)}, x.options().dtype(at::kByte)); };
-    return std::make_tuple(at::empty_like(x), at::empty({x.size(0), wg.size(0)}, x.options()), factor(), factor());
+    return std::make_tuple(rows_like(x), at::empty({x.size(0), wg.size(0)}, x.options()), factor(), factor());
   });
   m.impl("gated_ffn_bwd", [](const Tensor&, const Tensor& x, const Tensor&, const Tensor&, const Tensor&, const Tensor& wg,
                              const Tensor& wu, const Tensor& wd, bool, std::array<bool, 4> want) {
