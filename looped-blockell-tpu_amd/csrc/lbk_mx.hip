@@ -565,13 +565,20 @@ int mx_panel_slices(int64_t N, int TB, int tiles) {
   return best;
 }
 
+// Whether a product's panels times shares are more workgroups than a launch takes (its threads are a 32-bit
+// number).  Hidden features between 4800 and 9600 leave 32 tokens a panel, which passes it below the limit on tokens.
+template <int MODE>
+bool mx_panel_too_large(int64_t N, int F, const lbk_bell_mx& w) {
+  const int TB = mx_block_tokens(F);
+  return (N + TB - 1) / TB * mx_panel_slices<MODE>(N, TB, w.R * (w.B / 32)) > 0x3fffff;
+}
+
 template <int B, int MODE, int MT, bool BIAS, int FROM>
 int launch_mx_panel_t(MxPanelArgs a, hipStream_t st) {
   constexpr int NW = mx_panel_waves<MODE>(MT);
   auto* k = mx_panel_kernel<B, MODE, MT, NW, BIAS, FROM>;
   const int64_t lds = FROM == 2 ? 0 : panel_of(a.F / 32, 32 * MT).bytes, nb = (a.N + 32 * MT - 1) / (32 * MT);
   a.slices = mx_panel_slices<MODE>(a.N, 32 * MT, a.w0.R * (B / 32));
-  if (nb * a.slices > 0x3fffff) return -1;
   static std::atomic<uint64_t> done{0};
   if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), 160 * 1024, done) != 0) return -1;
   k<<<(unsigned)(nb * a.slices), NW * 64, lds, st>>>(a);
@@ -915,6 +922,7 @@ int lbk_mx_matmul_bf16(const uint16_t* x, int64_t N, int32_t in_features, const 
   if (too_many(N, in_features)) return LBK_ERR_TOO_LARGE;
   const size_t need = lbk_mx_matmul_workspace_bytes(N, in_features, w);
   if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
+  if (!decodes(N, {w}) && mx_panel_too_large<0>(N, in_features, *w)) return LBK_ERR_TOO_LARGE;
   MxPanelArgs a{};
   a.N = N; a.F = in_features; a.w0 = *w; a.b0 = bias; a.y = y;
   int err;
@@ -952,6 +960,8 @@ int lbk_mx_swiglu_fwd_bf16(const uint16_t* x, int64_t N, int32_t d_model, const 
   const size_t need = lbk_mx_swiglu_workspace_bytes(N, d_model, gate, up, down);
   if (!workspace || workspace_bytes < need) return LBK_ERR_WORKSPACE;
   const int d_ff = gate->R * gate->B;
+  if (!decodes(N, {gate, up, down}) && (mx_panel_too_large<1>(N, d_model, *gate) || mx_panel_too_large<0>(N, d_ff, *down)))
+    return LBK_ERR_TOO_LARGE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   MxPanelArgs g{}, d{};
   g.N = d.N = N; g.F = d_model; d.F = d_ff;

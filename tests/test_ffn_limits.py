@@ -2,6 +2,7 @@
 never narrowed.  The shape functions refuse as the operators do; expanded tensors (stride 0) stand for the large
 ones, since the refusal comes ahead of any copy."""
 
+import ctypes
 import os
 
 import pytest
@@ -9,6 +10,8 @@ import torch
 
 PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "looped-blockell-tpu_amd", "looped_blockell")
 needs_ext = pytest.mark.skipif(not os.path.exists(os.path.join(PKG, "_titan_ext.so")), reason="_titan_ext.so not built")
+
+needs_lib = pytest.mark.skipif(not os.path.exists(os.path.join(PKG, "liblbk.so")), reason="liblbk.so not built")
 
 F = 2 ** 32 + 64           # narrows to 64
 
@@ -54,3 +57,18 @@ def test_shape_functions_refuse(name):
 def test_operators_refuse(gpu, name):
     with pytest.raises(RuntimeError, match="more than 2\\^31 - 1"):
         _calls(gpu)[name]()
+
+
+@needs_lib
+@pytest.mark.parametrize("N", [2 ** 27, 2 ** 27 - 31])
+def test_grids_beyond_a_launch_are_refused_ahead_of_it(N):
+    """2^27 tokens of 32 features are within the limits, but their hidden state of 5120 features, in panels of 32
+    tokens, has more workgroups than a launch takes: refused by name, with nothing queued."""
+    from looped_blockell import abi as A
+    lib, P = A.load(), 0x1000                # an aligned address that no call reaches
+
+    def w(R):
+        return ctypes.byref(A.BellMx(P, P, P, R, 1, 32))
+
+    up, down = w(5120 // 32), w(1)
+    assert lib.lbk_mx_swiglu_fwd_bf16(P, N, 32, up, up, down, None, None, None, 0, P, P, 1 << 62, None) == A.LBK_ERR_TOO_LARGE
