@@ -81,7 +81,8 @@ __device__ __forceinline__ float gelu_gate(float z) {
 __device__ __forceinline__ float gelu_f(float z) { return z * gelu_gate(z); }
 __device__ __forceinline__ float gelu_grad_f(float z) {
   const float s = gelu_gate(z);
-  return s + z * s * (1.0f - s) * (1.5957691216f * (1.0f + 0.134145f * z * z));
+  // the bound (|z| = 273, where s is 0 or 1) keeps 0 from meeting an Inf once z^2 leaves fp32's range
+  return s + z * s * (1.0f - s) * (1.5957691216f * fminf(1.0f + 0.134145f * z * z, 1e4f));
 }
 
 // 1 KB from global memory to LDS: lane l's 16 bytes at p (or at base + off) land at lds + 16 l.  Inline
