@@ -488,7 +488,8 @@ def mx_dequantize_tiles(codes, scales, dtype: torch.dtype = torch.bfloat16):
 
 def mx_matmul(x, codes, scales, col_indices, bias=None):
     """x [..., C*B] -> [..., R*B] through a Block-ELL weight in 4 bits (``mx_quantize_tiles``), x
-    (rounded to bf16 if it is of another type) quantised in the call, sums in fp32; not differentiable."""
+    (rounded to bf16 first if it is of another type, so that its codes can differ from ``mx_quantize(x)``'s)
+    quantised in the call, sums in fp32; not differentiable."""
     _gpu(x, codes, scales, col_indices)
     if x.dim() == 2:
         return ops().block_ell_matmul_mx(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), codes, scales, col_indices,
@@ -517,7 +518,9 @@ def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", add_residual: b
     """``(act(x w_gate^T) * (x w_up^T)) w_down^T (+ x)`` with dense weights [out, in], all bf16 or all
     fp16; ``activation`` 'silu' or 'gelu' (tanh form); d_model and d_ff multiples of 8.
     Differentiable in x and the weights as one native autograd node (``titan::gated_ffn_train``),
-    gradients in the inputs' type; without gradients nothing is kept."""
+    gradients in the inputs' type; without gradients nothing is kept.  The hidden state, and in the backward the
+    gradients of both projections, are rounded to the inputs' type between the products: in fp16 what passes 65504
+    there is an Inf, even where the results would not be."""
     _gpu(x, w_gate, w_up, w_down)
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
