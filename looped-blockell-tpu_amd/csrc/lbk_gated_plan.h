@@ -12,7 +12,9 @@ constexpr int BK = 64;       // K of a stage
 
 // Whether the weights are streamed: where the tokens' own reads, once a workgroup, do not outweigh the tiled
 // kernel's idle columns.  us of a forward, streamed / tiled (33 tokens): 2048 / 8192 16 tokens 36 / 47, 32 tokens
-// 51 / 47; 1024 / 4096 32 tokens 20 / 25; 4096 / 14336 16 tokens 93 / 95, 8 tokens 80.
+// 51 / 47; 1024 / 4096 32 tokens 20 / 25; 4096 / 14336 16 tokens 93 / 95, 8 tokens 80.  Between 9 and 64 tokens either is far
+// from the weights' 20 us at 2048 / 8192 (38 at 16, 50 at 32, 53 at 64): every workgroup of 16 features reads all tokens
+// again here, and the tiled gate product has 128 workgroups for 256 CUs.
 inline bool skinny(int64_t N, int64_t D, int64_t F) { return N <= 16 || (N <= 32 && D * F <= (int64_t)1 << 23); }
 
 // How a product of M features, N columns and K (over all pairs) runs: output tiles of 256 or 128, K in

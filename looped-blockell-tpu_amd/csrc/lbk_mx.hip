@@ -24,7 +24,6 @@ namespace lbk {
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // fp4 x fp4; sa, sb: the scale bytes in bits 0 .. 7
@@ -290,9 +289,10 @@ struct MxPanelArgs {
 // their codes (16 bytes a lane), scale and column are loaded D positions ahead, always all three, so that the
 // compiler's load counters stay exact across tiles.  A dead slot, and the second half of an odd row's last
 // pair, multiplies zeros with unit scales.
-// MODE 1 is bound by the epilogue's vector work (silu's exp and reciprocal, the maximum and the conversion:
-// about 54 cycles a hidden value and wave, against 16 of the matrix unit at 8 slots), so four waves a SIMD of
-// 64 tokens beat two of 128, whose weights are read half as often.
+// MODE 1 (16384 tokens, 1024 -> 4096 at 0.25: 59 us) issues 30 us of vector instructions on every SIMD, counted at
+// four clocks each, and its exponentials and reciprocals, at a quarter of that rate, take 10 more; the matrix unit
+// is busy for 7 of them.  What the remaining time waits for is not measured.  Its 12 waves (three a SIMD) hold 64
+// accumulators each.
 // FROM: where a workgroup's tokens are: 0 a panel copied to LDS, 1 bf16 rows that it quantises into LDS itself,
 // 2 the panel in global memory (too wide for LDS: 32 lanes read 512 consecutive bytes there too).
 template <int B, int MODE, int MT, int NW, bool BIAS, int FROM>
@@ -610,9 +610,9 @@ int launch_quantize_panel(const uint16_t* x, int64_t N, int F, int TB, uint8_t* 
 // ------------------------------------------------------------------ few tokens
 // A workgroup of 8 waves makes one 32-row output tile of 32 tokens: the slots are dealt to the waves (MODE 1:
 // gate's to waves 0 .. 3, up's to 4 .. 7) and their sums joined through LDS in a fixed order.  The weights are
-// read once, four positions on their way per wave; tokens come as bf16 rows, quantised where they are used
-// (one launch less, and a row of the slot's columns is 64 bytes a lane), or as panels of 32 (XQ: the hidden
-// state).  Latency-bound at these sizes: 16 tokens, 4096 / 14336 at 0.1, 9 MB of weights.
+// read once, two positions on their way per wave where tokens come as bf16 rows, quantised where they are used
+// (one launch less, and a row of the slot's columns is 64 bytes a lane), four where they come as panels of 32 (XQ:
+// the hidden state).  Latency-bound at these sizes: 16 tokens, 4096 / 14336 at 0.1, 9 MB of weights.
 template <int B, int MODE, bool XQ>
 __global__ __launch_bounds__(512, 4) void mx_decode_kernel(MxPanelArgs a, const uint16_t* __restrict__ x) {
   constexpr int U = XQ ? 4 : 2, STEP = 64 / B, DEAL = MODE == 1 ? 4 : 8;
@@ -770,7 +770,6 @@ namespace {
 
 inline bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
-inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 constexpr int64_t kMaxThreads = 0xffffff00;     // of one launch
 constexpr int64_t kMaxTokens = (int64_t)1 << 27;  // the products' launches, 32 tokens a workgroup
 constexpr int32_t kMaxFeatures = 1 << 24;         // and slots of a row: places in a panel and in a row are 32-bit
