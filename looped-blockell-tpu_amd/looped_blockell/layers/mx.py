@@ -29,14 +29,14 @@ class MXBlockELLWeight(nn.Module):
     @classmethod
     @torch.no_grad()
     def from_values(cls, values: torch.Tensor, col_indices: torch.Tensor, bias: torch.Tensor | None = None):
-        """Quantise tiles [R,K,B_in,B_out] (bf16, fp16 or fp32) on the GPU."""
+        """Quantise tiles [R,K,B_in,B_out] (bf16, fp16 or fp32) on the GPU; columns and bias are copied."""
         codes, scales = kernels.mx_quantize_tiles(values.detach())
-        return cls(codes, scales, col_indices, bias)
+        return cls(codes, scales, col_indices.clone(), None if bias is None else bias.clone())
 
     @classmethod
     def from_linear(cls, linear):
         """Quantise a ``BlockELLLinear``, its pruned tiles as dead slots."""
-        return cls.from_values(linear.values, linear.effective_col_indices().clone(), linear.bias)
+        return cls.from_values(linear.values, linear.effective_col_indices(), linear.bias)
 
     def triple(self):
         return self.codes, self.scales, self.col_indices

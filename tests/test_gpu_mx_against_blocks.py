@@ -87,3 +87,23 @@ def test_ffn(gpu, N, tile):
         back = torch.argsort(src, 1)
         wrong = (cols[r, slot.gather(1, back)].long() * tile + back).flatten().cuda()
         assert ((y - h[:, wrong] * s).abs() > bound).any()
+
+
+def test_quantised_layers_are_copies(gpu):
+    """Training the source on, or loading a state into the quantised layer, leaves the other as it was."""
+    lin = BlockELLLinear(64, 128, tile_size=32, density=0.5, device="cuda")
+    x = torch.randn(5, 128, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        lin.bias.normal_()
+        cols = lin.col_indices.clone()
+        made = [MXBlockELLWeight.from_linear(lin), MXBlockELLWeight.from_values(lin.values, cols, lin.bias)]
+        before, bias = [w(x) for w in made], lin.bias.clone()
+        lin.bias.add_(1)
+        lin.values.mul_(2)
+        cols.fill_(-1)
+        lin.col_indices.fill_(0)
+        assert all(torch.equal(w(x), y) for w, y in zip(made, before))
+        lin.bias.copy_(bias)
+        for w in made:
+            w.load_state_dict({k: torch.zeros_like(v) for k, v in w.state_dict().items()})
+        assert torch.equal(lin.bias, bias)
