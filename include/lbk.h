@@ -843,6 +843,58 @@ int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const uint
                   const void* w_up, const void* w_down, int add_residual, void* dx, void* dw_gate, void* dw_up,
                   void* dw_down, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Dropout from a counter-based generator; the mask is made again wherever it is needed and never stored.
+ * Element (n, c) of x [N, F] has 16 bits u(n, c): Philox4x32 with 7 rounds (Salmon, Moraes, Dror and Shaw,
+ * "Parallel random numbers: as easy as 1, 2, 3", 2011), key = the low and high 32 bits of the seed, counter =
+ * (c / 8, the low and high 32 bits of n, stream_id); of the four words, word (c % 8) / 2 holds them, the even column
+ * low.  With cut = floor(65536 p + 0.5), y = u >= cut ? x 65536 / (65536 - cut) : 0, so p counts in steps of 2^-16.
+ * The backward is the same call on the gradient.  seed_dev (a device pointer) is read by the kernel in place of
+ * seed where it is given: a replayed graph follows it.  Rows of x are ldx elements apart, y is contiguous and may
+ * be x; both need an element's alignment only.  For the dropout of the reference's MLPBlock
+ * (looped_blockell/layers/mlp.py:98-168), whose generator is not reproduced.
+ */
+int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx, double p, const int64_t* seed_dev,
+                int64_t seed, uint32_t stream_id, void* y, void* stream);
+
+/*
+ * The seam between two applications of a residual block, in one pass over the rows:
+ *   z  = y / sqrt(mean(y^2) + eps) * post_scale              (z = y without post_scale)
+ *   h' = h + residual_scale * gate * drop(z)                 (drop: lbk_dropout's, from p, the seed and stream_id)
+ *   n  = h' / sqrt(mean(h'^2) + eps) * pre_scale             (only with pre_scale; of h' before it is rounded)
+ * h and h' are of state_type, y and n of `type`: the same one, or LBK_FP32 beside it.  Everything is contiguous
+ * [N, d], d <= 16384, and needs an element's alignment only.  gate [gate_rows, d]: row n takes gate row
+ * n / (N / gate_rows).  A row of zeros has a norm of zeros; with eps = 0 it is NaN.  h' may be h.
+ */
+typedef struct lbk_seam {
+    int64_t N;
+    int32_t d, state_type, type;
+    const float* post_scale;       /* [d] or NULL */
+    const float* pre_scale;        /* [d] or NULL */
+    const void* gate;              /* [gate_rows, d] of gate_type, or NULL */
+    int32_t gate_type;
+    int64_t gate_rows;             /* divides N */
+    float residual_scale, eps;
+    double p;
+    const int64_t* seed_dev;       /* device pointer or NULL (seed) */
+    int64_t seed;
+    uint32_t stream_id;
+} lbk_seam;
+
+/* rs_post, rs_pre [N]: 1 / sqrt(mean + eps) of the rows, for the backward (each NULL to skip). */
+int lbk_residual_norm_fwd(const lbk_seam* s, const void* h, const void* y, void* h_out, void* n_out, float* rs_post,
+                          float* rs_pre, void* stream);
+
+/*
+ * Gradients for dh_out (of h') and dn (of n), each NULL for none, from the forward's h and y and its rows' rs; each
+ * of dh, dy, d_post [d], d_gate (like gate) and d_pre [d] is optional.  Sums over rows run in a fixed order: no
+ * atomics.  dh may be dh_out.
+ */
+size_t lbk_residual_norm_bwd_workspace_bytes(const lbk_seam* s);
+int lbk_residual_norm_bwd(const lbk_seam* s, const void* h, const void* y, const float* rs_post, const float* rs_pre,
+                          const void* dh_out, const void* dn, void* dh, void* dy, float* d_post, void* d_gate, float* d_pre,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,689 @@
+// lbk_seam.hip — dropout from a counter-based generator, and the seam between two applications of a block: the
+// branch's norm, dropout, gate and scale, the residual sum and the norm ahead of the next application, with their
+// backward (gfx950), and their entry points of include/lbk.h.
+//
+//   z  = y rs(y) w_post            rs(v) = 1 / sqrt(mean(v^2) + eps)
+//   h' = h + alpha gate drop(z)
+//   n  = h' rs(h') w_pre
+//
+// All arithmetic is fp32; h', n and the gradients are rounded once, to their own types.
+#include "lbk.h"
+#include "lbk_device.h"
+#include "lbk_internal.h"
+
+#include <math.h>
+
+namespace lbk {
+namespace {
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+// rows of any length start at any element: 16-byte loads and stores that need no more than an element's alignment
+typedef u32x4 u32x4_2 __attribute__((aligned(2)));
+typedef f32x4 f32x4_4 __attribute__((aligned(4)));
+
+// ------------------------------------------------------------------ the generator
+// 16 bits for each of 8 consecutive columns of a row: Philox4x32 (Salmon, Moraes, Dror and Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", 2011) with the 7 rounds that the paper finds free of statistical defects, key =
+// seed, counter = (column / 8, row, stream).  A drop probability is then a multiple of 2^-16; words of 32 bits an
+// element would take twice the generator's arithmetic, which at 14 wide multiplications a block is what bounds a
+// dropout of 16-bit values next to memory.
+struct Random {
+  const int64_t* seed_dev;      // read by the kernel where it is given, so that a replayed graph follows it
+  int64_t seed;
+  uint32_t stream, cut;         // an element is dropped where its 16 bits are below cut
+  float keep;                   // 65536 / (65536 - cut)
+};
+
+__device__ __forceinline__ u32x4 random8(uint64_t key, uint32_t group, uint64_t row, uint32_t stream) {
+  uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
+  uint32_t c0 = group, c1 = (uint32_t)row, c2 = (uint32_t)(row >> 32), c3 = stream;
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)p1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)p0;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return u32x4{c0, c1, c2, c3};
+}
+
+// A dropped element is 0 whatever it held.
+__device__ __forceinline__ void drop8(float (&f)[8], const u32x4& w, uint32_t cut, float keep) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const uint32_t u = (q & 1) ? w[q >> 1] >> 16 : w[q >> 1] & 0xffffu;
+    f[q] = u >= cut ? f[q] * keep : 0.0f;
+  }
+}
+
+// ------------------------------------------------------------------ eight consecutive elements, n of them there
+template <int T> struct Elem { typedef uint16_t type; };
+template <> struct Elem<LBK_FP32> { typedef float type; };
+
+template <int T>
+__device__ __forceinline__ float to_f(typename Elem<T>::type v) {
+  if constexpr (T == LBK_FP32) return v;
+  else if constexpr (T == LBK_BF16) return bf2f(v);
+  else return (float)__builtin_bit_cast(_Float16, v);
+}
+template <int T>
+__device__ __forceinline__ typename Elem<T>::type from_f(float f) {
+  if constexpr (T == LBK_FP32) return f;
+  else if constexpr (T == LBK_BF16) return f2bf(f);
+  else return __builtin_bit_cast(uint16_t, (_Float16)f);
+}
+
+template <int T>
+__device__ __forceinline__ void load8(const void* base, int64_t at, int n, float (&f)[8]) {
+  const auto* p = static_cast<const typename Elem<T>::type*>(base) + at;
+  if (n >= 8) {
+    if constexpr (T == LBK_FP32) {
+      const f32x4 a = *reinterpret_cast<const f32x4_4*>(p), b = *reinterpret_cast<const f32x4_4*>(p + 4);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[q] = a[q], f[4 + q] = b[q];
+    } else {
+      const u32x4 v = *reinterpret_cast<const u32x4_2*>(p);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[2 * q] = to_f<T>((uint16_t)v[q]), f[2 * q + 1] = to_f<T>((uint16_t)(v[q] >> 16));
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = q < n ? to_f<T>(p[q]) : 0.0f;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack2_f16(float lo, float hi) {
+  const f16x2_t v = {(_Float16)lo, (_Float16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+template <int T>
+__device__ __forceinline__ void store8(void* base, int64_t at, int n, const float (&f)[8]) {
+  auto* p = static_cast<typename Elem<T>::type*>(base) + at;
+  if (n >= 8) {
+    if constexpr (T == LBK_FP32) {
+      *reinterpret_cast<f32x4_4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<f32x4_4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+    } else {
+      u32x4 v;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        v[q] = T == LBK_BF16 ? pack2_bf16(f[2 * q], f[2 * q + 1]) : pack2_f16(f[2 * q], f[2 * q + 1]);
+      *reinterpret_cast<u32x4_2*>(p) = v;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < n) p[q] = from_f<T>(f[q]);
+  }
+}
+
+// of a type known at run time only (the gate's)
+__device__ __forceinline__ void load8_any(int type, const void* base, int64_t at, int n, float (&f)[8]) {
+  if (type == LBK_FP32) load8<LBK_FP32>(base, at, n, f);
+  else if (type == LBK_BF16) load8<LBK_BF16>(base, at, n, f);
+  else load8<LBK_FP16>(base, at, n, f);
+}
+__device__ __forceinline__ void store8_any(int type, void* base, int64_t at, int n, const float (&f)[8]) {
+  if (type == LBK_FP32) store8<LBK_FP32>(base, at, n, f);
+  else if (type == LBK_BF16) store8<LBK_BF16>(base, at, n, f);
+  else store8<LBK_FP16>(base, at, n, f);
+}
+
+// ------------------------------------------------------------------ dropout
+struct DropArgs {
+  const void* x;
+  void* y;
+  int64_t N, ldx;
+  int F, G;                     // G: groups of 8 columns in a row
+  uint32_t magic, shift;        // n / G = n magic >> shift for n < 2^31
+  Random r;
+};
+
+constexpr int DROP_GROUPS = 4;  // of a thread
+
+template <int T>
+__global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
+  const uint64_t key = (uint64_t)(a.r.seed_dev ? *a.r.seed_dev : a.r.seed);
+  const int64_t first = (int64_t)blockIdx.x * (256 * DROP_GROUPS), row0 = first / a.G;
+  const uint32_t g0 = (uint32_t)(first - row0 * a.G) + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < DROP_GROUPS; ++k) {
+    const uint32_t off = g0 + 256 * k, dr = (uint32_t)((uint64_t)off * a.magic >> a.shift), g = off - dr * a.G;
+    const int64_t row = row0 + dr;
+    if (row >= a.N) return;
+    const int n = a.F - 8 * (int)g;
+    float f[8];
+    load8<T>(a.x, row * a.ldx + 8 * (int64_t)g, n, f);
+    drop8(f, random8(key, g, row, a.r.stream), a.r.cut, a.r.keep);
+    store8<T>(a.y, row * a.F + 8 * (int64_t)g, n, f);
+  }
+}
+
+// ------------------------------------------------------------------ rows
+template <int CTRL>
+__device__ __forceinline__ float lane_dpp(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+struct Add { static __device__ __forceinline__ float of(float a, float b) { return a + b; } };
+struct Max { static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); } };
+
+// over the 64 lanes, the result in every lane: neighbours, pairs, quads and halves of 16 by DPP, then the rows of 16
+// and the halves of the wave against each other
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float x) {
+  x = Op::of(x, lane_dpp<0xB1>(x));
+  x = Op::of(x, lane_dpp<0x4E>(x));
+  x = Op::of(x, lane_dpp<0x141>(x));
+  x = Op::of(x, lane_dpp<0x140>(x));
+  auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = Op::of(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return Op::of(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// A row belongs to NW waves (those of a workgroup where NW > 1), a lane's E vectors of 8 columns lie 512 NW apart.
+struct RowSum {
+  float (*buf)[16];
+  int NW, w, turn;
+  template <class Op>
+  __device__ __forceinline__ float over(float x) {
+    x = wave_reduce<Op>(x);
+    if (NW == 1) return x;
+    turn ^= 1;                        // two buffers: a wave that is a reduction ahead writes the other
+    if ((threadIdx.x & 63) == 0) buf[turn][w] = x;
+    __syncthreads();
+    float v = buf[turn][0];
+    for (int k = 1; k < NW; ++k) v = Op::of(v, buf[turn][k]);
+    return v;
+  }
+};
+
+// rs of a row.  Squares pass fp32 from 1.8e19 on, which bf16 and fp32 rows may hold: such a row's are summed
+// again of values scaled by a power of two.  (The condition is the same in all waves of the row.)
+template <int E>
+__device__ __forceinline__ float row_rs(const float (&v)[E][8], int d, float eps, RowSum& rows) {
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) ss += v[e][q] * v[e][q];
+  ss = rows.over<Add>(ss);
+  float rs = 1.0f / sqrtf(ss / (float)d + eps);
+  if (ss > 3.0e38f) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) top = fmaxf(top, fabsf(v[e][q]));
+    top = rows.over<Max>(top);
+    if (top <= 3.4028235e38f) {
+      constexpr float s = 0x1p-80f;   // d <= 2^14: the sum lies between 2^-48 and 2^110
+      ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) ss += v[e][q] * s * (v[e][q] * s);
+      ss = rows.over<Add>(ss);
+      rs = s / sqrtf(ss / (float)d + eps * s * s);
+    }
+  }
+  return rs;
+}
+
+struct SeamArgs {
+  int64_t N;
+  int d, NW;
+  const void *h, *y;
+  const float *post, *pre;
+  const void* gate;
+  int gate_type;
+  int64_t gate_rows, per;       // rows of the gate, and rows of h that share one
+  float alpha, eps;
+  Random r;
+  void *h_out, *n_out;
+  float *rs_post, *rs_pre;
+  // backward
+  const void *dh_out, *dn;
+  void *dh, *dy;
+  float* part;                  // [vectors][blocks][d]
+  void* d_gate;
+  int64_t W, blocks, bpg;       // rows of a worker, workgroups, workgroups of a gate row (0: gate rows lie in workers)
+};
+
+template <int TH, int TY, int E, bool DROP>
+__global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
+  __shared__ float buf[2][16];
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+  const int worker = a.NW == 1 ? wv : 0, w = a.NW == 1 ? 0 : wv, R = a.NW == 1 ? (int)(blockDim.x >> 6) : 1;
+  RowSum rows{buf, a.NW, w, 0};
+  const int64_t row = (int64_t)blockIdx.x * R + worker;
+  if (row >= a.N) return;           // one worker a workgroup where there are barriers
+  float h[E][8], y[E][8];
+  int col[E], n[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    col[e] = 8 * ((e * a.NW + w) * 64 + lane);
+    n[e] = a.d - col[e];
+    load8<TY>(a.y, row * a.d + col[e], n[e], y[e]);
+    load8<TH>(a.h, row * a.d + col[e], n[e], h[e]);
+  }
+  if (a.post) {
+    const float rs = row_rs<E>(y, a.d, a.eps, rows);
+    if (a.rs_post && lane == 0 && w == 0) a.rs_post[row] = rs;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float p[8];
+      load8<LBK_FP32>(a.post, col[e], n[e], p);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[e][q] = y[e][q] * rs * p[q];
+    }
+  }
+  const uint64_t key = DROP ? (uint64_t)(a.r.seed_dev ? *a.r.seed_dev : a.r.seed) : 0;
+  const int64_t grow = a.gate ? (a.gate_rows == 1 ? 0 : (int64_t)((uint32_t)row / (uint32_t)a.per)) : 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if constexpr (DROP) drop8(y[e], random8(key, (uint32_t)col[e] >> 3, row, a.r.stream), a.r.cut, a.r.keep);
+    if (a.gate) {
+      float g[8];
+      load8_any(a.gate_type, a.gate, grow * a.d + col[e], n[e], g);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[e][q] *= g[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) h[e][q] += a.alpha * y[e][q];
+    store8<TH>(a.h_out, row * a.d + col[e], n[e], h[e]);
+  }
+  if (a.pre) {
+    const float rs = row_rs<E>(h, a.d, a.eps, rows);
+    if (a.rs_pre && lane == 0 && w == 0) a.rs_pre[row] = rs;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float p[8];
+      load8<LBK_FP32>(a.pre, col[e], n[e], p);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) h[e][q] = h[e][q] * rs * p[q];
+      store8<TY>(a.n_out, row * a.d + col[e], n[e], h[e]);
+    }
+  }
+}
+
+// The backward of a row.  h' is made again from h and y, in fp32: what was stored of it is rounded.  With
+// q = w_pre dn, x2 = h' rs(h'), x1 = y rs(y):
+//   t  = dh' + rs(h') (q - x2 mean(q x2)) = dh          d_pre  = sum of dn x2
+//   s  = alpha gate t, dropped as z was                 d_gate = sum of alpha t drop(z), d_post = sum of s x1
+//   dy = rs(y) (v - x1 mean(v x1)),  v = w_post s
+// A workgroup takes consecutive rows, a worker (one wave, or all of them) W of these, and keeps the columns' sums in
+// registers.  Sums go to `part`, one row a workgroup, and are added in a fixed order by seam_sum_kernel: no atomics.  A
+// gate's rows either lie in one worker each (bpg = 0: written at once) or take bpg workgroups each.
+template <int TH, int TY, int E, bool DROP>
+__global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
+  __shared__ float buf[2][16];
+  extern __shared__ float sums[];   // [workers][d]
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
+  const int worker = a.NW == 1 ? wv : 0, w = a.NW == 1 ? 0 : wv, R = a.NW == 1 ? (int)(blockDim.x >> 6) : 1;
+  RowSum rows{buf, a.NW, w, 0};
+  int64_t r0, end;
+  if (a.bpg) {                      // workgroups of one gate row
+    const int64_t g = blockIdx.x / a.bpg, c = blockIdx.x - g * a.bpg;
+    r0 = g * a.per + (c * R + worker) * a.W;
+    end = min(r0 + a.W, (g + 1) * a.per);
+  } else {
+    r0 = ((int64_t)blockIdx.x * R + worker) * a.W;
+    end = min(r0 + a.W, a.N);
+  }
+  const uint64_t key = DROP ? (uint64_t)(a.r.seed_dev ? *a.r.seed_dev : a.r.seed) : 0;
+  float s_pre[E][8] = {}, s_post[E][8] = {}, s_gate[E][8] = {};
+  int col[E], n[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    col[e] = 8 * ((e * a.NW + w) * 64 + lane);
+    n[e] = a.d - col[e];
+  }
+  int64_t grow = a.gate && a.gate_rows > 1 && r0 < a.N ? r0 / a.per : 0, gend = (grow + 1) * a.per;
+  for (int64_t row = r0; row < end; ++row) {
+    const int64_t at = row * a.d;
+    if (a.gate && row >= gend) ++grow, gend += a.per;
+    const float rs1 = a.post ? a.rs_post[row] : 1.0f;
+    float t[E][8], y[E][8], z[E][8], g[E][8];
+    u32x4 rnd[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (a.dh_out) load8<TH>(a.dh_out, at + col[e], n[e], t[e]);
+      else
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t[e][q] = 0.f;
+      load8<TY>(a.y, at + col[e], n[e], y[e]);
+      if (a.gate) load8_any(a.gate_type, a.gate, grow * a.d + col[e], n[e], g[e]);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        y[e][q] *= rs1;             // x1
+        z[e][q] = y[e][q];
+        if (!a.gate) g[e][q] = 1.0f;
+      }
+      if (a.post) {
+        float p[8];
+        load8<LBK_FP32>(a.post, col[e], n[e], p);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) z[e][q] *= p[q];
+      }
+      if constexpr (DROP) {
+        rnd[e] = random8(key, (uint32_t)col[e] >> 3, row, a.r.stream);
+        drop8(z[e], rnd[e], a.r.cut, a.r.keep);
+      }
+    }
+    if (a.dn) {
+      const float rs = a.rs_pre[row];
+      float x[E][8], v[E][8], dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float p[8];
+        load8<TH>(a.h, at + col[e], n[e], x[e]);
+        load8<TY>(a.dn, at + col[e], n[e], v[e]);
+        load8<LBK_FP32>(a.pre, col[e], n[e], p);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          x[e][q] = (x[e][q] + a.alpha * (z[e][q] * g[e][q])) * rs;
+          s_pre[e][q] += v[e][q] * x[e][q];
+          v[e][q] *= p[q];
+          dot += v[e][q] * x[e][q];
+        }
+      }
+      dot = rows.over<Add>(dot) / (float)a.d;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t[e][q] += rs * (v[e][q] - x[e][q] * dot);
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (a.dh) store8<TH>(a.dh, at + col[e], n[e], t[e]);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        t[e][q] *= a.alpha;
+        s_gate[e][q] += t[e][q] * z[e][q];
+        t[e][q] *= g[e][q];
+      }
+      if constexpr (DROP) drop8(t[e], rnd[e], a.r.cut, a.r.keep);
+      if (a.post) {
+        float p[8];
+        load8<LBK_FP32>(a.post, col[e], n[e], p);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          s_post[e][q] += t[e][q] * y[e][q];
+          t[e][q] *= p[q];
+          dot += t[e][q] * y[e][q];
+        }
+      }
+    }
+    if (a.post) {
+      dot = rows.over<Add>(dot) / (float)a.d;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t[e][q] = rs1 * (t[e][q] - y[e][q] * dot);
+    }
+    if (a.dy)
+#pragma unroll
+      for (int e = 0; e < E; ++e) store8<TY>(a.dy, at + col[e], n[e], t[e]);
+    if (a.d_gate && a.bpg == 0 && row + 1 == gend) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        store8_any(a.gate_type, a.d_gate, grow * a.d + col[e], n[e], s_gate[e]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s_gate[e][q] = 0.f;
+      }
+    }
+  }
+  if (!a.part) return;
+  // the workers' sums in their order, one vector after the other through LDS
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (k == 2 && (!a.d_gate || a.bpg == 0)) break;
+    float* dst = a.part + (k * a.blocks + blockIdx.x) * a.d;
+    if (R == 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) store8<LBK_FP32>(dst, col[e], n[e], k == 0 ? s_pre[e] : k == 1 ? s_post[e] : s_gate[e]);
+      continue;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < n[e]) sums[worker * a.d + col[e] + q] = k == 0 ? s_pre[e][q] : k == 1 ? s_post[e][q] : s_gate[e][q];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+      float v = sums[c];
+      for (int j = 1; j < R; ++j) v += sums[j * a.d + c];
+      dst[c] = v;
+    }
+  }
+}
+
+// d_pre, d_post (jobs 0 and 1) and the gate's rows (2 ..): sums of `part` over a job's workgroups
+struct SumArgs {
+  const float* part;
+  int64_t blocks, bpg;
+  int d, gate_type, chunks;         // chunks: workgroups of a job
+  float *d_pre, *d_post;
+  void* d_gate;
+};
+
+__global__ __launch_bounds__(1024) void seam_sum_kernel(SumArgs a) {
+  __shared__ float sums[16][64];
+  const int64_t job = blockIdx.x / a.chunks;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = (int)(blockIdx.x - job * a.chunks) * 64 + lane;
+  const int64_t first = job < 2 ? job * a.blocks : 2 * a.blocks + (job - 2) * a.bpg, count = job < 2 ? a.blocks : a.bpg;
+  const bool wanted = job == 0 ? a.d_pre != nullptr : job == 1 ? a.d_post != nullptr : true;
+  if (!wanted) return;
+  float v = 0.f;
+  if (c < a.d)
+    for (int64_t b = w; b < count; b += 16) v += a.part[(first + b) * a.d + c];
+  sums[w][lane] = v;
+  __syncthreads();
+  if (w || c >= a.d) return;
+  for (int k = 1; k < 16; ++k) v += sums[k][lane];
+  if (job == 0) a.d_pre[c] = v;
+  else if (job == 1) a.d_post[c] = v;
+  else {
+    const int64_t at = (job - 2) * a.d + c;
+    if (a.gate_type == LBK_FP32) static_cast<float*>(a.d_gate)[at] = v;
+    else static_cast<uint16_t*>(a.d_gate)[at] = a.gate_type == LBK_BF16 ? from_f<LBK_BF16>(v) : from_f<LBK_FP16>(v);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
+inline int launched() { return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH; }
+inline bool elem_aligned(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == LBK_FP32 ? 3u : 1u)) == 0; }
+
+bool random_of(double p, const int64_t* seed_dev, int64_t seed, uint32_t stream, Random& r) {
+  if (!(p >= 0.0 && p <= 1.0)) return false;
+  r.seed_dev = seed_dev, r.seed = seed, r.stream = stream;
+  r.cut = (uint32_t)floor(p * 65536.0 + 0.5);
+  r.keep = (float)(65536.0 / (65536.0 - r.cut));     // unused at cut = 65536
+  return true;
+}
+
+// vectors of 8 a lane (E) and waves a row
+struct RowPlan {
+  int E, NW;
+};
+RowPlan row_plan(int d) {
+  if (d <= 512) return {1, 1};
+  if (d > 8192) return {4, 8};
+  int NW = 1;
+  while (NW * 1024 < d) NW *= 2;
+  return {2, NW};
+}
+
+// rows of a worker and workgroups of the backward
+struct BwdPlan {
+  RowPlan row;
+  int R;
+  int64_t W, blocks, bpg;
+};
+BwdPlan bwd_plan(int64_t N, int d, bool gate, int64_t gate_rows) {
+  BwdPlan p;
+  p.row = row_plan(d);
+  p.R = p.row.NW == 1 ? 4 : 1;
+  const int64_t target = p.R == 4 ? 512 : 1024;
+  const int64_t W = N / (target * p.R) > 0 ? (N + target * p.R - 1) / (target * p.R) : 1;
+  const int64_t per = gate ? N / gate_rows : N;
+  p.W = W;
+  if (!gate) {
+    p.bpg = 0;
+    p.blocks = (N + W * p.R - 1) / (W * p.R);
+  } else if (per >= W * p.R) {
+    p.bpg = (per + W * p.R - 1) / (W * p.R);
+    p.blocks = p.bpg * gate_rows;
+  } else {
+    p.W = W > per ? W / per * per : per;
+    p.bpg = 0;
+    p.blocks = (N + p.W * p.R - 1) / (p.W * p.R);
+  }
+  return p;
+}
+
+constexpr int MAX_D = 16384;
+
+int check_seam(const lbk_seam* s, SeamArgs& a) {
+  if (!s) return LBK_ERR_NULL;
+  const bool types = (s->state_type == s->type || s->state_type == LBK_FP32) && s->type >= LBK_BF16 && s->type <= LBK_FP32;
+  if (!types || s->N < 0 || !(s->eps >= 0.0f) || !random_of(s->p, s->seed_dev, s->seed, s->stream_id, a.r)) return LBK_ERR_ARG;
+  if (s->d <= 0) return LBK_ERR_SHAPE;
+  if (s->d > MAX_D || s->N > 0x7fffffff) return LBK_ERR_TOO_LARGE;
+  if (s->gate) {
+    if (s->gate_type < LBK_BF16 || s->gate_type > LBK_FP32) return LBK_ERR_ARG;
+    if (s->gate_rows <= 0 || s->N % s->gate_rows) return LBK_ERR_SHAPE;
+    if (!elem_aligned(s->gate, s->gate_type)) return LBK_ERR_ALIGN;
+  }
+  if (!elem_aligned(s->post_scale, LBK_FP32) || !elem_aligned(s->pre_scale, LBK_FP32)) return LBK_ERR_ALIGN;
+  a.N = s->N, a.d = s->d;
+  a.post = s->post_scale, a.pre = s->pre_scale;
+  a.gate = s->gate, a.gate_type = s->gate_type;
+  a.gate_rows = s->gate ? s->gate_rows : 1, a.per = a.N / a.gate_rows;
+  a.alpha = s->residual_scale, a.eps = s->eps;
+  return LBK_OK;
+}
+
+template <int TH, int TY, bool BWD>
+int launch_seam_t(const SeamArgs& a, int E, int64_t blocks, int threads, int lds, hipStream_t st) {
+  auto go = [&](auto* k) {
+    k<<<(unsigned)blocks, threads, lds, st>>>(a);
+    return launched();
+  };
+  const bool drop = a.r.cut > 0;
+  if constexpr (BWD) {
+    if (E == 1) return drop ? go(seam_bwd_kernel<TH, TY, 1, true>) : go(seam_bwd_kernel<TH, TY, 1, false>);
+    if (E == 2) return drop ? go(seam_bwd_kernel<TH, TY, 2, true>) : go(seam_bwd_kernel<TH, TY, 2, false>);
+    return drop ? go(seam_bwd_kernel<TH, TY, 4, true>) : go(seam_bwd_kernel<TH, TY, 4, false>);
+  } else {
+    if (E == 1) return drop ? go(seam_fwd_kernel<TH, TY, 1, true>) : go(seam_fwd_kernel<TH, TY, 1, false>);
+    if (E == 2) return drop ? go(seam_fwd_kernel<TH, TY, 2, true>) : go(seam_fwd_kernel<TH, TY, 2, false>);
+    return drop ? go(seam_fwd_kernel<TH, TY, 4, true>) : go(seam_fwd_kernel<TH, TY, 4, false>);
+  }
+}
+template <bool BWD>
+int launch_seam(int state, int type, const SeamArgs& a, int E, int64_t blocks, int threads, int lds, hipStream_t st) {
+  if (state == LBK_FP32) {
+    if (type == LBK_BF16) return launch_seam_t<LBK_FP32, LBK_BF16, BWD>(a, E, blocks, threads, lds, st);
+    if (type == LBK_FP16) return launch_seam_t<LBK_FP32, LBK_FP16, BWD>(a, E, blocks, threads, lds, st);
+    return launch_seam_t<LBK_FP32, LBK_FP32, BWD>(a, E, blocks, threads, lds, st);
+  }
+  if (type == LBK_BF16) return launch_seam_t<LBK_BF16, LBK_BF16, BWD>(a, E, blocks, threads, lds, st);
+  return launch_seam_t<LBK_FP16, LBK_FP16, BWD>(a, E, blocks, threads, lds, st);
+}
+
+}  // namespace
+}  // namespace lbk
+
+using namespace lbk;
+
+extern "C" {
+
+int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx, double p, const int64_t* seed_dev,
+                int64_t seed, uint32_t stream_id, void* y, void* stream) {
+  DropArgs a{};
+  if (dtype < LBK_BF16 || dtype > LBK_FP32 || N < 0 || ldx < F || !random_of(p, seed_dev, seed, stream_id, a.r)) return LBK_ERR_ARG;
+  if (F <= 0) return LBK_ERR_SHAPE;
+  if (N == 0) return LBK_OK;
+  if (!x || !y) return LBK_ERR_NULL;
+  if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype)) return LBK_ERR_ALIGN;
+  const int64_t G = ((int64_t)F + 7) / 8;
+  if (N > INT64_MAX / 64 / ldx || N > ((int64_t)0x7fffffff * 256) / G) return LBK_ERR_TOO_LARGE;
+  a.x = x, a.y = y, a.N = N, a.ldx = ldx, a.F = F, a.G = (int)G;
+  uint32_t s = 0;
+  while (((int64_t)1 << s) < G) ++s;
+  a.shift = 31 + s;
+  a.magic = (uint32_t)((((uint64_t)1 << a.shift) + G - 1) / G);
+  const int64_t blocks = (N * G + 256 * DROP_GROUPS - 1) / (256 * DROP_GROUPS);
+  const auto k = dtype == LBK_BF16 ? dropout_kernel<LBK_BF16> : dtype == LBK_FP16 ? dropout_kernel<LBK_FP16> : dropout_kernel<LBK_FP32>;
+  k<<<(unsigned)blocks, 256, 0, S(stream)>>>(a);
+  return launched();
+}
+
+int lbk_residual_norm_fwd(const lbk_seam* s, const void* h, const void* y, void* h_out, void* n_out, float* rs_post,
+                          float* rs_pre, void* stream) {
+  SeamArgs a{};
+  if (int st = check_seam(s, a)) return st;
+  if (a.N == 0) return LBK_OK;
+  if (!h || !y || !h_out || (a.pre && !n_out)) return LBK_ERR_NULL;
+  if (!elem_aligned(h, s->state_type) || !elem_aligned(h_out, s->state_type) || !elem_aligned(y, s->type) ||
+      !elem_aligned(n_out, s->type) || !elem_aligned(rs_post, LBK_FP32) || !elem_aligned(rs_pre, LBK_FP32))
+    return LBK_ERR_ALIGN;
+  a.h = h, a.y = y, a.h_out = h_out, a.n_out = n_out, a.rs_post = rs_post, a.rs_pre = rs_pre;
+  const RowPlan p = row_plan(a.d);
+  a.NW = p.NW;
+  const int R = p.NW == 1 ? 4 : 1;
+  return launch_seam<false>(s->state_type, s->type, a, p.E, (a.N + R - 1) / R, 64 * p.NW * R, 0, S(stream));
+}
+
+size_t lbk_residual_norm_bwd_workspace_bytes(const lbk_seam* s) {
+  SeamArgs a{};
+  if (check_seam(s, a)) return 0;
+  if (a.N == 0) return 0;
+  const BwdPlan p = bwd_plan(a.N, a.d, a.gate != nullptr, a.gate_rows);
+  return ((size_t)3 * p.blocks * a.d * 4 + 255) & ~(size_t)255;
+}
+
+int lbk_residual_norm_bwd(const lbk_seam* s, const void* h, const void* y, const float* rs_post, const float* rs_pre,
+                          const void* dh_out, const void* dn, void* dh, void* dy, float* d_post, void* d_gate, float* d_pre,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  SeamArgs a{};
+  if (int st = check_seam(s, a)) return st;
+  if ((dn && !a.pre) || (d_pre && !a.pre) || (d_post && !a.post) || (d_gate && !a.gate)) return LBK_ERR_ARG;
+  if (a.N > 0 && (!y || (dn && (!h || !rs_pre)) || (a.post && !rs_post))) return LBK_ERR_NULL;
+  if (!elem_aligned(y, s->type) || !elem_aligned(h, s->state_type) || !elem_aligned(dh_out, s->state_type) ||
+      !elem_aligned(dn, s->type) || !elem_aligned(dh, s->state_type) || !elem_aligned(dy, s->type) ||
+      !elem_aligned(d_gate, s->gate_type) || !elem_aligned(d_post, LBK_FP32) || !elem_aligned(d_pre, LBK_FP32) ||
+      !elem_aligned(rs_post, LBK_FP32) || !elem_aligned(rs_pre, LBK_FP32) || !elem_aligned(workspace, LBK_FP32))
+    return LBK_ERR_ALIGN;
+  const bool vectors = d_post || d_gate || d_pre;
+  const size_t need = vectors ? lbk_residual_norm_bwd_workspace_bytes(s) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return LBK_ERR_WORKSPACE;
+  BwdPlan p{};
+  if (a.N > 0) {
+    p = bwd_plan(a.N, a.d, a.gate != nullptr, a.gate_rows);
+    a.NW = p.row.NW, a.W = p.W, a.blocks = p.blocks, a.bpg = p.bpg;
+    a.h = h, a.y = y, a.rs_post = const_cast<float*>(rs_post), a.rs_pre = const_cast<float*>(rs_pre);
+    a.dh_out = dh_out, a.dn = dn, a.dh = dh, a.dy = dy, a.d_gate = d_gate;
+    a.part = vectors ? static_cast<float*>(workspace) : nullptr;
+    const int lds = p.R > 1 ? p.R * a.d * 4 : 0;      // at most 16 KB
+    if (int st = launch_seam<true>(s->state_type, s->type, a, p.row.E, p.blocks, 64 * p.row.NW * p.R, lds, S(stream))) return st;
+  }
+  if (!vectors) return LBK_OK;
+  SumArgs m{static_cast<float*>(workspace), p.blocks, p.bpg, a.d, a.gate_type, (a.d + 63) / 64, d_pre, d_post, d_gate};
+  // a gate without rows has no gradients to write, but for the one row that stands for none
+  const int64_t jobs = 2 + (d_gate && (p.bpg || a.N == 0) ? a.gate_rows : 0);
+  if (jobs * m.chunks > 0x7fffffff) return LBK_ERR_TOO_LARGE;
+  seam_sum_kernel<<<(unsigned)(jobs * m.chunks), 1024, 0, S(stream)>>>(m);
+  return launched();
+}
+
+}  // extern "C"

@@ -7,21 +7,10 @@ namespace {
 using at::Tensor;
 using OptTensor = c10::optional<at::Tensor>;
 
-int32_t elem_type(at::ScalarType t, const char* op, const char* name) {
-  TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, "titan::", op, ": ", name,
-              " must be bf16, fp16 or fp32, got ", t);
-  return t == at::kBFloat16 ? LBK_BF16 : t == at::kHalf ? LBK_FP16 : LBK_FP32;
-}
-
 // contiguous and 16-byte aligned (a view may start anywhere in its storage)
 Tensor dense16(const Tensor& t) {
   Tensor c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.data_ptr()) & 15 ? c.clone() : c;
-}
-
-void check_with(const Tensor& t, const Tensor& x, const char* op, const char* name) {
-  check_gpu(t, op, name);
-  TORCH_CHECK(t.device() == x.device(), "titan::", op, ": ", name, " is on ", t.device(), ", the input on ", x.device());
 }
 
 // of a weight [R, K, ...]

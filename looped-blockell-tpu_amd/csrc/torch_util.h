@@ -1,4 +1,4 @@
-// torch_util.h — what the operator registrations (torch_ops.cpp, torch_ffn.cpp) share: the current
+// torch_util.h — what the operator registrations (torch_ops.cpp, torch_ffn.cpp, torch_seam.cpp) share: the current
 // stream, status codes as errors, argument checks, workspaces.
 #pragma once
 
@@ -32,6 +32,17 @@ inline uint16_t* bfm(at::Tensor& t) { return reinterpret_cast<uint16_t*>(t.data_
 
 inline void check_gpu(const at::Tensor& t, const char* op, const char* name) {
   TORCH_CHECK(t.is_cuda(), "titan::", op, ": ", name, " must be a GPU (HIP) tensor");
+}
+
+inline void check_with(const at::Tensor& t, const at::Tensor& x, const char* op, const char* name) {
+  check_gpu(t, op, name);
+  TORCH_CHECK(t.device() == x.device(), "titan::", op, ": ", name, " is on ", t.device(), ", the input on ", x.device());
+}
+
+inline int32_t elem_type(at::ScalarType t, const char* op, const char* name) {
+  TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, "titan::", op, ": ", name,
+              " must be bf16, fp16 or fp32, got ", t);
+  return t == at::kBFloat16 ? LBK_BF16 : t == at::kHalf ? LBK_FP16 : LBK_FP32;
 }
 
 // a size as the C ABI's 32-bit argument

@@ -68,6 +68,15 @@ class CoreBlock(C.Structure):
                 ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("b_down", C.c_void_p)]
 
 
+class Seam(C.Structure):
+    """``lbk_seam``: the operands and options of the residual seam."""
+
+    _fields_ = [("N", C.c_int64), ("d", C.c_int32), ("state_type", C.c_int32), ("type", C.c_int32),
+                ("post_scale", C.c_void_p), ("pre_scale", C.c_void_p), ("gate", C.c_void_p), ("gate_type", C.c_int32),
+                ("gate_rows", C.c_int64), ("residual_scale", C.c_float), ("eps", C.c_float), ("p", C.c_double),
+                ("seed_dev", C.c_void_p), ("seed", C.c_int64), ("stream_id", C.c_uint32)]
+
+
 # (name, restype, argtypes) for every entry point of include/lbk.h
 _P = C.c_void_p
 _I64 = C.c_int64
@@ -77,6 +86,7 @@ _F = C.c_float
 _PB = C.POINTER(Bell)
 _PT = C.POINTER(BellTernary)
 _PM = C.POINTER(BellMx)
+_PS = C.POINTER(Seam)
 SIGNATURES = {
     "lbk_status_string": (C.c_char_p, [C.c_int]),
     "lbk_version": (C.c_int, []),
@@ -182,6 +192,10 @@ SIGNATURES = {
     "lbk_gated_bwd_workspace_bytes": (_SZ, [_I64, _I32, _I32]),
     "lbk_gated_bwd": (C.c_int, [_I32, _P, _P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P, C.c_int, _P, _P, _P, _P, _P,
                                 _SZ, _P]),
+    "lbk_dropout": (C.c_int, [_P, _I32, _I64, _I32, _I64, C.c_double, _P, _I64, C.c_uint32, _P, _P]),
+    "lbk_residual_norm_fwd": (C.c_int, [_PS, _P, _P, _P, _P, _P, _P, _P]),
+    "lbk_residual_norm_bwd_workspace_bytes": (_SZ, [_PS]),
+    "lbk_residual_norm_bwd": (C.c_int, [_PS, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -529,3 +529,49 @@ def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", add_residual: b
     else:
         y = ops().gated_ffn_fwd(x2, w_gate, w_up, w_down, activation, add_residual)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], y.shape[-1])
+
+
+# ---------------------------------------------------------------- around the FFN
+
+def _seed(seed):
+    """(seed tensor or None, seed as a signed 64-bit number) of an int or a GPU tensor of one int64."""
+    if isinstance(seed, torch.Tensor):
+        return seed, 0
+    return None, (int(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+
+def dropout(x, p: float, seed, stream: int = 0):
+    """Zeros each element of x [..., F] (bf16, fp16 or fp32) with probability p (in steps of 2^-16) and scales the
+    others by 1 / (1 - p).  The mask follows from ``seed`` (an int, or an int64 tensor of one element on x's GPU,
+    which a replayed graph reads anew), ``stream`` (0 .. 2^32 - 1: of calls that share a seed) and an element's row and
+    column (rows counted over the leading dimensions), as ``include/lbk.h`` defines; it is never stored.
+    Differentiable: the backward makes the same mask again."""
+    _gpu(x)
+    return ops().counter_dropout(x, float(p), *_seed(seed), int(stream))
+
+
+def residual_norm(h, y, post_scale=None, gate=None, pre_scale=None, residual_scale: float = 1.0, eps: float = 1e-5,
+                  p: float = 0.0, seed=0, stream: int = 0):
+    """The seam between two applications of a residual block, in one pass: ``(h', n)`` with
+
+      z  = y / sqrt(mean(y^2) + eps) * post_scale         (y itself without ``post_scale``)
+      h' = h + residual_scale * gate * dropout(z, p, seed, stream)
+      n  = h' / sqrt(mean(h'^2) + eps) * pre_scale        (None without ``pre_scale``)
+
+    h and y are [..., d], h of y's type or fp32 (the state of a looped block); h' is of h's type, n of y's and formed of
+    h' before that is rounded.  ``gate`` is [d], or [G, d] with one row for every N / G consecutive rows (a sequence's, a
+    token's).  ``post_scale`` and ``pre_scale`` are [d], used in fp32.  Differentiable in h, y and the three vectors."""
+    _gpu(h, y)
+    h2, y2 = (t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) for t in (h, y))
+    if h.shape != y.shape:
+        raise RuntimeError(f"h and y must have one shape, got {tuple(h.shape)} and {tuple(y.shape)}")
+    args = (h2, y2, post_scale, gate, pre_scale, float(residual_scale), float(eps), float(p), *_seed(seed), int(stream))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, y, post_scale, gate, pre_scale)):
+        _no_transforms()
+        hn, n = ops().residual_norm_train(*args)
+    else:
+        hn, n = ops().residual_norm(*args)
+    if h.dim() != 2:
+        hn = hn.reshape(h.shape)
+        n = n if pre_scale is None else n.reshape(h.shape)
+    return hn, (None if pre_scale is None else n)
