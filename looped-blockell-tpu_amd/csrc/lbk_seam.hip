@@ -76,23 +76,75 @@ __device__ __forceinline__ typename Elem<T>::type from_f(float f) {
   else return __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-template <int T>
-__device__ __forceinline__ void load8(const void* base, int64_t at, int n, float (&f)[8]) {
-  const auto* p = static_cast<const typename Elem<T>::type*>(base) + at;
-  if (n >= 8) {
-    if constexpr (T == LBK_FP32) {
-      const f32x4 a = *reinterpret_cast<const f32x4_4*>(p), b = *reinterpret_cast<const f32x4_4*>(p + 4);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f[q] = a[q], f[4 + q] = b[q];
-    } else {
-      const u32x4 v = *reinterpret_cast<const u32x4_2*>(p);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f[2 * q] = to_f<T>((uint16_t)v[q]), f[2 * q + 1] = to_f<T>((uint16_t)(v[q] >> 16));
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) f[q] = q < n ? to_f<T>(p[q]) : 0.0f;
+// A lane's 8 columns of a row of d, the last of them perhaps behind the row's end.  Such a lane loads the row's last 8
+// and moves them to their places after the wait: with loads one by one under a condition the waves that hold a row's end
+// wait for every array in turn (4097 x 1001, backward: 31.2 -> 28.1 us).
+struct Cols {
+  int col, n, from, shift;      // first column, columns there (< 8 or negative: the end), column loaded from, places to move by
+  bool tail;                    // of any lane of the wave
+  __device__ __forceinline__ Cols() {}
+  __device__ __forceinline__ Cols(int c, int d) : col(c), n(d - c) {
+    from = min(c, max(d - 8, 0));
+    shift = d >= 8 && n > 0 && n < 8 ? 8 - n : 0;
+    tail = __any(n < 8);
   }
+};
+
+// as loaded, so that a load can be in flight while something else is worked on
+template <int T> struct Raw8 { u32x4 v[T == LBK_FP32 ? 2 : 1]; };
+
+// SMALL: d may be less than 8 (one lane holds the row)
+template <int T, bool SMALL = false>
+__device__ __forceinline__ void fetch8(const void* base, int64_t row, int d, const Cols& c, Raw8<T>& r) {
+  // a base that all lanes share and 32-bit offsets: one register of an address in a lane
+  const auto* p = static_cast<const typename Elem<T>::type*>(base) + row * d;
+  if (!SMALL || d >= 8) {
+    const auto* q = reinterpret_cast<const u32x4_2*>(reinterpret_cast<const char*>(p) + (uint32_t)c.from * (uint32_t)sizeof(*p));
+    r.v[0] = q[0];
+    if constexpr (T == LBK_FP32) r.v[1] = q[1];
+    return;
+  }
+  uint32_t e[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    if constexpr (T == LBK_FP32) e[q] = __float_as_uint(p[min(q, d - 1)]);
+    else e[q] = p[min(q, d - 1)];
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (T == LBK_FP32) r.v[0][q] = e[q], r.v[1][q] = e[4 + q];
+    else r.v[0][q] = e[2 * q] | e[2 * q + 1] << 16;
+  }
+}
+template <int K>
+__device__ __forceinline__ void move_down(float (&f)[8], int shift) {
+  const uint32_t by = shift & K ? ~0u : 0u;
+#pragma unroll
+  for (int q = 0; q + K < 8; ++q) f[q] = __uint_as_float((__float_as_uint(f[q + K]) & by) | (__float_as_uint(f[q]) & ~by));
+}
+// ODD: a row's last columns may be fewer than 8; else a lane has all of its columns or none
+template <int T, bool ODD = true>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, const Cols& c, float (&f)[8]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (T == LBK_FP32) f[q] = __uint_as_float(r.v[0][q]), f[4 + q] = __uint_as_float(r.v[1][q]);
+    else f[2 * q] = to_f<T>((uint16_t)r.v[0][q]), f[2 * q + 1] = to_f<T>((uint16_t)(r.v[0][q] >> 16));
+  }
+  if (c.tail) {
+    if constexpr (ODD) {
+      move_down<4>(f, c.shift);
+      move_down<2>(f, c.shift);
+      move_down<1>(f, c.shift);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = (ODD ? q < c.n : c.n > 0) ? f[q] : 0.0f;
+  }
+}
+template <int T, bool ODD = true>
+__device__ __forceinline__ void load8(const void* base, int64_t row, int d, const Cols& c, float (&f)[8]) {
+  Raw8<T> r;
+  fetch8<T>(base, row, d, c, r);
+  unpack8<T, ODD>(r, c, f);
 }
 
 __device__ __forceinline__ uint32_t pack2_f16(float lo, float hi) {
@@ -100,10 +152,11 @@ __device__ __forceinline__ uint32_t pack2_f16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-template <int T>
-__device__ __forceinline__ void store8(void* base, int64_t at, int n, const float (&f)[8]) {
-  auto* p = static_cast<typename Elem<T>::type*>(base) + at;
-  if (n >= 8) {
+template <int T, bool ODD = true>
+__device__ __forceinline__ void store8(void* base, int64_t row, int d, const Cols& c, const float (&f)[8]) {
+  auto* b = static_cast<typename Elem<T>::type*>(base) + row * d;
+  auto* p = reinterpret_cast<decltype(b)>(reinterpret_cast<char*>(b) + (uint32_t)c.col * (uint32_t)sizeof(*b));
+  if (c.n >= 8) {
     if constexpr (T == LBK_FP32) {
       *reinterpret_cast<f32x4_4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
       *reinterpret_cast<f32x4_4*>(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
@@ -114,23 +167,25 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int n, const floa
         v[q] = T == LBK_BF16 ? pack2_bf16(f[2 * q], f[2 * q + 1]) : pack2_f16(f[2 * q], f[2 * q + 1]);
       *reinterpret_cast<u32x4_2*>(p) = v;
     }
-  } else {
+  } else if constexpr (ODD) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (q < n) p[q] = from_f<T>(f[q]);
+    for (int q = 0; q < 7; ++q)
+      if (q < c.n) p[q] = from_f<T>(f[q]);
   }
 }
 
 // of a type known at run time only (the gate's)
-__device__ __forceinline__ void load8_any(int type, const void* base, int64_t at, int n, float (&f)[8]) {
-  if (type == LBK_FP32) load8<LBK_FP32>(base, at, n, f);
-  else if (type == LBK_BF16) load8<LBK_BF16>(base, at, n, f);
-  else load8<LBK_FP16>(base, at, n, f);
+template <bool ODD>
+__device__ __forceinline__ void load8_any(int type, const void* base, int64_t row, int d, const Cols& c, float (&f)[8]) {
+  if (type == LBK_FP32) load8<LBK_FP32, ODD>(base, row, d, c, f);
+  else if (type == LBK_BF16) load8<LBK_BF16, ODD>(base, row, d, c, f);
+  else load8<LBK_FP16, ODD>(base, row, d, c, f);
 }
-__device__ __forceinline__ void store8_any(int type, void* base, int64_t at, int n, const float (&f)[8]) {
-  if (type == LBK_FP32) store8<LBK_FP32>(base, at, n, f);
-  else if (type == LBK_BF16) store8<LBK_BF16>(base, at, n, f);
-  else store8<LBK_FP16>(base, at, n, f);
+template <bool ODD>
+__device__ __forceinline__ void store8_any(int type, void* base, int64_t row, int d, const Cols& c, const float (&f)[8]) {
+  if (type == LBK_FP32) store8<LBK_FP32, ODD>(base, row, d, c, f);
+  else if (type == LBK_BF16) store8<LBK_BF16, ODD>(base, row, d, c, f);
+  else store8<LBK_FP16, ODD>(base, row, d, c, f);
 }
 
 // ------------------------------------------------------------------ dropout
@@ -145,21 +200,29 @@ struct DropArgs {
 
 constexpr int DROP_GROUPS = 4;  // of a thread
 
-template <int T>
+template <int T, bool SMALL>
 __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
   const uint64_t key = (uint64_t)(a.r.seed_dev ? *a.r.seed_dev : a.r.seed);
   const int64_t first = (int64_t)blockIdx.x * (256 * DROP_GROUPS), row0 = first / a.G;
   const uint32_t g0 = (uint32_t)(first - row0 * a.G) + threadIdx.x;
+  Raw8<T> raw[DROP_GROUPS];
+  Cols c[DROP_GROUPS];
+  int64_t row[DROP_GROUPS];
 #pragma unroll
   for (int k = 0; k < DROP_GROUPS; ++k) {
-    const uint32_t off = g0 + 256 * k, dr = (uint32_t)((uint64_t)off * a.magic >> a.shift), g = off - dr * a.G;
-    const int64_t row = row0 + dr;
-    if (row >= a.N) return;
-    const int n = a.F - 8 * (int)g;
+    const uint32_t off = g0 + 256 * k, dr = (uint32_t)((uint64_t)off * a.magic >> a.shift);
+    row[k] = row0 + dr;
+    c[k] = Cols(8 * (int)(off - dr * a.G), a.F);
+    const bool there = row[k] < a.N;
+    if (!there) c[k].n = 0;
+    fetch8<T, SMALL>(static_cast<const char*>(a.x) + (there ? row[k] : 0) * a.ldx * sizeof(typename Elem<T>::type), 0, a.F, c[k], raw[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < DROP_GROUPS; ++k) {
     float f[8];
-    load8<T>(a.x, row * a.ldx + 8 * (int64_t)g, n, f);
-    drop8(f, random8(key, g, row, a.r.stream), a.r.cut, a.r.keep);
-    store8<T>(a.y, row * a.F + 8 * (int64_t)g, n, f);
+    unpack8<T>(raw[k], c[k], f);
+    drop8(f, random8(key, (uint32_t)c[k].col >> 3, row[k], a.r.stream), a.r.cut, a.r.keep);
+    store8<T>(a.y, row[k], a.F, c[k], f);
   }
 }
 
@@ -185,19 +248,20 @@ __device__ __forceinline__ float wave_reduce(float x) {
   return Op::of(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
-// A row belongs to NW waves (those of a workgroup where NW > 1), a lane's E vectors of 8 columns lie 512 NW apart.
+// A row belongs to NW waves of a workgroup, `first` and those behind it; a lane's E vectors of 8 columns lie 512 NW
+// apart.
 struct RowSum {
   float (*buf)[16];
-  int NW, w, turn;
+  int NW, first, wave, turn;
   template <class Op>
   __device__ __forceinline__ float over(float x) {
     x = wave_reduce<Op>(x);
     if (NW == 1) return x;
     turn ^= 1;                        // two buffers: a wave that is a reduction ahead writes the other
-    if ((threadIdx.x & 63) == 0) buf[turn][w] = x;
+    if ((threadIdx.x & 63) == 0) buf[turn][wave] = x;
     __syncthreads();
-    float v = buf[turn][0];
-    for (int k = 1; k < NW; ++k) v = Op::of(v, buf[turn][k]);
+    float v = buf[turn][first];
+    for (int k = 1; k < NW; ++k) v = Op::of(v, buf[turn][first + k]);
     return v;
   }
 };
@@ -254,22 +318,27 @@ struct SeamArgs {
   int64_t W, blocks, bpg;       // rows of a worker, workgroups, workgroups of a gate row (0: gate rows lie in workers)
 };
 
-template <int TH, int TY, int E, bool DROP>
+template <int TH, int TY, int E, bool DROP, bool ODD>
 __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
   __shared__ float buf[2][16];
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
   const int worker = a.NW == 1 ? wv : 0, w = a.NW == 1 ? 0 : wv, R = a.NW == 1 ? (int)(blockDim.x >> 6) : 1;
-  RowSum rows{buf, a.NW, w, 0};
+  RowSum rows{buf, a.NW, 0, w, 0};
   const int64_t row = (int64_t)blockIdx.x * R + worker;
   if (row >= a.N) return;           // one worker a workgroup where there are barriers
   float h[E][8], y[E][8];
-  int col[E], n[E];
+  Cols c[E];
+  {
+    Raw8<TY> ry[E];
+    Raw8<TH> rh[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    col[e] = 8 * ((e * a.NW + w) * 64 + lane);
-    n[e] = a.d - col[e];
-    load8<TY>(a.y, row * a.d + col[e], n[e], y[e]);
-    load8<TH>(a.h, row * a.d + col[e], n[e], h[e]);
+    for (int e = 0; e < E; ++e) {
+      c[e] = Cols(8 * ((e * a.NW + w) * 64 + lane), a.d);
+      fetch8<TY>(a.y, row, a.d, c[e], ry[e]);
+      fetch8<TH>(a.h, row, a.d, c[e], rh[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) unpack8<TY, ODD>(ry[e], c[e], y[e]), unpack8<TH, ODD>(rh[e], c[e], h[e]);
   }
   if (a.post) {
     const float rs = row_rs<E>(y, a.d, a.eps, rows);
@@ -277,7 +346,7 @@ __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float p[8];
-      load8<LBK_FP32>(a.post, col[e], n[e], p);
+      load8<LBK_FP32, ODD>(a.post, 0, a.d, c[e], p);
 #pragma unroll
       for (int q = 0; q < 8; ++q) y[e][q] = y[e][q] * rs * p[q];
     }
@@ -286,16 +355,16 @@ __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
   const int64_t grow = a.gate ? (a.gate_rows == 1 ? 0 : (int64_t)((uint32_t)row / (uint32_t)a.per)) : 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if constexpr (DROP) drop8(y[e], random8(key, (uint32_t)col[e] >> 3, row, a.r.stream), a.r.cut, a.r.keep);
+    if constexpr (DROP) drop8(y[e], random8(key, (uint32_t)c[e].col >> 3, row, a.r.stream), a.r.cut, a.r.keep);
     if (a.gate) {
       float g[8];
-      load8_any(a.gate_type, a.gate, grow * a.d + col[e], n[e], g);
+      load8_any<ODD>(a.gate_type, a.gate, grow, a.d, c[e], g);
 #pragma unroll
       for (int q = 0; q < 8; ++q) y[e][q] *= g[q];
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) h[e][q] += a.alpha * y[e][q];
-    store8<TH>(a.h_out, row * a.d + col[e], n[e], h[e]);
+    store8<TH, ODD>(a.h_out, row, a.d, c[e], h[e]);
   }
   if (a.pre) {
     const float rs = row_rs<E>(h, a.d, a.eps, rows);
@@ -303,10 +372,10 @@ __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float p[8];
-      load8<LBK_FP32>(a.pre, col[e], n[e], p);
+      load8<LBK_FP32, ODD>(a.pre, 0, a.d, c[e], p);
 #pragma unroll
       for (int q = 0; q < 8; ++q) h[e][q] = h[e][q] * rs * p[q];
-      store8<TY>(a.n_out, row * a.d + col[e], n[e], h[e]);
+      store8<TY, ODD>(a.n_out, row, a.d, c[e], h[e]);
     }
   }
 }
@@ -316,16 +385,16 @@ __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
 //   t  = dh' + rs(h') (q - x2 mean(q x2)) = dh          d_pre  = sum of dn x2
 //   s  = alpha gate t, dropped as z was                 d_gate = sum of alpha t drop(z), d_post = sum of s x1
 //   dy = rs(y) (v - x1 mean(v x1)),  v = w_post s
-// A workgroup takes consecutive rows, a worker (one wave, or all of them) W of these, and keeps the columns' sums in
-// registers.  Sums go to `part`, one row a workgroup, and are added in a fixed order by seam_sum_kernel: no atomics.  A
+// A workgroup takes consecutive rows, a worker (NW waves) W of these, and keeps the columns' sums in registers; the
+// next row's loads are in flight while a row is worked on.  Sums go to `part`, one row a workgroup, and are added in a fixed order by seam_sum_kernel: no atomics.  A
 // gate's rows either lie in one worker each (bpg = 0: written at once) or take bpg workgroups each.
-template <int TH, int TY, int E, bool DROP>
+template <int TH, int TY, int E, bool DROP, bool ODD>
 __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
   __shared__ float buf[2][16];
   extern __shared__ float sums[];   // [workers][d]
-  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6);
-  const int worker = a.NW == 1 ? wv : 0, w = a.NW == 1 ? 0 : wv, R = a.NW == 1 ? (int)(blockDim.x >> 6) : 1;
-  RowSum rows{buf, a.NW, w, 0};
+  const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6), R = (int)(blockDim.x >> 6) / a.NW;
+  const int worker = uniform(wv / a.NW), w = wv - worker * a.NW;
+  RowSum rows{buf, a.NW, worker * a.NW, wv, 0};
   int64_t r0, end;
   if (a.bpg) {                      // workgroups of one gate row
     const int64_t g = blockIdx.x / a.bpg, c = blockIdx.x - g * a.bpg;
@@ -337,27 +406,41 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
   }
   const uint64_t key = DROP ? (uint64_t)(a.r.seed_dev ? *a.r.seed_dev : a.r.seed) : 0;
   float s_pre[E][8] = {}, s_post[E][8] = {}, s_gate[E][8] = {};
-  int col[E], n[E];
+  Cols c[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    col[e] = 8 * ((e * a.NW + w) * 64 + lane);
-    n[e] = a.d - col[e];
-  }
+  for (int e = 0; e < E; ++e) c[e] = Cols(8 * ((e * a.NW + w) * 64 + lane), a.d);
   int64_t grow = a.gate && a.gate_rows > 1 && r0 < a.N ? r0 / a.per : 0, gend = (grow + 1) * a.per;
-  for (int64_t row = r0; row < end; ++row) {
-    const int64_t at = row * a.d;
-    if (a.gate && row >= gend) ++grow, gend += a.per;
-    const float rs1 = a.post ? a.rs_post[row] : 1.0f;
+  Raw8<TH> rt[E], rh[E];
+  Raw8<TY> ry[E], rv[E];
+  // y and dn for the next row are loaded once this row's are unpacked, dh and h once the first sum has taken h's place
+  auto fetch_y = [&](int64_t row) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      fetch8<TY>(a.y, row, a.d, c[e], ry[e]);
+      if (a.dn) fetch8<TY>(a.dn, row, a.d, c[e], rv[e]);
+    }
+  };
+  auto fetch_h = [&](int64_t row) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (a.dn) fetch8<TH>(a.h, row, a.d, c[e], rh[e]);
+      if (a.dh_out) fetch8<TH>(a.dh_out, row, a.d, c[e], rt[e]);
+    }
+  };
+  if (r0 < end) fetch_y(r0), fetch_h(r0);
+  // All workers make W turns, for the barriers of a row of many waves; one past its rows' end works on the last one
+  // that it fetched, for nobody.
+  for (int64_t row = r0; row < r0 + a.W; ++row) {
+    const bool ok = row < end;
+    if (!ok && a.NW == 1) break;
+    if (a.gate && ok && row >= gend) ++grow, gend += a.per;
+    const float rs1 = a.post && ok ? a.rs_post[row] : 1.0f, rs2 = a.dn && ok ? a.rs_pre[row] : 1.0f;
     float t[E][8], y[E][8], z[E][8], g[E][8];
     u32x4 rnd[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (a.dh_out) load8<TH>(a.dh_out, at + col[e], n[e], t[e]);
-      else
-#pragma unroll
-        for (int q = 0; q < 8; ++q) t[e][q] = 0.f;
-      load8<TY>(a.y, at + col[e], n[e], y[e]);
-      if (a.gate) load8_any(a.gate_type, a.gate, grow * a.d + col[e], n[e], g[e]);
+      unpack8<TY, ODD>(ry[e], c[e], y[e]);
+      if (a.gate) load8_any<ODD>(a.gate_type, a.gate, grow, a.d, c[e], g[e]);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         y[e][q] *= rs1;             // x1
@@ -366,55 +449,63 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
       }
       if (a.post) {
         float p[8];
-        load8<LBK_FP32>(a.post, col[e], n[e], p);
+        load8<LBK_FP32, ODD>(a.post, 0, a.d, c[e], p);
 #pragma unroll
         for (int q = 0; q < 8; ++q) z[e][q] *= p[q];
       }
       if constexpr (DROP) {
-        rnd[e] = random8(key, (uint32_t)col[e] >> 3, row, a.r.stream);
+        rnd[e] = random8(key, (uint32_t)c[e].col >> 3, row, a.r.stream);
         drop8(z[e], rnd[e], a.r.cut, a.r.keep);
       }
     }
+    float x[E][8], v[E][8];
+#pragma unroll
+    for (int e = 0; e < E; ++e) unpack8<TY, ODD>(rv[e], c[e], v[e]);
+    if (row + 1 < end) fetch_y(row + 1);
+    float dot = 0.f;
     if (a.dn) {
-      const float rs = a.rs_pre[row];
-      float x[E][8], v[E][8], dot = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         float p[8];
-        load8<TH>(a.h, at + col[e], n[e], x[e]);
-        load8<TY>(a.dn, at + col[e], n[e], v[e]);
-        load8<LBK_FP32>(a.pre, col[e], n[e], p);
+        load8<LBK_FP32, ODD>(a.pre, 0, a.d, c[e], p);
+        unpack8<TH, ODD>(rh[e], c[e], x[e]);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          x[e][q] = (x[e][q] + a.alpha * (z[e][q] * g[e][q])) * rs;
-          s_pre[e][q] += v[e][q] * x[e][q];
+          x[e][q] = (x[e][q] + a.alpha * (z[e][q] * g[e][q])) * rs2;
+          if (ok) s_pre[e][q] += v[e][q] * x[e][q];
           v[e][q] *= p[q];
           dot += v[e][q] * x[e][q];
         }
       }
       dot = rows.over<Add>(dot) / (float)a.d;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int q = 0; q < 8; ++q) t[e][q] += rs * (v[e][q] - x[e][q] * dot);
     }
-    float dot = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (a.dh) store8<TH>(a.dh, at + col[e], n[e], t[e]);
+      unpack8<TH, ODD>(rt[e], c[e], t[e]);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (!a.dh_out) t[e][q] = 0.f;
+        if (a.dn) t[e][q] += rs2 * (v[e][q] - x[e][q] * dot);
+      }
+    }
+    if (row + 1 < end) fetch_h(row + 1);
+    dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (a.dh && ok) store8<TH, ODD>(a.dh, row, a.d, c[e], t[e]);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         t[e][q] *= a.alpha;
-        s_gate[e][q] += t[e][q] * z[e][q];
+        if (ok) s_gate[e][q] += t[e][q] * z[e][q];
         t[e][q] *= g[e][q];
       }
       if constexpr (DROP) drop8(t[e], rnd[e], a.r.cut, a.r.keep);
       if (a.post) {
         float p[8];
-        load8<LBK_FP32>(a.post, col[e], n[e], p);
+        load8<LBK_FP32, ODD>(a.post, 0, a.d, c[e], p);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          s_post[e][q] += t[e][q] * y[e][q];
+          if (ok) s_post[e][q] += t[e][q] * y[e][q];
           t[e][q] *= p[q];
           dot += t[e][q] * y[e][q];
         }
@@ -427,13 +518,13 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) t[e][q] = rs1 * (t[e][q] - y[e][q] * dot);
     }
-    if (a.dy)
+    if (a.dy && ok)
 #pragma unroll
-      for (int e = 0; e < E; ++e) store8<TY>(a.dy, at + col[e], n[e], t[e]);
-    if (a.d_gate && a.bpg == 0 && row + 1 == gend) {
+      for (int e = 0; e < E; ++e) store8<TY, ODD>(a.dy, row, a.d, c[e], t[e]);
+    if (a.d_gate && a.bpg == 0 && ok && row + 1 == gend) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        store8_any(a.gate_type, a.d_gate, grow * a.d + col[e], n[e], s_gate[e]);
+        store8_any<ODD>(a.gate_type, a.d_gate, grow, a.d, c[e], s_gate[e]);
 #pragma unroll
         for (int q = 0; q < 8; ++q) s_gate[e][q] = 0.f;
       }
@@ -447,7 +538,7 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
     float* dst = a.part + (k * a.blocks + blockIdx.x) * a.d;
     if (R == 1) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) store8<LBK_FP32>(dst, col[e], n[e], k == 0 ? s_pre[e] : k == 1 ? s_post[e] : s_gate[e]);
+      for (int e = 0; e < E; ++e) store8<LBK_FP32, ODD>(dst, 0, a.d, c[e], k == 0 ? s_pre[e] : k == 1 ? s_post[e] : s_gate[e]);
       continue;
     }
     __syncthreads();
@@ -455,7 +546,7 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int q = 0; q < 8; ++q)
-        if (q < n[e]) sums[worker * a.d + col[e] + q] = k == 0 ? s_pre[e][q] : k == 1 ? s_post[e][q] : s_gate[e][q];
+        if (q < c[e].n) sums[worker * a.d + c[e].col + q] = k == 0 ? s_pre[e][q] : k == 1 ? s_post[e][q] : s_gate[e][q];
     __syncthreads();
     for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
       float v = sums[c];
@@ -474,26 +565,37 @@ struct SumArgs {
   void* d_gate;
 };
 
+// A workgroup sums 64 columns, 4 a lane, in 64 slices of the rows: 16-byte loads, eight of a thread in flight (2-byte
+// aligned as everywhere, for odd d).
 __global__ __launch_bounds__(1024) void seam_sum_kernel(SumArgs a) {
-  __shared__ float sums[16][64];
+  __shared__ f32x4 sums[64][16];
   const int64_t job = blockIdx.x / a.chunks;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = (int)(blockIdx.x - job * a.chunks) * 64 + lane;
+  const int lane = threadIdx.x & 15, slice = threadIdx.x >> 4, c0 = (int)(blockIdx.x - job * a.chunks) * 64, c = c0 + 4 * lane;
   const int64_t first = job < 2 ? job * a.blocks : 2 * a.blocks + (job - 2) * a.bpg, count = job < 2 ? a.blocks : a.bpg;
   const bool wanted = job == 0 ? a.d_pre != nullptr : job == 1 ? a.d_post != nullptr : true;
   if (!wanted) return;
-  float v = 0.f;
-  if (c < a.d)
-    for (int64_t b = w; b < count; b += 16) v += a.part[(first + b) * a.d + c];
-  sums[w][lane] = v;
+  f32x4 v = {0, 0, 0, 0};
+  const float* p = a.part + first * a.d + c;
+  if (c + 4 <= a.d) {
+#pragma unroll 8
+    for (int64_t b = slice; b < count; b += 64) v += *reinterpret_cast<const f32x4_4*>(p + b * a.d);
+  } else if (c < a.d) {
+    for (int64_t b = slice; b < count; b += 64)
+      for (int q = 0; q < a.d - c; ++q) v[q] += p[b * a.d + q];
+  }
+  sums[slice][lane] = v;
   __syncthreads();
-  if (w || c >= a.d) return;
-  for (int k = 1; k < 16; ++k) v += sums[k][lane];
-  if (job == 0) a.d_pre[c] = v;
-  else if (job == 1) a.d_post[c] = v;
+  if (threadIdx.x >= 64 || c0 + (int)threadIdx.x >= a.d) return;
+  const int col = c0 + threadIdx.x;
+  float t = 0.f;
+#pragma unroll 16
+  for (int k = 0; k < 64; ++k) t += sums[k][threadIdx.x >> 2][threadIdx.x & 3];
+  if (job == 0) a.d_pre[col] = t;
+  else if (job == 1) a.d_post[col] = t;
   else {
-    const int64_t at = (job - 2) * a.d + c;
-    if (a.gate_type == LBK_FP32) static_cast<float*>(a.d_gate)[at] = v;
-    else static_cast<uint16_t*>(a.d_gate)[at] = a.gate_type == LBK_BF16 ? from_f<LBK_BF16>(v) : from_f<LBK_FP16>(v);
+    const int64_t at = (job - 2) * a.d + col;
+    if (a.gate_type == LBK_FP32) static_cast<float*>(a.d_gate)[at] = t;
+    else static_cast<uint16_t*>(a.d_gate)[at] = a.gate_type == LBK_BF16 ? from_f<LBK_BF16>(t) : from_f<LBK_FP16>(t);
   }
 }
 
@@ -510,16 +612,17 @@ bool random_of(double p, const int64_t* seed_dev, int64_t seed, uint32_t stream,
   return true;
 }
 
-// vectors of 8 a lane (E) and waves a row
+// Vectors of 8 a lane (E) and waves a row: one vector up to the 8 waves of a workgroup.  Two in half as many waves spare
+// the barriers of a row of 1024 and measure the same forward (41.9 and 42.4 us at 16384 x 1024 with dropout, 78.8 and 79.0
+// backward), but a lone row of 4096 takes 4.0 us instead of 3.4, and the backward has no registers left.
 struct RowPlan {
   int E, NW;
 };
 RowPlan row_plan(int d) {
-  if (d <= 512) return {1, 1};
-  if (d > 8192) return {4, 8};
   int NW = 1;
-  while (NW * 1024 < d) NW *= 2;
-  return {2, NW};
+  const int E = d <= 4096 ? 1 : 2;
+  while (NW * 512 * E < d) NW *= 2;
+  return {E, NW};
 }
 
 // rows of a worker and workgroups of the backward
@@ -531,9 +634,10 @@ struct BwdPlan {
 BwdPlan bwd_plan(int64_t N, int d, bool gate, int64_t gate_rows) {
   BwdPlan p;
   p.row = row_plan(d);
-  p.R = p.row.NW == 1 ? 4 : 1;
-  const int64_t target = p.R == 4 ? 512 : 1024;
-  const int64_t W = N / (target * p.R) > 0 ? (N + target * p.R - 1) / (target * p.R) : 1;
+  // workgroups of four waves, three on a CU, as the kernel's registers allow (16384 x 1024: 75.4 us; eight waves, one on a
+  // CU: 78.4, four waves, two on a CU: 82.1); rows of eight waves one on a CU
+  p.R = p.row.NW < 4 ? 4 / p.row.NW : 1;
+  const int64_t most = p.row.NW == 8 ? 256 : 768, W = (N + most * p.R - 1) / (most * p.R);
   const int64_t per = gate ? N / gate_rows : N;
   p.W = W;
   if (!gate) {
@@ -550,13 +654,13 @@ BwdPlan bwd_plan(int64_t N, int d, bool gate, int64_t gate_rows) {
   return p;
 }
 
-constexpr int MAX_D = 16384;
+constexpr int MAX_D = 8192;
 
 int check_seam(const lbk_seam* s, SeamArgs& a) {
   if (!s) return LBK_ERR_NULL;
   const bool types = (s->state_type == s->type || s->state_type == LBK_FP32) && s->type >= LBK_BF16 && s->type <= LBK_FP32;
   if (!types || s->N < 0 || !(s->eps >= 0.0f) || !random_of(s->p, s->seed_dev, s->seed, s->stream_id, a.r)) return LBK_ERR_ARG;
-  if (s->d <= 0) return LBK_ERR_SHAPE;
+  if (s->d < 8) return LBK_ERR_SHAPE;
   if (s->d > MAX_D || s->N > 0x7fffffff) return LBK_ERR_TOO_LARGE;
   if (s->gate) {
     if (s->gate_type < LBK_BF16 || s->gate_type > LBK_FP32) return LBK_ERR_ARG;
@@ -572,22 +676,23 @@ int check_seam(const lbk_seam* s, SeamArgs& a) {
   return LBK_OK;
 }
 
-template <int TH, int TY, bool BWD>
-int launch_seam_t(const SeamArgs& a, int E, int64_t blocks, int threads, int lds, hipStream_t st) {
+template <int TH, int TY, int E, bool ODD, bool BWD>
+int launch_seam_e(const SeamArgs& a, int64_t blocks, int threads, int lds, hipStream_t st) {
   auto go = [&](auto* k) {
     k<<<(unsigned)blocks, threads, lds, st>>>(a);
     return launched();
   };
-  const bool drop = a.r.cut > 0;
-  if constexpr (BWD) {
-    if (E == 1) return drop ? go(seam_bwd_kernel<TH, TY, 1, true>) : go(seam_bwd_kernel<TH, TY, 1, false>);
-    if (E == 2) return drop ? go(seam_bwd_kernel<TH, TY, 2, true>) : go(seam_bwd_kernel<TH, TY, 2, false>);
-    return drop ? go(seam_bwd_kernel<TH, TY, 4, true>) : go(seam_bwd_kernel<TH, TY, 4, false>);
-  } else {
-    if (E == 1) return drop ? go(seam_fwd_kernel<TH, TY, 1, true>) : go(seam_fwd_kernel<TH, TY, 1, false>);
-    if (E == 2) return drop ? go(seam_fwd_kernel<TH, TY, 2, true>) : go(seam_fwd_kernel<TH, TY, 2, false>);
-    return drop ? go(seam_fwd_kernel<TH, TY, 4, true>) : go(seam_fwd_kernel<TH, TY, 4, false>);
+  if constexpr (BWD) return a.r.cut ? go(seam_bwd_kernel<TH, TY, E, true, ODD>) : go(seam_bwd_kernel<TH, TY, E, false, ODD>);
+  else return a.r.cut ? go(seam_fwd_kernel<TH, TY, E, true, ODD>) : go(seam_fwd_kernel<TH, TY, E, false, ODD>);
+}
+template <int TH, int TY, bool BWD>
+int launch_seam_t(const SeamArgs& a, int E, int64_t blocks, int threads, int lds, hipStream_t st) {
+  if (a.d % 8) {
+    return E == 1 ? launch_seam_e<TH, TY, 1, true, BWD>(a, blocks, threads, lds, st)
+                  : launch_seam_e<TH, TY, 2, true, BWD>(a, blocks, threads, lds, st);
   }
+  return E == 1 ? launch_seam_e<TH, TY, 1, false, BWD>(a, blocks, threads, lds, st)
+                : launch_seam_e<TH, TY, 2, false, BWD>(a, blocks, threads, lds, st);
 }
 template <bool BWD>
 int launch_seam(int state, int type, const SeamArgs& a, int E, int64_t blocks, int threads, int lds, hipStream_t st) {
@@ -623,9 +728,13 @@ int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx,
   a.shift = 31 + s;
   a.magic = (uint32_t)((((uint64_t)1 << a.shift) + G - 1) / G);
   const int64_t blocks = (N * G + 256 * DROP_GROUPS - 1) / (256 * DROP_GROUPS);
-  const auto k = dtype == LBK_BF16 ? dropout_kernel<LBK_BF16> : dtype == LBK_FP16 ? dropout_kernel<LBK_FP16> : dropout_kernel<LBK_FP32>;
-  k<<<(unsigned)blocks, 256, 0, S(stream)>>>(a);
-  return launched();
+  auto go = [&](auto* k) {
+    k<<<(unsigned)blocks, 256, 0, S(stream)>>>(a);
+    return launched();
+  };
+  if (dtype == LBK_BF16) return F < 8 ? go(dropout_kernel<LBK_BF16, true>) : go(dropout_kernel<LBK_BF16, false>);
+  if (dtype == LBK_FP16) return F < 8 ? go(dropout_kernel<LBK_FP16, true>) : go(dropout_kernel<LBK_FP16, false>);
+  return F < 8 ? go(dropout_kernel<LBK_FP32, true>) : go(dropout_kernel<LBK_FP32, false>);
 }
 
 int lbk_residual_norm_fwd(const lbk_seam* s, const void* h, const void* y, void* h_out, void* n_out, float* rs_post,

@@ -89,7 +89,7 @@ Seam make_seam(const Tensor& h, const Tensor& y, const OptTensor& post, const Op
   TORCH_CHECK(h.dim() == 2 && y.sizes() == h.sizes(), "titan::", op, ": h and y must be one [N, d], got ", h.sizes(), " and ", y.sizes());
   TORCH_CHECK(th == ty || th == LBK_FP32, "titan::", op, ": h is ", h.scalar_type(), ", y ", y.scalar_type(),
               "; h must be of y's type or fp32");
-  TORCH_CHECK(h.size(1) > 0, "titan::", op, ": no features");
+  TORCH_CHECK(h.size(1) >= 8 && h.size(1) <= 8192, "titan::", op, ": d must lie between 8 and 8192, got ", h.size(1));
   TORCH_CHECK(o.eps >= 0, "titan::", op, ": eps must not be negative, got ", o.eps);
   const int64_t N = h.size(0), d = h.size(1);
   Seam r;

@@ -558,7 +558,7 @@ def residual_norm(h, y, post_scale=None, gate=None, pre_scale=None, residual_sca
       h' = h + residual_scale * gate * dropout(z, p, seed, stream)
       n  = h' / sqrt(mean(h'^2) + eps) * pre_scale        (None without ``pre_scale``)
 
-    h and y are [..., d], h of y's type or fp32 (the state of a looped block); h' is of h's type, n of y's and formed of
+    h and y are [..., d] (d from 8 to 8192), h of y's type or fp32 (the state of a looped block); h' is of h's type, n of y's and formed of
     h' before that is rounded.  ``gate`` is [d], or [G, d] with one row for every N / G consecutive rows (a sequence's, a
     token's).  ``post_scale`` and ``pre_scale`` are [d], used in fp32.  Differentiable in h, y and the three vectors."""
     _gpu(h, y)

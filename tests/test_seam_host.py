@@ -74,8 +74,8 @@ def test_seam_validation_codes():
     assert lib.lbk_residual_norm_fwd(None, P, P, P, P, None, None, None) == A.LBK_ERR_NULL
     for a in (s(st=0, t=1), s(st=1, t=2), s(t=3), s(t=-1), s(N=-1), s(eps=-1e-3), s(eps=float("nan")), s(p=2.0), s(gate=P, gt=5)):
         assert fwd(a) == A.LBK_ERR_ARG
-    assert fwd(s(d=0)) == A.LBK_ERR_SHAPE and fwd(s(gate=P, rows=3)) == A.LBK_ERR_SHAPE and fwd(s(gate=P, rows=0)) == A.LBK_ERR_SHAPE
-    assert fwd(s(d=16385)) == A.LBK_ERR_TOO_LARGE and fwd(s(N=1 << 31)) == A.LBK_ERR_TOO_LARGE
+    assert fwd(s(d=7)) == A.LBK_ERR_SHAPE and fwd(s(gate=P, rows=3)) == A.LBK_ERR_SHAPE and fwd(s(gate=P, rows=0)) == A.LBK_ERR_SHAPE
+    assert fwd(s(d=8193)) == A.LBK_ERR_TOO_LARGE and fwd(s(N=1 << 31)) == A.LBK_ERR_TOO_LARGE
     assert fwd(s(), h=None) == A.LBK_ERR_NULL and fwd(s(), n=None) == A.LBK_ERR_NULL
     assert fwd(s(post=P + 2)) == A.LBK_ERR_ALIGN and fwd(s(st=2), h=P + 2) == A.LBK_ERR_ALIGN and fwd(s(), y=P + 1) == A.LBK_ERR_ALIGN
     assert fwd(s(gate=P + 1)) == A.LBK_ERR_ALIGN
