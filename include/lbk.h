@@ -895,6 +895,45 @@ int lbk_residual_norm_bwd(const lbk_seam* s, const void* h, const void* y, const
                           const void* dh_out, const void* dn, void* dh, void* dy, float* d_post, void* d_gate, float* d_pre,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Low-rank adapters of many requests beside one shared projection:
+ *   out[t] = y[t] + scales[a] * b[a] (a[a] x[t]),  a = ids[t];   out[t] = y[t] where ids[t] lies outside [0, n)
+ * x [N, in], y and out [N, out], a [n, rank, in], b [n, out, rank], all of one type (LBK_BF16 or LBK_FP16), scales [n] fp32
+ * or NULL (1).  Sums and a x are fp32 (a x and, in the backward, b^T dout enter the second products in 16 bits of
+ * mantissa).  in and out are multiples of 8, rank 1 .. 256, n 1 .. 4096, N up to 2^30; rows of x, y, out and dout have a
+ * stride in elements, rows and pointers are 16-byte aligned; out may be y.  No counterpart in the reference.
+ *
+ * The plan holds the tokens sorted by adapter (stable), for any number of projections of one batch: an opaque device
+ * buffer of lbk_adapter_plan_bytes(N, n) (0: sizes that are refused), 16-byte aligned, that the calls below read with
+ * the same N and n.  id_bytes: 4 or 8 (int32, int64).
+ */
+size_t lbk_adapter_plan_bytes(int64_t N, int32_t n_adapters);
+int lbk_adapter_plan(const void* ids, int32_t id_bytes, int64_t N, int32_t n_adapters, void* plan, size_t plan_bytes, void* stream);
+
+typedef struct lbk_adapter {
+    const void* a;
+    const void* b;
+    const float* scales;
+    const int32_t* plan;
+    int64_t N;
+    int32_t n, rank, in_features, out_features, type;
+} lbk_adapter;
+
+/* planes (lbk_adapter_planes_bytes, or NULL): scales * a x as the backward's db needs it. */
+size_t lbk_adapter_planes_bytes(const lbk_adapter* d);
+size_t lbk_adapter_add_workspace_bytes(const lbk_adapter* d);
+int lbk_adapter_add(const lbk_adapter* d, const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo,
+                    void* planes, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients for dout [N, out] (y's is dout itself): dx [N, in] contiguous (zero for tokens without an adapter), da and
+ * db like a and b (zero for adapters without tokens), each optional (db needs planes).  Sums over tokens run in a fixed
+ * order: no atomics.
+ */
+size_t lbk_adapter_bwd_workspace_bytes(const lbk_adapter* d);
+int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void* dout, int64_t ldo, const void* planes, void* dx,
+                    void* da, void* db, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,778 @@
+// lbk_adapter.hip — low-rank adapters of many requests beside a shared projection, out = y + s B (A x) with each
+// token's own A, B and s, with the backward (gfx950, bf16 or fp16 MFMA, fp32 sums), and the entry points of
+// include/lbk.h.
+//
+// Tokens are sorted by adapter once for all projections (the plan) and taken in tiles of up to 64 tokens of one adapter:
+//   shrink  t = A x of a tile, K in shares, fp32 partial sums          expand  out = y + B t', t' = s (sum of t's shares)
+//   grad    dA = dt'^T x, dB = dy^T t' over an adapter's tiles         with dt' = s B^T dy by shrink, dx = A^T dt' by expand
+// t' and dt' enter the second products as two bf16 each (the upper 16 bits and the rest, 16 bits of mantissa in all): in
+// one they would add as much error as the results' own rounding, and with ranks of 16 the second fills a half of the
+// matrix instruction's K that would lie idle.  fp16 operands beside them are split the same way, which is exact.
+#include "lbk.h"
+#include "lbk_device.h"
+#include "lbk_internal.h"
+
+#include <algorithm>
+
+namespace lbk {
+namespace {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int TILE = 64;             // tokens of a tile: four subtiles of a matrix instruction's 16
+constexpr int MAX_ADAPTERS = 4096, MAX_RANK = 256;
+
+// ------------------------------------------------------------------ the plan
+// int32 words: seg [n + 2] (first place of each bin; bin n holds the tokens without an adapter), tstart [n + 2] (first
+// tile), tiles [max_tiles] of {adapter or -1, first place, tokens, bins with tokens before}, perm [N] (place -> token).
+struct Tile {
+  int32_t adapter, first, count, ord;
+};
+
+__host__ __device__ inline int64_t max_tiles(int64_t N, int n) { return N / TILE + (N < n + 1 ? N : n + 1); }
+inline int64_t plan_words(int64_t N, int n) { return 2 * ((int64_t)n + 2 + ((n & 1) ? 1 : 0)) + 4 * max_tiles(N, n) + N + 4; }
+
+struct Plan {
+  const int32_t *seg, *tstart, *perm;
+  const Tile* tiles;
+};
+__host__ __device__ inline Plan plan_view(const int32_t* p, int64_t N, int n) {
+  const int64_t w = ((int64_t)n + 2 + 1) & ~(int64_t)1;        // even: the tiles lie on 16 bytes
+  const int32_t* tiles = p + 2 * w;
+  return {p, p + w, tiles + 4 * max_tiles(N, n), reinterpret_cast<const Tile*>(tiles)};
+}
+
+// A tile as a kernel may use it, whatever buffer was passed for the plan; adapter -1: none
+__device__ __forceinline__ Tile tile_at(const Plan& p, int64_t k, int64_t N, int n) {
+  Tile t = p.tiles[k];
+  t.adapter = t.adapter < 0 || t.adapter > n || t.count < 1 ? -1 : t.adapter;
+  t.first = min((uint32_t)t.first, (uint32_t)(N - 1));
+  t.count = min(t.count, min(TILE, (int)(N - t.first)));
+  return t;
+}
+__device__ __forceinline__ int64_t row_at(const Plan& p, int place, int64_t N) { return min((uint32_t)p.perm[place], (uint32_t)(N - 1)); }
+
+// A stable counting sort by one workgroup.  Each wave counts a run of tokens of its own, the counts are added up bin by
+// bin and wave by wave, and each wave goes over its run again: a token's place is its bin's and wave's first one plus
+// the same bin's tokens before it, those of the wave's 64 found by comparing the bins' bits.
+template <typename I>
+__global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, int64_t N, int n, int waves, int32_t* __restrict__ plan) {
+  extern __shared__ int32_t lds[];
+  int32_t* cnt = lds;                        // [waves][n + 1]
+  int32_t* ts = lds + waves * (n + 1);       // [n + 2] tiles before a bin
+  __shared__ int32_t wsum[3][16];
+  const int tid = threadIdx.x, T = blockDim.x, lane = tid & 63, w = uniform(tid >> 6), nw = T >> 6;
+  const Plan pv = plan_view(plan, N, n);
+  int32_t *seg = const_cast<int32_t*>(pv.seg), *tstart = const_cast<int32_t*>(pv.tstart), *perm = const_cast<int32_t*>(pv.perm);
+  Tile* tiles = const_cast<Tile*>(pv.tiles);
+  for (int k = tid; k < waves * (n + 1); k += T) cnt[k] = 0;
+  __syncthreads();
+  auto bin = [&](int64_t t) {
+    const I a = ids[t];
+    return a >= 0 && a < n ? (int)a : n;
+  };
+  const int64_t run = ((N + waves - 1) / waves + 63) / 64 * 64, r0 = w * run, r1 = min(r0 + run, N);
+  if (w < waves)
+    for (int64_t t = r0 + lane; t < r1; t += 64) atomicAdd(&cnt[w * (n + 1) + bin(t)], 1);
+  __syncthreads();
+  // tokens, tiles and bins before each bin: every thread has a run of bins
+  const int per = (n + 1 + T - 1) / T, b0 = min(tid * per, n + 1), b1 = min(b0 + per, n + 1);
+  int s[3] = {0, 0, 0};
+  for (int b = b0; b < b1; ++b) {
+    int c = 0;
+    for (int k = 0; k < waves; ++k) c += cnt[k * (n + 1) + b];
+    s[0] += c, s[1] += (c + TILE - 1) / TILE, s[2] += c > 0;
+  }
+  int pre[3];
+  for (int k = 0; k < 3; ++k) {
+    int v = s[k];
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(v, o, 64);
+      if (lane >= o) v += u;
+    }
+    pre[k] = v - s[k];
+    if (lane == 63) wsum[k][w] = v;
+  }
+  __syncthreads();
+  for (int k = 0; k < 3; ++k)
+    for (int j = 0; j < w; ++j) pre[k] += wsum[k][j];
+  int total = 0;
+  for (int j = 0; j < nw; ++j) total += wsum[1][j];
+  for (int b = b0; b < b1; ++b) {
+    seg[b] = pre[0];
+    tstart[b] = ts[b] = pre[1];
+    int c = 0;
+    for (int k = 0; k < waves; ++k) {
+      int32_t& v = cnt[k * (n + 1) + b];
+      const int t = v;
+      v = pre[0] + c;                        // this wave's first place in the bin
+      c += t;
+    }
+    // the bin's first tile here, the others below
+    if (c) tiles[pre[1]] = {b, pre[0], min(c, TILE), pre[2]};
+    pre[0] += c, pre[1] += (c + TILE - 1) / TILE, pre[2] += c > 0;
+  }
+  if (tid == 0) seg[n + 1] = (int32_t)N, tstart[n + 1] = ts[n + 1] = total;
+  __threadfence_block();
+  __syncthreads();
+  for (int t = tid; t < (int)max_tiles(N, n); t += T) {
+    if (t >= total) {
+      tiles[t] = {-1, 0, 0, 0};
+      continue;
+    }
+    int lo = 0, hi = n;                      // the last bin that begins at or before t and is not empty
+    while (lo < hi) {
+      const int m = (lo + hi + 1) >> 1;
+      if (ts[m] <= t) lo = m;
+      else hi = m - 1;
+    }
+    if (t == ts[lo]) continue;
+    const Tile f = tiles[ts[lo]];
+    const int first = f.first + TILE * (t - ts[lo]);
+    tiles[t] = {lo, first, min(TILE, seg[lo + 1] - first), f.ord};
+  }
+  if (w >= waves) return;
+  int bits = 1;
+  while (n >> bits) ++bits;
+  for (int64_t t0 = r0; t0 < r1; t0 += 64) {
+    const int64_t t = t0 + lane;
+    const bool there = t < r1;
+    const int b = there ? bin(t) : -1;
+    uint64_t same = __ballot(there);
+    for (int k = 0; k < bits; ++k) {
+      const uint64_t m = __ballot(there && (b >> k & 1));
+      same &= (b >> k & 1) ? m : ~m;
+    }
+    const int before = __popcll(same & (((uint64_t)1 << lane) - 1));
+    const int at = there ? cnt[w * (n + 1) + b] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the wave has read before its leaders write
+    __builtin_amdgcn_wave_barrier();
+    if (there && before == 0) cnt[w * (n + 1) + b] = at + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    if (there) perm[at + before] = (int32_t)t;
+  }
+}
+
+// ------------------------------------------------------------------ values
+template <bool H>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (H) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else return mfma_bf16(a, b, c);
+}
+template <bool H> __device__ __forceinline__ float half_lo(uint32_t w) {
+  if constexpr (H) return (float)__builtin_bit_cast(f16x2_t, w)[0];
+  else return bf_lo(w);
+}
+template <bool H> __device__ __forceinline__ float half_hi(uint32_t w) {
+  if constexpr (H) return (float)__builtin_bit_cast(f16x2_t, w)[1];
+  else return bf_hi(w);
+}
+template <bool H> __device__ __forceinline__ uint32_t pack2h(float lo, float hi) {
+  if constexpr (H) {
+    const f16x2_t v = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    return pack2_bf16(lo, hi);
+  }
+}
+
+// v = its upper 16 bits + a rest that bf16 holds to 8 bits.  An Inf has no rest (Inf - Inf is none), a NaN's rest is NaN.
+__device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ float rest(float v) { return fabsf(v) == __builtin_inff() ? 0.0f : v - upper(v); }
+__device__ __forceinline__ void split8(const float (&f)[8], u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    hi[k] = __builtin_amdgcn_perm(__float_as_uint(f[2 * k + 1]), __float_as_uint(f[2 * k]), 0x07060302u);
+    lo[k] = pack2_bf16(rest(f[2 * k]), rest(f[2 * k + 1]));
+  }
+}
+// eight fp16 values as two bf16 each, exactly
+__device__ __forceinline__ void split_f16(const u32x4& v, u32x4& hi, u32x4& lo) {
+  float f[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[2 * k] = half_lo<true>(v[k]), f[2 * k + 1] = half_hi<true>(v[k]);
+  split8(f, hi, lo);
+}
+
+// ------------------------------------------------------------------ shrink
+// part[share][tile][slot][rank] = sum over a share of K of W[a][rank][k] x[token][k], W [n, r, K].  Memory-bound: x once
+// (long prompts) or W once (a token an adapter).  A workgroup takes a tile and a share of K, its waves 64 K at a time in
+// turn (a line of each row); a lane's operands are 16 bytes of a row, from memory to the matrix instruction.
+struct Shrink {
+  const uint16_t *x, *w;
+  int64_t ldx, N, tiles;
+  int n, r, K, shares, rs;      // rs: ranks rounded up to 4
+  const int32_t* plan;
+  float* part;
+};
+
+template <bool H, int RT>
+__global__ __launch_bounds__(256) void shrink_kernel(Shrink p) {
+  extern __shared__ f32x4 red[];              // [wave][RT * 4][64]
+  const Plan plan = plan_view(p.plan, p.N, p.n);
+  const Tile t = tile_at(plan, blockIdx.x, p.N, p.n);
+  if ((unsigned)t.adapter >= (unsigned)p.n) return;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+  const int subs = (t.count + 15) >> 4, r0 = blockIdx.z * 64;
+  const uint16_t* xr[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    xr[s] = p.x + row_at(plan, t.first + min(16 * s + i, t.count - 1), p.N) * p.ldx + 8 * q;
+  }
+  const uint16_t* wr[RT];
+#pragma unroll
+  for (int k = 0; k < RT; ++k) wr[k] = p.w + ((int64_t)t.adapter * p.r + min(r0 + 16 * k + i, p.r - 1)) * p.K + 8 * q;
+  const int units = (p.K + 63) / 64, u0 = (int)((int64_t)units * blockIdx.y / p.shares), u1 = (int)((int64_t)units * (blockIdx.y + 1) / p.shares);
+  f32x4 acc[RT][4] = {};
+  const u32x4 none = {0, 0, 0, 0};
+  for (int u = u0 + w; u < u1; u += 4) {
+    u32x4 xv[2][4], wv[2][RT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = 64 * u + 32 * h;
+      const bool in = k + 8 * q < p.K;
+#pragma unroll
+      for (int j = 0; j < RT; ++j) wv[h][j] = in ? *reinterpret_cast<const u32x4*>(wr[j] + k) : none;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s < subs) xv[h][s] = in ? *reinterpret_cast<const u32x4*>(xr[s] + k) : none;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s < subs)
+#pragma unroll
+          for (int j = 0; j < RT; ++j) acc[j][s] = mfma16<H>(wv[h][j], xv[h][s], acc[j][s]);
+  }
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (s < subs) red[(w * RT * 4 + j * 4 + s) * 64 + lane] = acc[j][s];
+  __syncthreads();
+  // entry (j, s) of a lane (i, q): token 16 s + i, ranks 16 j + 4 q .. + 3
+  for (int e = w; e < RT * 4; e += 4) {
+    const int j = e >> 2, s = e & 3, slot = 16 * s + i, rank = r0 + 16 * j + 4 * q;
+    if (slot >= t.count || rank >= p.rs) continue;
+    f32x4 v = red[e * 64 + lane];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) v += red[(k * RT * 4 + e) * 64 + lane];
+    *reinterpret_cast<f32x4*>(p.part + (((int64_t)blockIdx.y * p.tiles + blockIdx.x) * TILE + slot) * p.rs + rank) = v;
+  }
+}
+
+// ------------------------------------------------------------------ expand
+// out[token][f] = y[token][f] + sum over ranks of W[a][f][rank] t'[token][rank], W [n, F, r] with rows of ldw.
+// Memory-bound by y and out.  A workgroup takes a tile and a share of F: it adds up t's shares, splits t' into LDS in the
+// order of the matrix instruction's operand (`planes`: and for grad, ranks first), and its waves take 64 features at a
+// time.  The 32 features of two products are dealt so that a lane ends with 8 consecutive ones of a token.
+struct Expand {
+  const uint16_t *w, *y;        // y NULL: out is the product alone
+  uint16_t* out;
+  int64_t ldy, ldo, N, tiles;
+  int n, r, F, ldw, shares, chunks, rs;
+  const int32_t* plan;
+  const float *part, *scales;
+  uint16_t* planes;             // [tile][upper, rest][ranks to 16][64 slots], or NULL
+};
+
+// the operand of a lane: ranks k .. k + 7 of a row, those from r on zero.  RV: ranks that lie aligned together
+template <int RV>
+__device__ __forceinline__ u32x4 rank8(const uint16_t* row, int k, int r) {
+  if constexpr (RV == 8) {
+    return k < r ? *reinterpret_cast<const u32x4*>(row + k) : u32x4{0, 0, 0, 0};
+  } else if constexpr (RV == 4) {
+    const u32x2 z = {0, 0}, a = k < r ? *reinterpret_cast<const u32x2*>(row + k) : z, b = k + 4 < r ? *reinterpret_cast<const u32x2*>(row + k + 4) : z;
+    return u32x4{a[0], a[1], b[0], b[1]};
+  } else {
+    uint32_t e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = row[min(k + j, r - 1)];
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (k + 2 * j < r ? e[2 * j] : 0u) | (k + 2 * j + 1 < r ? e[2 * j + 1] << 16 : 0u);
+    return v;
+  }
+}
+
+template <bool H, int RV, bool ONE>          // ONE: r <= 16, upper and rest in one matrix instruction
+__global__ __launch_bounds__(256) void expand_kernel(Expand p) {
+  extern __shared__ u32x4 tf[];              // [step][subtile][64]
+  const Plan plan = plan_view(p.plan, p.N, p.n);
+  const Tile t = tile_at(plan, blockIdx.x, p.N, p.n);
+  if (t.adapter < 0) return;
+  const bool bare = t.adapter == p.n;        // tokens without an adapter
+  if (bare && p.y == p.out) return;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+  const int subs = (t.count + 15) >> 4;
+  int64_t row[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) row[s] = row_at(plan, t.first + min(16 * s + i, t.count - 1), p.N);
+  const int units = (p.F + 63) / 64, u0 = (int)((int64_t)units * blockIdx.y / p.chunks), u1 = (int)((int64_t)units * (blockIdx.y + 1) / p.chunks);
+  if (!bare) {
+    const int groups = ONE ? 2 : (p.r + 31) / 32 * 4, slot = lane;
+    const float scale = p.scales ? p.scales[t.adapter] : 1.0f;
+    for (int g = w; g < groups; g += 4) {
+      float f[8] = {};
+      if (slot < t.count) {
+        const float* at = p.part + ((int64_t)blockIdx.x * TILE + slot) * p.rs + 8 * g;
+        for (int k = 0; k < p.shares; ++k, at += p.tiles * TILE * p.rs) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (8 * g + 4 * h < p.r) {
+              const f32x4 v = *reinterpret_cast<const f32x4*>(at + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[4 * h + e] += v[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 8 * g + e < p.r ? f[e] * scale : 0.0f;
+      }
+      u32x4 hi, lo;
+      split8(f, hi, lo);
+      const int s = slot >> 4, l = slot & 15;
+      if constexpr (ONE) {
+        tf[s * 64 + 16 * g + l] = hi;
+        tf[s * 64 + 16 * (g + 2) + l] = lo;
+      } else {
+        tf[((g >> 2) * 8 + s) * 64 + 16 * (g & 3) + l] = hi;
+        tf[((g >> 2) * 8 + 4 + s) * 64 + 16 * (g & 3) + l] = lo;
+      }
+      if (p.planes && blockIdx.y == 0) {
+        const int r16 = (p.r + 15) & ~15;
+        uint16_t* pl = p.planes + (int64_t)blockIdx.x * 2 * r16 * TILE + slot;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * g + e < r16) {
+            pl[(8 * g + e) * TILE] = (uint16_t)(hi[e >> 1] >> (16 * (e & 1)));
+            pl[(r16 + 8 * g + e) * TILE] = (uint16_t)(lo[e >> 1] >> (16 * (e & 1)));
+          }
+      }
+    }
+    __syncthreads();
+  }
+  for (int u = u0 + w; u < u1; u += 4) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int f0 = 64 * u + 32 * g, fl = f0 + 8 * q;
+      u32x4 yv[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        yv[s] = p.y && s < subs && fl < p.F ? *reinterpret_cast<const u32x4*>(p.y + row[s] * p.ldy + fl) : u32x4{0, 0, 0, 0};
+      f32x4 acc[4][2] = {};
+      if (!bare) {
+        const uint16_t* wr[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          wr[j] = p.w + ((int64_t)t.adapter * p.F + min(f0 + 8 * (i >> 2) + 4 * j + (i & 3), p.F - 1)) * p.ldw;
+        const int steps = ONE ? 1 : (p.r + 31) / 32;
+        for (int k = 0; k < steps; ++k) {
+          u32x4 wv[2], wl[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            wv[j] = rank8<RV>(wr[j], ONE ? 8 * (q & 1) : 32 * k + 8 * q, p.r);
+            if constexpr (H) split_f16(wv[j], wv[j], wl[j]);
+          }
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            if (s < subs) {
+              const u32x4 a = tf[(k * 8 + s) * 64 + lane];
+              u32x4 b;
+              if constexpr (!ONE) b = tf[(k * 8 + 4 + s) * 64 + lane];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                acc[s][j] = mfma_bf16(wv[j], a, acc[s][j]);
+                if constexpr (!ONE) acc[s][j] = mfma_bf16(wv[j], b, acc[s][j]);
+                if constexpr (H) acc[s][j] = mfma_bf16(wl[j], a, acc[s][j]);
+                if constexpr (H && !ONE) acc[s][j] = mfma_bf16(wl[j], b, acc[s][j]);
+              }
+            }
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (16 * s + i < t.count && fl < p.F) {
+          u32x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x4& v = acc[s][e >> 1];
+            o[e] = pack2h<H>(half_lo<H>(yv[s][e]) + v[2 * (e & 1)], half_hi<H>(yv[s][e]) + v[2 * (e & 1) + 1]);
+          }
+          *reinterpret_cast<u32x4*>(p.out + row[s] * p.ldo + fl) = bare ? yv[s] : o;
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ grad
+// part[piece][rank][f] = sum over the tokens of a piece of P[token][rank] Q[token][f], P from planes, Q = x or dy.
+// Memory-bound by Q.  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens lie in an
+// LDS slice of its own and are read transposed.  Where the adapter changes on the way, a piece ends: piece number =
+// tile / turn + the adapter's number among those with tokens, which grows with either.
+struct Grad {
+  const uint16_t* q[2];
+  const uint16_t* planes[2];
+  float* part[2];
+  int64_t ldq[2], N, tiles;
+  int F[2], turn[2], pieces[2];
+  int n, r, rblocks;
+  const int32_t* plan;
+};
+
+constexpr int QROW = 72;             // elements of a token's row in LDS: 64 and 16 bytes, which moves the rows over the banks
+
+template <bool H, int RT>
+__global__ __launch_bounds__(256) void grad_kernel(Grad p) {
+  __shared__ __attribute__((aligned(16))) uint16_t slices[4][(H ? 2 : 1) * 32 * QROW];
+  const int z = blockIdx.z / p.rblocks, r0 = (blockIdx.z - z * p.rblocks) * 64;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+  const int F = p.F[z], f0 = (blockIdx.x * 4 + w) * 64, r16 = (p.r + 15) & ~15;
+  const int64_t t0 = (int64_t)blockIdx.y * p.turn[z], t1 = min(t0 + p.turn[z], p.tiles);
+  if (f0 >= F || t0 >= t1) return;
+  const Plan plan = plan_view(p.plan, p.N, p.n);
+  uint16_t* slice = slices[w];
+  const int fl = f0 + 8 * (lane & 7);
+  f32x4 acc[RT][4] = {};
+  auto flush = [&](int64_t tile, int ord) {
+    float* out = p.part[z] + (tile / p.turn[z] + ord) * p.r * F;
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+      for (int ft = 0; ft < 4; ++ft) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int rank = r0 + 16 * j + 4 * q + v, f = f0 + 16 * ft + i;
+          if (rank < p.r && f < F) out[(int64_t)rank * F + f] = acc[j][ft][v];
+        }
+        acc[j][ft] = f32x4{0, 0, 0, 0};
+      }
+  };
+  Tile t = tile_at(plan, t0, p.N, p.n);
+  for (int64_t tile = t0; tile < t1; ++tile) {
+    if ((unsigned)t.adapter >= (unsigned)p.n) return;         // tokens without an adapter, or no tile: nothing behind them
+    for (int half = 0; half < 2 && 32 * half < t.count; ++half) {
+      u32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int slot = 32 * half + 8 * j + (lane >> 3);
+        const int64_t row = row_at(plan, t.first + min(slot, t.count - 1), p.N);
+        v[j] = slot < t.count && fl < F ? *reinterpret_cast<const u32x4*>(p.q[z] + row * p.ldq[z] + fl) : u32x4{0, 0, 0, 0};
+      }
+      u32x4 a[RT][2];
+      const uint16_t* pl = p.planes[z] + (tile * 2 * r16 + r0 + i) * TILE + 32 * half + 8 * q;
+#pragma unroll
+      for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          a[j][h] = r0 + 16 * j < r16 ? *reinterpret_cast<const u32x4*>(pl + (16 * j + h * r16) * TILE) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint16_t* at = slice + (8 * j + (lane >> 3)) * QROW + 8 * (lane & 7);
+        if constexpr (H) {
+          u32x4 hi, lo;
+          split_f16(v[j], hi, lo);
+          *reinterpret_cast<u32x4*>(at) = hi;
+          *reinterpret_cast<u32x4*>(at + 32 * QROW) = lo;
+        } else {
+          *reinterpret_cast<u32x4*>(at) = v[j];
+        }
+      }
+#pragma unroll
+      for (int ft = 0; ft < 4; ++ft) {
+        const u32x4 b = tr_frag(slice, QROW, 0, 16 * ft, lane);
+        u32x4 bl;
+        if constexpr (H) bl = tr_frag(slice + 32 * QROW, QROW, 0, 16 * ft, lane);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+          acc[j][ft] = mfma_bf16(a[j][0], b, acc[j][ft]);
+          acc[j][ft] = mfma_bf16(a[j][1], b, acc[j][ft]);
+          if constexpr (H) acc[j][ft] = mfma_bf16(a[j][1], bl, mfma_bf16(a[j][0], bl, acc[j][ft]));
+        }
+      }
+    }
+    const Tile next = tile + 1 < t1 ? tile_at(plan, tile + 1, p.N, p.n) : Tile{-1, 0, 0, 0};
+    if (next.adapter != t.adapter) flush(tile, min((uint32_t)t.ord, (uint32_t)min(p.N, (int64_t)p.n) - 1));
+    t = next;
+  }
+}
+
+// The pieces of every adapter in their order, rounded: dA [n, r, F] (z = 0), dB [n, F, r] (z = 1); adapters without tokens
+// get zeros.  A thread has a feature and 8 ranks.
+struct GradSum {
+  const float* part[2];
+  uint16_t* out[2];
+  int F[2], turn[2];
+  int64_t N;
+  int n, r, h;
+  const int32_t* plan;
+};
+
+__global__ __launch_bounds__(256) void grad_sum_kernel(GradSum p) {
+  const int z = blockIdx.z, F = p.F[z], groups = (p.r + 7) / 8, a = blockIdx.y;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (!p.out[z] || e >= (int64_t)F * groups) return;
+  const int g = (int)(e / F), f = (int)(e - (int64_t)g * F);
+  const Plan plan = plan_view(p.plan, p.N, p.n);
+  const int ta = plan.tstart[a], tb = plan.tstart[a + 1];
+  float v[8] = {};
+  if (tb > ta) {
+    const int ord = plan.tiles[ta].ord, s1 = (tb - 1) / p.turn[z] + ord;
+    for (int s = ta / p.turn[z] + ord; s <= s1; ++s) {
+      const float* at = p.part[z] + ((int64_t)s * p.r + 8 * g) * F + f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (8 * g + k < p.r) v[k] += at[(int64_t)k * F];
+    }
+  }
+  uint32_t o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = p.h ? pack2h<true>(v[2 * k], v[2 * k + 1]) : pack2h<false>(v[2 * k], v[2 * k + 1]);
+  if (z == 1 && p.r % 8 == 0) {
+    *reinterpret_cast<u32x4*>(p.out[1] + ((int64_t)a * F + f) * p.r + 8 * g) = u32x4{o[0], o[1], o[2], o[3]};
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (8 * g + k < p.r) {
+      const uint16_t h = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
+      if (z == 0) p.out[0][((int64_t)a * p.r + 8 * g + k) * F + f] = h;
+      else p.out[1][((int64_t)a * F + f) * p.r + 8 * g + k] = h;
+    }
+}
+
+// dst [n][cols][ld] = the transposes of src [n][rows][cols], rows to ld zero
+__global__ __launch_bounds__(256) void transpose_kernel(const uint16_t* __restrict__ src, int rows, int cols, int ld, uint16_t* __restrict__ dst) {
+  __shared__ uint16_t s[64][66];
+  const int64_t a = blockIdx.z;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  for (int k = y; k < 64; k += 4)
+    s[k][x] = r0 + k < rows && c0 + x < cols ? src[(a * rows + r0 + k) * cols + c0 + x] : (uint16_t)0;
+  __syncthreads();
+  for (int k = y; k < 64; k += 4)
+    if (c0 + k < cols && r0 + x < ld) dst[(a * cols + c0 + k) * ld + r0 + x] = s[x][k];
+}
+
+// ------------------------------------------------------------------ launches
+inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
+inline int launched() { return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH; }
+inline bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+constexpr int64_t WANTED = 1024;     // workgroups of a launch, four on a CU
+
+// shares of K of a shrink: enough workgroups, at least 256 K (one turn of the four waves) each
+int shares_of(int64_t tiles, int K) {
+  const int64_t s = (WANTED + tiles - 1) / tiles, most = (K + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min(s, most));
+}
+int chunks_of(int64_t tiles, int F) {
+  const int64_t s = (WANTED + tiles - 1) / tiles, most = (F + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min(s, most));
+}
+size_t part_bytes(int64_t tiles, int K, int r) { return align256((size_t)shares_of(tiles, K) * tiles * TILE * ((r + 3) & ~3) * 4); }
+size_t plane_bytes(int64_t tiles, int r) { return align256((size_t)tiles * 2 * ((r + 15) & ~15) * TILE * 2); }
+
+// tiles of a workgroup of grad, and its pieces
+int turn_of(int64_t tiles, int F) {
+  const int64_t fb = (F + 255) / 256;
+  return (int)std::max<int64_t>(1, tiles * fb / (WANTED / 2));
+}
+int64_t pieces_of(int64_t tiles, int64_t N, int n, int turn) { return (tiles + turn - 1) / turn + std::min<int64_t>(N, n); }
+
+int launch_shrink(bool h, const Shrink& p, hipStream_t st) {
+  const int rb = (p.r + 63) / 64, rt = std::min((p.r + 15) / 16, 4);
+  const dim3 grid((unsigned)p.tiles, p.shares, rb);
+  auto go = [&](auto* k, int RT) {
+    k<<<grid, 256, RT * 16384, st>>>(p);
+    return launched();
+  };
+  if (rt == 1) return h ? go(shrink_kernel<true, 1>, 1) : go(shrink_kernel<false, 1>, 1);
+  if (rt == 2) return h ? go(shrink_kernel<true, 2>, 2) : go(shrink_kernel<false, 2>, 2);
+  return h ? go(shrink_kernel<true, 4>, 4) : go(shrink_kernel<false, 4>, 4);
+}
+
+int launch_expand(bool h, const Expand& p, hipStream_t st) {
+  const bool one = p.r <= 16;
+  const int lds = one ? 4096 : (p.r + 31) / 32 * 8192, rv = p.ldw % 8 == 0 ? 8 : p.ldw % 4 == 0 ? 4 : 1;
+  const dim3 grid((unsigned)p.tiles, p.chunks);
+  auto go = [&](auto* k) {
+    k<<<grid, 256, lds, st>>>(p);
+    return launched();
+  };
+#define LBK_EXPAND(H)                                                                         \
+  if (rv == 8) return one ? go(expand_kernel<H, 8, true>) : go(expand_kernel<H, 8, false>);   \
+  if (rv == 4) return one ? go(expand_kernel<H, 4, true>) : go(expand_kernel<H, 4, false>);   \
+  return one ? go(expand_kernel<H, 1, true>) : go(expand_kernel<H, 1, false>);
+  if (h) {
+    LBK_EXPAND(true)
+  }
+  LBK_EXPAND(false)
+#undef LBK_EXPAND
+}
+
+int check_adapter(const lbk_adapter* d) {
+  if (!d) return LBK_ERR_NULL;
+  if ((d->type != LBK_BF16 && d->type != LBK_FP16) || d->N < 0) return LBK_ERR_ARG;
+  if (d->n < 1 || d->rank < 1 || d->in_features < 8 || d->out_features < 8 || d->in_features % 8 || d->out_features % 8) return LBK_ERR_SHAPE;
+  if (d->n > MAX_ADAPTERS || d->rank > MAX_RANK || d->N > (1 << 30) || d->in_features > (1 << 21) || d->out_features > (1 << 21))
+    return LBK_ERR_TOO_LARGE;
+  return LBK_OK;
+}
+
+}  // namespace
+}  // namespace lbk
+
+using namespace lbk;
+
+extern "C" {
+
+size_t lbk_adapter_plan_bytes(int64_t N, int32_t n_adapters) {
+  if (N < 0 || N > (1 << 30) || n_adapters < 1 || n_adapters > MAX_ADAPTERS) return 0;
+  return (size_t)plan_words(N, n_adapters) * 4;
+}
+
+int lbk_adapter_plan(const void* ids, int32_t id_bytes, int64_t N, int32_t n_adapters, void* plan, size_t plan_bytes, void* stream) {
+  if ((id_bytes != 4 && id_bytes != 8) || N < 0) return LBK_ERR_ARG;
+  if (n_adapters < 1) return LBK_ERR_SHAPE;
+  if (N > (1 << 30) || n_adapters > MAX_ADAPTERS) return LBK_ERR_TOO_LARGE;
+  if ((N > 0 && !ids) || !plan) return LBK_ERR_NULL;
+  if (!a16(plan) || (reinterpret_cast<uintptr_t>(ids) & (id_bytes - 1))) return LBK_ERR_ALIGN;
+  if (plan_bytes < lbk_adapter_plan_bytes(N, n_adapters)) return LBK_ERR_WORKSPACE;
+  // waves that count: as many as have 64 tokens and as 44 KB of counters hold
+  const int bins = n_adapters + 1;
+  const int waves = (int)std::max<int64_t>(1, std::min<int64_t>({16, 11264 / bins, (N + 63) / 64}));
+  const int lds = (waves * bins + bins + 1) * 4;
+  if (id_bytes == 4) plan_kernel<int32_t><<<1, 1024, lds, S(stream)>>>(static_cast<const int32_t*>(ids), N, n_adapters, waves, static_cast<int32_t*>(plan));
+  else plan_kernel<int64_t><<<1, 1024, lds, S(stream)>>>(static_cast<const int64_t*>(ids), N, n_adapters, waves, static_cast<int32_t*>(plan));
+  return launched();
+}
+
+size_t lbk_adapter_planes_bytes(const lbk_adapter* d) {
+  return check_adapter(d) || d->N == 0 ? 0 : plane_bytes(max_tiles(d->N, d->n), d->rank);
+}
+
+size_t lbk_adapter_add_workspace_bytes(const lbk_adapter* d) {
+  return check_adapter(d) || d->N == 0 ? 0 : part_bytes(max_tiles(d->N, d->n), d->in_features, d->rank);
+}
+
+int lbk_adapter_add(const lbk_adapter* d, const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo,
+                    void* planes, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = check_adapter(d)) return st;
+  if (ldx < d->in_features || ldy < d->out_features || ldo < d->out_features) return LBK_ERR_ARG;
+  if (d->N == 0) return LBK_OK;
+  if (!d->a || !d->b || !d->plan || !x || !y || !out) return LBK_ERR_NULL;
+  for (const void* p : {d->a, d->b, (const void*)d->plan, x, y, (const void*)out, (const void*)planes, (const void*)workspace})
+    if (!a16(p)) return LBK_ERR_ALIGN;
+  if (ldx % 8 || ldy % 8 || ldo % 8 || (reinterpret_cast<uintptr_t>(d->scales) & 3)) return LBK_ERR_ALIGN;
+  if (!workspace || workspace_bytes < lbk_adapter_add_workspace_bytes(d)) return LBK_ERR_WORKSPACE;
+  const bool h = d->type == LBK_FP16;
+  const int64_t tiles = max_tiles(d->N, d->n);
+  const int rs = (d->rank + 3) & ~3, shares = shares_of(tiles, d->in_features);
+  const Shrink s{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(d->a), ldx, d->N, tiles, d->n, d->rank, d->in_features, shares, rs,
+                 d->plan, static_cast<float*>(workspace)};
+  if (int st = launch_shrink(h, s, S(stream))) return st;
+  const Expand e{static_cast<const uint16_t*>(d->b), static_cast<const uint16_t*>(y), static_cast<uint16_t*>(out), ldy, ldo, d->N, tiles, d->n,
+                 d->rank, d->out_features, d->rank, shares, chunks_of(tiles, d->out_features), rs, d->plan, static_cast<const float*>(workspace),
+                 d->scales, static_cast<uint16_t*>(planes)};
+  return launch_expand(h, e, S(stream));
+}
+
+// shares of dy's shrink, planes of dt', the transposes of B and A, the pieces of dA and dB
+struct BwdParts {
+  size_t part, planes, bt, at, pa, pb, all;
+};
+static BwdParts bwd_parts(const lbk_adapter* d) {
+  const int64_t tiles = max_tiles(d->N, d->n);
+  BwdParts p;
+  p.part = part_bytes(tiles, d->out_features, d->rank);
+  p.planes = plane_bytes(tiles, d->rank);
+  p.bt = align256((size_t)d->n * d->rank * d->out_features * 2);
+  p.at = align256((size_t)d->n * ((d->rank + 7) & ~7) * d->in_features * 2);
+  auto pieces = [&](int F) { return align256((size_t)pieces_of(tiles, d->N, d->n, turn_of(tiles, F)) * d->rank * F * 4); };
+  p.pa = pieces(d->in_features);
+  p.pb = pieces(d->out_features);
+  p.all = p.part + p.planes + p.bt + p.at + p.pa + p.pb;
+  return p;
+}
+
+size_t lbk_adapter_bwd_workspace_bytes(const lbk_adapter* d) { return check_adapter(d) || d->N == 0 ? 0 : bwd_parts(d).all; }
+
+int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void* dout, int64_t ldo, const void* planes, void* dx,
+                    void* da, void* db, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = check_adapter(d)) return st;
+  if (ldx < d->in_features || ldo < d->out_features) return LBK_ERR_ARG;
+  if (!d->plan) return LBK_ERR_NULL;
+  const bool some = d->N > 0;
+  if (some && (!d->a || !d->b || !dout || (da && !x) || (db && !planes))) return LBK_ERR_NULL;
+  for (const void* p : {d->a, d->b, (const void*)d->plan, x, dout, planes, (const void*)dx, (const void*)da, (const void*)db, (const void*)workspace})
+    if (!a16(p)) return LBK_ERR_ALIGN;
+  if (ldx % 8 || ldo % 8 || (reinterpret_cast<uintptr_t>(d->scales) & 3)) return LBK_ERR_ALIGN;
+  if (some && (!workspace || workspace_bytes < lbk_adapter_bwd_workspace_bytes(d))) return LBK_ERR_WORKSPACE;
+  const bool h = d->type == LBK_FP16;
+  const int64_t tiles = max_tiles(d->N, d->n);
+  const int in = d->in_features, out = d->out_features, r = d->rank, rs = (r + 3) & ~3, r8 = (r + 7) & ~7;
+  hipStream_t st = S(stream);
+  BwdParts sz{};
+  if (some) sz = bwd_parts(d);
+  char* at = static_cast<char*>(workspace);
+  auto take = [&](size_t b) {
+    char* p = at;
+    at += b;
+    return p;
+  };
+  float* part = reinterpret_cast<float*>(take(sz.part));
+  uint16_t* dplanes = reinterpret_cast<uint16_t*>(take(sz.planes));
+  uint16_t* bt = reinterpret_cast<uint16_t*>(take(sz.bt));
+  uint16_t* att = reinterpret_cast<uint16_t*>(take(sz.at));
+  float* pa = reinterpret_cast<float*>(take(sz.pa));
+  float* pb = reinterpret_cast<float*>(take(sz.pb));
+  if (some && (dx || da)) {
+    transpose_kernel<<<dim3((r + 63) / 64, (out + 63) / 64, d->n), 256, 0, st>>>(static_cast<const uint16_t*>(d->b), out, r, out, bt);
+    if (int e = launched()) return e;
+    if (dx) {
+      transpose_kernel<<<dim3((in + 63) / 64, (r + 63) / 64, d->n), 256, 0, st>>>(static_cast<const uint16_t*>(d->a), r, in, r8, att);
+      if (int e = launched()) return e;
+    }
+    const int shares = shares_of(tiles, out);
+    const Shrink s{static_cast<const uint16_t*>(dout), bt, ldo, d->N, tiles, d->n, r, out, shares, rs, d->plan, part};
+    if (int e = launch_shrink(h, s, st)) return e;
+    const Expand e{att, nullptr, static_cast<uint16_t*>(dx), in, in, d->N, tiles, d->n, r, dx ? in : 0, r8, shares,
+                   dx ? chunks_of(tiles, in) : 1, rs, d->plan, part, d->scales, da ? dplanes : nullptr};
+    if (int k = launch_expand(h, e, st)) return k;
+  }
+  if (!da && !db) return LBK_OK;
+  Grad g{};
+  g.q[0] = static_cast<const uint16_t*>(x), g.q[1] = static_cast<const uint16_t*>(dout);
+  g.planes[0] = dplanes, g.planes[1] = static_cast<const uint16_t*>(planes);
+  g.part[0] = pa, g.part[1] = pb, g.ldq[0] = ldx, g.ldq[1] = ldo;
+  g.N = d->N, g.tiles = tiles, g.n = d->n, g.r = r, g.rblocks = (r + 63) / 64, g.plan = d->plan;
+  g.F[0] = da ? in : 0, g.F[1] = db ? out : 0;
+  g.turn[0] = some ? turn_of(tiles, in) : 1, g.turn[1] = some ? turn_of(tiles, out) : 1;
+  if (some) {
+    const int F = std::max(g.F[0], g.F[1]);
+    int64_t runs = 0;
+    for (int z = 0; z < 2; ++z)
+      if (g.F[z]) runs = std::max(runs, (tiles + g.turn[z] - 1) / g.turn[z]);
+    const dim3 grid((F + 255) / 256, (unsigned)runs, 2 * g.rblocks);
+    const int rt = std::min((r + 15) / 16, 4);
+    auto go = [&](auto* k) {
+      k<<<grid, 256, 0, st>>>(g);
+      return launched();
+    };
+    if (int e = rt == 1 ? (h ? go(grad_kernel<true, 1>) : go(grad_kernel<false, 1>))
+                : rt == 2 ? (h ? go(grad_kernel<true, 2>) : go(grad_kernel<false, 2>))
+                          : (h ? go(grad_kernel<true, 4>) : go(grad_kernel<false, 4>)))
+      return e;
+  }
+  GradSum m{};
+  m.part[0] = pa, m.part[1] = pb, m.out[0] = static_cast<uint16_t*>(da), m.out[1] = static_cast<uint16_t*>(db);
+  m.F[0] = in, m.F[1] = out, m.turn[0] = g.turn[0], m.turn[1] = g.turn[1], m.N = d->N, m.n = d->n, m.r = r, m.h = h, m.plan = d->plan;
+  const int64_t most = ((int64_t)std::max(da ? in : 0, db ? out : 0) * ((r + 7) / 8) + 255) / 256;
+  grad_sum_kernel<<<dim3((unsigned)most, d->n, 2), 256, 0, st>>>(m);
+  return launched();
+}
+
+}  // extern "C"

@@ -1,5 +1,5 @@
-// torch_util.h — what the operator registrations (torch_ops.cpp, torch_ffn.cpp, torch_seam.cpp) share: the current
-// stream, status codes as errors, argument checks, workspaces.
+// torch_util.h — what the operator registrations (torch_ops.cpp, torch_ffn.cpp, torch_seam.cpp, torch_adapter.cpp)
+// share: the current stream, status codes as errors, argument checks, workspaces.
 #pragma once
 
 #include <ATen/ATen.h>

@@ -77,6 +77,13 @@ class Seam(C.Structure):
                 ("seed_dev", C.c_void_p), ("seed", C.c_int64), ("stream_id", C.c_uint32)]
 
 
+class Adapter(C.Structure):
+    """``lbk_adapter``: low-rank adapters, the plan of a batch's tokens and their sizes."""
+
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scales", C.c_void_p), ("plan", C.c_void_p), ("N", C.c_int64),
+                ("n", C.c_int32), ("rank", C.c_int32), ("in_features", C.c_int32), ("out_features", C.c_int32), ("type", C.c_int32)]
+
+
 # (name, restype, argtypes) for every entry point of include/lbk.h
 _P = C.c_void_p
 _I64 = C.c_int64
@@ -87,6 +94,7 @@ _PB = C.POINTER(Bell)
 _PT = C.POINTER(BellTernary)
 _PM = C.POINTER(BellMx)
 _PS = C.POINTER(Seam)
+_PA = C.POINTER(Adapter)
 SIGNATURES = {
     "lbk_status_string": (C.c_char_p, [C.c_int]),
     "lbk_version": (C.c_int, []),
@@ -196,6 +204,13 @@ SIGNATURES = {
     "lbk_residual_norm_fwd": (C.c_int, [_PS, _P, _P, _P, _P, _P, _P, _P]),
     "lbk_residual_norm_bwd_workspace_bytes": (_SZ, [_PS]),
     "lbk_residual_norm_bwd": (C.c_int, [_PS, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "lbk_adapter_plan_bytes": (_SZ, [_I64, _I32]),
+    "lbk_adapter_plan": (C.c_int, [_P, _I32, _I64, _I32, _P, _SZ, _P]),
+    "lbk_adapter_planes_bytes": (_SZ, [_PA]),
+    "lbk_adapter_add_workspace_bytes": (_SZ, [_PA]),
+    "lbk_adapter_add": (C.c_int, [_PA, _P, _I64, _P, _I64, _P, _I64, _P, _P, _SZ, _P]),
+    "lbk_adapter_bwd_workspace_bytes": (_SZ, [_PA]),
+    "lbk_adapter_bwd": (C.c_int, [_PA, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -16,6 +16,7 @@ fills.
 from __future__ import annotations
 
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -575,3 +576,43 @@ def residual_norm(h, y, post_scale=None, gate=None, pre_scale=None, residual_sca
         hn = hn.reshape(h.shape)
         n = n if pre_scale is None else n.reshape(h.shape)
     return hn, (None if pre_scale is None else n)
+
+
+class AdapterPlan(NamedTuple):
+    """The tokens of a batch sorted by adapter (``adapter_plan``), for every projection that the batch passes."""
+
+    data: torch.Tensor
+    tokens: int
+    adapters: int
+
+
+def adapter_plan(ids, n_adapters: int) -> AdapterPlan:
+    """``ids`` (int32 or int64, any shape) holds each token's adapter, those outside [0, n_adapters) stand for none.  The
+    plan serves every ``adapter_add`` of the batch with the same ``n_adapters`` (1 .. 4096); it holds the ids of the time
+    of the call."""
+    _gpu(ids)
+    return AdapterPlan(ops().adapter_plan(ids, int(n_adapters)), ids.numel(), int(n_adapters))
+
+
+def adapter_add(y, x, a, b, plan: AdapterPlan, scales=None, inplace: bool = False):
+    """``y + scales[id] * (x a[id]^T) b[id]^T`` with each token's adapter, y as it is where a token has none: the
+    low-rank update beside a shared projection's y = base(x).  x is [..., in], y [..., out], a [n, rank, in] and b [n, out,
+    rank], all bf16 or all fp16 (features multiples of 8, rank 1 .. 256); scales [n] fp32 or None (1).  ``a x`` stays in
+    fp32 up to 16 bits of mantissa.  Differentiable in y, x, a and b as one native autograd node
+    (``titan::adapter_add_train``); ``inplace`` adds into y, without gradients."""
+    _gpu(y, x, a, b)
+    if plan.tokens * x.shape[-1] != x.numel() or plan.adapters != a.shape[0]:
+        raise RuntimeError(f"the plan is of {plan.tokens} tokens and {plan.adapters} adapters; x is {tuple(x.shape)}, a {tuple(a.shape)}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    y2 = y if y.dim() == 2 else (y.view if inplace else y.reshape)(-1, y.shape[-1])
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
+        if inplace:
+            raise RuntimeError("adapter_add into y has no gradients; call it without inplace or under torch.no_grad()")
+        _no_transforms()
+        out = ops().adapter_add_train(y2, x2, a, b, plan.data, scales)
+    elif inplace:
+        ops().adapter_add_(y2, x2, a, b, plan.data, scales)
+        return y
+    else:
+        out = ops().adapter_add(y2, x2, a, b, plan.data, scales)
+    return out if y.dim() == 2 else out.reshape(y.shape)
