@@ -68,13 +68,38 @@ __global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, i
   Tile* tiles = const_cast<Tile*>(pv.tiles);
   for (int k = tid; k < waves * (n + 1); k += T) cnt[k] = 0;
   __syncthreads();
-  auto bin = [&](int64_t t) {
-    const I a = ids[t];
-    return a >= 0 && a < n ? (int)a : n;
-  };
   const int64_t run = ((N + waves - 1) / waves + 63) / 64 * 64, r0 = w * run, r1 = min(r0 + run, N);
+  int bits = 1;
+  while (n >> bits) ++bits;
+  // the lanes whose token has this lane's bin (-1: no token): the first of them counts for all, as 64 additions to one
+  // counter would follow each other
+  auto alike = [&](int b) {
+    uint64_t same = __ballot(b >= 0);
+    for (int k = 0; k < bits; ++k) {
+      const uint64_t m = __ballot(b >= 0 && (b >> k & 1));
+      same &= (b >> k & 1) ? m : ~m;
+    }
+    return same;
+  };
+  constexpr int AHEAD = 8;                   // turns of 64 tokens whose ids are loaded together
+  auto load = [&](int64_t t0, int (&b)[AHEAD]) {
+    I v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) v[k] = t0 + 64 * k + lane < r1 ? ids[t0 + 64 * k + lane] : (I)0;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) b[k] = t0 + 64 * k + lane >= r1 ? -1 : v[k] >= 0 && v[k] < n ? (int)v[k] : n;
+  };
   if (w < waves)
-    for (int64_t t = r0 + lane; t < r1; t += 64) atomicAdd(&cnt[w * (n + 1) + bin(t)], 1);
+    for (int64_t t0 = r0; t0 < r1; t0 += 64 * AHEAD) {
+      int b[AHEAD];
+      load(t0, b);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (!__ballot(b[k] >= 0)) break;
+        const uint64_t same = alike(b[k]);
+        if (b[k] >= 0 && !(same & (((uint64_t)1 << lane) - 1))) cnt[w * (n + 1) + b[k]] += __popcll(same);
+      }
+    }
   __syncthreads();
   // tokens, tiles and bins before each bin: every thread has a run of bins
   const int per = (n + 1 + T - 1) / T, b0 = min(tid * per, n + 1), b1 = min(b0 + per, n + 1);
@@ -133,25 +158,24 @@ __global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, i
     tiles[t] = {lo, first, min(TILE, seg[lo + 1] - first), f.ord};
   }
   if (w >= waves) return;
-  int bits = 1;
-  while (n >> bits) ++bits;
-  for (int64_t t0 = r0; t0 < r1; t0 += 64) {
-    const int64_t t = t0 + lane;
-    const bool there = t < r1;
-    const int b = there ? bin(t) : -1;
-    uint64_t same = __ballot(there);
-    for (int k = 0; k < bits; ++k) {
-      const uint64_t m = __ballot(there && (b >> k & 1));
-      same &= (b >> k & 1) ? m : ~m;
+  for (int64_t t0 = r0; t0 < r1; t0 += 64 * AHEAD) {
+    int bins[AHEAD];
+    load(t0, bins);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int b = bins[j];
+      const bool there = b >= 0;
+      if (!__ballot(there)) break;
+      const uint64_t same = alike(b);
+      const int before = __popcll(same & (((uint64_t)1 << lane) - 1));
+      const int at = there ? cnt[w * (n + 1) + b] : 0;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");     // the wave has read before its leaders write
+      __builtin_amdgcn_wave_barrier();
+      if (there && before == 0) cnt[w * (n + 1) + b] = at + __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (there) perm[at + before] = (int32_t)(t0 + 64 * j + lane);
     }
-    const int before = __popcll(same & (((uint64_t)1 << lane) - 1));
-    const int at = there ? cnt[w * (n + 1) + b] : 0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the wave has read before its leaders write
-    __builtin_amdgcn_wave_barrier();
-    if (there && before == 0) cnt[w * (n + 1) + b] = at + __popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    if (there) perm[at + before] = (int32_t)t;
   }
 }
 
@@ -212,10 +236,11 @@ template <bool H, int RT>
 __global__ __launch_bounds__(256) void shrink_kernel(Shrink p) {
   extern __shared__ f32x4 red[];              // [wave][RT * 4][64]
   const Plan plan = plan_view(p.plan, p.N, p.n);
-  const Tile t = tile_at(plan, blockIdx.x, p.N, p.n);
+  const unsigned tile = blockIdx.x / p.shares, share = blockIdx.x - tile * p.shares;
+  const Tile t = tile_at(plan, tile, p.N, p.n);
   if ((unsigned)t.adapter >= (unsigned)p.n) return;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-  const int subs = (t.count + 15) >> 4, r0 = blockIdx.z * 64;
+  const int subs = (t.count + 15) >> 4, r0 = blockIdx.y * 64;
   const uint16_t* xr[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
@@ -224,28 +249,41 @@ __global__ __launch_bounds__(256) void shrink_kernel(Shrink p) {
   const uint16_t* wr[RT];
 #pragma unroll
   for (int k = 0; k < RT; ++k) wr[k] = p.w + ((int64_t)t.adapter * p.r + min(r0 + 16 * k + i, p.r - 1)) * p.K + 8 * q;
-  const int units = (p.K + 63) / 64, u0 = (int)((int64_t)units * blockIdx.y / p.shares), u1 = (int)((int64_t)units * (blockIdx.y + 1) / p.shares);
+  const int units = (p.K + 63) / 64, u0 = (int)((int64_t)units * share / p.shares), u1 = (int)((int64_t)units * (share + 1) / p.shares);
   f32x4 acc[RT][4] = {};
   const u32x4 none = {0, 0, 0, 0};
-  for (int u = u0 + w; u < u1; u += 4) {
-    u32x4 xv[2][4], wv[2][RT];
+  struct Unit {
+    u32x4 x[2][4], w[2][RT];
+  };
+  auto fetch = [&](int u, Unit& v) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = 64 * u + 32 * h;
       const bool in = k + 8 * q < p.K;
 #pragma unroll
-      for (int j = 0; j < RT; ++j) wv[h][j] = in ? *reinterpret_cast<const u32x4*>(wr[j] + k) : none;
+      for (int j = 0; j < RT; ++j) v.w[h][j] = in ? *reinterpret_cast<const u32x4*>(wr[j] + k) : none;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        if (s < subs) xv[h][s] = in ? *reinterpret_cast<const u32x4*>(xr[s] + k) : none;
+        if (s < subs) v.x[h][s] = in ? *reinterpret_cast<const u32x4*>(xr[s] + k) : none;
     }
+  };
+  // two units' operands in two sets of registers: a set is loaded again as soon as it is used up
+  auto turn = [&](int u, Unit& v) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         if (s < subs)
 #pragma unroll
-          for (int j = 0; j < RT; ++j) acc[j][s] = mfma16<H>(wv[h][j], xv[h][s], acc[j][s]);
+          for (int j = 0; j < RT; ++j) acc[j][s] = mfma16<H>(v.w[h][j], v.x[h][s], acc[j][s]);
+    if (u + 8 < u1) fetch(u + 8, v);
+  };
+  Unit v0, v1;
+  if (u0 + w < u1) fetch(u0 + w, v0);
+  if (u0 + w + 4 < u1) fetch(u0 + w + 4, v1);
+  for (int u = u0 + w; u < u1; u += 8) {
+    turn(u, v0);
+    if (u + 4 < u1) turn(u + 4, v1);
   }
 #pragma unroll
   for (int j = 0; j < RT; ++j)
@@ -260,7 +298,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(Shrink p) {
     f32x4 v = red[e * 64 + lane];
 #pragma unroll
     for (int k = 1; k < 4; ++k) v += red[(k * RT * 4 + e) * 64 + lane];
-    *reinterpret_cast<f32x4*>(p.part + (((int64_t)blockIdx.y * p.tiles + blockIdx.x) * TILE + slot) * p.rs + rank) = v;
+    *reinterpret_cast<f32x4*>(p.part + (((int64_t)share * p.tiles + tile) * TILE + slot) * p.rs + rank) = v;
   }
 }
 
@@ -274,6 +312,7 @@ struct Expand {
   uint16_t* out;
   int64_t ldy, ldo, N, tiles;
   int n, r, F, ldw, shares, chunks, rs;
+  bool few;
   const int32_t* plan;
   const float *part, *scales;
   uint16_t* planes;             // [tile][upper, rest][ranks to 16][64 slots], or NULL
@@ -298,52 +337,69 @@ __device__ __forceinline__ u32x4 rank8(const uint16_t* row, int k, int r) {
   }
 }
 
-template <bool H, int RV, bool ONE>          // ONE: r <= 16, upper and rest in one matrix instruction
-__global__ __launch_bounds__(256) void expand_kernel(Expand p) {
-  extern __shared__ u32x4 tf[];              // [step][subtile][64]
-  const Plan plan = plan_view(p.plan, p.N, p.n);
-  const Tile t = tile_at(plan, blockIdx.x, p.N, p.n);
-  if (t.adapter < 0) return;
-  const bool bare = t.adapter == p.n;        // tokens without an adapter
-  if (bare && p.y == p.out) return;
-  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-  const int subs = (t.count + 15) >> 4;
-  int64_t row[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s) row[s] = row_at(plan, t.first + min(16 * s + i, t.count - 1), p.N);
-  const int units = (p.F + 63) / 64, u0 = (int)((int64_t)units * blockIdx.y / p.chunks), u1 = (int)((int64_t)units * (blockIdx.y + 1) / p.chunks);
-  if (!bare) {
-    const int groups = ONE ? 2 : (p.r + 31) / 32 * 4, slot = lane;
-    const float scale = p.scales ? p.scales[t.adapter] : 1.0f;
-    for (int g = w; g < groups; g += 4) {
+// Ranks up to 16 take one matrix instruction, upper and rest side by side in its K; more go 32 at a time, upper and rest
+// one after the other.
+enum { R16, R32, R64, RMORE };
+
+// over lanes l, l + 16, l + 32 and l + 48
+__device__ __forceinline__ float rows_sum(float x) {
+  auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// t' of a tile, its shares summed and scaled, split into LDS: [step of 32 ranks][upper, rest][subtile][lane] (R16: [subtile]
+// [lane]).  A wave takes 8 ranks; its lanes the 64 tokens, or (FEW) the 16 of a subtile and every fourth share each.
+template <int RK, bool FEW>
+__device__ __forceinline__ void split_t(const Expand& p, const Tile& t, unsigned tile, bool planes, u32x4* tf) {
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+  const int eights = RK == R16 ? 2 : (p.r + 31) / 32 * 4, turns = !FEW ? 1 : planes ? 4 : (t.count + 15) >> 4;
+  const float scale = p.scales ? p.scales[t.adapter] : 1.0f;
+  const int64_t share = p.tiles * TILE * p.rs;
+  for (int g = w; g < eights; g += 4)
+    for (int turn = 0; turn < turns; ++turn) {
+      const int slot = FEW ? 16 * turn + (lane & 15) : lane;
       float f[8] = {};
-      if (slot < t.count) {
-        const float* at = p.part + ((int64_t)blockIdx.x * TILE + slot) * p.rs + 8 * g;
-        for (int k = 0; k < p.shares; ++k, at += p.tiles * TILE * p.rs) {
+      if (slot < t.count && 8 * g < p.r) {
+        // the second four ranks are there or are not added
+        const float* at = p.part + ((int64_t)tile * TILE + slot) * p.rs + 8 * g;
+        const int second = 8 * g + 4 < p.rs ? 4 : 0;
+        // four shares' loads at a time (FEW: two), the last ones read again for nothing
+        constexpr int AT = FEW ? 2 : 4, BY = FEW ? 4 : 1;
+        for (int k = FEW ? lane >> 4 : 0; k < p.shares; k += AT * BY) {
+          f32x4 v[AT][2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (8 * g + 4 * h < p.r) {
-              const f32x4 v = *reinterpret_cast<const f32x4*>(at + 4 * h);
+          for (int j = 0; j < AT; ++j) {
+            const float* a = at + min(k + j * BY, p.shares - 1) * share;
+            v[j][0] = *reinterpret_cast<const f32x4*>(a), v[j][1] = *reinterpret_cast<const f32x4*>(a + second);
+          }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) f[4 * h + e] += v[e];
-            }
+          for (int j = 0; j < AT; ++j)
+            if (k + j * BY < p.shares)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] += v[j][0][e], f[4 + e] += v[j][1][e];
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = 8 * g + e < p.r ? f[e] * scale : 0.0f;
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (FEW) f[e] = rows_sum(f[e]);
+        f[e] = 8 * g + e < p.r ? f[e] * scale : 0.0f;
+      }
+      if (FEW && lane >= 16) continue;
       u32x4 hi, lo;
       split8(f, hi, lo);
       const int s = slot >> 4, l = slot & 15;
-      if constexpr (ONE) {
+      if constexpr (RK == R16) {
         tf[s * 64 + 16 * g + l] = hi;
         tf[s * 64 + 16 * (g + 2) + l] = lo;
       } else {
         tf[((g >> 2) * 8 + s) * 64 + 16 * (g & 3) + l] = hi;
         tf[((g >> 2) * 8 + 4 + s) * 64 + 16 * (g & 3) + l] = lo;
       }
-      if (p.planes && blockIdx.y == 0) {
+      if (planes) {
         const int r16 = (p.r + 15) & ~15;
-        uint16_t* pl = p.planes + (int64_t)blockIdx.x * 2 * r16 * TILE + slot;
+        uint16_t* pl = p.planes + (int64_t)tile * 2 * r16 * TILE + slot;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (8 * g + e < r16) {
@@ -352,59 +408,228 @@ __global__ __launch_bounds__(256) void expand_kernel(Expand p) {
           }
       }
     }
+}
+
+// 32 features of 16 tokens, ranks of one step: the product added to acc[0 .. 1]
+template <bool H, bool ONE>
+__device__ __forceinline__ void add_step(const u32x4 (&w)[2], const u32x4& ta, const u32x4& tb, f32x4 (&acc)[2]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    u32x4 wv = w[j], wl;
+    if constexpr (H) split_f16(w[j], wv, wl);
+    acc[j] = mfma_bf16(wv, ta, acc[j]);
+    if constexpr (!ONE) acc[j] = mfma_bf16(wv, tb, acc[j]);
+    if constexpr (H) acc[j] = mfma_bf16(wl, ta, acc[j]);
+    if constexpr (H && !ONE) acc[j] = mfma_bf16(wl, tb, acc[j]);
+  }
+}
+template <bool H>
+__device__ __forceinline__ u32x4 plus(const u32x4& y, const f32x4 (&acc)[2]) {
+  u32x4 o;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    o[c] = pack2h<H>(half_lo<H>(y[c]) + acc[c >> 1][2 * (c & 1)], half_hi<H>(y[c]) + acc[c >> 1][2 * (c & 1) + 1]);
+  return o;
+}
+// the row of W that row i of the j-th matrix instruction of 32 features takes: two of them leave a lane 8 consecutive ones
+__device__ __forceinline__ int feature(int i, int j) { return 8 * (i >> 2) + 4 * j + (i & 3); }
+
+// Tiles that mostly have up to 16 tokens: bound by W, of which a wave has 64 features in work and 64 in flight, from memory
+// to the matrix instruction; further subtiles one after the other
+template <bool H, int RV, int RK>
+__device__ __forceinline__ void expand_few(const Expand& p, const Plan& plan, const Tile& t, unsigned tile, unsigned chunk, u32x4* tf) {
+  constexpr bool ONE = RK == R16;
+  constexpr int STEPS = RK == R64 ? 2 : 1;   // of 32 ranks, loaded ahead (RMORE: none)
+  const bool bare = t.adapter == p.n;        // tokens without an adapter
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+  const int units = (p.F + 63) / 64, u0 = (int)((int64_t)units * chunk / p.chunks) + w, u1 = (int)((int64_t)units * (chunk + 1) / p.chunks);
+  const uint16_t* wa = p.w + (int64_t)t.adapter * p.F * p.ldw;
+  auto weights = [&](int f0, int step, u32x4 (&v)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) v[j] = rank8<RV>(wa + (int64_t)min(f0 + feature(i, j), p.F - 1) * p.ldw, ONE ? 8 * (q & 1) : 32 * step + 8 * q, p.r);
+  };
+  struct Unit {
+    u32x4 y[2], w[2][STEPS][2];
+  };
+  int64_t row = 0;
+  auto fetch_w = [&](int u, Unit& g) {
+    if (bare || RK == RMORE) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) weights(64 * u + 32 * e, st, g.w[e][st]);
+  };
+  auto fetch_y = [&](int u, Unit& g) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int fl = 64 * u + 32 * e + 8 * q;
+      g.y[e] = p.y && fl < p.F ? *reinterpret_cast<const u32x4*>(p.y + row * p.ldy + fl) : u32x4{0, 0, 0, 0};
+    }
+  };
+  Unit v0, v1;                               // a set is loaded again as soon as it is used up
+  if (u0 < u1) fetch_w(u0, v0);              // they need no more than the tile
+  if (u0 + 4 < u1) fetch_w(u0 + 4, v1);
+  row = row_at(plan, t.first + min(i, t.count - 1), p.N);
+  if (u0 < u1) fetch_y(u0, v0);
+  if (u0 + 4 < u1) fetch_y(u0 + 4, v1);
+  if (!bare) {
+    split_t<RK, true>(p, t, tile, p.planes && chunk == 0, tf);
     __syncthreads();
   }
-  for (int u = u0 + w; u < u1; u += 4) {
+  int sub = 0;
+  u32x4 t16;
+  auto turn = [&](int u, Unit& v) {
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int f0 = 64 * u + 32 * g, fl = f0 + 8 * q;
-      u32x4 yv[4];
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        yv[s] = p.y && s < subs && fl < p.F ? *reinterpret_cast<const u32x4*>(p.y + row[s] * p.ldy + fl) : u32x4{0, 0, 0, 0};
-      f32x4 acc[4][2] = {};
+    for (int e = 0; e < 2; ++e) {
+      f32x4 acc[2] = {};
       if (!bare) {
-        const uint16_t* wr[2];
+        if constexpr (ONE) {
+          add_step<H, true>(v.w[e][0], t16, t16, acc);
+        } else if constexpr (RK == RMORE) {
+          for (int st = 0; st < (p.r + 31) / 32; ++st) {
+            u32x4 w2[2];
+            weights(64 * u + 32 * e, st, w2);
+            add_step<H, false>(w2, tf[st * 512 + sub * 64 + lane], tf[st * 512 + 256 + sub * 64 + lane], acc);
+          }
+        } else {
+#pragma unroll
+          for (int st = 0; st < STEPS; ++st) add_step<H, false>(v.w[e][st], tf[st * 512 + sub * 64 + lane], tf[st * 512 + 256 + sub * 64 + lane], acc);
+        }
+      }
+      const int fl = 64 * u + 32 * e + 8 * q;
+      if (16 * sub + i < t.count && fl < p.F) *reinterpret_cast<u32x4*>(p.out + row * p.ldo + fl) = bare ? v.y[e] : plus<H>(v.y[e], acc);
+    }
+    if (u + 8 < u1) fetch_w(u + 8, v), fetch_y(u + 8, v);
+  };
+  for (;;) {
+    if (ONE && !bare) t16 = tf[sub * 64 + lane];
+    for (int u = u0; u < u1; u += 8) {
+      turn(u, v0);
+      if (u + 4 < u1) turn(u + 4, v1);
+    }
+    if (16 * ++sub >= t.count) return;
+    row = row_at(plan, t.first + min(16 * sub + i, t.count - 1), p.N);
+    if (u0 < u1) fetch_w(u0, v0), fetch_y(u0, v0);
+    if (u0 + 4 < u1) fetch_w(u0 + 4, v1), fetch_y(u0 + 4, v1);
+  }
+}
+
+// A lane has 8 features of its token in each of two groups of 32 (x, y): lanes of the upper eight tokens of 16 give theirs
+// of the first group for the lower eight's of the second.  Then x holds whole 128-byte lines of the lower tokens' rows
+// across the wave, y of the upper ones', where x and y before held halves of 16 rows' lines; the same again undoes it.
+__device__ __forceinline__ void trade(u32x4& x, u32x4& y, bool upper) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t give = upper ? x[c] : y[c];
+    const uint32_t got = __builtin_amdgcn_update_dpp(0, give, 0x128, 0xf, 0xf, true);      // from the lane 8 on in its 16
+    x[c] = upper ? got : x[c];
+    y[c] = upper ? y[c] : got;
+  }
+}
+
+// Larger tiles: bound by y and out.  A wave takes 128 features, whose part of W it holds in registers for all subtiles, one
+// subtile after the other: the four waves of a workgroup work on 1 KB of 16 rows at a time.
+template <bool H, int RV, int RK>
+__device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, const Tile& t, unsigned tile, unsigned chunk, u32x4* tf) {
+  constexpr bool ONE = RK == R16;
+  constexpr int STEPS = RK == R64 || RK == RMORE ? 2 : 1;      // of 32 ranks, held at a time
+  const bool bare = t.adapter == p.n;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
+  const int subs = (t.count + 15) >> 4;
+  const int units = (p.F + 127) / 128, u0 = (int)((int64_t)units * chunk / p.chunks) + w, u1 = (int)((int64_t)units * (chunk + 1) / p.chunks);
+  const uint16_t* wa = p.w + (int64_t)t.adapter * p.F * p.ldw;
+  u32x4 wv[4][STEPS][2];
+  auto fetch_w = [&](int u, int rb) {
+    if (bare) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          wr[j] = p.w + ((int64_t)t.adapter * p.F + min(f0 + 8 * (i >> 2) + 4 * j + (i & 3), p.F - 1)) * p.ldw;
-        const int steps = ONE ? 1 : (p.r + 31) / 32;
-        for (int k = 0; k < steps; ++k) {
-          u32x4 wv[2], wl[2];
+          wv[e][st][j] = rank8<RV>(wa + (int64_t)min(128 * u + 32 * e + feature(i, j), p.F - 1) * p.ldw, ONE ? 8 * (q & 1) : 64 * rb + 32 * st + 8 * q, p.r);
+  };
+  if (u0 < u1 && RK != RMORE) fetch_w(u0, 0);                  // it needs no more than the tile
+  // y and out by whole lines: of tokens i % 8 and 8 + i % 8 of a subtile, features 64 g + 32 (i / 8) + 8 q on
+  const bool upper = i >= 8;
+  int32_t row[4][2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            wv[j] = rank8<RV>(wr[j], ONE ? 8 * (q & 1) : 32 * k + 8 * q, p.r);
-            if constexpr (H) split_f16(wv[j], wv[j], wl[j]);
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) row[s][e] = (int32_t)row_at(plan, t.first + min(16 * s + 8 * e + (i & 7), t.count - 1), p.N);
+  auto column = [&](int u, int g) { return 128 * u + 64 * g + 32 * (i >> 3) + 8 * q; };
+  auto fetch_y = [&](int u, int s, u32x4 (&y)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int fl = column(u, e >> 1);
+      y[e] = p.y && s < subs && fl < p.F ? *reinterpret_cast<const u32x4*>(p.y + row[s][e & 1] * p.ldy + fl) : u32x4{0, 0, 0, 0};
+    }
+  };
+  u32x4 y0[4], y1[4];                                          // subtiles in turn, loaded again as soon as they are used up
+  if (u0 < u1) fetch_y(u0, 0, y0), fetch_y(u0, 1, y1);
+  if (!bare) {
+    split_t<RK, false>(p, t, tile, p.planes && chunk == 0, tf);
+    __syncthreads();
+  }
+  auto turn = [&](int u, int s, u32x4 (&y)[4]) {
+    if (s < subs) {
+      f32x4 acc[4][2] = {};
+      if (!bare) {
+        const int blocks = RK == RMORE ? (p.r + 63) / 64 : 1;
+        for (int rb = 0; rb < blocks; ++rb) {
+          if (RK == RMORE) fetch_w(u, rb);
+#pragma unroll
+          for (int st = 0; st < STEPS; ++st) {
+            const int step = 2 * rb + st;
+            if (RK == RMORE && 32 * step >= p.r) break;
+            u32x4 ta, tb;
+            if constexpr (ONE) ta = tb = tf[s * 64 + lane];
+            else ta = tf[step * 512 + s * 64 + lane], tb = tf[step * 512 + 256 + s * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add_step<H, ONE>(wv[e][st], ta, tb, acc[e]);
           }
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            if (s < subs) {
-              const u32x4 a = tf[(k * 8 + s) * 64 + lane];
-              u32x4 b;
-              if constexpr (!ONE) b = tf[(k * 8 + 4 + s) * 64 + lane];
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                acc[s][j] = mfma_bf16(wv[j], a, acc[s][j]);
-                if constexpr (!ONE) acc[s][j] = mfma_bf16(wv[j], b, acc[s][j]);
-                if constexpr (H) acc[s][j] = mfma_bf16(wl[j], a, acc[s][j]);
-                if constexpr (H && !ONE) acc[s][j] = mfma_bf16(wl[j], b, acc[s][j]);
-              }
-            }
         }
       }
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (16 * s + i < t.count && fl < p.F) {
-          u32x4 o;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f32x4& v = acc[s][e >> 1];
-            o[e] = pack2h<H>(half_lo<H>(yv[s][e]) + v[2 * (e & 1)], half_hi<H>(yv[s][e]) + v[2 * (e & 1) + 1]);
-          }
-          *reinterpret_cast<u32x4*>(p.out + row[s] * p.ldo + fl) = bare ? yv[s] : o;
+      for (int g = 0; g < 2; ++g) {
+        u32x4 o[2] = {y[2 * g], y[2 * g + 1]};
+        if (!bare) {
+          trade(o[0], o[1], upper);
+          o[0] = plus<H>(o[0], acc[2 * g]);
+          o[1] = plus<H>(o[1], acc[2 * g + 1]);
+          trade(o[0], o[1], upper);
         }
+        const int fl = column(u, g);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (16 * s + 8 * e + (i & 7) < t.count && fl < p.F) *reinterpret_cast<u32x4*>(p.out + row[s][e] * p.ldo + fl) = o[e];
+      }
     }
+    if (s < 2) fetch_y(u, s + 2, y);
+    else if (u + 4 < u1) fetch_y(u + 4, s - 2, y);
+  };
+  for (int u = u0; u < u1; u += 4) {
+    turn(u, 0, y0);
+    turn(u, 1, y1);
+    turn(u, 2, y0);
+    turn(u, 3, y1);
+    if (u + 4 < u1 && RK != RMORE) fetch_w(u + 4, 0);
   }
+}
+
+template <bool H, int RV, int RK, bool FEW>
+__global__ __launch_bounds__(256) void expand_kernel(Expand p) {
+  extern __shared__ u32x4 tf[];
+  const Plan plan = plan_view(p.plan, p.N, p.n);
+  // a tile's shares of F in consecutive workgroups: at any time all of a row's stretch is in work, not one share of all
+  // rows, whose stride would put it on part of the memory channels; and a power of two of them, so that an XCD meets
+  // its own features of an adapter again and again
+  const unsigned tile = blockIdx.x / p.chunks, chunk = blockIdx.x - tile * p.chunks;
+  const Tile t = tile_at(plan, tile, p.N, p.n);
+  if (t.adapter < 0) return;
+  if (t.adapter == p.n && p.y == p.out) return;
+  if constexpr (FEW) expand_few<H, RV, RK>(p, plan, t, tile, chunk, tf);
+  else expand_many<H, RV, RK>(p, plan, t, tile, chunk, tf);
 }
 
 // ------------------------------------------------------------------ grad
@@ -417,7 +642,8 @@ struct Grad {
   const uint16_t* planes[2];
   float* part[2];
   int64_t ldq[2], N, tiles;
-  int F[2], turn[2], pieces[2];
+  int F[2], turn[2];
+  int64_t first;               // workgroups of dA, ahead of those of dB
   int n, r, rblocks;
   const int32_t* plan;
 };
@@ -427,17 +653,75 @@ constexpr int QROW = 72;             // elements of a token's row in LDS: 64 and
 template <bool H, int RT>
 __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
   __shared__ __attribute__((aligned(16))) uint16_t slices[4][(H ? 2 : 1) * 32 * QROW];
-  const int z = blockIdx.z / p.rblocks, r0 = (blockIdx.z - z * p.rblocks) * 64;
+  const int z = blockIdx.x >= p.first, F = p.F[z], fb = (F + 255) / 256;
+  const unsigned id = blockIdx.x - (z ? (unsigned)p.first : 0), run = id / fb;
+  const int r0 = blockIdx.y * 64;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
-  const int F = p.F[z], f0 = (blockIdx.x * 4 + w) * 64, r16 = (p.r + 15) & ~15;
-  const int64_t t0 = (int64_t)blockIdx.y * p.turn[z], t1 = min(t0 + p.turn[z], p.tiles);
+  const int f0 = ((id - run * fb) * 4 + w) * 64, r16 = (p.r + 15) & ~15;
+  const int64_t t0 = (int64_t)run * p.turn[z], t1 = min(t0 + p.turn[z], p.tiles);
   if (f0 >= F || t0 >= t1) return;
   const Plan plan = plan_view(p.plan, p.N, p.n);
   uint16_t* slice = slices[w];
   const int fl = f0 + 8 * (lane & 7);
+
+  // The steps of 32 tokens.  Two of them have their rows and planes in registers, in sets that are loaded again as soon as
+  // they are used up, and the places of the rows behind these are there already.
+  struct Step {
+    int64_t tile;
+    Tile t;
+    int half;
+    bool ok;
+  };
+  auto open = [&](int64_t tile) {
+    Step s;
+    s.tile = tile, s.half = 0;
+    s.ok = tile < t1;
+    if (s.ok) {
+      s.t = tile_at(plan, tile, p.N, p.n);
+      s.ok = (unsigned)s.t.adapter < (unsigned)p.n;      // else tokens without an adapter, or no tile: nothing behind them
+    }
+    return s;
+  };
+  auto after = [&](const Step& s) {
+    if (!s.ok) return s;
+    if (32 * (s.half + 1) < s.t.count) {
+      Step n = s;
+      ++n.half;
+      return n;
+    }
+    return open(s.tile + 1);
+  };
+  auto places = [&](const Step& s, int32_t (&row)[4]) {
+    if (s.ok)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row[j] = plan.perm[s.t.first + min(32 * s.half + 8 * j + (lane >> 3), s.t.count - 1)];
+  };
+  struct Set {
+    u32x4 v[4], a[RT][2];
+  };
+  auto rows = [&](const Step& s, const int32_t (&row)[4], Set& g) {
+    if (s.ok)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool there = 32 * s.half + 8 * j + (lane >> 3) < s.t.count && fl < F;
+        g.v[j] = there ? *reinterpret_cast<const u32x4*>(p.q[z] + (int64_t)min((uint32_t)row[j], (uint32_t)(p.N - 1)) * p.ldq[z] + fl)
+                       : u32x4{0, 0, 0, 0};
+      }
+  };
+  auto factors = [&](const Step& s, Set& g) {
+    if (!s.ok) return;
+    const uint16_t* pl = p.planes[z] + (s.tile * 2 * r16 + r0 + i) * TILE + 32 * s.half + 8 * q;
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        g.a[j][h] = r0 + 16 * j < r16 ? *reinterpret_cast<const u32x4*>(pl + (16 * j + h * r16) * TILE) : u32x4{0, 0, 0, 0};
+  };
+
   f32x4 acc[RT][4] = {};
-  auto flush = [&](int64_t tile, int ord) {
-    float* out = p.part[z] + (tile / p.turn[z] + ord) * p.r * F;
+  auto flush = [&](const Step& s) {
+    const int ord = min((uint32_t)s.t.ord, (uint32_t)min(p.N, (int64_t)p.n) - 1);
+    float* out = p.part[z] + (s.tile / p.turn[z] + ord) * p.r * F;
 #pragma unroll
     for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -450,57 +734,57 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
         acc[j][ft] = f32x4{0, 0, 0, 0};
       }
   };
-  Tile t = tile_at(plan, t0, p.N, p.n);
-  for (int64_t tile = t0; tile < t1; ++tile) {
-    if ((unsigned)t.adapter >= (unsigned)p.n) return;         // tokens without an adapter, or no tile: nothing behind them
-    for (int half = 0; half < 2 && 32 * half < t.count; ++half) {
-      u32x4 v[4];
+  Step now = open(t0), next = after(now), third = after(next);
+  int32_t row[4];
+  Set g0, g1;
+  places(now, row);
+  rows(now, row, g0);
+  factors(now, g0);
+  places(next, row);
+  rows(next, row, g1);
+  factors(next, g1);
+  places(third, row);
+  auto turn = [&](Set& g) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int slot = 32 * half + 8 * j + (lane >> 3);
-        const int64_t row = row_at(plan, t.first + min(slot, t.count - 1), p.N);
-        v[j] = slot < t.count && fl < F ? *reinterpret_cast<const u32x4*>(p.q[z] + row * p.ldq[z] + fl) : u32x4{0, 0, 0, 0};
-      }
-      u32x4 a[RT][2];
-      const uint16_t* pl = p.planes[z] + (tile * 2 * r16 + r0 + i) * TILE + 32 * half + 8 * q;
-#pragma unroll
-      for (int j = 0; j < RT; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          a[j][h] = r0 + 16 * j < r16 ? *reinterpret_cast<const u32x4*>(pl + (16 * j + h * r16) * TILE) : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint16_t* at = slice + (8 * j + (lane >> 3)) * QROW + 8 * (lane & 7);
-        if constexpr (H) {
-          u32x4 hi, lo;
-          split_f16(v[j], hi, lo);
-          *reinterpret_cast<u32x4*>(at) = hi;
-          *reinterpret_cast<u32x4*>(at + 32 * QROW) = lo;
-        } else {
-          *reinterpret_cast<u32x4*>(at) = v[j];
-        }
-      }
-#pragma unroll
-      for (int ft = 0; ft < 4; ++ft) {
-        const u32x4 b = tr_frag(slice, QROW, 0, 16 * ft, lane);
-        u32x4 bl;
-        if constexpr (H) bl = tr_frag(slice + 32 * QROW, QROW, 0, 16 * ft, lane);
-#pragma unroll
-        for (int j = 0; j < RT; ++j) {
-          acc[j][ft] = mfma_bf16(a[j][0], b, acc[j][ft]);
-          acc[j][ft] = mfma_bf16(a[j][1], b, acc[j][ft]);
-          if constexpr (H) acc[j][ft] = mfma_bf16(a[j][1], bl, mfma_bf16(a[j][0], bl, acc[j][ft]));
-        }
+    for (int j = 0; j < 4; ++j) {
+      uint16_t* at = slice + (8 * j + (lane >> 3)) * QROW + 8 * (lane & 7);
+      if constexpr (H) {
+        u32x4 hi, lo;
+        split_f16(g.v[j], hi, lo);
+        *reinterpret_cast<u32x4*>(at) = hi;
+        *reinterpret_cast<u32x4*>(at + 32 * QROW) = lo;
+      } else {
+        *reinterpret_cast<u32x4*>(at) = g.v[j];
       }
     }
-    const Tile next = tile + 1 < t1 ? tile_at(plan, tile + 1, p.N, p.n) : Tile{-1, 0, 0, 0};
-    if (next.adapter != t.adapter) flush(tile, min((uint32_t)t.ord, (uint32_t)min(p.N, (int64_t)p.n) - 1));
-    t = next;
+    rows(third, row, g);
+    const Step fourth = after(third);
+    places(fourth, row);
+#pragma unroll
+    for (int ft = 0; ft < 4; ++ft) {
+      const u32x4 b = tr_frag(slice, QROW, 0, 16 * ft, lane);
+      u32x4 bl;
+      if constexpr (H) bl = tr_frag(slice + 32 * QROW, QROW, 0, 16 * ft, lane);
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        acc[j][ft] = mfma_bf16(g.a[j][0], b, acc[j][ft]);
+        acc[j][ft] = mfma_bf16(g.a[j][1], b, acc[j][ft]);
+        if constexpr (H) acc[j][ft] = mfma_bf16(g.a[j][1], bl, mfma_bf16(g.a[j][0], bl, acc[j][ft]));
+      }
+    }
+    factors(third, g);
+    if (!next.ok || next.t.adapter != now.t.adapter) flush(now);
+    now = next, next = third, third = fourth;
+  };
+  while (now.ok) {
+    turn(g0);
+    if (now.ok) turn(g1);
   }
 }
 
-// The pieces of every adapter in their order, rounded: dA [n, r, F] (z = 0), dB [n, F, r] (z = 1); adapters without tokens
-// get zeros.  A thread has a feature and 8 ranks.
+// The pieces of every adapter in their order, rounded: dA [n, r, F] (z even), dB [n, F, r] (z odd); adapters without
+// tokens get zeros.  A workgroup takes 64 features and 16 ranks, a thread 4 features of a rank, with eight pieces' loads in
+// flight; dB turns through LDS.
 struct GradSum {
   const float* part[2];
   uint16_t* out[2];
@@ -511,43 +795,56 @@ struct GradSum {
 };
 
 __global__ __launch_bounds__(256) void grad_sum_kernel(GradSum p) {
-  const int z = blockIdx.z, F = p.F[z], groups = (p.r + 7) / 8, a = blockIdx.y;
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (!p.out[z] || e >= (int64_t)F * groups) return;
-  const int g = (int)(e / F), f = (int)(e - (int64_t)g * F);
+  __shared__ uint16_t s[64][18];
+  const int z = blockIdx.z & 1, F = p.F[z], a = blockIdx.y, f0 = blockIdx.x * 64, r0 = (blockIdx.z >> 1) * 16;
+  if (!p.out[z] || f0 >= F) return;
+  const int k = threadIdx.x >> 4, rank = r0 + k, f = f0 + 4 * (threadIdx.x & 15);
   const Plan plan = plan_view(p.plan, p.N, p.n);
   const int ta = plan.tstart[a], tb = plan.tstart[a + 1];
-  float v[8] = {};
-  if (tb > ta) {
-    const int ord = plan.tiles[ta].ord, s1 = (tb - 1) / p.turn[z] + ord;
-    for (int s = ta / p.turn[z] + ord; s <= s1; ++s) {
-      const float* at = p.part[z] + ((int64_t)s * p.r + 8 * g) * F + f;
+  f32x4 v = {0, 0, 0, 0};
+  if (tb > ta && rank < p.r && f < F) {
+    const int ord = plan.tiles[ta].ord, s0 = ta / p.turn[z] + ord, pieces = (tb - 1) / p.turn[z] + ord - s0 + 1;
+    const float* at = p.part[z] + ((int64_t)s0 * p.r + rank) * F + f;
+    const int64_t piece = (int64_t)p.r * F;
+    for (int j0 = 0; j0 < pieces; j0 += 8) {
+      f32x4 u[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (8 * g + k < p.r) v[k] += at[(int64_t)k * F];
+      for (int j = 0; j < 8; ++j) u[j] = *reinterpret_cast<const f32x4*>(at + min(j0 + j, pieces - 1) * piece);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < pieces) v += u[j];
     }
   }
-  uint32_t o[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) o[k] = p.h ? pack2h<true>(v[2 * k], v[2 * k + 1]) : pack2h<false>(v[2 * k], v[2 * k + 1]);
-  if (z == 1 && p.r % 8 == 0) {
-    *reinterpret_cast<u32x4*>(p.out[1] + ((int64_t)a * F + f) * p.r + 8 * g) = u32x4{o[0], o[1], o[2], o[3]};
+  const uint32_t lo = p.h ? pack2h<true>(v[0], v[1]) : pack2h<false>(v[0], v[1]), hi = p.h ? pack2h<true>(v[2], v[3]) : pack2h<false>(v[2], v[3]);
+  if (z == 0) {
+    if (rank < p.r && f < F) *reinterpret_cast<u32x2*>(p.out[0] + ((int64_t)a * p.r + rank) * F + f) = u32x2{lo, hi};
     return;
   }
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (8 * g + k < p.r) {
-      const uint16_t h = (uint16_t)(o[k >> 1] >> (16 * (k & 1)));
-      if (z == 0) p.out[0][((int64_t)a * p.r + 8 * g + k) * F + f] = h;
-      else p.out[1][((int64_t)a * F + f) * p.r + 8 * g + k] = h;
-    }
+  const int c = 4 * (threadIdx.x & 15);
+  s[c][k] = (uint16_t)lo, s[c + 1][k] = (uint16_t)(lo >> 16), s[c + 2][k] = (uint16_t)hi, s[c + 3][k] = (uint16_t)(hi >> 16);
+  __syncthreads();
+  const int ranks = min(16, p.r - r0);
+  uint16_t* out = p.out[1] + ((int64_t)a * F + f0) * p.r + r0;
+  for (int e = threadIdx.x; e < min(64, F - f0) * ranks; e += 256) out[(int64_t)(e / ranks) * p.r + e % ranks] = s[e / ranks][e % ranks];
 }
 
-// dst [n][cols][ld] = the transposes of src [n][rows][cols], rows to ld zero
-__global__ __launch_bounds__(256) void transpose_kernel(const uint16_t* __restrict__ src, int rows, int cols, int ld, uint16_t* __restrict__ dst) {
+// dst [n][cols][ld] = the transposes of src [n][rows][cols], rows to ld zero; two of them in one launch (z: 2 n)
+struct Transpose {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int rows[2], cols[2], ld[2], n;
+};
+
+__global__ __launch_bounds__(256) void transpose_kernel(Transpose p) {
   __shared__ uint16_t s[64][66];
-  const int64_t a = blockIdx.z;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int which = blockIdx.z >= p.n, rows = p.rows[which], cols = p.cols[which], ld = p.ld[which];
+  const int64_t a = blockIdx.z - which * p.n;
+  const int tc = (cols + 63) / 64, tr = (ld + 63) / 64;
+  if ((int)blockIdx.x >= tc * tr) return;
+  const int c0 = (blockIdx.x % tc) * 64, r0 = (blockIdx.x / tc) * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const uint16_t* src = p.src[which];
+  uint16_t* dst = p.dst[which];
+#pragma unroll 8
   for (int k = y; k < 64; k += 4)
     s[k][x] = r0 + k < rows && c0 + x < cols ? src[(a * rows + r0 + k) * cols + c0 + x] : (uint16_t)0;
   __syncthreads();
@@ -561,16 +858,21 @@ inline int launched() { return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ER
 inline bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-constexpr int64_t WANTED = 1024;     // workgroups of a launch, four on a CU
+// Whether tiles have few tokens: on average up to 16, were every adapter (and none) to occur.  64 tokens of 128 adapters,
+// 4096 -> 14336, rank 16: expand 10 us this way, 15 the other; 16384 tokens of 4, 1024 -> 4096: 85 and 55.
+bool few_of(int64_t N, int n) { return N <= 16 * (int64_t)(n + 1); }
 
-// shares of K of a shrink: enough workgroups, at least 256 K (one turn of the four waves) each
+// Shares of K of a shrink, two workgroups on a CU and at least 512 K each: every workgroup of expand adds a tile's shares up.
 int shares_of(int64_t tiles, int K) {
-  const int64_t s = (WANTED + tiles - 1) / tiles, most = (K + 255) / 256;
+  const int64_t s = (512 + tiles - 1) / tiles, most = (K + 511) / 512;
   return (int)std::max<int64_t>(1, std::min(s, most));
 }
-int chunks_of(int64_t tiles, int F) {
-  const int64_t s = (WANTED + tiles - 1) / tiles, most = (F + 255) / 256;
-  return (int)std::max<int64_t>(1, std::min(s, most));
+// Shares of F of an expand: a power of two, up to about 1100 workgroups, a unit of features for every wave at least
+int chunks_of(int64_t tiles, int F, bool few) {
+  int64_t c = 1;
+  while (2 * c * tiles <= 1100 && c < 64) c *= 2;
+  const int unit = few ? 256 : 512;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(c, (F + unit - 1) / unit));
 }
 size_t part_bytes(int64_t tiles, int K, int r) { return align256((size_t)shares_of(tiles, K) * tiles * TILE * ((r + 3) & ~3) * 4); }
 size_t plane_bytes(int64_t tiles, int r) { return align256((size_t)tiles * 2 * ((r + 15) & ~15) * TILE * 2); }
@@ -578,13 +880,13 @@ size_t plane_bytes(int64_t tiles, int r) { return align256((size_t)tiles * 2 * (
 // tiles of a workgroup of grad, and its pieces
 int turn_of(int64_t tiles, int F) {
   const int64_t fb = (F + 255) / 256;
-  return (int)std::max<int64_t>(1, tiles * fb / (WANTED / 2));
+  return (int)std::max<int64_t>(1, tiles * fb / 512);
 }
 int64_t pieces_of(int64_t tiles, int64_t N, int n, int turn) { return (tiles + turn - 1) / turn + std::min<int64_t>(N, n); }
 
 int launch_shrink(bool h, const Shrink& p, hipStream_t st) {
   const int rb = (p.r + 63) / 64, rt = std::min((p.r + 15) / 16, 4);
-  const dim3 grid((unsigned)p.tiles, p.shares, rb);
+  const dim3 grid((unsigned)(p.tiles * p.shares), rb);
   auto go = [&](auto* k, int RT) {
     k<<<grid, 256, RT * 16384, st>>>(p);
     return launched();
@@ -594,24 +896,22 @@ int launch_shrink(bool h, const Shrink& p, hipStream_t st) {
   return h ? go(shrink_kernel<true, 4>, 4) : go(shrink_kernel<false, 4>, 4);
 }
 
-int launch_expand(bool h, const Expand& p, hipStream_t st) {
-  const bool one = p.r <= 16;
-  const int lds = one ? 4096 : (p.r + 31) / 32 * 8192, rv = p.ldw % 8 == 0 ? 8 : p.ldw % 4 == 0 ? 4 : 1;
-  const dim3 grid((unsigned)p.tiles, p.chunks);
-  auto go = [&](auto* k) {
-    k<<<grid, 256, lds, st>>>(p);
-    return launched();
-  };
-#define LBK_EXPAND(H)                                                                         \
-  if (rv == 8) return one ? go(expand_kernel<H, 8, true>) : go(expand_kernel<H, 8, false>);   \
-  if (rv == 4) return one ? go(expand_kernel<H, 4, true>) : go(expand_kernel<H, 4, false>);   \
-  return one ? go(expand_kernel<H, 1, true>) : go(expand_kernel<H, 1, false>);
-  if (h) {
-    LBK_EXPAND(true)
-  }
-  LBK_EXPAND(false)
-#undef LBK_EXPAND
+template <bool H, int RV, int RK>
+int launch_expand_t(const Expand& p, hipStream_t st) {
+  const int lds = (RK == R16 ? 256 : (p.r + 31) / 32 * 512) * 16;      // t': at most 64 KB
+  if (p.few) expand_kernel<H, RV, RK, true><<<(unsigned)(p.tiles * p.chunks), 256, lds, st>>>(p);
+  else expand_kernel<H, RV, RK, false><<<(unsigned)(p.tiles * p.chunks), 256, lds, st>>>(p);
+  return launched();
 }
+template <bool H>
+int launch_expand_h(const Expand& p, hipStream_t st) {
+  const int rv = p.ldw % 8 == 0 ? 8 : p.ldw % 4 == 0 ? 4 : 1;
+  if (p.r <= 16) return rv == 8 ? launch_expand_t<H, 8, R16>(p, st) : rv == 4 ? launch_expand_t<H, 4, R16>(p, st) : launch_expand_t<H, 1, R16>(p, st);
+  if (rv == 8 && p.r <= 32) return launch_expand_t<H, 8, R32>(p, st);
+  if (rv == 8 && p.r <= 64) return launch_expand_t<H, 8, R64>(p, st);
+  return rv == 8 ? launch_expand_t<H, 8, RMORE>(p, st) : rv == 4 ? launch_expand_t<H, 4, RMORE>(p, st) : launch_expand_t<H, 1, RMORE>(p, st);
+}
+int launch_expand(bool h, const Expand& p, hipStream_t st) { return h ? launch_expand_h<true>(p, st) : launch_expand_h<false>(p, st); }
 
 int check_adapter(const lbk_adapter* d) {
   if (!d) return LBK_ERR_NULL;
@@ -675,7 +975,8 @@ int lbk_adapter_add(const lbk_adapter* d, const void* x, int64_t ldx, const void
                  d->plan, static_cast<float*>(workspace)};
   if (int st = launch_shrink(h, s, S(stream))) return st;
   const Expand e{static_cast<const uint16_t*>(d->b), static_cast<const uint16_t*>(y), static_cast<uint16_t*>(out), ldy, ldo, d->N, tiles, d->n,
-                 d->rank, d->out_features, d->rank, shares, chunks_of(tiles, d->out_features), rs, d->plan, static_cast<const float*>(workspace),
+                 d->rank, d->out_features, d->rank, shares, chunks_of(tiles, d->out_features, few_of(d->N, d->n)), rs, few_of(d->N, d->n),
+                 d->plan, static_cast<const float*>(workspace),
                  d->scales, static_cast<uint16_t*>(planes)};
   return launch_expand(h, e, S(stream));
 }
@@ -730,17 +1031,17 @@ int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void
   float* pa = reinterpret_cast<float*>(take(sz.pa));
   float* pb = reinterpret_cast<float*>(take(sz.pb));
   if (some && (dx || da)) {
-    transpose_kernel<<<dim3((r + 63) / 64, (out + 63) / 64, d->n), 256, 0, st>>>(static_cast<const uint16_t*>(d->b), out, r, out, bt);
+    Transpose tp{};
+    tp.src[0] = static_cast<const uint16_t*>(d->b), tp.dst[0] = bt, tp.rows[0] = out, tp.cols[0] = r, tp.ld[0] = out;
+    tp.src[1] = static_cast<const uint16_t*>(d->a), tp.dst[1] = att, tp.rows[1] = r, tp.cols[1] = in, tp.ld[1] = r8, tp.n = d->n;
+    const int most = std::max((out + 63) / 64, dx ? (in + 63) / 64 : 0) * ((r8 + 63) / 64);
+    transpose_kernel<<<dim3(most, 1, dx ? 2 * d->n : d->n), 256, 0, st>>>(tp);
     if (int e = launched()) return e;
-    if (dx) {
-      transpose_kernel<<<dim3((in + 63) / 64, (r + 63) / 64, d->n), 256, 0, st>>>(static_cast<const uint16_t*>(d->a), r, in, r8, att);
-      if (int e = launched()) return e;
-    }
     const int shares = shares_of(tiles, out);
     const Shrink s{static_cast<const uint16_t*>(dout), bt, ldo, d->N, tiles, d->n, r, out, shares, rs, d->plan, part};
     if (int e = launch_shrink(h, s, st)) return e;
     const Expand e{att, nullptr, static_cast<uint16_t*>(dx), in, in, d->N, tiles, d->n, r, dx ? in : 0, r8, shares,
-                   dx ? chunks_of(tiles, in) : 1, rs, d->plan, part, d->scales, da ? dplanes : nullptr};
+                   dx ? chunks_of(tiles, in, few_of(d->N, d->n)) : 1, rs, few_of(d->N, d->n), d->plan, part, d->scales, da ? dplanes : nullptr};
     if (int k = launch_expand(h, e, st)) return k;
   }
   if (!da && !db) return LBK_OK;
@@ -752,11 +1053,10 @@ int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void
   g.F[0] = da ? in : 0, g.F[1] = db ? out : 0;
   g.turn[0] = some ? turn_of(tiles, in) : 1, g.turn[1] = some ? turn_of(tiles, out) : 1;
   if (some) {
-    const int F = std::max(g.F[0], g.F[1]);
-    int64_t runs = 0;
-    for (int z = 0; z < 2; ++z)
-      if (g.F[z]) runs = std::max(runs, (tiles + g.turn[z] - 1) / g.turn[z]);
-    const dim3 grid((F + 255) / 256, (unsigned)runs, 2 * g.rblocks);
+    int64_t blocks[2];
+    for (int z = 0; z < 2; ++z) blocks[z] = (int64_t)((g.F[z] + 255) / 256) * ((tiles + g.turn[z] - 1) / g.turn[z]);
+    g.first = blocks[0];
+    const dim3 grid((unsigned)(blocks[0] + blocks[1]), g.rblocks);
     const int rt = std::min((r + 15) / 16, 4);
     auto go = [&](auto* k) {
       k<<<grid, 256, 0, st>>>(g);
@@ -770,8 +1070,8 @@ int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void
   GradSum m{};
   m.part[0] = pa, m.part[1] = pb, m.out[0] = static_cast<uint16_t*>(da), m.out[1] = static_cast<uint16_t*>(db);
   m.F[0] = in, m.F[1] = out, m.turn[0] = g.turn[0], m.turn[1] = g.turn[1], m.N = d->N, m.n = d->n, m.r = r, m.h = h, m.plan = d->plan;
-  const int64_t most = ((int64_t)std::max(da ? in : 0, db ? out : 0) * ((r + 7) / 8) + 255) / 256;
-  grad_sum_kernel<<<dim3((unsigned)most, d->n, 2), 256, 0, st>>>(m);
+  const int most = (std::max(da ? in : 0, db ? out : 0) + 63) / 64;
+  grad_sum_kernel<<<dim3(most, d->n, 2 * ((r + 15) / 16)), 256, 0, st>>>(m);
   return launched();
 }
 
