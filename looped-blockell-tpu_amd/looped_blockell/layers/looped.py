@@ -23,18 +23,42 @@ from .norms import RMSNorm
 
 
 class LoopedSwiGLU(nn.Module):
+    """``h <- h + MLP(RMSNorm(h))``, L times; with any of the last four options
+    ``h <- h + residual_scale * gate * dropout(post_norm(MLP(norm(h))))``, an application's branch and the next one's norm
+    joined by ``kernels.residual_norm`` on the fp32 state.  ``gate``: a parameter [d_model] (ones), or per call a
+    tensor [G, d_model] with a row for every N / G consecutive tokens in its place.  ``dropout`` drops with the
+    ``dropout_seed`` of a call (application t with stream t), and not at all without one."""
+
     def __init__(self, d_model: int, d_ff: int, L: int, tile_size: int = 16, density: float = 1.0,
-                 eps: float = 1e-5, device=None, bias: bool = True):
+                 eps: float = 1e-5, device=None, bias: bool = True, post_norm: bool = False, gate: bool = False,
+                 residual_scale: float = 1.0, dropout: float = 0.0):
         super().__init__()
         self.L = L
         self.norm = RMSNorm(d_model, eps=eps, device=device)
         self.mlp = MLPBlock(d_model, d_ff, use_swiglu=True, tile_size=tile_size, density=density, device=device,
                             bias=bias)
+        self.post_norm = RMSNorm(d_model, eps=eps, device=device) if post_norm else None
+        self.gate = nn.Parameter(torch.ones(d_model, device=device)) if gate else None
+        self.residual_scale, self.dropout = residual_scale, dropout
 
-    def forward(self, h: torch.Tensor) -> torch.Tensor:
+    def _seams(self, h2: torch.Tensor, gate, seed) -> torch.Tensor:
+        hf, n = h2.float(), self.norm(h2)
+        post = None if self.post_norm is None else self.post_norm.scale
+        p = self.dropout if seed is not None else 0.0
+        for t in range(self.L):
+            pre = self.norm.scale if t + 1 < self.L else None
+            hf, n = kernels.residual_norm(hf, self.mlp(n), post, gate, pre, self.residual_scale, self.norm.eps, p,
+                                          0 if seed is None else seed, t)
+        return hf.to(torch.bfloat16)
+
+    def forward(self, h: torch.Tensor, gate: torch.Tensor | None = None, dropout_seed=None) -> torch.Tensor:
         lead = h.shape[:-1]
         d = h.shape[-1]
         h2 = h.reshape(-1, d).to(torch.bfloat16).contiguous()
+        gate = self.gate if gate is None else gate
+        if (self.post_norm is not None or gate is not None or self.residual_scale != 1.0
+                or (self.dropout > 0.0 and dropout_seed is not None)):
+            return self._seams(h2, gate, dropout_seed).reshape(*lead, d)
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters())):
             if (self.L >= 1 and h2.shape[0] > 0 and d == self.mlp.d_model and _plain(self.norm, RMSNorm)
                     and _plain(self.mlp, MLPBlock) and self.mlp.use_swiglu and self.mlp._fp32_values()):

@@ -236,7 +236,9 @@ class MLPBlock(nn.Module):
             out = kernels.gelu_fwd_prepacked(x2, p1, v1, c1, p2, v2, c2, fc1.bias, fc2.bias)
         return out if x.dim() == 2 else out.reshape(*x.shape[:-1], out.shape[-1])
 
-    def forward(self, x: torch.Tensor, deterministic: bool = True) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, deterministic: bool = True, dropout_seed=None, dropout_stream: int = 0) -> torch.Tensor:
+        """With ``deterministic`` False the result is dropped out: by torch's generator, or with ``dropout_seed`` (an int
+        or a GPU tensor of one int64) by ``kernels.dropout``, which stores no mask."""
         if self.use_swiglu:
             x2 = x.reshape(-1, self.d_model).to(torch.bfloat16).contiguous()
             bg, bu, bd = self.swiglu_biases()
@@ -253,5 +255,8 @@ class MLPBlock(nn.Module):
         else:                       # the two layers one by one: their hooks and overrides see each
             out = self.fc2(F.gelu(self.fc1(x).float(), approximate="tanh").to(torch.bfloat16))
         if self.dropout > 0.0 and not deterministic:
-            out = F.dropout(out, p=self.dropout, training=True)
+            if dropout_seed is None:
+                out = F.dropout(out, p=self.dropout, training=True)
+            else:
+                out = kernels.dropout(out, self.dropout, dropout_seed, dropout_stream)
         return out
