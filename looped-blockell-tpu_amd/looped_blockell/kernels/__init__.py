@@ -548,6 +548,7 @@ def dropout(x, p: float, seed, stream: int = 0):
     column (rows counted over the leading dimensions), as ``include/lbk.h`` defines; it is never stored.
     Differentiable: the backward makes the same mask again."""
     _gpu(x)
+    _no_transforms()
     return ops().counter_dropout(x, float(p), *_seed(seed), int(stream))
 
 
@@ -563,19 +564,20 @@ def residual_norm(h, y, post_scale=None, gate=None, pre_scale=None, residual_sca
     h' before that is rounded.  ``gate`` is [d], or [G, d] with one row for every N / G consecutive rows (a sequence's, a
     token's).  ``post_scale`` and ``pre_scale`` are [d], used in fp32.  Differentiable in h, y and the three vectors."""
     _gpu(h, y)
-    h2, y2 = (t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) for t in (h, y))
     if h.shape != y.shape:
         raise RuntimeError(f"h and y must have one shape, got {tuple(h.shape)} and {tuple(y.shape)}")
-    args = (h2, y2, post_scale, gate, pre_scale, float(residual_scale), float(eps), float(p), *_seed(seed), int(stream))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, y, post_scale, gate, pre_scale)):
+    flat = h.dim() == 2
+    h2, y2 = (h, y) if flat else (h.reshape(-1, h.shape[-1]), y.reshape(-1, y.shape[-1]))
+    t, s = _seed(seed)
+    if torch.is_grad_enabled() and (h.requires_grad or y.requires_grad or any(
+            v is not None and v.requires_grad for v in (post_scale, gate, pre_scale))):
         _no_transforms()
-        hn, n = ops().residual_norm_train(*args)
+        hn, n = ops().residual_norm_train(h2, y2, post_scale, gate, pre_scale, residual_scale, eps, p, t, s, stream)
     else:
-        hn, n = ops().residual_norm(*args)
-    if h.dim() != 2:
-        hn = hn.reshape(h.shape)
-        n = n if pre_scale is None else n.reshape(h.shape)
-    return hn, (None if pre_scale is None else n)
+        hn, n = ops().residual_norm(h2, y2, post_scale, gate, pre_scale, residual_scale, eps, p, t, s, stream)
+    if pre_scale is None:
+        return (hn if flat else hn.reshape(h.shape)), None
+    return (hn, n) if flat else (hn.reshape(h.shape), n.reshape(h.shape))
 
 
 class AdapterPlan(NamedTuple):

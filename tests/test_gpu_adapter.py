@@ -254,6 +254,51 @@ def test_deterministic_and_on_another_stream(gpu, K):
     assert all(torch.equal(p, q) for p, q in zip(first, second))
 
 
+def test_offsets_beyond_32_bits(gpu, K):
+    """y and out of more than 2^31 elements: the last tokens as alone, into a new tensor and in place, and their gradients."""
+    N, fin, fout = 263000, 64, 8192
+    g = torch.Generator().manual_seed(6)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()
+    x, y = torch.zeros(N, fin, dtype=BF, device="cuda"), torch.zeros(N, fout, dtype=BF, device="cuda")
+    x[-70:], y[-70:] = r(70, fin), r(70, fout)
+    a, b = r(2, 16, fin), r(2, fout, 16)
+    ids = torch.full((N,), -1, dtype=torch.int32)
+    ids[-70:] = torch.arange(70) % 2
+    dout = r(70, fout)
+    want = ref.adapter(y[-70:], x[-70:], a, b, ids[-70:].cuda(), None, dout)
+    plan = K.adapter_plan(ids.cuda(), 2)
+    for t in (x, a, b):
+        t.requires_grad_(True)
+    out = K.adapter_add(y, x, a, b, plan)
+    ref.close(out[-70:].detach(), want["out"])
+    assert not bool(out[:-70].any())
+    full = torch.zeros(N, fout, dtype=BF, device="cuda")
+    full[-70:] = dout
+    dx, da, db = torch.autograd.grad(out, [x, a, b], full)
+    ref.close(dx[-70:], want["dx"])
+    ref.close(da, want["da"])
+    ref.close(db, want["db"])
+    with torch.no_grad():
+        K.adapter_add(y, x, a, b, plan, inplace=True)
+        assert torch.equal(y[-70:], out[-70:]) and not bool(y[:-70].any())
+
+
+def test_into_its_own_input_and_single_tokens(gpu, K):
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()
+    a, b = r(2, 8, 64), r(2, 64, 8)
+    x = r(40, 64)
+    plan = K.adapter_plan((torch.arange(40) % 3).cuda(), 2)
+    want = K.adapter_add(x, x, a, b, plan)
+    assert torch.equal(K.adapter_add(x, x, a, b, plan, inplace=True), want)
+    with torch.inference_mode():                              # a token alone, without leading dimensions
+        one = K.adapter_plan(torch.tensor(1, device="cuda"), 2)
+        v, w = r(64), r(64)
+        out = K.adapter_add(v, w, a, b, one)
+        assert out.shape == (64,) and torch.equal(out, K.adapter_add(v[None], w[None], a, b, one)[0])
+        assert torch.equal(K.adapter_add(v, w, a, b, one, inplace=True), out)
+
+
 def test_refusals(gpu, K):
     z = lambda *s, dt=BF: torch.zeros(*s, dtype=dt, device="cuda")
     y, x, a, b = z(4, 64), z(4, 32), z(2, 8, 32), z(2, 64, 8)

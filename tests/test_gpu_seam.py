@@ -274,6 +274,33 @@ def test_captured_training_step(gpu, K):
         last = got[1]
 
 
+def test_seam_of_many_rows(gpu, K):
+    """Elements beyond 2^31, forward and backward: the last rows as alone."""
+    N, d = 263000, 8192
+    h = torch.zeros(N, d, dtype=BF, device="cuda")
+    g = torch.Generator().manual_seed(8)
+    y, tail = h.clone(), 3
+    h[-tail:], y[-tail:] = randn(g, tail, d, dtype=BF), randn(g, tail, d, dtype=BF)
+    w = 1 + 0.1 * randn(g, d)
+    a, b = h[-tail:].clone().requires_grad_(True), y[-tail:].clone().requires_grad_(True)
+    want = K.residual_norm(a, b, w, w, w)
+    grads = torch.autograd.grad([t.sum() for t in want], [a, b])
+    h.requires_grad_(True), y.requires_grad_(True)
+    got = K.residual_norm(h, y, w, w, w)
+    assert all(torch.equal(p[-tail:], q) for p, q in zip(got, want))
+    one = torch.ones(1, dtype=BF, device="cuda").expand(N, d)
+    dh, dy = torch.autograd.grad(got, [h, y], [one, one])
+    assert torch.equal(dh[-tail:], grads[0]) and torch.equal(dy[-tail:], grads[1])
+
+
+def test_transforms_are_refused(gpu, K):
+    x = torch.ones(3, 4, 16, device="cuda")
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.vmap(lambda t: K.dropout(t, 0.5, 1))(x)
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda t: K.residual_norm(t, t)[0].sum())(x[0])
+
+
 def test_seed_changed_before_the_backward(gpu, K):
     x = torch.ones(4, 8, device="cuda", requires_grad=True)
     seed = torch.tensor([1], device="cuda")
