@@ -53,7 +53,8 @@ __device__ __forceinline__ Tile tile_at(const Plan& p, int64_t k, int64_t N, int
 }
 __device__ __forceinline__ int64_t row_at(const Plan& p, int place, int64_t N) { return min((uint32_t)p.perm[place], (uint32_t)(N - 1)); }
 
-// A stable counting sort by one workgroup.  Each wave counts a run of tokens of its own, the counts are added up bin by
+// A stable counting sort by one workgroup, once for all projections of a batch (16384 tokens: 19 us, 64: 5.6).  Each wave
+// counts a run of tokens of its own, the counts are added up bin by
 // bin and wave by wave, and each wave goes over its run again: a token's place is its bin's and wave's first one plus
 // the same bin's tokens before it, those of the wave's 64 found by comparing the bins' bits.
 template <typename I>
@@ -67,7 +68,6 @@ __global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, i
   int32_t *seg = const_cast<int32_t*>(pv.seg), *tstart = const_cast<int32_t*>(pv.tstart), *perm = const_cast<int32_t*>(pv.perm);
   Tile* tiles = const_cast<Tile*>(pv.tiles);
   for (int k = tid; k < waves * (n + 1); k += T) cnt[k] = 0;
-  __syncthreads();
   const int64_t run = ((N + waves - 1) / waves + 63) / 64 * 64, r0 = w * run, r1 = min(r0 + run, N);
   int bits = 1;
   while (n >> bits) ++bits;
@@ -89,10 +89,16 @@ __global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, i
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) b[k] = t0 + 64 * k + lane >= r1 ? -1 : v[k] >= 0 && v[k] < n ? (int)v[k] : n;
   };
+  int kept[AHEAD];                           // the run's first ones, for the second time too
+  if (w < waves) load(r0, kept);
+  __syncthreads();
   if (w < waves)
     for (int64_t t0 = r0; t0 < r1; t0 += 64 * AHEAD) {
       int b[AHEAD];
-      load(t0, b);
+      if (t0 > r0) load(t0, b);
+      else
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) b[k] = kept[k];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         if (!__ballot(b[k] >= 0)) break;
@@ -160,7 +166,10 @@ __global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, i
   if (w >= waves) return;
   for (int64_t t0 = r0; t0 < r1; t0 += 64 * AHEAD) {
     int bins[AHEAD];
-    load(t0, bins);
+    if (t0 > r0) load(t0, bins);
+    else
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) bins[k] = kept[k];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int b = bins[j];
@@ -222,8 +231,10 @@ __device__ __forceinline__ void split_f16(const u32x4& v, u32x4& hi, u32x4& lo) 
 
 // ------------------------------------------------------------------ shrink
 // part[share][tile][slot][rank] = sum over a share of K of W[a][rank][k] x[token][k], W [n, r, K].  Memory-bound: x once
-// (long prompts) or W once (a token an adapter).  A workgroup takes a tile and a share of K, its waves 64 K at a time in
-// turn (a line of each row); a lane's operands are 16 bytes of a row, from memory to the matrix instruction.
+// (long prompts: 134 MB of 16384 x 4096 in 28 us) or W once (a token an adapter).  A workgroup takes a tile and a share of
+// K, its waves 64 K at a time in turn (a line of each row); a lane's operands are 16 bytes of a row, from memory to the
+// matrix instruction.  A tile's shares lie in consecutive workgroups, so that all of a row is in work at a time (16384 x 1024:
+// 15.5 -> 13.3 us).
 struct Shrink {
   const uint16_t *x, *w;
   int64_t ldx, N, tiles;
@@ -304,9 +315,10 @@ __global__ __launch_bounds__(256) void shrink_kernel(Shrink p) {
 
 // ------------------------------------------------------------------ expand
 // out[token][f] = y[token][f] + sum over ranks of W[a][f][rank] t'[token][rank], W [n, F, r] with rows of ldw.
-// Memory-bound by y and out.  A workgroup takes a tile and a share of F: it adds up t's shares, splits t' into LDS in the
-// order of the matrix instruction's operand (`planes`: and for grad, ranks first), and its waves take 64 features at a
-// time.  The 32 features of two products are dealt so that a lane ends with 8 consecutive ones of a token.
+// Memory-bound by y and out (16384 tokens, 1024 / 4096, rank 16: 268 MB in 55 us), or by W (64 tokens, an adapter each,
+// 4096 / 14336: 27 MB in 10 us).  A workgroup takes a tile and a share of F: it adds up t's shares, splits t' into LDS in
+// the order of the matrix instruction's operand (`planes`: and for grad, ranks first), and its waves share the features.
+// The 32 features of two products are dealt so that a lane ends with 8 consecutive ones of a token.
 struct Expand {
   const uint16_t *w, *y;        // y NULL: out is the product alone
   uint16_t* out;
@@ -350,64 +362,69 @@ __device__ __forceinline__ float rows_sum(float x) {
 }
 
 // t' of a tile, its shares summed and scaled, split into LDS: [step of 32 ranks][upper, rest][subtile][lane] (R16: [subtile]
-// [lane]).  A wave takes 8 ranks; its lanes the 64 tokens, or (FEW) the 16 of a subtile and every fourth share each.
+// [lane]); slots without a token hold anything, as they stay in their columns of the products.  A thread has 4 ranks of a
+// token, the threads beside it the next ones (a token's 8 ranks each were 32 bytes of every row at a time: expand of 4099
+// tokens, 2048 / 8192, rank 64 43.9 -> 42.9 us).  FEW: lanes 16 apart take every fourth share each.
 template <int RK, bool FEW>
-__device__ __forceinline__ void split_t(const Expand& p, const Tile& t, unsigned tile, bool planes, u32x4* tf) {
+__device__ __forceinline__ void split_t(const Expand& p, const Tile& t, unsigned tile, u32x4* tf) {
+  constexpr int QB = RK == R16 ? 2 : 3;      // fours of a step's ranks: 4 (two halves of a K), 8
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
-  const int eights = RK == R16 ? 2 : (p.r + 31) / 32 * 4, turns = !FEW ? 1 : planes ? 4 : (t.count + 15) >> 4;
   const float scale = p.scales ? p.scales[t.adapter] : 1.0f;
   const int64_t share = p.tiles * TILE * p.rs;
-  for (int g = w; g < eights; g += 4)
-    for (int turn = 0; turn < turns; ++turn) {
-      const int slot = FEW ? 16 * turn + (lane & 15) : lane;
-      float f[8] = {};
-      if (slot < t.count && 8 * g < p.r) {
-        // the second four ranks are there or are not added
-        const float* at = p.part + ((int64_t)tile * TILE + slot) * p.rs + 8 * g;
-        const int second = 8 * g + 4 < p.rs ? 4 : 0;
-        // four shares' loads at a time (FEW: two), the last ones read again for nothing
-        constexpr int AT = FEW ? 2 : 4, BY = FEW ? 4 : 1;
-        for (int k = FEW ? lane >> 4 : 0; k < p.shares; k += AT * BY) {
-          f32x4 v[AT][2];
+  const int items = (RK == R16 ? 1 : (p.r + 31) / 32) * 4 << (QB + 4);
+  u32x2* out = reinterpret_cast<u32x2*>(tf);
+  constexpr int AT = FEW ? 2 : 4, BY = FEW ? 4 : 1, PASS = FEW ? 64 : 256;
+#pragma unroll 2
+  for (int k0 = 0; k0 < items; k0 += PASS) {
+    const int item = k0 + (FEW ? 16 * w + (lane & 15) : (int)threadIdx.x);
+    const int four = item & ((1 << QB) - 1), l = item >> QB & 15, s = item >> (QB + 4) & 3, step = item >> (QB + 6);
+    const int slot = 16 * s + l, rank = 32 * step + 4 * four;
+    f32x4 f = {0, 0, 0, 0};
+    if (slot < t.count && rank < p.r) {
+      const float* at = p.part + ((int64_t)tile * TILE + slot) * p.rs + rank;
+      for (int k = FEW ? lane >> 4 : 0; k < p.shares; k += AT * BY) {       // the last shares are read again for nothing
+        f32x4 v[AT];
 #pragma unroll
-          for (int j = 0; j < AT; ++j) {
-            const float* a = at + min(k + j * BY, p.shares - 1) * share;
-            v[j][0] = *reinterpret_cast<const f32x4*>(a), v[j][1] = *reinterpret_cast<const f32x4*>(a + second);
-          }
+        for (int j = 0; j < AT; ++j) v[j] = *reinterpret_cast<const f32x4*>(at + min(k + j * BY, p.shares - 1) * share);
 #pragma unroll
-          for (int j = 0; j < AT; ++j)
-            if (k + j * BY < p.shares)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) f[e] += v[j][0][e], f[4 + e] += v[j][1][e];
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (FEW) f[e] = rows_sum(f[e]);
-        f[e] = 8 * g + e < p.r ? f[e] * scale : 0.0f;
-      }
-      if (FEW && lane >= 16) continue;
-      u32x4 hi, lo;
-      split8(f, hi, lo);
-      const int s = slot >> 4, l = slot & 15;
-      if constexpr (RK == R16) {
-        tf[s * 64 + 16 * g + l] = hi;
-        tf[s * 64 + 16 * (g + 2) + l] = lo;
-      } else {
-        tf[((g >> 2) * 8 + s) * 64 + 16 * (g & 3) + l] = hi;
-        tf[((g >> 2) * 8 + 4 + s) * 64 + 16 * (g & 3) + l] = lo;
-      }
-      if (planes) {
-        const int r16 = (p.r + 15) & ~15;
-        uint16_t* pl = p.planes + (int64_t)tile * 2 * r16 * TILE + slot;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (8 * g + e < r16) {
-            pl[(8 * g + e) * TILE] = (uint16_t)(hi[e >> 1] >> (16 * (e & 1)));
-            pl[(r16 + 8 * g + e) * TILE] = (uint16_t)(lo[e >> 1] >> (16 * (e & 1)));
-          }
+        for (int j = 0; j < AT; ++j)
+          if (k + j * BY < p.shares) f += v[j];
       }
     }
+    if (16 * s >= t.count) continue;         // the same for all lanes of a wave
+    u32x2 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (FEW) f[e] = rows_sum(f[e]);
+      f[e] = rank + e < p.r ? f[e] * scale : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      hi[e] = __builtin_amdgcn_perm(__float_as_uint(f[2 * e + 1]), __float_as_uint(f[2 * e]), 0x07060302u);
+      lo[e] = pack2_bf16(rest(f[2 * e]), rest(f[2 * e + 1]));
+    }
+    if (FEW && lane >= 16) continue;
+    const int at = RK == R16 ? s * 64 + 16 * (four >> 1) + l : (step * 8 + s) * 64 + 16 * (four >> 1) + l;
+    out[2 * at + (four & 1)] = hi;
+    out[2 * (at + (RK == R16 ? 32 : 256)) + (four & 1)] = lo;
+  }
+}
+
+// t' from LDS for grad: ranks first, slots without a token zero
+template <int RK>
+__device__ __forceinline__ void put_planes(const Expand& p, const Tile& t, unsigned tile, const u32x4* tf) {
+  const int slot = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), s = slot >> 4, l = slot & 15, r16 = (p.r + 15) & ~15;
+  const u32x4 none = {0, 0, 0, 0};
+  for (int g = w; 8 * g < r16; g += 4) {
+    const int at = RK == R16 ? s * 64 + 16 * g + l : ((g >> 2) * 8 + s) * 64 + 16 * (g & 3) + l;
+    const u32x4 hi = slot < t.count ? tf[at] : none, lo = slot < t.count ? tf[at + (RK == R16 ? 32 : 256)] : none;
+    uint16_t* pl = p.planes + ((int64_t)tile * 2 * r16 + 8 * g) * TILE + slot;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      pl[e * TILE] = (uint16_t)(hi[e >> 1] >> (16 * (e & 1)));
+      pl[(r16 + e) * TILE] = (uint16_t)(lo[e >> 1] >> (16 * (e & 1)));
+    }
+  }
 }
 
 // 32 features of 16 tokens, ranks of one step: the product added to acc[0 .. 1]
@@ -473,8 +490,9 @@ __device__ __forceinline__ void expand_few(const Expand& p, const Plan& plan, co
   if (u0 < u1) fetch_y(u0, v0);
   if (u0 + 4 < u1) fetch_y(u0 + 4, v1);
   if (!bare) {
-    split_t<RK, true>(p, t, tile, p.planes && chunk == 0, tf);
+    split_t<RK, true>(p, t, tile, tf);
     __syncthreads();
+    if (p.planes && chunk == 0) put_planes<RK>(p, t, tile, tf);
   }
   int sub = 0;
   u32x4 t16;
@@ -528,7 +546,10 @@ __device__ __forceinline__ void trade(u32x4& x, u32x4& y, bool upper) {
 }
 
 // Larger tiles: bound by y and out.  A wave takes 128 features, whose part of W it holds in registers for all subtiles, one
-// subtile after the other: the four waves of a workgroup work on 1 KB of 16 rows at a time.
+// subtile after the other: the four waves of a workgroup work on 1 KB of 16 rows at a time.  What counts is how much of a
+// row is in work together: 16384 tokens, 1024 / 4096, rank 16, took 85 us with 64 bytes of 64 rows a wave, 62 with 256 bytes
+// of 16 rows and a subtile a wave, 59 with W through LDS and whole lines a load, and 55 so; rank 64 (4099 tokens, 2048 /
+// 8192) 64, 81, 50 and 43.
 template <bool H, int RV, int RK>
 __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, const Tile& t, unsigned tile, unsigned chunk, u32x4* tf) {
   constexpr bool ONE = RK == R16;
@@ -568,8 +589,9 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
   u32x4 y0[4], y1[4];                                          // subtiles in turn, loaded again as soon as they are used up
   if (u0 < u1) fetch_y(u0, 0, y0), fetch_y(u0, 1, y1);
   if (!bare) {
-    split_t<RK, false>(p, t, tile, p.planes && chunk == 0, tf);
+    split_t<RK, false>(p, t, tile, tf);
     __syncthreads();
+    if (p.planes && chunk == 0) put_planes<RK>(p, t, tile, tf);
   }
   auto turn = [&](int u, int s, u32x4 (&y)[4]) {
     if (s < subs) {
@@ -636,8 +658,9 @@ __global__ __launch_bounds__(256) void expand_kernel(Expand p) {
 
 // ------------------------------------------------------------------ grad
 // part[piece][rank][f] = sum over the tokens of a piece of P[token][rank] Q[token][f], P from planes, Q = x or dy.
-// Memory-bound by Q.  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens lie in an
-// LDS slice of its own and are read transposed.  Where the adapter changes on the way, a piece ends: piece number =
+// Memory-bound by Q (dA and dB of 16384 tokens, 1024 / 4096, rank 16: 168 MB in 34 us; 53 while three of four workgroups
+// of the grid had nothing to do).  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens
+// lie in an LDS slice of its own and are read transposed.  Where the adapter changes on the way, a piece ends: piece number =
 // tile / turn + the adapter's number among those with tokens, which grows with either.
 struct Grad {
   const uint16_t* q[2];
@@ -786,7 +809,7 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
 
 // The pieces of every adapter in their order, rounded: dA [n, r, F] (z even), dB [n, F, r] (z odd); adapters without
 // tokens get zeros.  A workgroup takes 64 features and 16 ranks, a thread 4 features of a rank, with eight pieces' loads in
-// flight; dB turns through LDS.
+// flight (one piece at a time: 91 us instead of 7 at 16384 tokens, 1024 / 4096, rank 16); dB turns through LDS.
 struct GradSum {
   const float* part[2];
   uint16_t* out[2];
@@ -947,8 +970,9 @@ int lbk_adapter_plan(const void* ids, int32_t id_bytes, int64_t N, int32_t n_ada
   const int bins = n_adapters + 1;
   const int waves = (int)std::max<int64_t>(1, std::min<int64_t>({16, 11264 / bins, (N + 63) / 64}));
   const int lds = (waves * bins + bins + 1) * 4;
-  if (id_bytes == 4) plan_kernel<int32_t><<<1, 1024, lds, S(stream)>>>(static_cast<const int32_t*>(ids), N, n_adapters, waves, static_cast<int32_t*>(plan));
-  else plan_kernel<int64_t><<<1, 1024, lds, S(stream)>>>(static_cast<const int64_t*>(ids), N, n_adapters, waves, static_cast<int32_t*>(plan));
+  const int threads = waves <= 4 && bins <= 1024 ? 256 : 1024;
+  if (id_bytes == 4) plan_kernel<int32_t><<<1, threads, lds, S(stream)>>>(static_cast<const int32_t*>(ids), N, n_adapters, waves, static_cast<int32_t*>(plan));
+  else plan_kernel<int64_t><<<1, threads, lds, S(stream)>>>(static_cast<const int64_t*>(ids), N, n_adapters, waves, static_cast<int32_t*>(plan));
   return launched();
 }
 
