@@ -170,6 +170,7 @@ struct AdapterTrain : public torch::autograd::Function<AdapterTrain> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list r(6);
     if (!grads[0].defined()) return r;
+    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
     const std::array<bool, 3> want = {ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)};
     const Tensor dout = grads[0].to(s[0].scalar_type());
@@ -184,12 +185,14 @@ struct AdapterTrain : public torch::autograd::Function<AdapterTrain> {
   }
 };
 
-Tensor adapter_add_train(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
-  return std::get<0>(call_fwd_train(y, x, a, b, plan, scales));
-}
-Tensor adapter_add_train_autograd(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
-  TORCH_CHECK(!scales.has_value() || !scales->requires_grad(), "titan::adapter_add_train: scales have no gradient");
-  return AdapterTrain::apply(y, x, a, b, plan, scales);
+Tensor adapter_add_autograd(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK(!needs_grad(scales), "titan::adapter_add: scales have no gradient");
+    if (y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()) return AdapterTrain::apply(y, x, a, b, plan, scales);
+  }
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("titan::adapter_add", "").typed<decltype(adapter_add)>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(y, x, a, b, plan, scales);
 }
 void adapter_add_inplace_autograd(Tensor y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !(y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()),
@@ -207,7 +210,6 @@ TORCH_LIBRARY_FRAGMENT(titan, m) {
   m.def("adapter_plan(Tensor ids, int n_adapters) -> Tensor");
   m.def("adapter_add(Tensor y, " ADAPTER_ARGS ") -> Tensor");
   m.def("adapter_add_(Tensor(a!) y, " ADAPTER_ARGS ") -> ()");
-  m.def("adapter_add_train(Tensor y, " ADAPTER_ARGS ") -> Tensor");
   m.def("adapter_add_fwd_train(Tensor y, " ADAPTER_ARGS ") -> (Tensor, Tensor)");
   m.def("adapter_add_bwd(Tensor grad_out, Tensor x, Tensor a, Tensor b, Tensor plan, Tensor planes, Tensor? scales, bool[3] want) "
         "-> (Tensor, Tensor, Tensor)");
@@ -217,15 +219,15 @@ TORCH_LIBRARY_IMPL(titan, CUDA, m) {
   m.impl("adapter_plan", &adapter_plan);
   m.impl("adapter_add", &adapter_add);
   m.impl("adapter_add_", &adapter_add_);
-  m.impl("adapter_add_train", &adapter_add_train);
   m.impl("adapter_add_fwd_train", &adapter_add_fwd_train);
   m.impl("adapter_add_bwd", &adapter_add_bwd);
 }
 
 TORCH_LIBRARY_IMPL(titan, Autograd, m) {
-  m.impl("adapter_add_train", &adapter_add_train_autograd);
+  m.impl("adapter_plan", torch::CppFunction::makeFallthrough());      // whole numbers
+  m.impl("adapter_add", &adapter_add_autograd);
   m.impl("adapter_add_", &adapter_add_inplace_autograd);
-  for (const char* name : {"adapter_plan", "adapter_add", "adapter_add_fwd_train", "adapter_add_bwd"})
+  for (const char* name : {"adapter_add_fwd_train", "adapter_add_bwd"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }
 
@@ -239,7 +241,6 @@ TORCH_LIBRARY_IMPL(titan, Meta, m) {
     return at::empty(y.sizes(), y.options());
   };
   m.impl("adapter_add", add);
-  m.impl("adapter_add_train", add);
   m.impl("adapter_add_", [](Tensor, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&) {});
   m.impl("adapter_add_fwd_train", [add](const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
     lbk_adapter d{};

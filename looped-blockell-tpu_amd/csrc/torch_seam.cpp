@@ -59,6 +59,7 @@ struct Dropout : public torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list r(5);
+    const BelowAutograd below;
     if (grads[0].defined())
       r[0] = call_dropout(grads[0], ctx->saved_data["p"].toDouble(), or_none(ctx->get_saved_variables()[0]),
                           ctx->saved_data["seed"].toInt(), ctx->saved_data["stream"].toInt());
@@ -67,7 +68,9 @@ struct Dropout : public torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout_autograd(const Tensor& x, double p, const OptTensor& seed_tensor, int64_t seed, int64_t stream) {
-  return Dropout::apply(x, p, seed_tensor, seed, stream);
+  if (at::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, p, seed_tensor, seed, stream);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_dropout(x, p, seed_tensor, seed, stream);
 }
 
 // ------------------------------------------------------------------ the seam
@@ -226,6 +229,7 @@ struct SeamTrain : public torch::autograd::Function<SeamTrain> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list r(11);
     if (!grads[0].defined() && !grads[1].defined()) return r;
+    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
     auto& v = ctx->saved_data;
     std::array<bool, 5> want;
@@ -243,16 +247,18 @@ struct SeamTrain : public torch::autograd::Function<SeamTrain> {
   }
 };
 
-std::tuple<Tensor, Tensor> seam_train(const Tensor& h, const Tensor& y, const OptTensor& post, const OptTensor& gate, const OptTensor& pre,
-                                      double scale, double eps, double p, const OptTensor& seed_tensor, int64_t seed, int64_t stream) {
-  auto [hn, n, r1, r2] = call_seam_fwd_train(h, y, post, gate, pre, scale, eps, p, seed_tensor, seed, stream);
-  return {hn, n};
-}
-std::tuple<Tensor, Tensor> seam_train_autograd(const Tensor& h, const Tensor& y, const OptTensor& post, const OptTensor& gate,
-                                               const OptTensor& pre, double scale, double eps, double p, const OptTensor& seed_tensor,
-                                               int64_t seed, int64_t stream) {
-  auto r = SeamTrain::apply(h, y, post, gate, pre, scale, eps, p, seed_tensor, seed, stream);
-  return {r[0], r[1]};
+using Two = std::tuple<Tensor, Tensor>;
+
+Two seam_autograd(const Tensor& h, const Tensor& y, const OptTensor& post, const OptTensor& gate, const OptTensor& pre, double scale,
+                  double eps, double p, const OptTensor& seed_tensor, int64_t seed, int64_t stream) {
+  if (at::GradMode::is_enabled() &&
+      (h.requires_grad() || y.requires_grad() || needs_grad(post) || needs_grad(gate) || needs_grad(pre))) {
+    auto r = SeamTrain::apply(h, y, post, gate, pre, scale, eps, p, seed_tensor, seed, stream);
+    return {r[0], r[1]};
+  }
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("titan::residual_norm", "").typed<decltype(seam_fwd)>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(h, y, post, gate, pre, scale, eps, p, seed_tensor, seed, stream);
 }
 
 // for the shape functions: the operators' results are contiguous, whatever the arguments' strides
@@ -266,7 +272,6 @@ Tensor rows_like(const Tensor& x) { return at::empty(x.sizes(), x.options()); }
 TORCH_LIBRARY_FRAGMENT(titan, m) {
   m.def("counter_dropout(Tensor x, float p, Tensor? seed_tensor, int seed, int stream) -> Tensor");
   m.def("residual_norm(Tensor h, Tensor y, " SEAM_ARGS ") -> (Tensor, Tensor)");
-  m.def("residual_norm_train(Tensor h, Tensor y, " SEAM_ARGS ") -> (Tensor, Tensor)");
   m.def("residual_norm_fwd_train(Tensor h, Tensor y, " SEAM_ARGS ") -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("residual_norm_bwd(Tensor? grad_h, Tensor? grad_n, Tensor h, Tensor y, Tensor rs_post, Tensor rs_pre, " SEAM_ARGS
         ", bool[5] want) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
@@ -275,15 +280,14 @@ TORCH_LIBRARY_FRAGMENT(titan, m) {
 TORCH_LIBRARY_IMPL(titan, CUDA, m) {
   m.impl("counter_dropout", &dropout);
   m.impl("residual_norm", &seam_fwd);
-  m.impl("residual_norm_train", &seam_train);
   m.impl("residual_norm_fwd_train", &seam_fwd_train);
   m.impl("residual_norm_bwd", &seam_bwd);
 }
 
 TORCH_LIBRARY_IMPL(titan, Autograd, m) {
   m.impl("counter_dropout", &dropout_autograd);
-  m.impl("residual_norm_train", &seam_train_autograd);
-  for (const char* name : {"residual_norm", "residual_norm_fwd_train", "residual_norm_bwd"})
+  m.impl("residual_norm", &seam_autograd);
+  for (const char* name : {"residual_norm_fwd_train", "residual_norm_bwd"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }
 
@@ -298,7 +302,6 @@ TORCH_LIBRARY_IMPL(titan, Meta, m) {
     return std::make_tuple(rows_like(h), pre.has_value() && pre->defined() ? rows_like(y) : at::empty({0}, y.options()));
   };
   m.impl("residual_norm", two);
-  m.impl("residual_norm_train", two);
   m.impl("residual_norm_fwd_train", [two](const Tensor& h, const Tensor& y, const OptTensor& post, const OptTensor& gate, const OptTensor& pre,
                                           double a, double b, double c, const OptTensor& s, int64_t e, int64_t f) {
     auto [hn, n] = two(h, y, post, gate, pre, a, b, c, s, e, f);

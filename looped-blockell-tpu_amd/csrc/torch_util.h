@@ -71,6 +71,17 @@ inline at::Tensor opt_bias(const c10::optional<at::Tensor>& b, int64_t n, const 
   if (b->scalar_type() == at::kFloat && b->device() == x.device() && b->is_contiguous()) return *b;
   return b->to(x.device(), at::kFloat).contiguous();
 }
+inline bool needs_grad(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); }
+
+// For a backward that calls operators: past the Autograd key, whose fallback boxes every argument, unless a graph of the
+// gradients is asked for (which those operators then refuse or, having a formula, record).
+struct BelowAutograd {
+  c10::optional<at::AutoDispatchBelowADInplaceOrView> guard;
+  BelowAutograd() {
+    if (!at::GradMode::is_enabled()) guard.emplace();
+  }
+};
+
 inline const float* fptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
 }  // namespace

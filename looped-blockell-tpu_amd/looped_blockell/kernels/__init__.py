@@ -568,13 +568,8 @@ def residual_norm(h, y, post_scale=None, gate=None, pre_scale=None, residual_sca
         raise RuntimeError(f"h and y must have one shape, got {tuple(h.shape)} and {tuple(y.shape)}")
     flat = h.dim() == 2
     h2, y2 = (h, y) if flat else (h.reshape(-1, h.shape[-1]), y.reshape(-1, y.shape[-1]))
-    t, s = _seed(seed)
-    if torch.is_grad_enabled() and (h.requires_grad or y.requires_grad or any(
-            v is not None and v.requires_grad for v in (post_scale, gate, pre_scale))):
-        _no_transforms()
-        hn, n = ops().residual_norm_train(h2, y2, post_scale, gate, pre_scale, residual_scale, eps, p, t, s, stream)
-    else:
-        hn, n = ops().residual_norm(h2, y2, post_scale, gate, pre_scale, residual_scale, eps, p, t, s, stream)
+    _no_transforms()
+    hn, n = ops().residual_norm(h2, y2, post_scale, gate, pre_scale, residual_scale, eps, p, *_seed(seed), stream)
     if pre_scale is None:
         return (hn if flat else hn.reshape(h.shape)), None
     return (hn, n) if flat else (hn.reshape(h.shape), n.reshape(h.shape))
@@ -600,21 +595,16 @@ def adapter_add(y, x, a, b, plan: AdapterPlan, scales=None, inplace: bool = Fals
     """``y + scales[id] * (x a[id]^T) b[id]^T`` with each token's adapter, y as it is where a token has none: the
     low-rank update beside a shared projection's y = base(x).  x is [..., in], y [..., out], a [n, rank, in] and b [n, out,
     rank], all bf16 or all fp16 (features multiples of 8, rank 1 .. 256); scales [n] fp32 or None (1).  ``a x`` stays in
-    fp32 up to 16 bits of mantissa.  Differentiable in y, x, a and b as one native autograd node
-    (``titan::adapter_add_train``); ``inplace`` adds into y, without gradients."""
+    fp32 up to 16 bits of mantissa.  Differentiable in y, x, a and b as one native autograd node;
+    ``inplace`` adds into y, without gradients."""
     _gpu(y, x, a, b)
     if plan.tokens * x.shape[-1] != x.numel() or plan.adapters != a.shape[0]:
         raise RuntimeError(f"the plan is of {plan.tokens} tokens and {plan.adapters} adapters; x is {tuple(x.shape)}, a {tuple(a.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     y2 = y if y.dim() == 2 else (y.view if inplace else y.reshape)(-1, y.shape[-1])
-    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
-        if inplace:
-            raise RuntimeError("adapter_add into y has no gradients; call it without inplace or under torch.no_grad()")
-        _no_transforms()
-        out = ops().adapter_add_train(y2, x2, a, b, plan.data, scales)
-    elif inplace:
+    _no_transforms()
+    if inplace:
         ops().adapter_add_(y2, x2, a, b, plan.data, scales)
         return y
-    else:
-        out = ops().adapter_add(y2, x2, a, b, plan.data, scales)
+    out = ops().adapter_add(y2, x2, a, b, plan.data, scales)
     return out if y.dim() == 2 else out.reshape(y.shape)

@@ -327,5 +327,7 @@ def test_refusals(gpu, K):
                 lambda: K.residual_norm(x, x.cpu()), lambda: K.residual_norm(x.cpu(), x)):
         with pytest.raises((RuntimeError, TypeError)):
             bad()
-    with pytest.raises(RuntimeError):                       # the plain operator has no gradient of its own
-        K.ops().residual_norm(x.clone().requires_grad_(True), x, None, None, None, 1.0, 1e-5, 0.0, None, 0, 0)[0].sum().backward()
+    xl = x.clone().requires_grad_(True)                     # no second derivative
+    (d,) = torch.autograd.grad(K.residual_norm(x, xl, post_scale=x[0])[0].sum(), xl, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
