@@ -825,10 +825,10 @@ __global__ __launch_bounds__(256) void grad_sum_kernel(GradSum p) {
   if (!p.out[z] || f0 >= F) return;
   const int k = threadIdx.x >> 4, rank = r0 + k, f = f0 + 4 * (threadIdx.x & 15);
   const Plan plan = plan_view(p.plan, p.N, p.n);
-  const int ta = plan.tstart[a], tb = plan.tstart[a + 1];
+  const int tiles = (int)max_tiles(p.N, p.n), ta = max(plan.tstart[a], 0), tb = min(plan.tstart[a + 1], tiles);      // as tile_at
   f32x4 v = {0, 0, 0, 0};
   if (tb > ta && rank < p.r && f < F) {
-    const int ord = plan.tiles[ta].ord, s0 = ta / p.turn[z] + ord, pieces = (tb - 1) / p.turn[z] + ord - s0 + 1;
+    const int ord = min((uint32_t)plan.tiles[ta].ord, (uint32_t)min(p.N, (int64_t)p.n) - 1), s0 = ta / p.turn[z] + ord, pieces = (tb - 1) / p.turn[z] + ord - s0 + 1;
     const float* at = p.part[z] + ((int64_t)s0 * p.r + rank) * F + f;
     const int64_t piece = (int64_t)p.r * F;
     for (int j0 = 0; j0 < pieces; j0 += 8) {
@@ -853,7 +853,8 @@ __global__ __launch_bounds__(256) void grad_sum_kernel(GradSum p) {
   for (int e = threadIdx.x; e < min(64, F - f0) * ranks; e += 256) out[(int64_t)(e / ranks) * p.r + e % ranks] = s[e / ranks][e % ranks];
 }
 
-// dst [n][cols][ld] = the transposes of src [n][rows][cols], rows to ld zero; two of them in one launch (z: 2 n)
+// dst [n][cols][ld] = the transposes of src [n][rows][cols], rows to ld zero; two of them in one launch (z: 2 n).  A thread's
+// 16 loads are all in flight before the first is used (4 adapters of rank 16, 1024 / 4096: 10 -> 4 us, which is latency).
 struct Transpose {
   const uint16_t* src[2];
   uint16_t* dst[2];
@@ -869,9 +870,11 @@ __global__ __launch_bounds__(256) void transpose_kernel(Transpose p) {
   const int c0 = (blockIdx.x % tc) * 64, r0 = (blockIdx.x / tc) * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
   const uint16_t* src = p.src[which];
   uint16_t* dst = p.dst[which];
-#pragma unroll 8
-  for (int k = y; k < 64; k += 4)
-    s[k][x] = r0 + k < rows && c0 + x < cols ? src[(a * rows + r0 + k) * cols + c0 + x] : (uint16_t)0;
+  uint16_t v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] = src[(a * rows + min(r0 + 4 * k + y, rows - 1)) * cols + min(c0 + x, cols - 1)];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) s[4 * k + y][x] = r0 + 4 * k + y < rows && c0 + x < cols ? v[k] : (uint16_t)0;
   __syncthreads();
   for (int k = y; k < 64; k += 4)
     if (c0 + k < cols && r0 + x < ld) dst[(a * cols + c0 + k) * ld + r0 + x] = s[x][k];
