@@ -549,7 +549,7 @@ __device__ __forceinline__ void trade(u32x4& x, u32x4& y, bool upper) {
 // subtile after the other: the four waves of a workgroup work on 1 KB of 16 rows at a time.  What counts is how much of a
 // row is in work together: 16384 tokens, 1024 / 4096, rank 16, took 85 us with 64 bytes of 64 rows a wave, 62 with 256 bytes
 // of 16 rows and a subtile a wave, 59 with W through LDS and whole lines a load, and 55 so; rank 64 (4099 tokens, 2048 /
-// 8192) 64, 81, 50 and 43.
+// 8192) 64, 81, 50 and 42.
 template <bool H, int RV, int RK>
 __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, const Tile& t, unsigned tile, unsigned chunk, u32x4* tf) {
   constexpr bool ONE = RK == R16;
@@ -594,8 +594,8 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
     if (p.planes && chunk == 0) put_planes<RK>(p, t, tile, tf);
   }
   auto turn = [&](int u, int s, u32x4 (&y)[4]) {
+    f32x4 acc[4][2] = {};
     if (s < subs) {
-      f32x4 acc[4][2] = {};
       if (!bare) {
         const int blocks = RK == RMORE ? (p.r + 63) / 64 : 1;
         for (int rb = 0; rb < blocks; ++rb) {
@@ -612,6 +612,10 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
           }
         }
       }
+    }
+    // ahead of the stores: they would have to end before it is there (rank 64: 43.3 -> 42.1 us)
+    if (s == 3 && u + 4 < u1 && RK != RMORE) fetch_w(u + 4, 0);
+    if (s < subs) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         u32x4 o[2] = {y[2 * g], y[2 * g + 1]};
@@ -635,7 +639,6 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
     turn(u, 1, y1);
     turn(u, 2, y0);
     turn(u, 3, y1);
-    if (u + 4 < u1 && RK != RMORE) fetch_w(u + 4, 0);
   }
 }
 
@@ -890,9 +893,10 @@ inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 // 4096 -> 14336, rank 16: expand 10 us this way, 15 the other; 16384 tokens of 4, 1024 -> 4096: 85 and 55.
 bool few_of(int64_t N, int n) { return N <= 16 * (int64_t)(n + 1); }
 
-// Shares of K of a shrink, two workgroups on a CU and at least 512 K each: every workgroup of expand adds a tile's shares up.
+// Shares of K of a shrink, up to four workgroups on a CU and at least 512 K each: every workgroup of expand adds a tile's shares
+// up (dy of 16384 x 4096, 260 tiles: 2 shares 40 us and 12.8 in expand, 4 shares 35.5 and 13.7, 6 shares 36.7 and 15.1).
 int shares_of(int64_t tiles, int K) {
-  const int64_t s = (512 + tiles - 1) / tiles, most = (K + 511) / 512;
+  const int64_t s = (1024 + tiles - 1) / tiles, most = (K + 511) / 512;
   return (int)std::max<int64_t>(1, std::min(s, most));
 }
 // Shares of F of an expand: a power of two, up to about 1100 workgroups, a unit of features for every wave at least
