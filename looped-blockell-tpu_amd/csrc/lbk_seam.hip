@@ -390,11 +390,13 @@ __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
 // A workgroup takes consecutive rows, a worker (NW waves) W of these, and keeps the columns' sums in registers; the next
 // row's loads are in flight while a row is worked on.  Sums go to `part`, one row a workgroup, and are added in a fixed
 // order by seam_sum_kernel: no atomics.  A gate's rows either lie in one worker each (bpg = 0: written at once) or take bpg
-// workgroups each.  Memory-bound: 302 MB of 16384 x 1024 (fp32 state, bf16 branch) in 75 us with dropout.
-template <int TH, int TY, int E, bool DROP, bool ODD>
+// workgroups each.  Memory-bound: 302 MB of 16384 x 1024 (fp32 state, bf16 branch) in 61 us with dropout, which is the copy's rate
+// (FULL; with post, pre and gate loaded in every row, which waits for the next row's loads too, 75).
+template <int TH, int TY, int E, bool DROP, bool ODD, bool FULL>
 __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
   __shared__ float buf[2][16];
-  extern __shared__ float sums[];   // [workers][d]
+  extern __shared__ __attribute__((aligned(16))) float shared[];    // [workers][d]; FULL: and ahead of it post, pre, gate, 512 NW each
+  const bool with_dn = FULL || a.dn, with_dh = FULL || a.dh_out, with_post = FULL || a.post;
   const int lane = threadIdx.x & 63, wv = uniform(threadIdx.x >> 6), R = (int)(blockDim.x >> 6) / a.NW;
   const int worker = uniform(wv / a.NW), w = wv - worker * a.NW;
   RowSum rows{buf, a.NW, worker * a.NW, wv, 0};
@@ -415,44 +417,94 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
   int64_t grow = a.gate && a.gate_rows > 1 && r0 < a.N ? r0 / a.per : 0, gend = (grow + 1) * a.per;
   Raw8<TH> rt[E], rh[E];
   Raw8<TY> ry[E], rv[E];
-  // y and dn for the next row are loaded once this row's are unpacked, dh and h once the first sum has taken h's place
+  float next1 = 1.0f, next2 = 1.0f;
+  // y and dn for the next row are loaded once this row's are unpacked, dh and h once the first sum has taken h's place.
+  // Loads end in their order, so nothing else is loaded in between: what all rows share lies in LDS (FULL), and a load that
+  // some path left out would count as one that has ended (behind the last row it is loaded again).
   auto fetch_y = [&](int64_t row) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       fetch8<TY>(a.y, row, a.d, c[e], ry[e]);
-      if (a.dn) fetch8<TY>(a.dn, row, a.d, c[e], rv[e]);
+      if (with_dn) fetch8<TY>(a.dn, row, a.d, c[e], rv[e]);
     }
+    if (with_post) next1 = a.rs_post[row];
+    if (with_dn) next2 = a.rs_pre[row];
   };
   auto fetch_h = [&](int64_t row) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (a.dn) fetch8<TH>(a.h, row, a.d, c[e], rh[e]);
-      if (a.dh_out) fetch8<TH>(a.dh_out, row, a.d, c[e], rt[e]);
+      if (with_dn) fetch8<TH>(a.h, row, a.d, c[e], rh[e]);
+      if (with_dh) fetch8<TH>(a.dh_out, row, a.d, c[e], rt[e]);
     }
   };
+  // computed here, before the registers that it was computed from are loaded again
+  auto settle = [](float (&f)[8]) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) asm volatile("" : "+v"(f[q]));
+  };
   if (r0 < end) fetch_y(r0), fetch_h(r0);
-  // All workers make W turns, for the barriers of a row of many waves; one past its rows' end works on the last one
-  // that it fetched, for nobody.
+  if constexpr (FULL) {
+    static_assert(E == 1);
+    const int P = 512 * a.NW;
+    const float* from[2] = {a.post, a.pre};
+    for (int k = threadIdx.x; k < P; k += blockDim.x) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) shared[j * P + k] = k < a.d ? from[j][k] : 0.0f;
+    }
+    if (threadIdx.x < P / 8) {
+      const Cols o(8 * threadIdx.x, a.d);
+      float g[8];
+      if (a.gate) load8_any<ODD>(a.gate_type, a.gate, a.bpg ? blockIdx.x / a.bpg : 0, a.d, o, g);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) shared[2 * P + o.col + q] = a.gate ? g[q] : 1.0f;
+    }
+    __syncthreads();
+  }
+  auto param = [&](int k, const void* from, int e, float (&f)[8]) {
+    if constexpr (FULL) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(shared + k * 512 * a.NW + c[0].col);
+      const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[q] = lo[q], f[4 + q] = hi[q];
+    } else {
+      load8<LBK_FP32, ODD>(from, 0, a.d, c[e], f);
+    }
+  };
+  // All workers make W turns, for the barriers of a row of many waves; one past its rows' end only takes part in these.
   for (int64_t row = r0; row < r0 + a.W; ++row) {
-    const bool ok = row < end;
-    if (!ok && a.NW == 1) break;
-    if (a.gate && ok && row >= gend) ++grow, gend += a.per;
-    const float rs1 = a.post && ok ? a.rs_post[row] : 1.0f, rs2 = a.dn && ok ? a.rs_pre[row] : 1.0f;
+    if (row >= end) {
+      if (a.NW == 1) break;
+      if (with_dn) rows.over<Add>(0.f);
+      if (with_post) rows.over<Add>(0.f);
+      continue;
+    }
+    if (a.gate && row >= gend) ++grow, gend += a.per;
+    const float rs1 = next1, rs2 = next2;
     float t[E][8], y[E][8], z[E][8], g[E][8];
     u32x4 rnd[E];
+    float x[E][8], v[E][8];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       unpack8<TY, ODD>(ry[e], c[e], y[e]);
-      if (a.gate) load8_any<ODD>(a.gate_type, a.gate, grow, a.d, c[e], g[e]);
+      unpack8<TY, ODD>(rv[e], c[e], v[e]);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[e][q] *= rs1;             // x1
+      settle(y[e]), settle(v[e]);
+    }
+    const int64_t next = min(row + 1, end - 1);
+    fetch_y(next);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (FULL) param(2, nullptr, e, g[e]);
+      else if (a.gate) load8_any<ODD>(a.gate_type, a.gate, grow, a.d, c[e], g[e]);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        y[e][q] *= rs1;             // x1
         z[e][q] = y[e][q];
-        if (!a.gate) g[e][q] = 1.0f;
+        if (!FULL && !a.gate) g[e][q] = 1.0f;
       }
-      if (a.post) {
+      if (with_post) {
         float p[8];
-        load8<LBK_FP32, ODD>(a.post, 0, a.d, c[e], p);
+        param(0, a.post, e, p);
 #pragma unroll
         for (int q = 0; q < 8; ++q) z[e][q] *= p[q];
       }
@@ -461,21 +513,17 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
         drop8(z[e], rnd[e], a.r.cut, a.r.keep);
       }
     }
-    float x[E][8], v[E][8];
-#pragma unroll
-    for (int e = 0; e < E; ++e) unpack8<TY, ODD>(rv[e], c[e], v[e]);
-    if (row + 1 < end) fetch_y(row + 1);
     float dot = 0.f;
-    if (a.dn) {
+    if (with_dn) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         float p[8];
-        load8<LBK_FP32, ODD>(a.pre, 0, a.d, c[e], p);
+        param(1, a.pre, e, p);
         unpack8<TH, ODD>(rh[e], c[e], x[e]);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           x[e][q] = (x[e][q] + a.alpha * (z[e][q] * g[e][q])) * rs2;
-          if (ok) s_pre[e][q] += v[e][q] * x[e][q];
+          s_pre[e][q] += v[e][q] * x[e][q];
           v[e][q] *= p[q];
           dot += v[e][q] * x[e][q];
         }
@@ -487,44 +535,45 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
       unpack8<TH, ODD>(rt[e], c[e], t[e]);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        if (!a.dh_out) t[e][q] = 0.f;
-        if (a.dn) t[e][q] += rs2 * (v[e][q] - x[e][q] * dot);
+        if (!with_dh) t[e][q] = 0.f;
+        if (with_dn) t[e][q] += rs2 * (v[e][q] - x[e][q] * dot);
       }
+      settle(t[e]);
     }
-    if (row + 1 < end) fetch_h(row + 1);
+    fetch_h(next);
     dot = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (a.dh && ok) store8<TH, ODD>(a.dh, row, a.d, c[e], t[e]);
+      if (FULL || a.dh) store8<TH, ODD>(a.dh, row, a.d, c[e], t[e]);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         t[e][q] *= a.alpha;
-        if (ok) s_gate[e][q] += t[e][q] * z[e][q];
+        s_gate[e][q] += t[e][q] * z[e][q];
         t[e][q] *= g[e][q];
       }
       if constexpr (DROP) drop8(t[e], rnd[e], a.r.cut, a.r.keep);
-      if (a.post) {
+      if (with_post) {
         float p[8];
-        load8<LBK_FP32, ODD>(a.post, 0, a.d, c[e], p);
+        param(0, a.post, e, p);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          if (ok) s_post[e][q] += t[e][q] * y[e][q];
+          s_post[e][q] += t[e][q] * y[e][q];
           t[e][q] *= p[q];
           dot += t[e][q] * y[e][q];
         }
       }
     }
-    if (a.post) {
+    if (with_post) {
       dot = rows.over<Add>(dot) / (float)a.d;
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
         for (int q = 0; q < 8; ++q) t[e][q] = rs1 * (t[e][q] - y[e][q] * dot);
     }
-    if (a.dy && ok)
+    if (FULL || a.dy)
 #pragma unroll
       for (int e = 0; e < E; ++e) store8<TY, ODD>(a.dy, row, a.d, c[e], t[e]);
-    if (a.d_gate && a.bpg == 0 && ok && row + 1 == gend) {
+    if (!FULL && a.d_gate && a.bpg == 0 && row + 1 == gend) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         store8_any<ODD>(a.gate_type, a.d_gate, grow, a.d, c[e], s_gate[e]);
@@ -533,6 +582,7 @@ __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
       }
     }
   }
+  float* sums = shared + (FULL ? 3 * 512 * a.NW : 0);
   if (!a.part) return;
   // the workers' sums in their order, one vector after the other through LDS
 #pragma unroll
@@ -637,10 +687,10 @@ struct BwdPlan {
 BwdPlan bwd_plan(int64_t N, int d, bool gate, int64_t gate_rows) {
   BwdPlan p;
   p.row = row_plan(d);
-  // workgroups of four waves, three on a CU, as the kernel's registers allow (16384 x 1024: 75.4 us; eight waves, one on a
-  // CU: 78.4, four waves, two on a CU: 82.1); rows of eight waves one on a CU
-  p.R = p.row.NW < 4 ? 4 / p.row.NW : 1;
-  const int64_t most = p.row.NW == 8 ? 256 : 768, W = (N + most * p.R - 1) / (most * p.R);
+  // workgroups of eight waves, one on a CU (backward and sums of 16384 x 1024: 64.9 us, of 4097 x 1001 in fp16 25.5; four
+  // waves, two on a CU: 64.0 and 28.5, three: 65.9 and 29.3; eight waves, two on a CU: 68.5 and 34.5)
+  p.R = 8 / p.row.NW;
+  const int64_t most = 256, W = (N + most * p.R - 1) / (most * p.R);
   const int64_t per = gate ? N / gate_rows : N;
   p.W = W;
   if (!gate) {
@@ -681,11 +731,17 @@ int check_seam(const lbk_seam* s, SeamArgs& a) {
 
 template <int TH, int TY, int E, bool ODD, bool BWD>
 int launch_seam_e(const SeamArgs& a, int64_t blocks, int threads, int lds, hipStream_t st) {
-  auto go = [&](auto* k) {
-    k<<<(unsigned)blocks, threads, lds, st>>>(a);
+  auto go = [&](auto* k, int more = 0) {
+    k<<<(unsigned)blocks, threads, lds + more, st>>>(a);
     return launched();
   };
-  if constexpr (BWD) return a.r.cut ? go(seam_bwd_kernel<TH, TY, E, true, ODD>) : go(seam_bwd_kernel<TH, TY, E, false, ODD>);
+  if constexpr (BWD && E == 1) {
+    // a training step's call, all operands of its rows there and a workgroup's rows under one gate
+    if (a.dn && a.dh_out && a.post && a.dh && a.dy && (!a.gate || a.bpg))
+      return a.r.cut ? go(seam_bwd_kernel<TH, TY, E, true, ODD, true>, 3 * 2048 * a.NW)
+                     : go(seam_bwd_kernel<TH, TY, E, false, ODD, true>, 3 * 2048 * a.NW);
+  }
+  if constexpr (BWD) return a.r.cut ? go(seam_bwd_kernel<TH, TY, E, true, ODD, false>) : go(seam_bwd_kernel<TH, TY, E, false, ODD, false>);
   else return a.r.cut ? go(seam_fwd_kernel<TH, TY, E, true, ODD>) : go(seam_fwd_kernel<TH, TY, E, false, ODD>);
 }
 template <int TH, int TY, bool BWD>
