@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void shrink_kernel(Shrink p) {
 
 // ------------------------------------------------------------------ expand
 // out[token][f] = y[token][f] + sum over ranks of W[a][f][rank] t'[token][rank], W [n, F, r] with rows of ldw.
-// Memory-bound by y and out (16384 tokens, 1024 / 4096, rank 16: 268 MB in 55 us), or by W (64 tokens, an adapter each,
+// Memory-bound by y and out (16384 tokens, 1024 / 4096, rank 16: 268 MB in 53 us), or by W (64 tokens, an adapter each,
 // 4096 / 14336: 27 MB in 10 us).  A workgroup takes a tile and a share of F: it adds up t's shares, splits t' into LDS in
 // the order of the matrix instruction's operand (`planes`: and for grad, ranks first), and its waves share the features.
 // The 32 features of two products are dealt so that a lane ends with 8 consecutive ones of a token.
@@ -548,20 +548,22 @@ __device__ __forceinline__ void trade(u32x4& x, u32x4& y, bool upper) {
 // Larger tiles: bound by y and out.  A wave takes 128 features, whose part of W it holds in registers for all subtiles, one
 // subtile after the other: the four waves of a workgroup work on 1 KB of 16 rows at a time.  What counts is how much of a
 // row is in work together: 16384 tokens, 1024 / 4096, rank 16, took 85 us with 64 bytes of 64 rows a wave, 62 with 256 bytes
-// of 16 rows and a subtile a wave, 59 with W through LDS and whole lines a load, and 55 so; rank 64 (4099 tokens, 2048 /
-// 8192) 64, 81, 50 and 42.
-template <bool H, int RV, int RK>
+// of 16 rows and a subtile a wave, 59 with W through LDS and whole lines a load, 55 so, and 53 with loads that no path leaves out; rank 64
+// (4099 tokens, 2048 / 8192) 64, 81, 50 and 42, rank 16 there 42 and 35 (with loads left out for subtiles that are not there).
+template <bool H, int RV, int RK, bool Y>
 __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, const Tile& t, unsigned tile, unsigned chunk, u32x4* tf) {
   constexpr bool ONE = RK == R16;
   constexpr int STEPS = RK == R64 || RK == RMORE ? 2 : 1;      // of 32 ranks, held at a time
-  const bool bare = t.adapter == p.n;
+  // Loads end in their order, and one that some path leaves out counts as ended, so that the others are waited for with
+  // those behind them.  Up to 32 ranks, all loads are made and all four subtiles taken, whether there or not.  More ranks leave
+  // too few registers for that, and there a subtile that is not there costs more.
+  constexpr bool ALL = STEPS == 1;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), i = lane & 15, q = lane >> 4;
   const int subs = (t.count + 15) >> 4;
   const int units = (p.F + 127) / 128, u0 = (int)((int64_t)units * chunk / p.chunks) + w, u1 = (int)((int64_t)units * (chunk + 1) / p.chunks);
   const uint16_t* wa = p.w + (int64_t)t.adapter * p.F * p.ldw;
   u32x4 wv[4][STEPS][2];
   auto fetch_w = [&](int u, int rb) {
-    if (bare) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -570,7 +572,7 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
         for (int j = 0; j < 2; ++j)
           wv[e][st][j] = rank8<RV>(wa + (int64_t)min(128 * u + 32 * e + feature(i, j), p.F - 1) * p.ldw, ONE ? 8 * (q & 1) : 64 * rb + 32 * st + 8 * q, p.r);
   };
-  if (u0 < u1 && RK != RMORE) fetch_w(u0, 0);                  // it needs no more than the tile
+  if (RK != RMORE && u0 < u1) fetch_w(u0, 0);                  // it needs no more than the tile
   // y and out by whole lines: of tokens i % 8 and 8 + i % 8 of a subtile, features 64 g + 32 (i / 8) + 8 q on
   const bool upper = i >= 8;
   int32_t row[4][2];
@@ -583,56 +585,54 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int fl = column(u, e >> 1);
-      y[e] = p.y && s < subs && fl < p.F ? *reinterpret_cast<const u32x4*>(p.y + row[s][e & 1] * p.ldy + fl) : u32x4{0, 0, 0, 0};
+      if (Y && (ALL || (s < subs && fl < p.F))) y[e] = *reinterpret_cast<const u32x4*>(p.y + row[s][e & 1] * p.ldy + min(fl, p.F - 8));
+      else y[e] = u32x4{0, 0, 0, 0};
     }
   };
   u32x4 y0[4], y1[4];                                          // subtiles in turn, loaded again as soon as they are used up
   if (u0 < u1) fetch_y(u0, 0, y0), fetch_y(u0, 1, y1);
-  if (!bare) {
-    split_t<RK, false>(p, t, tile, tf);
-    __syncthreads();
-    if (p.planes && chunk == 0) put_planes<RK>(p, t, tile, tf);
-  }
+  split_t<RK, false>(p, t, tile, tf);
+  __syncthreads();
+  if (p.planes && chunk == 0) put_planes<RK>(p, t, tile, tf);
   auto turn = [&](int u, int s, u32x4 (&y)[4]) {
+    const bool here = ALL || s < subs, more = ALL || u + 4 < u1;
+    const int next = ALL ? min(u + 4, units - 1) : u + 4;
     f32x4 acc[4][2] = {};
-    if (s < subs) {
-      if (!bare) {
-        const int blocks = RK == RMORE ? (p.r + 63) / 64 : 1;
-        for (int rb = 0; rb < blocks; ++rb) {
-          if (RK == RMORE) fetch_w(u, rb);
+    if (here) {
+      const int blocks = RK == RMORE ? (p.r + 63) / 64 : 1;
+      for (int rb = 0; rb < blocks; ++rb) {
+        if (RK == RMORE) fetch_w(u, rb);
 #pragma unroll
-          for (int st = 0; st < STEPS; ++st) {
-            const int step = 2 * rb + st;
-            if (RK == RMORE && 32 * step >= p.r) break;
-            u32x4 ta, tb;
-            if constexpr (ONE) ta = tb = tf[s * 64 + lane];
-            else ta = tf[step * 512 + s * 64 + lane], tb = tf[step * 512 + 256 + s * 64 + lane];
+        for (int st = 0; st < STEPS; ++st) {
+          const int step = 2 * rb + st;
+          if (RK == RMORE && 32 * step >= p.r) break;
+          u32x4 ta, tb;
+          if constexpr (ONE) ta = tb = tf[s * 64 + lane];
+          else ta = tf[step * 512 + s * 64 + lane], tb = tf[step * 512 + 256 + s * 64 + lane];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) add_step<H, ONE>(wv[e][st], ta, tb, acc[e]);
-          }
+          for (int e = 0; e < 4; ++e) add_step<H, ONE>(wv[e][st], ta, tb, acc[e]);
         }
       }
     }
     // ahead of the stores: they would have to end before it is there (rank 64: 43.3 -> 42.1 us)
-    if (s == 3 && u + 4 < u1 && RK != RMORE) fetch_w(u + 4, 0);
-    if (s < subs) {
+    if (s == 3 && more && RK != RMORE) fetch_w(next, 0);
+    u32x4 o[4] = {y[0], y[1], y[2], y[3]};
+    if (here)
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        u32x4 o[2] = {y[2 * g], y[2 * g + 1]};
-        if (!bare) {
-          trade(o[0], o[1], upper);
-          o[0] = plus<H>(o[0], acc[2 * g]);
-          o[1] = plus<H>(o[1], acc[2 * g + 1]);
-          trade(o[0], o[1], upper);
-        }
-        const int fl = column(u, g);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (16 * s + 8 * e + (i & 7) < t.count && fl < p.F) *reinterpret_cast<u32x4*>(p.out + row[s][e] * p.ldo + fl) = o[e];
+        trade(o[2 * g], o[2 * g + 1], upper);
+        o[2 * g] = plus<H>(o[2 * g], acc[2 * g]);
+        o[2 * g + 1] = plus<H>(o[2 * g + 1], acc[2 * g + 1]);
+        trade(o[2 * g], o[2 * g + 1], upper);
       }
-    }
-    if (s < 2) fetch_y(u, s + 2, y);
-    else if (u + 4 < u1) fetch_y(u + 4, s - 2, y);
+    if (ALL) fetch_y(s < 2 ? u : next, s ^ 2, y);
+    if (here)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int fl = column(u, e >> 1);
+        if (16 * s + 8 * (e & 1) + (i & 7) < t.count && fl < p.F) *reinterpret_cast<u32x4*>(p.out + row[s][e & 1] * p.ldo + fl) = o[e];
+      }
+    if (!ALL && (s < 2 || more)) fetch_y(s < 2 ? u : next, s ^ 2, y);
   };
   for (int u = u0; u < u1; u += 4) {
     turn(u, 0, y0);
@@ -642,10 +642,30 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
   }
 }
 
+// Tokens without an adapter: out = y (or zero)
+__device__ __forceinline__ void copy_rows(const Expand& p, const Plan& plan, const Tile& t, unsigned chunk) {
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+  const int units = (p.F + 511) / 512, u0 = (int)((int64_t)units * chunk / p.chunks), u1 = (int)((int64_t)units * (chunk + 1) / p.chunks);
+  const int f0 = 512 * u0 + 8 * lane, f1 = min(512 * u1, p.F);
+  for (int s = 4 * w; s < t.count; s += 16) {      // four rows in flight
+    int64_t row[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) row[j] = row_at(plan, t.first + min(s + j, t.count - 1), p.N);
+    for (int f = f0; f < f1; f += 512) {
+      u32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = p.y ? *reinterpret_cast<const u32x4*>(p.y + row[j] * p.ldy + f) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (s + j < t.count) *reinterpret_cast<u32x4*>(p.out + row[j] * p.ldo + f) = v[j];
+    }
+  }
+}
+
 // (registers for two waves a SIMD where tiles are large: held to three, the kernel is slower, 57 against 44 us at rank 64 and 63
 // against 56 at rank 16, as more rows are open in memory at a time)
 template <bool H, int RV, int RK, bool FEW>
-__global__ __launch_bounds__(256) void expand_kernel(Expand p) {
+__global__ __launch_bounds__(256, FEW || RK == R64 ? 1 : 2) void expand_kernel(Expand p) {
   extern __shared__ u32x4 tf[];
   const Plan plan = plan_view(p.plan, p.N, p.n);
   // a tile's shares of F in consecutive workgroups: at any time all of a row's stretch is in work, not one share of all
@@ -656,7 +676,9 @@ __global__ __launch_bounds__(256) void expand_kernel(Expand p) {
   if (t.adapter < 0) return;
   if (t.adapter == p.n && p.y == p.out) return;
   if constexpr (FEW) expand_few<H, RV, RK>(p, plan, t, tile, chunk, tf);
-  else expand_many<H, RV, RK>(p, plan, t, tile, chunk, tf);
+  else if (t.adapter == p.n) copy_rows(p, plan, t, chunk);
+  else if (p.y) expand_many<H, RV, RK, true>(p, plan, t, tile, chunk, tf);
+  else expand_many<H, RV, RK, false>(p, plan, t, tile, chunk, tf);
 }
 
 // ------------------------------------------------------------------ grad
