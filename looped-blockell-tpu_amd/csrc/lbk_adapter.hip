@@ -973,6 +973,8 @@ int check_adapter(const lbk_adapter* d) {
   if (d->n < 1 || d->rank < 1 || d->in_features < 8 || d->out_features < 8 || d->in_features % 8 || d->out_features % 8) return LBK_ERR_SHAPE;
   if (d->n > MAX_ADAPTERS || d->rank > MAX_RANK || d->N > (1 << 30) || d->in_features > (1 << 21) || d->out_features > (1 << 21))
     return LBK_ERR_TOO_LARGE;
+  // a launch takes fewer than 2^32 threads; so many tiles are not split into shares
+  if (max_tiles(d->N, d->n) > (int64_t)UINT32_MAX / 256) return LBK_ERR_TOO_LARGE;
   return LBK_OK;
 }
 

@@ -69,6 +69,20 @@ def test_adapter_validation_codes():
         assert q(C.byref(d())) > 0 and q(C.byref(d(N=0))) == 0 and q(C.byref(d(r=0))) == 0
 
 
+@needs_lib
+def test_calls_beyond_a_launch():
+    """Tiles of 2^32 threads or more are refused before anything is queued (the pointers are never read)."""
+    from looped_blockell import abi as A
+    lib = A.load()
+    most = (2 ** 24 - 1 - 5) * 64 + 63
+    for N, fits in ((most, True), (most + 1, False)):
+        k = A.Adapter(P, P, None, P, N, 4, 16, 8, 8, 0)
+        ws = 1 << 44 if not fits else 0
+        add = lib.lbk_adapter_add(C.byref(k), P, 8, P, 8, P, 8, None, P, ws, None)
+        bwd = lib.lbk_adapter_bwd(C.byref(k), P, 8, P, 8, P, P, P, P, P, ws, None)
+        assert add == bwd == (A.LBK_ERR_WORKSPACE if fits else A.LBK_ERR_TOO_LARGE)
+
+
 @needs_ext
 def test_shape_functions_and_refusals():
     from looped_blockell import kernels as K
