@@ -655,6 +655,8 @@ __global__ __launch_bounds__(1024) void seam_sum_kernel(SumArgs a) {
 // ------------------------------------------------------------------ launches
 inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 inline int launched() { return hipGetLastError() == hipSuccess ? LBK_OK : LBK_ERR_LAUNCH; }
+// a launch takes fewer than 2^32 threads
+inline bool too_many(int64_t blocks, int threads) { return blocks > (int64_t)UINT32_MAX / threads; }
 inline bool elem_aligned(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == LBK_FP32 ? 3u : 1u)) == 0; }
 
 bool random_of(double p, const int64_t* seed_dev, int64_t seed, uint32_t stream, Random& r) {
@@ -787,6 +789,7 @@ int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx,
   a.shift = 31 + s;
   a.magic = (uint32_t)((((uint64_t)1 << a.shift) + G - 1) / G);
   const int64_t blocks = (N * G + 256 * DROP_GROUPS - 1) / (256 * DROP_GROUPS);
+  if (too_many(blocks, 256)) return LBK_ERR_TOO_LARGE;
   auto go = [&](auto* k) {
     k<<<(unsigned)blocks, 256, 0, S(stream)>>>(a);
     return launched();
@@ -809,6 +812,7 @@ int lbk_residual_norm_fwd(const lbk_seam* s, const void* h, const void* y, void*
   const RowPlan p = row_plan(a.d);
   a.NW = p.NW;
   const int R = p.NW == 1 ? 4 : 1;
+  if (too_many((a.N + R - 1) / R, 64 * p.NW * R)) return LBK_ERR_TOO_LARGE;
   return launch_seam<false>(s->state_type, s->type, a, p.E, (a.N + R - 1) / R, 64 * p.NW * R, 0, S(stream));
 }
 
@@ -849,7 +853,7 @@ int lbk_residual_norm_bwd(const lbk_seam* s, const void* h, const void* y, const
   SumArgs m{static_cast<float*>(workspace), p.blocks, p.bpg, a.d, a.gate_type, (a.d + 63) / 64, d_pre, d_post, d_gate};
   // a gate without rows has no gradients to write, but for the one row that stands for none
   const int64_t jobs = 2 + (d_gate && (p.bpg || a.N == 0) ? a.gate_rows : 0);
-  if (jobs * m.chunks > 0x7fffffff) return LBK_ERR_TOO_LARGE;
+  if (too_many(jobs * m.chunks, 1024)) return LBK_ERR_TOO_LARGE;
   seam_sum_kernel<<<(unsigned)(jobs * m.chunks), 1024, 0, S(stream)>>>(m);
   return launched();
 }

@@ -94,6 +94,21 @@ def test_seam_validation_codes():
     assert bwd(s(N=0), y=None, h=None, r1=None, r2=None, dh_out=None, dn=None, dh=None, dy=None, dpost=None, dpre=None, ws=None, nb=0) == A.LBK_OK
 
 
+@needs_lib
+def test_calls_beyond_a_launch():
+    """2^32 threads or more are refused before anything is queued (the pointers are never read)."""
+    from looped_blockell import abi as A
+    lib = A.load()
+    a = A.Seam(1 << 26, 8, 0, 0, None, None, None, 0, 1, 1.0, 1e-5, 0.0, None, 0, 0)
+    assert lib.lbk_residual_norm_fwd(C.byref(a), P, P, P, None, None, None, None) == A.LBK_ERR_TOO_LARGE
+    a.d = 8192
+    assert lib.lbk_residual_norm_fwd(C.byref(a), P, P, P, None, None, None, None) == A.LBK_ERR_TOO_LARGE
+    assert lib.lbk_dropout(P, 0, 1 << 34, 8, 8, 0.5, None, 0, 0, P, None) == A.LBK_ERR_TOO_LARGE
+    a.N, a.d, a.gate, a.gate_type, a.gate_rows = 0, 8, P, 0, 1 << 22
+    assert lib.lbk_residual_norm_bwd(C.byref(a), None, None, None, None, None, None, None, None, None, P, None, None, 0,
+                                     None) == A.LBK_ERR_TOO_LARGE
+
+
 @needs_ext
 def test_shape_functions():
     from looped_blockell import kernels as K
