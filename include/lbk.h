@@ -899,8 +899,7 @@ int lbk_residual_norm_bwd(const lbk_seam* s, const void* h, const void* y, const
  * Low-rank adapters of many requests beside one shared projection:
  *   out[t] = y[t] + scales[a] * b[a] (a[a] x[t]),  a = ids[t];   out[t] = y[t] where ids[t] lies outside [0, n)
  * x [N, in], y and out [N, out], a [n, rank, in], b [n, out, rank], all of one type (LBK_BF16 or LBK_FP16), scales [n] fp32
- * or NULL (1).  Sums and a x are fp32 (a x and, in the backward, b^T dout enter the second products in 16 bits of
- * mantissa).  in and out are multiples of 8, rank 1 .. 256, n 1 .. 4096, N / 64 + n below 2^24 - 1; rows of x, y, out and dout have a
+ * or NULL (1).  Sums, a x and, in the backward, b^T dout are fp32 and enter the second products as such.  in and out are multiples of 8, rank 1 .. 256, n 1 .. 4096, N / 64 + n below 2^24 - 1; rows of x, y, out and dout have a
  * stride in elements, rows and pointers are 16-byte aligned; out may be y.  No counterpart in the reference.
  *
  * The plan holds the tokens sorted by adapter (stable), for any number of projections of one batch: an opaque device

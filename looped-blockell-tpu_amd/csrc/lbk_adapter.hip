@@ -5,9 +5,9 @@
 // Tokens are sorted by adapter once for all projections (the plan) and taken in tiles of up to 64 tokens of one adapter:
 //   shrink  t = A x of a tile, K in shares, fp32 partial sums          expand  out = y + B t', t' = s (sum of t's shares)
 //   grad    dA = dt'^T x, dB = dy^T t' over an adapter's tiles         with dt' = s B^T dy by shrink, dx = A^T dt' by expand
-// t' and dt' enter the second products as two bf16 each (the upper 16 bits and the rest, 16 bits of mantissa in all): in
-// one they would add as much error as the results' own rounding, and with ranks of 16 the second fills a half of the
-// matrix instruction's K that would lie idle.  fp16 operands beside them are split the same way, which is exact.
+// t' and dt' enter the second products as three bf16 each, which hold all 24 bits of an fp32 mantissa (8 bits at a time, cut
+// off and not rounded): fp32 sums as the first products', at three matrix instructions where these calls wait for memory.
+// fp16 operands beside them are two bf16, which is exact; of the six products the last, below 2^-24 of the whole, is left out.
 #include "lbk.h"
 #include "lbk_device.h"
 #include "lbk_internal.h"
@@ -211,22 +211,21 @@ template <bool H> __device__ __forceinline__ uint32_t pack2h(float lo, float hi)
   }
 }
 
-// v = its upper 16 bits + a rest that bf16 holds to 8 bits.  An Inf has no rest (Inf - Inf is none), a NaN's rest is NaN.
+// v = its upper 16 bits + a rest; an Inf has no rest (Inf - Inf is none), a NaN's rest is NaN.  The rest's upper 16 bits and
+// what is left of it are bf16 again, exactly.
 __device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ float rest(float v) { return fabsf(v) == __builtin_inff() ? 0.0f : v - upper(v); }
-__device__ __forceinline__ void split8(const float (&f)[8], u32x4& hi, u32x4& lo) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    hi[k] = __builtin_amdgcn_perm(__float_as_uint(f[2 * k + 1]), __float_as_uint(f[2 * k]), 0x07060302u);
-    lo[k] = pack2_bf16(rest(f[2 * k]), rest(f[2 * k + 1]));
-  }
+__device__ __forceinline__ uint32_t upper2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 // eight fp16 values as two bf16 each, exactly
 __device__ __forceinline__ void split_f16(const u32x4& v, u32x4& hi, u32x4& lo) {
-  float f[8];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) f[2 * k] = half_lo<true>(v[k]), f[2 * k + 1] = half_hi<true>(v[k]);
-  split8(f, hi, lo);
+  for (int k = 0; k < 4; ++k) {
+    const float a = half_lo<true>(v[k]), b = half_hi<true>(v[k]);
+    hi[k] = upper2(a, b);
+    lo[k] = upper2(rest(a), rest(b));
+  }
 }
 
 // ------------------------------------------------------------------ shrink
@@ -327,7 +326,7 @@ struct Expand {
   bool few;
   const int32_t* plan;
   const float *part, *scales;
-  uint16_t* planes;             // [tile][upper, rest][ranks to 16][64 slots], or NULL
+  uint16_t* planes;             // [tile][three parts][ranks to 16][64 slots], or NULL
 };
 
 // the operand of a lane: ranks k .. k + 7 of a row, those from r on zero.  RV: ranks that lie aligned together
@@ -349,9 +348,12 @@ __device__ __forceinline__ u32x4 rank8(const uint16_t* row, int k, int r) {
   }
 }
 
-// Ranks up to 16 take one matrix instruction, upper and rest side by side in its K; more go 32 at a time, upper and rest
-// one after the other.
+// Ranks up to 16 take two matrix instructions, two parts of t' side by side in the first's K and the third in the second's;
+// more go 32 at a time, the parts one after the other.
 enum { R16, R32, R64, RMORE };
+// places of a step's second and third parts behind its first
+template <int RK> constexpr int second = RK == R16 ? 32 : 256;
+template <int RK> constexpr int third = RK == R16 ? 256 : 512;
 
 // over lanes l, l + 16, l + 32 and l + 48
 __device__ __forceinline__ float rows_sum(float x) {
@@ -361,8 +363,8 @@ __device__ __forceinline__ float rows_sum(float x) {
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// t' of a tile, its shares summed and scaled, split into LDS: [step of 32 ranks][upper, rest][subtile][lane] (R16: [subtile]
-// [lane]); slots without a token hold anything, as they stay in their columns of the products.  A thread has 4 ranks of a
+// t' of a tile, its shares summed and scaled, split into LDS: [step of 32 ranks][part][subtile][lane] (R16: [two parts, the
+// third][subtile][lane]); slots without a token hold anything, as they stay in their columns of the products.  A thread has 4 ranks of a
 // token, the threads beside it the next ones (a token's 8 ranks each were 32 bytes of every row at a time: expand of 4099
 // tokens, 2048 / 8192, rank 64 43.9 -> 42.9 us).  FEW: lanes 16 apart take every fourth share each.
 template <int RK, bool FEW>
@@ -392,21 +394,20 @@ __device__ __forceinline__ void split_t(const Expand& p, const Tile& t, unsigned
       }
     }
     if (16 * s >= t.count) continue;         // the same for all lanes of a wave
-    u32x2 hi, lo;
+    float r[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (FEW) f[e] = rows_sum(f[e]);
       f[e] = rank + e < p.r ? f[e] * scale : 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      hi[e] = __builtin_amdgcn_perm(__float_as_uint(f[2 * e + 1]), __float_as_uint(f[2 * e]), 0x07060302u);
-      lo[e] = pack2_bf16(rest(f[2 * e]), rest(f[2 * e + 1]));
+      r[e] = rest(f[e]);
     }
     if (FEW && lane >= 16) continue;
-    const int at = RK == R16 ? s * 64 + 16 * (four >> 1) + l : (step * 8 + s) * 64 + 16 * (four >> 1) + l;
-    out[2 * at + (four & 1)] = hi;
-    out[2 * (at + (RK == R16 ? 32 : 256)) + (four & 1)] = lo;
+    const int at = RK == R16 ? s * 64 + 16 * (four >> 1) + l : (step * 12 + s) * 64 + 16 * (four >> 1) + l;
+    u32x2* const to = out + 2 * at + (four & 1);
+    to[0] = u32x2{upper2(f[0], f[1]), upper2(f[2], f[3])};
+    to[2 * second<RK>] = u32x2{upper2(r[0], r[1]), upper2(r[2], r[3])};
+    to[2 * third<RK>] = u32x2{upper2(rest(r[0]), rest(r[1])), upper2(rest(r[2]), rest(r[3]))};
+    if constexpr (RK == R16) to[2 * (third<RK> + 32)] = u32x2{0, 0};
   }
 }
 
@@ -416,28 +417,39 @@ __device__ __forceinline__ void put_planes(const Expand& p, const Tile& t, unsig
   const int slot = threadIdx.x & 63, w = uniform(threadIdx.x >> 6), s = slot >> 4, l = slot & 15, r16 = (p.r + 15) & ~15;
   const u32x4 none = {0, 0, 0, 0};
   for (int g = w; 8 * g < r16; g += 4) {
-    const int at = RK == R16 ? s * 64 + 16 * g + l : ((g >> 2) * 8 + s) * 64 + 16 * (g & 3) + l;
-    const u32x4 hi = slot < t.count ? tf[at] : none, lo = slot < t.count ? tf[at + (RK == R16 ? 32 : 256)] : none;
-    uint16_t* pl = p.planes + ((int64_t)tile * 2 * r16 + 8 * g) * TILE + slot;
+    const int at = RK == R16 ? s * 64 + 16 * g + l : ((g >> 2) * 12 + s) * 64 + 16 * (g & 3) + l;
+    const u32x4 part[3] = {slot < t.count ? tf[at] : none, slot < t.count ? tf[at + second<RK>] : none, slot < t.count ? tf[at + third<RK>] : none};
+    uint16_t* pl = p.planes + ((int64_t)tile * 3 * r16 + 8 * g) * TILE + slot;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      pl[e * TILE] = (uint16_t)(hi[e >> 1] >> (16 * (e & 1)));
-      pl[(r16 + e) * TILE] = (uint16_t)(lo[e >> 1] >> (16 * (e & 1)));
-    }
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pl[(k * r16 + e) * TILE] = (uint16_t)(part[k][e >> 1] >> (16 * (e & 1)));
   }
 }
 
+// t' of a subtile and step as the matrix instructions take it (R16: two of them)
+template <int RK> struct Parts { u32x4 v[RK == R16 ? 2 : 3]; };
+template <int RK>
+__device__ __forceinline__ Parts<RK> parts_of(const u32x4* tf, int step, int sub, int lane) {
+  const u32x4* at = tf + (step * 12 + sub) * 64 + lane;
+  if constexpr (RK == R16) return {{at[0], at[third<RK>]}};
+  else return {{at[0], at[second<RK>], at[third<RK>]}};
+}
+
 // 32 features of 16 tokens, ranks of one step: the product added to acc[0 .. 1]
-template <bool H, bool ONE>
-__device__ __forceinline__ void add_step(const u32x4 (&w)[2], const u32x4& ta, const u32x4& tb, f32x4 (&acc)[2]) {
+template <bool H, int RK>
+__device__ __forceinline__ void add_step(const u32x4 (&w)[2], const Parts<RK>& t, f32x4 (&acc)[2]) {
+  constexpr int P = RK == R16 ? 2 : 3;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     u32x4 wv = w[j], wl;
     if constexpr (H) split_f16(w[j], wv, wl);
-    acc[j] = mfma_bf16(wv, ta, acc[j]);
-    if constexpr (!ONE) acc[j] = mfma_bf16(wv, tb, acc[j]);
-    if constexpr (H) acc[j] = mfma_bf16(wl, ta, acc[j]);
-    if constexpr (H && !ONE) acc[j] = mfma_bf16(wl, tb, acc[j]);
+#pragma unroll
+    for (int k = 0; k < P; ++k) acc[j] = mfma_bf16(wv, t.v[k], acc[j]);
+    if constexpr (H) {
+#pragma unroll
+      for (int k = 0; k + 1 < P; ++k) acc[j] = mfma_bf16(wl, t.v[k], acc[j]);
+    }
   }
 }
 template <bool H>
@@ -495,23 +507,23 @@ __device__ __forceinline__ void expand_few(const Expand& p, const Plan& plan, co
     if (p.planes && chunk == 0) put_planes<RK>(p, t, tile, tf);
   }
   int sub = 0;
-  u32x4 t16;
+  Parts<RK> t16;
   auto turn = [&](int u, Unit& v) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       f32x4 acc[2] = {};
       if (!bare) {
         if constexpr (ONE) {
-          add_step<H, true>(v.w[e][0], t16, t16, acc);
+          add_step<H, RK>(v.w[e][0], t16, acc);
         } else if constexpr (RK == RMORE) {
           for (int st = 0; st < (p.r + 31) / 32; ++st) {
             u32x4 w2[2];
             weights(64 * u + 32 * e, st, w2);
-            add_step<H, false>(w2, tf[st * 512 + sub * 64 + lane], tf[st * 512 + 256 + sub * 64 + lane], acc);
+            add_step<H, RK>(w2, parts_of<RK>(tf, st, sub, lane), acc);
           }
         } else {
 #pragma unroll
-          for (int st = 0; st < STEPS; ++st) add_step<H, false>(v.w[e][st], tf[st * 512 + sub * 64 + lane], tf[st * 512 + 256 + sub * 64 + lane], acc);
+          for (int st = 0; st < STEPS; ++st) add_step<H, RK>(v.w[e][st], parts_of<RK>(tf, st, sub, lane), acc);
         }
       }
       const int fl = 64 * u + 32 * e + 8 * q;
@@ -520,7 +532,7 @@ __device__ __forceinline__ void expand_few(const Expand& p, const Plan& plan, co
     if (u + 8 < u1) fetch_w(u + 8, v), fetch_y(u + 8, v);
   };
   for (;;) {
-    if (ONE && !bare) t16 = tf[sub * 64 + lane];
+    if (ONE && !bare) t16 = parts_of<RK>(tf, 0, sub, lane);
     for (int u = u0; u < u1; u += 8) {
       turn(u, v0);
       if (u + 4 < u1) turn(u + 4, v1);
@@ -606,11 +618,9 @@ __device__ __forceinline__ void expand_many(const Expand& p, const Plan& plan, c
         for (int st = 0; st < STEPS; ++st) {
           const int step = 2 * rb + st;
           if (RK == RMORE && 32 * step >= p.r) break;
-          u32x4 ta, tb;
-          if constexpr (ONE) ta = tb = tf[s * 64 + lane];
-          else ta = tf[step * 512 + s * 64 + lane], tb = tf[step * 512 + 256 + s * 64 + lane];
+          const Parts<RK> parts = parts_of<RK>(tf, step, s, lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) add_step<H, ONE>(wv[e][st], ta, tb, acc[e]);
+          for (int e = 0; e < 4; ++e) add_step<H, RK>(wv[e][st], parts, acc[e]);
         }
       }
     }
@@ -684,7 +694,8 @@ __global__ __launch_bounds__(256, FEW || RK == R64 ? 1 : 2) void expand_kernel(E
 // ------------------------------------------------------------------ grad
 // part[piece][rank][f] = sum over the tokens of a piece of P[token][rank] Q[token][f], P from planes, Q = x or dy.
 // Memory-bound by Q (dA and dB of 16384 tokens, 1024 / 4096, rank 16: 168 MB in 34 us; 53 while three of four workgroups
-// of the grid had nothing to do).  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens
+// of the grid had nothing to do; held to the registers of four waves a SIMD at ranks up to 16, which is 7 of 166 us of the whole
+// training step).  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens
 // lie in an LDS slice of its own and are read transposed.  Where the adapter changes on the way, a piece ends: piece number =
 // tile / turn + the adapter's number among those with tokens, which grows with either.
 struct Grad {
@@ -701,7 +712,7 @@ struct Grad {
 constexpr int QROW = 72;             // elements of a token's row in LDS: 64 and 16 bytes, which moves the rows over the banks
 
 template <bool H, int RT>
-__global__ __launch_bounds__(256) void grad_kernel(Grad p) {
+__global__ __launch_bounds__(256, RT == 1 ? 4 : 1) void grad_kernel(Grad p) {
   __shared__ __attribute__((aligned(16))) uint16_t slices[4][(H ? 2 : 1) * 32 * QROW];
   const int z = blockIdx.x >= p.first, F = p.F[z], fb = (F + 255) / 256;
   const unsigned id = blockIdx.x - (z ? (unsigned)p.first : 0), run = id / fb;
@@ -747,7 +758,7 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
       for (int j = 0; j < 4; ++j) row[j] = plan.perm[s.t.first + min(32 * s.half + 8 * j + (lane >> 3), s.t.count - 1)];
   };
   struct Set {
-    u32x4 v[4], a[RT][2];
+    u32x4 v[4], a[RT][3];
   };
   auto rows = [&](const Step& s, const int32_t (&row)[4], Set& g) {
     if (s.ok)
@@ -760,11 +771,11 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
   };
   auto factors = [&](const Step& s, Set& g) {
     if (!s.ok) return;
-    const uint16_t* pl = p.planes[z] + (s.tile * 2 * r16 + r0 + i) * TILE + 32 * s.half + 8 * q;
+    const uint16_t* pl = p.planes[z] + (s.tile * 3 * r16 + r0 + i) * TILE + 32 * s.half + 8 * q;
 #pragma unroll
     for (int j = 0; j < RT; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 3; ++h)
         g.a[j][h] = r0 + 16 * j < r16 ? *reinterpret_cast<const u32x4*>(pl + (16 * j + h * r16) * TILE) : u32x4{0, 0, 0, 0};
   };
 
@@ -817,8 +828,8 @@ __global__ __launch_bounds__(256) void grad_kernel(Grad p) {
       if constexpr (H) bl = tr_frag(slice + 32 * QROW, QROW, 0, 16 * ft, lane);
 #pragma unroll
       for (int j = 0; j < RT; ++j) {
-        acc[j][ft] = mfma_bf16(g.a[j][0], b, acc[j][ft]);
-        acc[j][ft] = mfma_bf16(g.a[j][1], b, acc[j][ft]);
+#pragma unroll
+        for (int h = 0; h < 3; ++h) acc[j][ft] = mfma_bf16(g.a[j][h], b, acc[j][ft]);
         if constexpr (H) acc[j][ft] = mfma_bf16(g.a[j][1], bl, mfma_bf16(g.a[j][0], bl, acc[j][ft]));
       }
     }
@@ -929,7 +940,7 @@ int chunks_of(int64_t tiles, int F, bool few) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(c, (F + unit - 1) / unit));
 }
 size_t part_bytes(int64_t tiles, int K, int r) { return align256((size_t)shares_of(tiles, K) * tiles * TILE * ((r + 3) & ~3) * 4); }
-size_t plane_bytes(int64_t tiles, int r) { return align256((size_t)tiles * 2 * ((r + 15) & ~15) * TILE * 2); }
+size_t plane_bytes(int64_t tiles, int r) { return align256((size_t)tiles * 3 * ((r + 15) & ~15) * TILE * 2); }
 
 // tiles of a workgroup of grad, and its pieces
 int turn_of(int64_t tiles, int F) {
@@ -950,12 +961,18 @@ int launch_shrink(bool h, const Shrink& p, hipStream_t st) {
   return h ? go(shrink_kernel<true, 4>, 4) : go(shrink_kernel<false, 4>, 4);
 }
 
+template <bool H, int RV, int RK, bool FEW>
+int launch_expand_f(const Expand& p, hipStream_t st) {
+  static std::atomic<uint64_t> limit{0};
+  const int lds = (RK == R16 ? 512 : (p.r + 31) / 32 * 768) * 16;      // t': at most 96 KB
+  const auto k = expand_kernel<H, RV, RK, FEW>;
+  if (lds > 65536 && set_lds_limit_once(reinterpret_cast<const void*>(k), MAX_RANK / 32 * 768 * 16, limit)) return LBK_ERR_LAUNCH;
+  k<<<(unsigned)(p.tiles * p.chunks), 256, lds, st>>>(p);
+  return launched();
+}
 template <bool H, int RV, int RK>
 int launch_expand_t(const Expand& p, hipStream_t st) {
-  const int lds = (RK == R16 ? 256 : (p.r + 31) / 32 * 512) * 16;      // t': at most 64 KB
-  if (p.few) expand_kernel<H, RV, RK, true><<<(unsigned)(p.tiles * p.chunks), 256, lds, st>>>(p);
-  else expand_kernel<H, RV, RK, false><<<(unsigned)(p.tiles * p.chunks), 256, lds, st>>>(p);
-  return launched();
+  return p.few ? launch_expand_f<H, RV, RK, true>(p, st) : launch_expand_f<H, RV, RK, false>(p, st);
 }
 template <bool H>
 int launch_expand_h(const Expand& p, hipStream_t st) {

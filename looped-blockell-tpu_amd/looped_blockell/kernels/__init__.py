@@ -595,7 +595,7 @@ def adapter_add(y, x, a, b, plan: AdapterPlan, scales=None, inplace: bool = Fals
     """``y + scales[id] * (x a[id]^T) b[id]^T`` with each token's adapter, y as it is where a token has none: the
     low-rank update beside a shared projection's y = base(x).  x is [..., in], y [..., out], a [n, rank, in] and b [n, out,
     rank], all bf16 or all fp16 (features multiples of 8, rank 1 .. 256); scales [n] fp32 or None (1).  ``a x`` stays in
-    fp32 up to 16 bits of mantissa.  Differentiable in y, x, a and b as one native autograd node;
+    fp32.  Differentiable in y, x, a and b as one native autograd node;
     ``inplace`` adds into y, without gradients."""
     _gpu(y, x, a, b)
     if plan.tokens * x.shape[-1] != x.numel() or plan.adapters != a.shape[0]:
