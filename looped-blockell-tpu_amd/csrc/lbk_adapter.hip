@@ -211,10 +211,16 @@ template <bool H> __device__ __forceinline__ uint32_t pack2h(float lo, float hi)
   }
 }
 
-// v = its upper 16 bits + a rest; an Inf has no rest (Inf - Inf is none), a NaN's rest is NaN.  The rest's upper 16 bits and
-// what is left of it are bf16 again, exactly.
+// v = its upper 16 bits + a rest, whose upper 16 bits and what is left of it are bf16 again, exactly.  Where nothing is left (of
+// an Inf too) the part is 2^-60 of the whole, which no fp32 sum beside the whole sees: a part of 0 times an Inf would be NaN
+// where the whole times the Inf is one (from |v| = 2^-73 on; parts of smaller values end as 0).  All parts have the whole's
+// sign, a NaN's are NaN.
 __device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
-__device__ __forceinline__ float rest(float v) { return fabsf(v) == __builtin_inff() ? 0.0f : v - upper(v); }
+__device__ __forceinline__ float faint(float v) { return v * 0x1p-60f; }
+__device__ __forceinline__ float rest(float v, float whole) {
+  const float r = v - upper(v);
+  return fabsf(r) > 0.0f ? r : faint(whole);
+}
 __device__ __forceinline__ uint32_t upper2(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
@@ -224,7 +230,7 @@ __device__ __forceinline__ void split_f16(const u32x4& v, u32x4& hi, u32x4& lo) 
   for (int k = 0; k < 4; ++k) {
     const float a = half_lo<true>(v[k]), b = half_hi<true>(v[k]);
     hi[k] = upper2(a, b);
-    lo[k] = upper2(rest(a), rest(b));
+    lo[k] = upper2(rest(a, a), rest(b, b));
   }
 }
 
@@ -399,15 +405,15 @@ __device__ __forceinline__ void split_t(const Expand& p, const Tile& t, unsigned
     for (int e = 0; e < 4; ++e) {
       if constexpr (FEW) f[e] = rows_sum(f[e]);
       f[e] = rank + e < p.r ? f[e] * scale : 0.0f;
-      r[e] = rest(f[e]);
+      r[e] = rest(f[e], f[e]);
     }
     if (FEW && lane >= 16) continue;
     const int at = RK == R16 ? s * 64 + 16 * (four >> 1) + l : (step * 12 + s) * 64 + 16 * (four >> 1) + l;
     u32x2* const to = out + 2 * at + (four & 1);
     to[0] = u32x2{upper2(f[0], f[1]), upper2(f[2], f[3])};
     to[2 * second<RK>] = u32x2{upper2(r[0], r[1]), upper2(r[2], r[3])};
-    to[2 * third<RK>] = u32x2{upper2(rest(r[0]), rest(r[1])), upper2(rest(r[2]), rest(r[3]))};
-    if constexpr (RK == R16) to[2 * (third<RK> + 32)] = u32x2{0, 0};
+    to[2 * third<RK>] = u32x2{upper2(rest(r[0], f[0]), rest(r[1], f[1])), upper2(rest(r[2], f[2]), rest(r[3], f[3]))};
+    if constexpr (RK == R16) to[2 * (third<RK> + 32)] = u32x2{upper2(faint(f[0]), faint(f[1])), upper2(faint(f[2]), faint(f[3]))};
   }
 }
 
