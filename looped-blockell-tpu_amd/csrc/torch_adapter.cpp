@@ -186,6 +186,7 @@ struct AdapterTrain : public torch::autograd::Function<AdapterTrain> {
 };
 
 Tensor adapter_add_autograd(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
+  no_tangents("adapter_add", y, x, a, b, scales);
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK(!needs_grad(scales), "titan::adapter_add: scales have no gradient");
     if (y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()) return AdapterTrain::apply(y, x, a, b, plan, scales);
@@ -195,6 +196,7 @@ Tensor adapter_add_autograd(const Tensor& y, const Tensor& x, const Tensor& a, c
   return op.call(y, x, a, b, plan, scales);
 }
 void adapter_add_inplace_autograd(Tensor y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
+  no_tangents("adapter_add_", y, x, a, b, scales);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()),
               "titan::adapter_add_ has no gradient");
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("titan::adapter_add_", "").typed<decltype(adapter_add_)>();

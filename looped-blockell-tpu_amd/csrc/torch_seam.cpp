@@ -68,6 +68,7 @@ struct Dropout : public torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout_autograd(const Tensor& x, double p, const OptTensor& seed_tensor, int64_t seed, int64_t stream) {
+  no_tangents("counter_dropout", x);
   if (at::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, p, seed_tensor, seed, stream);
   at::AutoDispatchBelowADInplaceOrView below;
   return call_dropout(x, p, seed_tensor, seed, stream);
@@ -251,6 +252,7 @@ using Two = std::tuple<Tensor, Tensor>;
 
 Two seam_autograd(const Tensor& h, const Tensor& y, const OptTensor& post, const OptTensor& gate, const OptTensor& pre, double scale,
                   double eps, double p, const OptTensor& seed_tensor, int64_t seed, int64_t stream) {
+  no_tangents("residual_norm", h, y, post, gate, pre);
   if (at::GradMode::is_enabled() &&
       (h.requires_grad() || y.requires_grad() || needs_grad(post) || needs_grad(gate) || needs_grad(pre))) {
     auto r = SeamTrain::apply(h, y, post, gate, pre, scale, eps, p, seed_tensor, seed, stream);

@@ -73,6 +73,14 @@ inline at::Tensor opt_bias(const c10::optional<at::Tensor>& b, int64_t n, const 
 }
 inline bool needs_grad(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
+// Forward-mode derivatives: refused, as an operator below autograd would return its result without the tangent.
+inline bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+inline bool has_tangent(const c10::optional<at::Tensor>& t) { return t.has_value() && has_tangent(*t); }
+template <class... T>
+inline void no_tangents(const char* op, const T&... operands) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(operands) || ...), "titan::", op, " has no forward-mode derivative");
+}
+
 // For a backward that calls operators: past the Autograd key, whose fallback boxes every argument, unless a graph of the
 // gradients is asked for (which those operators then refuse or, having a formula, record).
 struct BelowAutograd {
