@@ -93,13 +93,13 @@ struct Cols {
 // as loaded, so that a load can be in flight while something else is worked on
 template <int T> struct Raw8 { u32x4 v[T == LBK_FP32 ? 2 : 1]; };
 
-// SMALL: d may be less than 8 (one lane holds the row)
-template <int T, bool SMALL = false>
+// SMALL: d may be less than 8 (one lane holds the row).  Off: of a column's offset in bytes.  Where all lanes share the base and
+// rows are short, 32 bits make that one register of an address in a lane; a row of 2^30 fp32 columns or more needs 64.
+template <int T, bool SMALL = false, class Off = uint32_t>
 __device__ __forceinline__ void fetch8(const void* base, int64_t row, int d, const Cols& c, Raw8<T>& r) {
-  // a base that all lanes share and 32-bit offsets: one register of an address in a lane
   const auto* p = static_cast<const typename Elem<T>::type*>(base) + row * d;
   if (!SMALL || d >= 8) {
-    const auto* q = reinterpret_cast<const u32x4_2*>(reinterpret_cast<const char*>(p) + (uint32_t)c.from * (uint32_t)sizeof(*p));
+    const auto* q = reinterpret_cast<const u32x4_2*>(reinterpret_cast<const char*>(p) + (Off)c.from * (Off)sizeof(*p));
     r.v[0] = q[0];
     if constexpr (T == LBK_FP32) r.v[1] = q[1];
     return;
@@ -152,10 +152,10 @@ __device__ __forceinline__ uint32_t pack2_f16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
-template <int T, bool ODD = true>
+template <int T, bool ODD = true, class Off = uint32_t>
 __device__ __forceinline__ void store8(void* base, int64_t row, int d, const Cols& c, const float (&f)[8]) {
   auto* b = static_cast<typename Elem<T>::type*>(base) + row * d;
-  auto* p = reinterpret_cast<decltype(b)>(reinterpret_cast<char*>(b) + (uint32_t)c.col * (uint32_t)sizeof(*b));
+  auto* p = reinterpret_cast<decltype(b)>(reinterpret_cast<char*>(b) + (Off)c.col * (Off)sizeof(*b));
   if (c.n >= 8) {
     if constexpr (T == LBK_FP32) {
       *reinterpret_cast<f32x4_4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
@@ -215,14 +215,14 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
     c[k] = Cols(8 * (int)(off - dr * a.G), a.F);
     const bool there = row[k] < a.N;
     if (!there) c[k].n = 0;
-    fetch8<T, SMALL>(static_cast<const char*>(a.x) + (there ? row[k] : 0) * a.ldx * sizeof(typename Elem<T>::type), 0, a.F, c[k], raw[k]);
+    fetch8<T, SMALL, uint64_t>(static_cast<const char*>(a.x) + (there ? row[k] : 0) * a.ldx * sizeof(typename Elem<T>::type), 0, a.F, c[k], raw[k]);
   }
 #pragma unroll
   for (int k = 0; k < DROP_GROUPS; ++k) {
     float f[8];
     unpack8<T>(raw[k], c[k], f);
     drop8(f, random8(key, (uint32_t)c[k].col >> 3, row[k], a.r.stream), a.r.cut, a.r.keep);
-    store8<T>(a.y, row[k], a.F, c[k], f);
+    store8<T, true, uint64_t>(a.y, row[k], a.F, c[k], f);
   }
 }
 
