@@ -11,8 +11,9 @@ import torch.nn.functional as F
 from torch import nn
 
 from .. import kernels
-from .mlp import BlockELLLinear, _plain
-from .mx import MXBlockELLWeight
+from .dense import DenseMLPBlock
+from .mlp import _HOOKS, BlockELLLinear, MLPBlock, _plain
+from .mx import MXBlockELLWeight, MXMLPBlock
 
 
 def _features(base):
@@ -58,12 +59,26 @@ class AdapterLinear(nn.Module):
         return kernels.adapter_add(y, x, a, b, plan, scales=self.scales, inplace=own)
 
 
+def _takes_over(mlp) -> bool:
+    """Whether ``mlp`` is no more than its projections and the activation that its class puts between them."""
+    cls = next((c for c in (MLPBlock, MXMLPBlock, DenseMLPBlock) if isinstance(mlp, c)), None)
+    own = ("forward", "swiglu_weights", "swiglu_biases")
+    return (cls is not None and all(getattr(type(mlp), m, None) is getattr(cls, m, None) and m not in mlp.__dict__ for m in own)
+            and not any(mlp.__dict__[h] for h in _HOOKS))
+
+
 class AdapterMLPBlock(nn.Module):
-    """The FFN of an ``MLPBlock`` (SwiGLU or GELU) or an ``MXMLPBlock`` with adapters beside each projection.  The
-    projections run one by one, as an adapter's update comes before the activation."""
+    """The FFN of an ``MLPBlock`` (SwiGLU or GELU), an ``MXMLPBlock`` or a ``DenseMLPBlock`` (either activation, parameters of
+    its dtype) with adapters beside each projection.  The projections run one by one, as an adapter's update comes before
+    the activation.  Any other block, one whose forward is replaced and one with hooks are refused: only the projections
+    and the activation are taken over."""
 
     def __init__(self, mlp: nn.Module, n_adapters: int, rank: int, **kw):
         super().__init__()
+        if not _takes_over(mlp):
+            raise ValueError("adapters go beside the projections of an MLPBlock, an MXMLPBlock or a DenseMLPBlock without hooks and "
+                             f"with that class's forward, not of {type(mlp).__name__}")
+        self.activation = getattr(mlp, "activation", "silu") if hasattr(mlp, "w_gate") else "gelu"
         self.names = ("w_gate", "w_up", "w_down") if hasattr(mlp, "w_gate") else ("fc1", "fc2")
         inner, last = getattr(mlp, self.names[0]), getattr(mlp, self.names[-1])
         d_model, d_ff = _features(last)[1], _features(inner)[1]
@@ -74,10 +89,10 @@ class AdapterMLPBlock(nn.Module):
     def forward(self, x: torch.Tensor, plan=None, dropout_seed=None) -> torch.Tensor:
         lin = [getattr(self, n) for n in self.names]
         first = [m(x, plan, dropout_seed, k) for k, m in enumerate(lin[:-1])]
+        h = first[0].float()
+        h = F.silu(h) if self.activation == "silu" else F.gelu(h, approximate="tanh")
         if len(first) == 2:
-            h = F.silu(first[0].float()) * first[1].float()
-        else:
-            h = F.gelu(first[0].float(), approximate="tanh")
+            h = h * first[1].float()
         return lin[-1](h.to(first[0].dtype), plan, dropout_seed, len(first))
 
 

@@ -1,0 +1,98 @@
+"""``AdapterMLPBlock`` keeps what the block it is made of does: its activation and its dropout, or refuses the block.  Without a
+plan no kernel of the adapters runs, so a dense block's form is checked on the CPU."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+BF = torch.bfloat16
+
+
+def layers():
+    from looped_blockell import layers as L
+    return L
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_dense_block_keeps_its_activation(activation):
+    L = layers()
+    torch.manual_seed(0)
+    mlp = L.DenseMLPBlock(32, 64, activation=activation)
+    for p in mlp.parameters():
+        torch.nn.init.normal_(p, std=0.3)
+    x = torch.randn(7, 32).to(BF)
+    act = F.silu if activation == "silu" else lambda z: F.gelu(z, approximate="tanh")
+    with torch.no_grad():
+        h = (act(mlp.w_gate(x).float()) * mlp.w_up(x).float()).to(BF)
+        want = mlp.w_down(h)
+        assert torch.equal(L.AdapterMLPBlock(mlp, 2, 4)(x), want)
+
+
+def test_other_blocks_are_refused():
+    L = layers()
+
+    class Mine(torch.nn.Module):
+        def __init__(self, of):
+            super().__init__()
+            self.w_gate, self.w_up, self.w_down = of.w_gate, of.w_up, of.w_down
+
+    class Squared(L.MLPBlock):
+        def forward(self, x):
+            return super().forward(x) ** 2
+
+    class Alike(L.MLPBlock):
+        pass
+
+    dense = L.DenseMLPBlock(32, 64)
+    hooked = L.MLPBlock(32, 64, use_swiglu=True)
+    hooked.register_forward_hook(lambda m, a, y: None)
+    replaced = L.MLPBlock(32, 64)
+    replaced.forward = lambda x: x
+    for bad in (Mine(dense), Squared(32, 64, use_swiglu=True), hooked, replaced, torch.nn.Linear(32, 32)):
+        with pytest.raises(ValueError, match="adapters go beside"):
+            L.AdapterMLPBlock(bad, 2, 4)
+    for good in (L.MLPBlock(32, 64), L.MLPBlock(32, 64, use_swiglu=True), Alike(32, 64), dense):
+        L.AdapterMLPBlock(good, 2, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+def test_dense_block_with_adapters(gpu, activation, dtype):
+    """Against 64 bits, serving and with gradients: at most eight roundings of half a step one after the other (the products',
+    the adapters', the hidden state's and the gradients' own), whose gains are near one."""
+    from looped_blockell import kernels as K
+    L = layers()
+    g = torch.Generator().manual_seed(3)
+
+    def r(*s, scale=1.0):
+        return (torch.randn(*s, generator=g) * scale).to(gpu, dtype)
+
+    mlp = L.DenseMLPBlock(64, 128, activation=activation, dtype=dtype, device=gpu)
+    m = L.AdapterMLPBlock(mlp, 3, 4, dtype=dtype, device=gpu)
+    with torch.no_grad():
+        for name, p in m.named_parameters():
+            p.copy_(r(*p.shape, scale=p.shape[-1] ** -0.5))
+    ids = torch.randint(-1, 3, (40,), generator=g)
+    plan = K.adapter_plan(ids.to(gpu), 3)
+    x, dy = r(40, 64).requires_grad_(True), r(40, 64)
+    out = m(x, plan)
+    leaves = [x] + [p for _, p in m.named_parameters()]
+    got = torch.autograd.grad(out, leaves, dy)
+    p64 = {k: p.detach().double().requires_grad_(True) for k, p in m.named_parameters()}
+    x64 = x.detach().double().requires_grad_(True)
+
+    def lin(name, v):
+        k = ids.clamp(0).to(gpu)
+        d = (p64[name + ".b"][k] @ (p64[name + ".a"][k] @ v[:, :, None]))[:, :, 0]
+        return v @ p64[name + ".base.weight"].T + d * (ids >= 0).to(gpu)[:, None]
+
+    act = F.silu if activation == "silu" else lambda z: F.gelu(z, approximate="tanh")
+    want = lin("w_down", act(lin("w_gate", x64)) * lin("w_up", x64))
+    grads = torch.autograd.grad(want, [x64] + list(p64.values()), dy.double())
+    for a, b in zip([out, *got], [want, *grads]):
+        off = float((a.detach().double() - b.detach()).norm() / b.detach().norm())
+        assert off <= 8 * torch.finfo(dtype).eps / 2, off
+    with torch.no_grad():
+        served = m(x, plan)
+        assert float((served.double() - want).norm() / want.norm()) <= 8 * torch.finfo(dtype).eps / 2
