@@ -70,8 +70,12 @@ def _takes_over(mlp) -> bool:
 class AdapterMLPBlock(nn.Module):
     """The FFN of an ``MLPBlock`` (SwiGLU or GELU), an ``MXMLPBlock`` or a ``DenseMLPBlock`` (either activation, parameters of
     its dtype) with adapters beside each projection.  The projections run one by one, as an adapter's update comes before
-    the activation.  Any other block, one whose forward is replaced and one with hooks are refused: only the projections
-    and the activation are taken over."""
+    the activation.  Any other block, one whose forward is replaced and one with hooks are refused: only the projections,
+    the activation and the dropout of the result are taken over.
+
+    The result's dropout is the block's own (``MLPBlock``): with ``deterministic`` False, by torch's generator, or by
+    ``kernels.dropout`` with a ``dropout_seed``, which the adapters' dropout follows too.  The projections' streams are
+    ``dropout_stream`` and those behind it, in their order, the result's comes next: four of a gated block, three else."""
 
     def __init__(self, mlp: nn.Module, n_adapters: int, rank: int, **kw):
         super().__init__()
@@ -79,6 +83,7 @@ class AdapterMLPBlock(nn.Module):
             raise ValueError("adapters go beside the projections of an MLPBlock, an MXMLPBlock or a DenseMLPBlock without hooks and "
                              f"with that class's forward, not of {type(mlp).__name__}")
         self.activation = getattr(mlp, "activation", "silu") if hasattr(mlp, "w_gate") else "gelu"
+        self.dropout = getattr(mlp, "dropout", 0.0)
         self.names = ("w_gate", "w_up", "w_down") if hasattr(mlp, "w_gate") else ("fc1", "fc2")
         inner, last = getattr(mlp, self.names[0]), getattr(mlp, self.names[-1])
         d_model, d_ff = _features(last)[1], _features(inner)[1]
@@ -86,14 +91,20 @@ class AdapterMLPBlock(nn.Module):
             fin = d_ff if name == self.names[-1] else d_model
             setattr(self, name, AdapterLinear(getattr(mlp, name), n_adapters, rank, in_features=fin, **kw))
 
-    def forward(self, x: torch.Tensor, plan=None, dropout_seed=None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, plan=None, dropout_seed=None, dropout_stream: int = 0, deterministic: bool = True) -> torch.Tensor:
         lin = [getattr(self, n) for n in self.names]
-        first = [m(x, plan, dropout_seed, k) for k, m in enumerate(lin[:-1])]
+        first = [m(x, plan, dropout_seed, dropout_stream + k) for k, m in enumerate(lin[:-1])]
         h = first[0].float()
         h = F.silu(h) if self.activation == "silu" else F.gelu(h, approximate="tanh")
         if len(first) == 2:
             h = h * first[1].float()
-        return lin[-1](h.to(first[0].dtype), plan, dropout_seed, len(first))
+        out = lin[-1](h.to(first[0].dtype), plan, dropout_seed, dropout_stream + len(first))
+        if self.dropout > 0.0 and not deterministic:
+            if dropout_seed is None:
+                out = F.dropout(out, p=self.dropout, training=True)
+            else:
+                out = kernels.dropout(out, self.dropout, dropout_seed, dropout_stream + len(lin))
+        return out
 
 
 def set_adapter_plan(module: nn.Module, plan) -> None:

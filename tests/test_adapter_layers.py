@@ -96,3 +96,41 @@ def test_dense_block_with_adapters(gpu, activation, dtype):
     with torch.no_grad():
         served = m(x, plan)
         assert float((served.double() - want).norm() / want.norm()) <= 8 * torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("swiglu", [True, False])
+def test_dropout_of_the_block(gpu, swiglu):
+    """An ``MLPBlock``'s dropout of its result, by seed and by torch's generator; streams are counted from the call's."""
+    from looped_blockell import kernels as K
+    L = layers()
+    torch.manual_seed(4)
+    mlp = L.MLPBlock(64, 128, use_swiglu=swiglu, dropout=0.25, tile_size=16, device=gpu)
+    m = L.AdapterMLPBlock(mlp, 3, 4, dropout=0.5, device=gpu)
+    with torch.no_grad():
+        for n in m.names:
+            getattr(m, n).b.normal_(std=0.5)
+    x, dy = torch.randn(2, 15, 64, device=gpu, dtype=BF, requires_grad=True), torch.randn(2, 15, 64, device=gpu, dtype=BF)
+    plan = K.adapter_plan(torch.randint(-1, 3, (2, 15), device=gpu), 3)
+    last = len(m.names)
+    y = m(x, plan)
+    assert torch.equal(m(x, plan, deterministic=True), y)
+    torch.manual_seed(5)
+    a = m(x, plan, deterministic=False)
+    torch.manual_seed(5)
+    assert torch.equal(a, F.dropout(y, 0.25))
+    y = m(x, plan, 9, 20)                                   # the adapters' dropout alone
+    assert not torch.equal(y, m(x, plan, 9)) and not torch.equal(y, m(x, plan))
+    z = m(x, plan, dropout_seed=9, dropout_stream=20, deterministic=False)
+    assert torch.equal(z, K.dropout(y, 0.25, 9, 20 + last))
+    (d1,) = torch.autograd.grad(z, x, dy)
+    (d2,) = torch.autograd.grad(y, x, K.dropout(dy, 0.25, 9, 20 + last))
+    assert torch.equal(d1, d2)
+    # stream by stream: the projections' as they count, the result's behind them
+    h = [getattr(m, n)(x, plan, 9, 20 + k) for k, n in enumerate(m.names[:-1])]
+    act = F.silu(h[0].float()) * h[1].float() if swiglu else F.gelu(h[0].float(), approximate="tanh")
+    assert torch.equal(y, getattr(m, m.names[-1])(act.to(BF), plan, 9, 20 + last - 1))
+    with torch.no_grad():
+        served = m(x, plan, 9, 20, deterministic=False)
+        kept = K.dropout(torch.ones_like(served), 0.25, 9, 20 + last) != 0
+        assert not bool(served[~kept].any()) and torch.equal(served != 0, kept)
