@@ -25,7 +25,7 @@ from .norms import RMSNorm
 class LoopedSwiGLU(nn.Module):
     """``h <- h + MLP(RMSNorm(h))``, L times; with any of the last four options
     ``h <- h + residual_scale * gate * dropout(post_norm(MLP(norm(h))))``, an application's branch and the next one's norm
-    joined by ``kernels.residual_norm`` on the fp32 state.  ``gate``: a parameter [d_model] (ones), or per call a
+    joined by ``kernels.residual_norm`` on the fp32 state (a norm with hooks or of another class is called for itself).  ``gate``: a parameter [d_model] (ones), or per call a
     tensor [G, d_model] with a row for every N / G consecutive tokens in its place.  ``dropout`` drops with the
     ``dropout_seed`` of a call (application t with stream t), and not at all without one."""
 
@@ -42,13 +42,20 @@ class LoopedSwiGLU(nn.Module):
         self.residual_scale, self.dropout = residual_scale, dropout
 
     def _seams(self, h2: torch.Tensor, gate, seed) -> torch.Tensor:
-        hf, n = h2.float(), self.norm(h2)
-        post = None if self.post_norm is None else self.post_norm.scale
+        hf, n = h2.float(), None
+        # the norms' scales go into the joining operator; a norm with hooks, of another class or (of the branch) with
+        # another eps is called for itself, on a state rounded to bf16
+        fused = _plain(self.norm, RMSNorm)
+        eps = self.norm.eps if fused else getattr(self.post_norm, "eps", 1e-5)
+        fused_post = self.post_norm is not None and _plain(self.post_norm, RMSNorm) and self.post_norm.eps == eps
+        post = self.post_norm.scale if fused_post else None
         p = self.dropout if seed is not None else 0.0
         for t in range(self.L):
-            pre = self.norm.scale if t + 1 < self.L else None
-            hf, n = kernels.residual_norm(hf, self.mlp(n), post, gate, pre, self.residual_scale, self.norm.eps, p,
-                                          0 if seed is None else seed, t)
+            y = self.mlp(self.norm(hf.to(torch.bfloat16)) if n is None else n)
+            if self.post_norm is not None and not fused_post:
+                y = self.post_norm(y)
+            pre = self.norm.scale if fused and t + 1 < self.L else None
+            hf, n = kernels.residual_norm(hf, y, post, gate, pre, self.residual_scale, eps, p, 0 if seed is None else seed, t)
         return hf.to(torch.bfloat16)
 
     def forward(self, h: torch.Tensor, gate: torch.Tensor | None = None, dropout_seed=None) -> torch.Tensor:
