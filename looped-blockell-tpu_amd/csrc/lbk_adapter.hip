@@ -104,6 +104,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(const I* __restrict__ ids, i
         if (!__ballot(b[k] >= 0)) break;
         const uint64_t same = alike(b[k]);
         if (b[k] >= 0 && !(same & (((uint64_t)1 << lane) - 1))) cnt[w * (n + 1) + b[k]] += __popcll(same);
+        // a counter's next addition may be another lane's
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
     }
   __syncthreads();
