@@ -197,7 +197,8 @@ Tensor adapter_add_autograd(const Tensor& y, const Tensor& x, const Tensor& a, c
 }
 void adapter_add_inplace_autograd(Tensor y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& plan, const OptTensor& scales) {
   no_tangents("adapter_add_", y, x, a, b, scales);
-  TORCH_CHECK(!at::GradMode::is_enabled() || !(y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad()),
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(y.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad() || needs_grad(scales)),
               "titan::adapter_add_ has no gradient");
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("titan::adapter_add_", "").typed<decltype(adapter_add_)>();
   at::AutoDispatchBelowADInplaceOrView below;
