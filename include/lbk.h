@@ -927,8 +927,10 @@ int lbk_adapter_add(const lbk_adapter* d, const void* x, int64_t ldx, const void
 /*
  * Gradients for dout [N, out] (y's is dout itself): dx [N, in] contiguous (zero for tokens without an adapter), da and
  * db like a and b (zero for adapters without tokens), each optional (db needs planes).  Sums over tokens run in a fixed
- * order: no atomics.
+ * order: no atomics.  The workspace is that of the gradients passed (.._for), or of all three; most of it are the fp32 pieces of
+ * da and db, which grow with the smaller of N and n.
  */
+size_t lbk_adapter_bwd_workspace_bytes_for(const lbk_adapter* d, int dx, int da, int db);
 size_t lbk_adapter_bwd_workspace_bytes(const lbk_adapter* d);
 int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void* dout, int64_t ldo, const void* planes, void* dx,
                     void* da, void* db, void* workspace, size_t workspace_bytes, void* stream);

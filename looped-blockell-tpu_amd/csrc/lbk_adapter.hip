@@ -1064,25 +1064,28 @@ int lbk_adapter_add(const lbk_adapter* d, const void* x, int64_t ldx, const void
   return launch_expand(h, e, S(stream));
 }
 
-// shares of dy's shrink, planes of dt', the transposes of B and A, the pieces of dA and dB
+// shares of dy's shrink, planes of dt', the transposes of B and A, the pieces of dA and dB: what the wanted gradients need
 struct BwdParts {
   size_t part, planes, bt, at, pa, pb, all;
 };
-static BwdParts bwd_parts(const lbk_adapter* d) {
+static BwdParts bwd_parts(const lbk_adapter* d, bool dx, bool da, bool db) {
   const int64_t tiles = max_tiles(d->N, d->n);
-  BwdParts p;
-  p.part = part_bytes(tiles, d->out_features, d->rank);
-  p.planes = plane_bytes(tiles, d->rank);
-  p.bt = align256((size_t)d->n * d->rank * d->out_features * 2);
-  p.at = align256((size_t)d->n * ((d->rank + 7) & ~7) * d->in_features * 2);
+  BwdParts p{};
+  if (dx || da) p.part = part_bytes(tiles, d->out_features, d->rank);
+  if (dx || da) p.bt = align256((size_t)d->n * d->rank * d->out_features * 2);
+  if (da) p.planes = plane_bytes(tiles, d->rank);
+  if (dx) p.at = align256((size_t)d->n * ((d->rank + 7) & ~7) * d->in_features * 2);
   auto pieces = [&](int F) { return align256((size_t)pieces_of(tiles, d->N, d->n, turn_of(tiles, F)) * d->rank * F * 4); };
-  p.pa = pieces(d->in_features);
-  p.pb = pieces(d->out_features);
+  if (da) p.pa = pieces(d->in_features);
+  if (db) p.pb = pieces(d->out_features);
   p.all = p.part + p.planes + p.bt + p.at + p.pa + p.pb;
   return p;
 }
 
-size_t lbk_adapter_bwd_workspace_bytes(const lbk_adapter* d) { return check_adapter(d) || d->N == 0 ? 0 : bwd_parts(d).all; }
+size_t lbk_adapter_bwd_workspace_bytes_for(const lbk_adapter* d, int dx, int da, int db) {
+  return check_adapter(d) || d->N == 0 ? 0 : bwd_parts(d, dx, da, db).all;
+}
+size_t lbk_adapter_bwd_workspace_bytes(const lbk_adapter* d) { return lbk_adapter_bwd_workspace_bytes_for(d, 1, 1, 1); }
 
 int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void* dout, int64_t ldo, const void* planes, void* dx,
                     void* da, void* db, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1094,13 +1097,13 @@ int lbk_adapter_bwd(const lbk_adapter* d, const void* x, int64_t ldx, const void
   for (const void* p : {d->a, d->b, (const void*)d->plan, x, dout, planes, (const void*)dx, (const void*)da, (const void*)db, (const void*)workspace})
     if (!a16(p)) return LBK_ERR_ALIGN;
   if (ldx % 8 || ldo % 8 || (reinterpret_cast<uintptr_t>(d->scales) & 3)) return LBK_ERR_ALIGN;
-  if (some && (!workspace || workspace_bytes < lbk_adapter_bwd_workspace_bytes(d))) return LBK_ERR_WORKSPACE;
+  BwdParts sz{};
+  if (some) sz = bwd_parts(d, dx, da, db);
+  if (sz.all && (!workspace || workspace_bytes < sz.all)) return LBK_ERR_WORKSPACE;
   const bool h = d->type == LBK_FP16;
   const int64_t tiles = max_tiles(d->N, d->n);
   const int in = d->in_features, out = d->out_features, r = d->rank, rs = (r + 3) & ~3, r8 = (r + 7) & ~7;
   hipStream_t st = S(stream);
-  BwdParts sz{};
-  if (some) sz = bwd_parts(d);
   char* at = static_cast<char*>(workspace);
   auto take = [&](size_t b) {
     char* p = at;

@@ -141,7 +141,7 @@ Three adapter_add_bwd(const Tensor& dout_, const Tensor& x_, const Tensor& a, co
     d[j] = want[j] ? at::empty(like[j]->sizes(), x.options()) : at::empty({0}, x.options());
     q[j] = want[j] ? d[j].data_ptr() : nullptr;
   }
-  const size_t wsb = lbk_adapter_bwd_workspace_bytes(&k.d);
+  const size_t wsb = lbk_adapter_bwd_workspace_bytes_for(&k.d, want[0], want[1], want[2]);
   Tensor ws = workspace(wsb, x);
   LBK_CALL("adapter_add_bwd", lbk_adapter_bwd(&k.d, x.data_ptr(), ld(x), dout.data_ptr(), ld(dout), want[2] ? planes.data_ptr() : nullptr, q[0],
                                               q[1], q[2], ws.data_ptr(), wsb, cur_stream(x)));

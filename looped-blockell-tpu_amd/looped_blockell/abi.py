@@ -209,6 +209,7 @@ SIGNATURES = {
     "lbk_adapter_planes_bytes": (_SZ, [_PA]),
     "lbk_adapter_add_workspace_bytes": (_SZ, [_PA]),
     "lbk_adapter_add": (C.c_int, [_PA, _P, _I64, _P, _I64, _P, _I64, _P, _P, _SZ, _P]),
+    "lbk_adapter_bwd_workspace_bytes_for": (_SZ, [_PA, C.c_int, C.c_int, C.c_int]),
     "lbk_adapter_bwd_workspace_bytes": (_SZ, [_PA]),
     "lbk_adapter_bwd": (C.c_int, [_PA, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
 }
