@@ -864,7 +864,8 @@ int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx,
  *   n  = h' / sqrt(mean(h'^2) + eps) * pre_scale             (only with pre_scale; of h' before it is rounded)
  * h and h' are of state_type, y and n of `type`: the same one, or LBK_FP32 beside it.  Everything is contiguous
  * [N, d], 8 <= d <= 8192, and needs an element's alignment only.  gate [gate_rows, d]: row n takes gate row
- * n / (N / gate_rows).  A row of zeros has a norm of zeros; with eps = 0 it is NaN.  h' may be h.
+ * n / (N / gate_rows).  A row of zeros has a norm of zeros; with eps = 0 it is NaN, and rows below fp32's normal numbers
+ * (a root mean square under 2^-126) have no finite norm.  h' may be h.
  */
 typedef struct lbk_seam {
     int64_t N;

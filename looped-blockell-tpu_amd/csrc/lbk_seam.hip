@@ -266,8 +266,9 @@ struct RowSum {
   }
 };
 
-// rs of a row.  Squares pass fp32 from 1.8e19 on, which bf16 and fp32 rows may hold: such a row's are summed
-// again of values scaled by a power of two.  (The condition is the same in all waves of the row.)
+// rs of a row.  Squares pass fp32 from 1.8e19 on and lose bits below 1e-19 (which shows where eps is as small), and bf16 and fp32
+// rows may hold such values: their squares are summed again of values scaled by a power of two.  (The condition is the
+// same in all waves of the row.)
 template <int E>
 __device__ __forceinline__ float row_rs(const float (&v)[E][8], int d, float eps, RowSum& rows) {
   float ss = 0.f;
@@ -277,15 +278,15 @@ __device__ __forceinline__ float row_rs(const float (&v)[E][8], int d, float eps
     for (int q = 0; q < 8; ++q) ss += v[e][q] * v[e][q];
   ss = rows.over<Add>(ss);
   float rs = 1.0f / sqrtf(ss / (float)d + eps);
-  if (ss > 3.0e38f) {
+  if (ss > 3.0e38f || (ss < 0x1p-90f && eps < 0x1p-90f)) {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int q = 0; q < 8; ++q) top = fmaxf(top, fabsf(v[e][q]));
     top = rows.over<Max>(top);
-    if (top <= 3.4028235e38f) {
-      constexpr float s = 0x1p-80f;   // d <= 2^14: the sum lies between 2^-48 and 2^110
+    if (top > 0.0f && top <= 3.4028235e38f) {
+      const float s = ss > 1.0f ? 0x1p-80f : 0x1p80f;   // d <= 2^14: the sum lies between 2^-48 and 2^110, or 2^-138 and 2^84
       ss = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e)
