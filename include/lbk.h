@@ -851,7 +851,7 @@ int lbk_gated_bwd(int32_t dtype, const void* grad_out, const void* x, const uint
  * low.  With cut = floor(65536 p + 0.5), y = u >= cut ? x 65536 / (65536 - cut) : 0, so p counts in steps of 2^-16.
  * The backward is the same call on the gradient.  seed_dev (a device pointer) is read by the kernel in place of
  * seed where it is given: a replayed graph follows it.  Rows of x are ldx elements apart, y is contiguous and may
- * be x; both need an element's alignment only.  For the dropout of the reference's MLPBlock
+ * be x where ldx is F; both need an element's alignment only.  For the dropout of the reference's MLPBlock
  * (looped_blockell/layers/mlp.py:98-168), whose generator is not reproduced.
  */
 int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx, double p, const int64_t* seed_dev,
@@ -901,7 +901,7 @@ int lbk_residual_norm_bwd(const lbk_seam* s, const void* h, const void* y, const
  *   out[t] = y[t] + scales[a] * b[a] (a[a] x[t]),  a = ids[t];   out[t] = y[t] where ids[t] lies outside [0, n)
  * x [N, in], y and out [N, out], a [n, rank, in], b [n, out, rank], all of one type (LBK_BF16 or LBK_FP16), scales [n] fp32
  * or NULL (1).  Sums, a x and, in the backward, b^T dout are fp32 and enter the second products as such.  in and out are multiples of 8, rank 1 .. 256, n 1 .. 4096, N / 64 + n below 2^24 - 1; rows of x, y, out and dout have a
- * stride in elements, rows and pointers are 16-byte aligned; out may be y.  No counterpart in the reference.
+ * stride in elements, rows and pointers are 16-byte aligned; out may be y with its stride.  No counterpart in the reference.
  *
  * The plan holds the tokens sorted by adapter (stable), for any number of projections of one batch: an opaque device
  * buffer of lbk_adapter_plan_bytes(N, n) (0: sizes that are refused), 16-byte aligned, that the calls below read with

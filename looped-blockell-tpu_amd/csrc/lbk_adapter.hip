@@ -1050,6 +1050,7 @@ int lbk_adapter_add(const lbk_adapter* d, const void* x, int64_t ldx, const void
   for (const void* p : {d->a, d->b, (const void*)d->plan, x, y, (const void*)out, (const void*)planes, (const void*)workspace})
     if (!a16(p)) return LBK_ERR_ALIGN;
   if (ldx % 8 || ldy % 8 || ldo % 8 || (reinterpret_cast<uintptr_t>(d->scales) & 3)) return LBK_ERR_ALIGN;
+  if (out == y && ldo != ldy && d->N > 1) return LBK_ERR_ARG;      // rows of out would lie over other rows of y
   if (!workspace || workspace_bytes < lbk_adapter_add_workspace_bytes(d)) return LBK_ERR_WORKSPACE;
   const bool h = d->type == LBK_FP16;
   const int64_t tiles = max_tiles(d->N, d->n);

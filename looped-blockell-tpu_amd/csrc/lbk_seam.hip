@@ -781,6 +781,7 @@ int lbk_dropout(const void* x, int32_t dtype, int64_t N, int32_t F, int64_t ldx,
   if (F <= 0) return LBK_ERR_SHAPE;
   if (N == 0) return LBK_OK;
   if (!x || !y) return LBK_ERR_NULL;
+  if (x == y && ldx != F && N > 1) return LBK_ERR_ARG;      // rows of y would lie over other rows of x
   if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype)) return LBK_ERR_ALIGN;
   const int64_t G = ((int64_t)F + 7) / 8;
   if (N > INT64_MAX / 64 / ldx || N > ((int64_t)0x7fffffff * 256) / G) return LBK_ERR_TOO_LARGE;
