@@ -703,8 +703,9 @@ __global__ __launch_bounds__(256, FEW || RK == R64 ? 1 : 2) void expand_kernel(E
 // ------------------------------------------------------------------ grad
 // part[piece][rank][f] = sum over the tokens of a piece of P[token][rank] Q[token][f], P from planes, Q = x or dy.
 // Memory-bound by Q (dA and dB of 16384 tokens, 1024 / 4096, rank 16: 168 MB in 34 us; 53 while three of four workgroups
-// of the grid had nothing to do; held to the registers of four waves a SIMD at ranks up to 16, which is 7 of 166 us of the whole
-// training step).  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens
+// of the grid had nothing to do).  Registers are held to four waves a SIMD at ranks up to 16 (whole training step 159 us, at
+// three 166) and two above 32 (rank 64: 275 us, at one 308), and left to the compiler between (rank 32: 194 us, held to
+// three 200).  A workgroup takes `turn` tiles in a row, its waves 64 features each; a wave's 32 tokens
 // lie in an LDS slice of its own and are read transposed.  Where the adapter changes on the way, a piece ends: piece number =
 // tile / turn + the adapter's number among those with tokens, which grows with either.
 struct Grad {
@@ -721,7 +722,7 @@ struct Grad {
 constexpr int QROW = 72;             // elements of a token's row in LDS: 64 and 16 bytes, which moves the rows over the banks
 
 template <bool H, int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 4 : 1) void grad_kernel(Grad p) {
+__global__ __launch_bounds__(256, RT == 1 ? 4 : RT == 2 ? 1 : 2) void grad_kernel(Grad p) {
   __shared__ __attribute__((aligned(16))) uint16_t slices[4][(H ? 2 : 1) * 32 * QROW];
   const int z = blockIdx.x >= p.first, F = p.F[z], fb = (F + 255) / 256;
   const unsigned id = blockIdx.x - (z ? (unsigned)p.first : 0), run = id / fb;
