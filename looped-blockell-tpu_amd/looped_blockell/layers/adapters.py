@@ -84,6 +84,7 @@ class AdapterMLPBlock(nn.Module):
                              f"with that class's forward, not of {type(mlp).__name__}")
         self.activation = getattr(mlp, "activation", "silu") if hasattr(mlp, "w_gate") else "gelu"
         self.dropout = getattr(mlp, "dropout", 0.0)
+        self.dtype = mlp.dtype if isinstance(mlp, DenseMLPBlock) else None      # the others' projections round x
         self.names = ("w_gate", "w_up", "w_down") if hasattr(mlp, "w_gate") else ("fc1", "fc2")
         inner, last = getattr(mlp, self.names[0]), getattr(mlp, self.names[-1])
         d_model, d_ff = _features(last)[1], _features(inner)[1]
@@ -93,6 +94,8 @@ class AdapterMLPBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, plan=None, dropout_seed=None, dropout_stream: int = 0, deterministic: bool = True) -> torch.Tensor:
         lin = [getattr(self, n) for n in self.names]
+        if self.dtype is not None:
+            x = x.to(self.dtype)
         first = [m(x, plan, dropout_seed, dropout_stream + k) for k, m in enumerate(lin[:-1])]
         h = first[0].float()
         h = F.silu(h) if self.activation == "silu" else F.gelu(h, approximate="tanh")

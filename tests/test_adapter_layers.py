@@ -26,6 +26,7 @@ def test_dense_block_keeps_its_activation(activation):
         h = (act(mlp.w_gate(x).float()) * mlp.w_up(x).float()).to(BF)
         want = mlp.w_down(h)
         assert torch.equal(L.AdapterMLPBlock(mlp, 2, 4)(x), want)
+        assert torch.equal(L.AdapterMLPBlock(mlp, 2, 4)(x.float()), want)      # x is rounded to the block's dtype
 
 
 def test_other_blocks_are_refused():
