@@ -215,7 +215,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
     c[k] = Cols(8 * (int)(off - dr * a.G), a.F);
     const bool there = row[k] < a.N;
     if (!there) c[k].n = 0;
-    fetch8<T, SMALL, uint64_t>(static_cast<const char*>(a.x) + (there ? row[k] : 0) * a.ldx * sizeof(typename Elem<T>::type), 0, a.F, c[k], raw[k]);
+    const char* from = static_cast<const char*>(a.x) + (there ? row[k] : 0) * a.ldx * sizeof(typename Elem<T>::type);
+    fetch8<T, SMALL, uint64_t>(from, 0, a.F, c[k], raw[k]);
   }
 #pragma unroll
   for (int k = 0; k < DROP_GROUPS; ++k) {
@@ -391,8 +392,8 @@ __global__ __launch_bounds__(512) void seam_fwd_kernel(SeamArgs a) {
 // A workgroup takes consecutive rows, a worker (NW waves) W of these, and keeps the columns' sums in registers; the next
 // row's loads are in flight while a row is worked on.  Sums go to `part`, one row a workgroup, and are added in a fixed
 // order by seam_sum_kernel: no atomics.  A gate's rows either lie in one worker each (bpg = 0: written at once) or take bpg
-// workgroups each.  Memory-bound: 302 MB of 16384 x 1024 (fp32 state, bf16 branch) in 61 us with dropout, which is the copy's rate
-// (FULL; with post, pre and gate loaded in every row, which waits for the next row's loads too, 75).
+// workgroups each.  Memory-bound: 302 MB of 16384 x 1024 (fp32 state, bf16 branch) in 61 to 65 us by the card with dropout,
+// which is the copy's rate (FULL; with post, pre and gate loaded in every row, which waits for the next row's loads too, 75).
 template <int TH, int TY, int E, bool DROP, bool ODD, bool FULL>
 __global__ __launch_bounds__(512) void seam_bwd_kernel(SeamArgs a) {
   __shared__ float buf[2][16];
